@@ -18,6 +18,8 @@ FMT_F32, FMT_IQ4_NL, FMT_IQ4_XS = 0, 1, 2
 MODE_CONCAT_F32, MODE_PAIRSUM_ADD_BF16 = 0, 1
 MAX_HEADS, MAX_CTX = 32, 4
 
+DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
+
 FMT_NAMES = {"f32": FMT_F32, "iq4_nl": FMT_IQ4_NL, "iq4_xs": FMT_IQ4_XS}
 
 _ERR_TEXT = {
@@ -162,6 +164,15 @@ SIGNATURES = {
     "engram_ple_conv": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                   C.c_int64, C.c_void_p, C.c_int32, C.c_int32, C.c_int64, C.c_int32, C.c_int32,
                                   C.c_void_p, C.c_void_p]),
+    "engram_adapter_workspace_bytes": (C.c_int64, [C.c_int64, C.c_int32, C.c_int32, C.c_int64, C.c_int64, C.c_int32]),
+    "engram_adapter_forward": (C.c_int, [C.c_int32, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p,
+                                         C.c_void_p, C.c_int64, C.c_int32, C.c_int32, C.c_int64, C.c_int64,
+                                         C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64,
+                                         C.c_void_p]),
+    "engram_adapter_backward": (C.c_int, [C.c_int32, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p,
+                                          C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_int32,
+                                          C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64,
+                                          C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
     "engram_selftest_mod": (C.c_int, [C.c_void_p, C.c_int64, C.c_uint32, C.c_void_p]),
     "engram_launch_count": (C.c_int64, []),
 }

@@ -51,6 +51,11 @@ extern "C" {
 #define ENGRAM_ERR_WORKSPACE (-4) /* scratch buffer too small                   */
 #define ENGRAM_ERR_CUDA (-5)      /* a launch failed (cudaGetLastError)         */
 
+/* ---- element types of the adapter and orthogonalisation entry points ------ */
+#define ENGRAM_DTYPE_F32 0
+#define ENGRAM_DTYPE_BF16 1
+#define ENGRAM_DTYPE_F16 2
+
 /* ---- row formats of the resident table ---------------------------------- */
 #define ENGRAM_FMT_F32 0    /* dim floats per row                              */
 #define ENGRAM_FMT_IQ4_NL 1 /* ggml IQ4_NL, dim/32 blocks (the reference table) */
@@ -660,6 +665,45 @@ ENGRAM_API int engram_gemm_tf32(int32_t n_terms, const float* const* a, const fl
 ENGRAM_API int engram_gemm_3xtf32(const float* a_hi, const float* a_lo, const float* b_hi, const float* b_lo,
                                   int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb, float* c, int64_t ldc,
                                   int32_t* err, void* stream);
+
+/*
+ * Low-rank adapters of many requests beside a shared projection (no reference
+ * counterpart; ple_forward applies them beside the PLE block's projections):
+ *   out[t, :] = base[t, :] + scale[i] * b[i] @ (a[i] @ x[t, :]),  i = index[t],
+ * with x [T, K], a [n_adapters, rank, K], b [n_adapters, N, rank] (both
+ * contiguous), index int32 [T], scale float [n_adapters] (nullable: 1), base
+ * [T, N] (nullable: zeros) and out [T, N]; ldx, ldbase, ldout: row strides in
+ * elements, at least the width.  An index outside [0, n_adapters) means no
+ * adapter: the row is base's.  out may be base itself (same pointer and
+ * stride).  x, a, b, base and out are of one element type (dtype); a[i] @ x[t]
+ * is kept in fp32 and out is rounded once.  rank <= 128, n_adapters <= 16384.
+ * 16-byte aligned rows (pointers, strides, K and N) take wide loads.
+ * workspace: device scratch, 16-byte aligned, of
+ * engram_adapter_workspace_bytes(..., backward = 0) bytes.
+ * Sums run in one fixed order: the same inputs give the same bits.
+ */
+ENGRAM_API int64_t engram_adapter_workspace_bytes(int64_t T, int32_t n_adapters, int32_t rank, int64_t K, int64_t N,
+                                                  int32_t backward);
+ENGRAM_API int engram_adapter_forward(int32_t dtype, const void* x, int64_t ldx, const void* a, const void* b,
+                                      const int32_t* index, const float* scale, int64_t T, int32_t n_adapters,
+                                      int32_t rank, int64_t K, int64_t N, const void* base, int64_t ldbase, void* out,
+                                      int64_t ldout, void* workspace, int64_t workspace_bytes, void* stream);
+/*
+ * Its gradients, from grad [T, N] (row stride ldgrad), the gradient of out
+ * (which is also base's):
+ *   dh[t] = scale[i] * b[i].T @ grad[t]
+ *   dx[t] = dx_base[t] + a[i].T @ dh[t]    (dx_base nullable: zeros; it may be dx)
+ *   da[i] = sum over i's t of dh[t] x[t].T,  db[i] = sum of scale[i] grad[t] (a[i] @ x[t]).T
+ * dx [T, K] (row stride lddx), da and db (contiguous, as a and b) are each
+ * nullable: not wanted.  Every row of dx is written (dx_base's, or zero, where
+ * there is no adapter) and all of da and db (zero for an adapter no position
+ * uses).  workspace: ..._workspace_bytes(..., backward = 1).
+ */
+ENGRAM_API int engram_adapter_backward(int32_t dtype, const void* grad, int64_t ldgrad, const void* x, int64_t ldx,
+                                       const void* a, const void* b, const int32_t* index, const float* scale,
+                                       int64_t T, int32_t n_adapters, int32_t rank, int64_t K, int64_t N,
+                                       const void* dx_base, int64_t lddx_base, void* dx, int64_t lddx, void* da,
+                                       void* db, void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

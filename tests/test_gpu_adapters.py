@@ -1,0 +1,222 @@
+"""adapter_add and its gradients on the GPU against the formula in 64 bits.
+
+Bounds.  A product of fp32 operands in three TF32 terms is off by at most
+2^-21 of it (each operand's remainder is read to 2^-22, the dropped term is
+2^-24); a sum of k products in fp32 adds at most k 2^-23 of the sum of their
+magnitudes (tensor-core partial sums round toward zero: a whole step).  With
+M = the sum of magnitudes of the inner sums carried through the outer one, an
+element is off by at most (2^-20 + (k + r) 2^-23) M, plus the half step of its
+own type.  k is the length of the inner sum, r of the outer one.
+"""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import engraft_ngram_b200 as eb
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+def make(T, K, N, rank, n, dtype, index="random", seed=0, scale=True):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+
+    def normal(*shape):
+        return torch.randn(*shape, device=DEV, generator=g).to(dtype)
+
+    if index == "random":
+        ix = torch.randint(-1, n, (T,), device=DEV, generator=g)
+    elif index == "segments":
+        ix = torch.sort(torch.randint(-1, n, (T,), device=DEV, generator=g)).values
+    elif index == "none":
+        ix = torch.full((T,), -1, device=DEV)
+    elif index == "outside":  # everything past the stack is no adapter either
+        ix = torch.randint(-5, n + 5, (T,), device=DEV, generator=g)
+        ix[0], ix[-1] = 2 ** 31 - 1, -2 ** 31
+    else:  # one adapter for all
+        ix = torch.full((T,), int(index), device=DEV)
+    s = 0.5 + torch.rand(n, device=DEV, generator=g) if scale else None
+    return dict(base=normal(T, N), x=normal(T, K), a=normal(n, rank, K), b=normal(n, N, rank),
+                index=ix.to(torch.int32), scale=s), normal(T, N)
+
+
+def formula(c, grad, mag=False):
+    """out, dx, da, db in 64 bits; mag: of the magnitudes (each sum without cancellation)."""
+    f = (lambda v: v.double().abs()) if mag else (lambda v: v.double())
+    base, x, a, b, grad = f(c["base"]), f(c["x"]), f(c["a"]), f(c["b"]), f(grad)
+    n = a.shape[0]
+    out, dx, da, db = base.clone(), torch.zeros_like(x), torch.zeros_like(a), torch.zeros_like(b)
+    for i in range(n):
+        t = (c["index"] == i).nonzero().flatten()
+        s = 1.0 if c["scale"] is None else float(c["scale"][i])
+        h, dh = s * (x[t] @ a[i].T), s * (grad[t] @ b[i])
+        out[t] += h @ b[i].T
+        dx[t] = dh @ a[i]
+        da[i] = dh.T @ x[t]
+        db[i] = grad[t].T @ h
+    return out, dx, da, db
+
+
+def check(got, want, mag, k, dtype):
+    half = torch.finfo(dtype).eps / 2
+    tiny = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    bound = (2.0 ** -20 + k * 2.0 ** -23) * mag * (1 + half) + half * want.abs() + tiny
+    off = (got.double() - want).abs() / bound
+    assert got.dtype == dtype and torch.isfinite(got).all()
+    assert float(off.max() if off.numel() else 0) <= 1.0, float(off.max())
+
+
+CASES = [
+    (1, 2560, 12800, 16, 4, BF16, "0"), (1, 64, 40, 1, 1, F32, "0"), (3, 1, 1, 1, 2, F32, "random"),
+    (256, 512, 640, 16, 40, F32, "random"), (300, 256, 384, 32, 3, BF16, "segments"),
+    (129, 130, 77, 11, 5, F16, "random"), (517, 97, 515, 7, 9, BF16, "random"), (200, 96, 72, 24, 2, F32, "segments"),
+    (65, 264, 136, 64, 1, BF16, "0"), (260, 264, 136, 64, 2, F32, "segments"), (130, 64, 96, 128, 3, F32, "random"),
+    (130, 64, 96, 100, 3, F16, "segments"), (90, 72, 1000, 33, 90, F32, "random"), (64, 64, 64, 8, 3, F32, "none"),
+    (64, 64, 64, 8, 3, BF16, "outside"), (2049, 80, 48, 16, 5, F32, "random"), (33, 40, 24, 16, 300, F32, "random"),
+    (5000, 16, 16, 4, 2000, F32, "random"),
+]
+
+
+@pytest.mark.parametrize("case", CASES, ids=str)
+def test_forward_and_gradients_match_the_formula(case):
+    T, K, N, rank, n, dtype, index = case
+    c, grad = make(*case, scale=T % 2 == 0)
+    want, mag = formula(c, grad), formula(c, grad, mag=True)
+    out = eb.adapter_add(**c)
+    check(out, want[0], mag[0], K + rank, dtype)
+    dx, da, db = eb.adapter_gradients(grad, c["x"], c["a"], c["b"], c["index"], c["scale"])
+    check(dx, want[1], mag[1], N + rank, dtype)
+    check(da, want[2], mag[2], N + T, dtype)
+    check(db, want[3], mag[3], K + T, dtype)
+    again = eb.adapter_add(**c)
+    assert torch.equal(out, again)
+    assert all(torch.equal(u, v) for u, v in zip((dx, da, db), eb.adapter_gradients(
+        grad, c["x"], c["a"], c["b"], c["index"], c["scale"])))
+
+
+def test_rows_without_an_adapter_keep_base_bit_for_bit_and_their_inputs_are_not_read():
+    c, grad = make(100, 64, 48, 8, 4, F32, "random", seed=3)
+    c["index"][::3] = -1
+    free = c["index"] < 0
+    c["x"][free] = float("nan")
+    c["base"][free] = float("inf")
+    grad[free] = float("nan")
+    out = eb.adapter_add(**c)
+    dx, da, db = eb.adapter_gradients(grad, c["x"], c["a"], c["b"], c["index"], c["scale"])
+    assert torch.equal(out[free], c["base"][free]) and torch.isfinite(out[~free]).all()
+    assert (dx[free] == 0).all()
+    assert torch.isfinite(dx).all() and torch.isfinite(da).all() and torch.isfinite(db).all()
+
+
+def test_in_place_without_base_and_into_a_view():
+    c, _ = make(77, 96, 136, 16, 3, BF16, "random", seed=4)
+    want = eb.adapter_add(**c)
+    wide = torch.zeros(77, 200, dtype=BF16, device=DEV)
+    wide[:, 8:144] = c["base"]
+    got = eb.adapter_add(wide[:, 8:144], c["x"], c["a"], c["b"], c["index"], c["scale"], out=wide[:, 8:144])
+    assert torch.equal(got, want) and (wide[:, :8] == 0).all() and (wide[:, 144:] == 0).all()
+    c["base"] = torch.zeros_like(c["base"])
+    assert torch.equal(eb.adapter_add(**c), eb.adapter_add(None, *list(c.values())[1:]))
+
+
+@pytest.mark.parametrize("shift", [1, 3])
+def test_unaligned_rows_match_aligned_ones(shift):
+    c, grad = make(150, 64, 48, 8, 4, BF16, "random", seed=5)
+    odd = {k: torch.empty(150, v.shape[1] + 5, dtype=BF16, device=DEV)[:, shift:shift + v.shape[1]].copy_(v)
+           for k, v in (("x", c["x"]), ("base", c["base"]), ("grad", grad))}
+    want, mag = formula(c, grad), formula(c, grad, mag=True)
+    rest = (c["a"], c["b"], c["index"], c["scale"])
+    check(eb.adapter_add(odd["base"], odd["x"], *rest), want[0], mag[0], 72, BF16)
+    for got, w, m in zip(eb.adapter_gradients(odd["grad"], odd["x"], *rest), want[1:], mag[1:]):
+        check(got, w, m, 250, BF16)
+
+
+def test_autograd_matches_the_gradients_and_differences():
+    c, grad = make(60, 40, 56, 12, 3, F32, "random", seed=6)
+    leaves = {k: c[k].clone().requires_grad_() for k in ("base", "x", "a", "b")}
+    out = eb.adapter_add(leaves["base"], leaves["x"], leaves["a"], leaves["b"], c["index"], c["scale"])
+    out.backward(grad)
+    dx, da, db = eb.adapter_gradients(grad, c["x"], c["a"], c["b"], c["index"], c["scale"])
+    assert torch.equal(leaves["base"].grad, grad) and torch.equal(leaves["x"].grad, dx)
+    assert torch.equal(leaves["a"].grad, da) and torch.equal(leaves["b"].grad, db)
+    # the product is linear in each argument, so a central difference is its derivative: what is left
+    # is rounding, of 2^-20 + (K + rank) 2^-23 of the magnitudes on either side
+    mag = formula(c, grad, mag=True)[0]
+    for k in ("x", "a", "b"):
+        d = torch.randn_like(c[k])
+        up, down = eb.adapter_add(**{**c, k: c[k] + d}), eb.adapter_add(**{**c, k: c[k] - d})
+        slope = float(((up.double() - down.double()) / 2 * grad.double()).sum())
+        want = float((leaves[k].grad.double() * d.double()).sum())
+        wider = formula({**c, k: c[k].abs() + d.abs()}, grad, mag=True)[0]
+        bound = (2.0 ** -20 + 120 * 2.0 ** -23) * float(((mag + 2 * wider) * grad.double().abs()).sum())
+        assert abs(slope - want) <= bound, k
+
+
+def test_only_the_gradients_asked_for():
+    c, grad = make(60, 40, 56, 12, 3, F32, "random", seed=7)
+    full = eb.adapter_gradients(grad, c["x"], c["a"], c["b"], c["index"], c["scale"])
+    for k, i in (("x", 0), ("a", 1), ("b", 2)):
+        leaf = c[k].clone().requires_grad_()
+        eb.adapter_add(**{**c, k: leaf}).backward(grad)
+        assert torch.equal(leaf.grad, full[i])
+    leaf = c["x"].clone().requires_grad_()
+    out = eb.adapter_add(None, leaf, c["a"], c["b"], c["index"])
+    (g,) = torch.autograd.grad(out.sum(), leaf, create_graph=True)
+    with pytest.raises(RuntimeError):  # once differentiable
+        g.sum().backward()
+
+
+def test_nothing_to_do():
+    c, grad = make(0, 40, 56, 12, 3, F32, "random")
+    assert eb.adapter_add(**c).shape == (0, 56)
+    dx, da, db = eb.adapter_gradients(grad, c["x"], c["a"], c["b"], c["index"], c["scale"])
+    assert dx.shape == (0, 40) and (da == 0).all() and (db == 0).all()
+    c, grad = make(6, 40, 56, 12, 1, F32, "none")
+    c["a"], c["b"], c["scale"] = c["a"][:0], c["b"][:0], None
+    assert torch.equal(eb.adapter_add(**c), c["base"])
+    dx, da, db = eb.adapter_gradients(grad, c["x"], c["a"], c["b"], c["index"])
+    assert (dx == 0).all() and da.shape == (0, 12, 40) and db.shape == (0, 56, 12)
+
+
+def test_another_stream_and_a_captured_call_replayed_on_new_inputs():
+    c, grad = make(256, 128, 160, 16, 12, F32, "random", seed=8)
+    d, _ = make(256, 128, 160, 16, 12, F32, "segments", seed=9)
+    want_c, want_d = eb.adapter_add(**c), eb.adapter_add(**d)
+    grads_d = eb.adapter_gradients(grad, d["x"], d["a"], d["b"], d["index"], d["scale"])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = eb.adapter_add(**c)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want_c)
+    held = {k: v.clone() for k, v in c.items()}
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = eb.adapter_add(**held)
+        grads = eb.adapter_gradients(grad, held["x"], held["a"], held["b"], held["index"], held["scale"])
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want_c)
+    for k in held:
+        held[k].copy_(d[k])
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want_d) and all(torch.equal(u, v) for u, v in zip(grads, grads_d))
+
+
+@pytest.mark.parametrize("bad, text", [
+    (lambda c: dict(x=c["x"].double()), "x:"), (lambda c: dict(a=c["a"][:, :, :-1]), "a "),
+    (lambda c: dict(a=c["a"].transpose(1, 2).contiguous().transpose(1, 2)), "contiguous"),
+    (lambda c: dict(b=c["b"].to(BF16)), "b:"), (lambda c: dict(index=c["index"].long()), "index"),
+    (lambda c: dict(index=c["index"][:-1]), "index"), (lambda c: dict(scale=c["scale"].double()), "scale"),
+    (lambda c: dict(scale=c["scale"][:-1]), "scale"), (lambda c: dict(base=c["base"][:, :-1]), "base"),
+    (lambda c: dict(base=c["base"].cpu()), "base"), (lambda c: dict(base=c["base"][:1].expand(20, -1)), "strides"),
+    (lambda c: dict(x=c["x"].t().contiguous().t()), "strides"),
+    (lambda c: dict(a=c["a"].repeat(1, 17, 1), b=c["b"].repeat(1, 1, 17)), "rank")])
+def test_refusals(bad, text):
+    c, _ = make(20, 16, 24, 8, 3, F32)
+    with pytest.raises(ValueError, match=text):
+        eb.adapter_add(**{**c, **bad(c)})
