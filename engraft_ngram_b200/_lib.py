@@ -173,6 +173,12 @@ SIGNATURES = {
                                           C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_int32,
                                           C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64,
                                           C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
+    "engram_orthogonalize_workspace_bytes": (C.c_int64, [C.c_int32, C.c_int64, C.c_int64, C.c_int64]),
+    "engram_orthogonalize": (C.c_int, [C.c_int32, C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_int32, C.c_void_p,
+                                       C.c_double, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
+    "engram_muon_step": (C.c_int, [C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64,
+                                   C.c_int64, C.c_int64, C.c_double, C.c_double, C.c_int32, C.c_double, C.c_int32,
+                                   C.c_void_p, C.c_double, C.c_void_p, C.c_int64, C.c_void_p]),
     "engram_selftest_mod": (C.c_int, [C.c_void_p, C.c_int64, C.c_uint32, C.c_void_p]),
     "engram_launch_count": (C.c_int64, []),
 }

@@ -106,6 +106,7 @@ def forward_into(out, base, x, a, b, index, scale) -> torch.Tensor:
                                         L.ptr(scale), T, n, rank, K, N, L.ptr(base), ldbase, out.data_ptr(), ldout,
                                         ws.data_ptr(), ws.numel(), L.stream_of(dev))
     L.check(st, "engram_adapter_forward")
+    torch.autograd.graph.increment_version(out)
     return out
 
 

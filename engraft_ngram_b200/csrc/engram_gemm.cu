@@ -28,12 +28,7 @@
 // stops its loop; the CTA still drains its TMA loads and MMAs (bounded waits
 // again) and frees its TMEM before it returns.  Rows, columns and K beyond the
 // operands are zero-filled by the TMA unit and never stored.
-#include <cuda.h>
-#include <cudaTypedefs.h>
-
-#include <mutex>
-
-#include "engram_common.cuh"
+#include "engram_tensor.cuh"
 
 using namespace engram;
 
@@ -59,47 +54,11 @@ static_assert(Cfg<true>::STAGE_BYTES == Cfg<false>::STAGE_BYTES, "one shared-mem
 constexpr int kThreads = 192;
 constexpr int kMaxTerms = 3;
 constexpr uint32_t kTmemCols = 256;
-constexpr long long kSpinLimit = 1ll << 24;
 
 struct GemmMaps {
     CUtensorMap a[kMaxTerms];  // fused: a[0] = A_hi, a[1] = A_lo
     CUtensorMap b[kMaxTerms];  // fused: b[0] = B_hi, b[1] = B_lo
 };
-
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
-__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
-}
-__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-// Bounded wait for the phase with the given parity; false (and *err raised) on timeout.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int* err) {
-    for (long long it = 0; it < kSpinLimit; it++)
-        if (mbar_try_wait(bar, parity)) return true;
-    if (err) atomicAdd(err, 1);
-    return false;
-}
-
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
-            dst),
-        "l"(map), "r"(x), "r"(y), "r"(bar)
-        : "memory");
-}
 
 // Shared-memory matrix descriptor of a K-major tile written by TMA with a
 // 128-byte (layout type 2) or 64-byte (type 4) swizzle: rows of 128 or 64
@@ -127,11 +86,6 @@ __device__ __forceinline__ void umma_tf32(uint32_t tmem_d, uint64_t da, uint64_t
         "l"(da), "l"(db), "r"(kInstrDesc), "r"(accumulate)
         : "memory");
 }
-__device__ __forceinline__ void umma_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
-                 : "memory");
-}
-
 template <bool FUSED>
 __global__ void __launch_bounds__(kThreads, 1) k_gemm_tf32(const __grid_constant__ GemmMaps maps, int n_terms,
                                                            int64_t M, int64_t N, int64_t K, float* __restrict__ c,
@@ -265,19 +219,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_gemm_tf32(const __grid_constant
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
     }
-}
-
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-    static std::once_flag once;
-    std::call_once(once, [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-    });
-    return fn;
 }
 
 // 2-D map of a row-major fp32 matrix [rows, K] (row stride ld floats), boxes of

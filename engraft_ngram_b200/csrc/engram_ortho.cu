@@ -1,0 +1,903 @@
+// engram_ortho.cu -- orthogonalising an update by Newton-Schulz products, and the
+// optimizer step that applies it.  Each matrix U of a stack is divided by its
+// Frobenius norm and taken through steps of an odd polynomial,
+//   X <- c0 X + (c1 G + c2 G G) X,   G = X X^T (the short side),
+// which moves every singular value toward 1 and leaves the singular vectors.
+//
+// Short sides up to 64 (adapter factors): all steps act on the short side only.
+// With G0 = U U^T / |U|^2, every iterate is X = P X0 with P a polynomial of G0, so
+// U is read once for G0, the small matrices are iterated by one block, and U is
+// read once more for P U.  That needs G0 and P far beyond fp32 (P cancels: it holds
+// c0^steps, 485 for the default, along the weak directions and 1 / sigma along the
+// strong ones), so this path sums in fp64 on the fp64 tensor cores
+// (mma.sync m8n8k4).  It is one pass over U, and one more with the output.
+//
+// Longer sides: three tcgen05 products a step on planes of fp16.  A value is
+// kept as y = 2^12 x = hi + lo, two fp16 (22 significant bits); a product is
+// hi hi + hi lo + lo hi in fp32 accumulators in tensor memory.  Every iterate has
+// entries below 16 (checked for the coefficients on the host), so hi is far from
+// fp16's limits, and lo's steps of 2^-24 are 2^-36 of x.  Results rounded to bf16
+// take one product of the hi planes: 2^-12 a rounding, eight times finer than
+// the result's own.  G and G G are symmetric: only tiles that reach the diagonal
+// or lie above it are computed and stored twice.  c0 is added to the diagonal of
+// the polynomial, so X' is one product.  The planes are read in the layout in which
+// U was given: tall matrices use U^T U and X P, so nothing is transposed in memory;
+// the descriptors take each operand along K or across it.
+#include "engram_tensor.cuh"
+
+using namespace engram;
+
+namespace {
+
+constexpr int kMaxSteps = 32;
+constexpr int kSmallSide = 64;
+
+struct Poly {
+    double c[kMaxSteps][3];
+    int steps;
+};
+
+template <typename T> __device__ __forceinline__ float to_f32(T v);
+template <> __device__ __forceinline__ float to_f32(float v) { return v; }
+template <> __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <> __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half from_f32(float v) { return __float2half_rn(v); }
+
+// Where U comes from and where the result goes.  Plain: U = x, the result is out.
+// Muon: m' = m + (1 - beta)(g - m), U = g + beta (m' - g) (Nesterov) or m'; the first
+// pass writes m', the later one reads it; the result O gives p' = decay p - step O.
+template <typename T>
+struct Plain {
+    const T* x;
+    T* out;
+    __device__ __forceinline__ float first(int64_t i) const { return to_f32(x[i]); }
+    __device__ __forceinline__ float again(int64_t i) const { return to_f32(x[i]); }
+    __device__ __forceinline__ void store(int64_t i, float o) const { out[i] = from_f32<T>(o); }
+};
+template <typename T>
+struct MuonIo {
+    const T* g;
+    const float* m;
+    float* m_out;
+    const float* p;
+    float* p_out;
+    float beta, rest, decay, step;
+    bool nesterov;
+    __device__ __forceinline__ float update(float gv, float mv) const {
+        return nesterov ? __fmaf_rn(beta, mv - gv, gv) : mv;
+    }
+    __device__ __forceinline__ float first(int64_t i) const {
+        const float gv = to_f32(g[i]), mv = m[i], mn = __fmaf_rn(rest, gv - mv, mv);
+        m_out[i] = mn;
+        return update(gv, mn);
+    }
+    __device__ __forceinline__ float again(int64_t i) const { return update(to_f32(g[i]), m_out[i]); }
+    __device__ __forceinline__ void store(int64_t i, float o) const { p_out[i] = __fmaf_rn(-step, o, decay * p[i]); }
+};
+
+// ---- short sides up to 64 -------------------------------------------------------
+
+__device__ __forceinline__ void dmma(double* d, double a, double b) {
+    asm volatile("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0, %1}, {%2}, {%3}, {%0, %1};"
+                 : "+d"(d[0]), "+d"(d[1])
+                 : "d"(a), "d"(b));
+}
+
+constexpr int kSmallThreads = 256;
+constexpr int KT = 64;        // long-side columns of a tile in shared memory
+constexpr int KTS = KT + 4;   // its row stride: rows 8 apart in a quarter fall on unlike banks
+
+// Columns k0 .. k0 + KT - 1 (below k_end) of the m x L matrix from element base on into tile
+// [8 MB][KTS], zeros outside.  tall: stored [L][m], else [m][L].
+template <int MB, typename F>
+__device__ __forceinline__ void load_tile(float* tile, int64_t base, int m, int64_t L, int64_t k0, int64_t k_end,
+                                          bool tall, F value) {
+    if (tall) {
+        const int64_t left = k_end - k0;
+        const int cols = left < KT ? (int)left : KT;
+        for (int e = threadIdx.x; e < KT * 8 * MB; e += kSmallThreads) {
+            const int k = e / (8 * MB), i = e % (8 * MB);
+            tile[i * KTS + k] = (i < m && k < cols) ? value(base + (k0 + k) * m + i) : 0.f;
+        }
+    } else {
+        for (int e = threadIdx.x; e < KT * 8 * MB; e += kSmallThreads) {
+            const int k = e % KT, i = e / KT;
+            tile[i * KTS + k] = (i < m && k0 + k < k_end) ? value(base + (int64_t)i * L + k0 + k) : 0.f;
+        }
+    }
+}
+
+// part[s, chunk] = U U^T over the chunk's columns, fp64, [8 MB][8 MB] (blocks of 8 on and above the
+// diagonal).  Warp w sums columns 8 w .. 8 w + 7 of each tile; the warps are added in their order.
+template <int MB, typename Io>
+__global__ void __launch_bounds__(kSmallThreads) k_small_gram(Io io, int m, int64_t L, bool tall, int64_t chunk,
+                                                              double* __restrict__ part) {
+    constexpr int RM = 8 * MB, NT = MB * (MB + 1) / 2;
+    // the tile, and after the last one the sums
+    __shared__ __align__(16) double sum[RM * RM > RM * KTS / 2 ? RM * RM : RM * KTS / 2];
+    float* tile = reinterpret_cast<float*>(sum);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
+    const int64_t base = (int64_t)blockIdx.y * m * L, k_begin = blockIdx.x * chunk;
+    const int64_t k_end = k_begin + chunk < L ? k_begin + chunk : L;
+    double acc[NT][2];
+#pragma unroll
+    for (int i = 0; i < NT; i++) acc[i][0] = acc[i][1] = 0.0;
+    for (int64_t k0 = k_begin; k0 < k_end; k0 += KT) {
+        __syncthreads();
+        load_tile<MB>(tile, base, m, L, k0, k_end, tall, [&](int64_t i) { return io.first(i); });
+        __syncthreads();
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            double f[MB];
+#pragma unroll
+            for (int i = 0; i < MB; i++) f[i] = (double)tile[(8 * i + g) * KTS + 8 * warp + 4 * s + q];
+            int at = 0;
+#pragma unroll
+            for (int i = 0; i < MB; i++)
+#pragma unroll
+                for (int j = i; j < MB; j++) dmma(acc[at++], f[i], f[j]);
+        }
+    }
+    __syncthreads();
+    for (int w = 0; w < kSmallThreads / 32; w++) {
+        if (w == warp) {
+            int at = 0;
+#pragma unroll
+            for (int i = 0; i < MB; i++)
+#pragma unroll
+                for (int j = i; j < MB; j++, at++)
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        double* d = sum + (8 * i + g) * RM + 8 * j + 2 * q + c;
+                        *d = w ? *d + acc[at][c] : acc[at][c];
+                    }
+        }
+        __syncthreads();
+    }
+    double* dst = part + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * RM * RM;
+    for (int e = threadIdx.x; e < RM * RM; e += kSmallThreads)
+        if (e % RM >= (e / RM & ~7)) dst[e] = sum[e];
+}
+
+// z = x y for symmetric matrices that commute (so z is symmetric): blocks of 8 on and above the
+// diagonal, mirrored.  f(i, j, v) gives the stored value.
+template <int MB, typename F>
+__device__ __forceinline__ void small_product(const double* x, const double* y, double* z, F f) {
+    constexpr int S = 8 * MB + 4, NT = MB * (MB + 1) / 2;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
+    for (int at = warp; at < NT; at += kSmallThreads / 32) {
+        int i = 0, left = at;
+        while (left >= MB - i) left -= MB - i, i++;
+        const int j = i + left;
+        double d[2][2] = {{0.0, 0.0}, {0.0, 0.0}};
+#pragma unroll
+        for (int s = 0; s < 2 * MB; s++)
+            dmma(d[s & 1], x[(8 * i + g) * S + 4 * s + q], y[(8 * j + g) * S + 4 * s + q]);
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            const int r = 8 * i + g, col = 8 * j + 2 * q + c;
+            const double v = f(r, col, d[0][c] + d[1][c]);
+            z[r * S + col] = v;
+            if (i != j) z[col * S + r] = v;
+        }
+    }
+    __syncthreads();
+}
+
+// The steps on the small matrices: pmat[s] = P / max(|U|, eps).
+template <int MB>
+__global__ void __launch_bounds__(kSmallThreads) k_small_poly(const double* __restrict__ part, int chunks, int m,
+                                                              Poly poly, double eps, double* __restrict__ pmat) {
+    constexpr int RM = 8 * MB, S = RM + 4;
+    extern __shared__ double sd[];
+    double *A = sd, *B = A + RM * S, *P = B + RM * S, *Q = P + RM * S;
+    __shared__ double inv_norm;
+    const double* src = part + (int64_t)blockIdx.x * chunks * RM * RM;
+    for (int e = threadIdx.x; e < RM * RM; e += kSmallThreads) {
+        const int i = e / RM, j = e % RM;
+        if (j < (i & ~7)) continue;
+        double v = 0.0;
+        for (int c = 0; c < chunks; c++) v += src[(int64_t)c * RM * RM + e];
+        A[i * S + j] = v;
+        if (j / 8 != i / 8) A[j * S + i] = v;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double t = 0.0;
+        for (int i = 0; i < m; i++) t += A[i * S + i];
+        const double norm = sqrt(t);
+        inv_norm = 1.0 / (norm < eps ? eps : norm);  // a NaN stays one
+    }
+    __syncthreads();
+    const double inv = inv_norm;
+    for (int e = threadIdx.x; e < RM * RM; e += kSmallThreads) {
+        const int i = e / RM, j = e % RM;
+        A[i * S + j] *= inv * inv;
+        P[i * S + j] = i == j ? inv : 0.0;
+    }
+    __syncthreads();
+    for (int s = 0; s < poly.steps; s++) {
+        const double c0 = poly.c[s][0], c1 = poly.c[s][1], c2 = poly.c[s][2];
+        // B = M = c0 + c1 A + c2 A A, then P <- M P and A <- M A M
+        small_product<MB>(A, A, B, [&](int i, int j, double v) { return (i == j ? c0 : 0.0) + c1 * A[i * S + j] + c2 * v; });
+        small_product<MB>(B, P, Q, [](int, int, double v) { return v; });
+        double* t = P;
+        P = Q, Q = t;
+        if (s + 1 < poly.steps) {
+            small_product<MB>(B, A, Q, [](int, int, double v) { return v; });
+            small_product<MB>(B, Q, A, [](int, int, double v) { return v; });
+        }
+    }
+    for (int e = threadIdx.x; e < RM * RM; e += kSmallThreads)
+        pmat[(int64_t)blockIdx.x * RM * RM + e] = P[(e / RM) * S + e % RM];
+}
+
+// The result P U, tile by tile.
+template <int MB, typename Io>
+__global__ void __launch_bounds__(kSmallThreads) k_small_apply(Io io, int m, int64_t L, bool tall, int64_t chunk,
+                                                               const double* __restrict__ pmat) {
+    constexpr int RM = 8 * MB, S = RM + 4;
+    extern __shared__ double sd[];
+    double* P = sd;
+    float* tile = reinterpret_cast<float*>(P + RM * S);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
+    const int64_t base = (int64_t)blockIdx.y * m * L, k_begin = blockIdx.x * chunk;
+    const int64_t k_end = k_begin + chunk < L ? k_begin + chunk : L;
+    for (int e = threadIdx.x; e < RM * RM; e += kSmallThreads)
+        P[(e / RM) * S + e % RM] = pmat[(int64_t)blockIdx.y * RM * RM + e];
+    for (int64_t k0 = k_begin; k0 < k_end; k0 += KT) {
+        __syncthreads();
+        load_tile<MB>(tile, base, m, L, k0, k_end, tall, [&](int64_t i) { return io.again(i); });
+        __syncthreads();
+        double acc[MB][2];
+#pragma unroll
+        for (int i = 0; i < MB; i++) acc[i][0] = acc[i][1] = 0.0;
+#pragma unroll
+        for (int s = 0; s < 2 * MB; s++) {  // warp w: columns 8 w .. 8 w + 7
+            const double b = (double)tile[(4 * s + q) * KTS + 8 * warp + g];
+#pragma unroll
+            for (int i = 0; i < MB; i++) dmma(acc[i], P[(8 * i + g) * S + 4 * s + q], b);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < MB; i++) {
+            tile[(8 * i + g) * KTS + 8 * warp + 2 * q] = (float)acc[i][0];
+            tile[(8 * i + g) * KTS + 8 * warp + 2 * q + 1] = (float)acc[i][1];
+        }
+        __syncthreads();
+        const int64_t left = k_end - k0;
+        const int cols = left < KT ? (int)left : KT;
+        if (tall) {
+            for (int e = threadIdx.x; e < cols * RM; e += kSmallThreads) {
+                const int k = e / RM, i = e % RM;
+                if (i < m) io.store(base + (k0 + k) * m + i, tile[i * KTS + k]);
+            }
+        } else {
+            for (int e = threadIdx.x; e < KT * m; e += kSmallThreads) {
+                const int k = e % KT, i = e / KT;
+                if (k < cols) io.store(base + (int64_t)i * L + k0 + k, tile[i * KTS + k]);
+            }
+        }
+    }
+}
+
+// ---- longer sides: planes ---------------------------------------------------------
+
+constexpr float kPlaneScale = 4096.f;
+constexpr int kNormThreads = 256;
+
+// part[s, block] = the block's share of |U|^2, fp64 (updates of 1e-20 and of 1e20 alike).
+template <typename Io>
+__global__ void __launch_bounds__(kNormThreads) k_norm(Io io, int64_t size, double* __restrict__ part) {
+    __shared__ double warp_sum[kNormThreads / 32];
+    const int64_t base = blockIdx.y * size;
+    double v = 0.0;
+    for (int64_t i = blockIdx.x * (int64_t)kNormThreads + threadIdx.x; i < size; i += (int64_t)gridDim.x * kNormThreads) {
+        const double u = (double)io.first(base + i);
+        v += u * u;
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+    if ((threadIdx.x & 31) == 0) warp_sum[threadIdx.x >> 5] = v;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < kNormThreads / 32; w++) v += warp_sum[w];
+        part[(int64_t)blockIdx.y * gridDim.x + blockIdx.x] = v;
+    }
+}
+
+struct Planes {
+    __half *hi, *lo;  // lo null: one product
+    int64_t ld, stride;
+};
+
+__device__ __forceinline__ void put(const Planes& p, int64_t i, float y) {
+    const __half h = __float2half_rn(y);
+    p.hi[i] = h;
+    if (p.lo) p.lo[i] = __float2half_rn(y - __half2float(h));
+}
+
+// planes = 2^12 U / max(|U|, eps); a warp takes a row at a time.
+template <typename Io>
+__global__ void __launch_bounds__(kNormThreads) k_planes(Io io, int64_t rows, int64_t cols,
+                                                         const double* __restrict__ part, int parts, double eps,
+                                                         Planes out) {
+    __shared__ double total;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (warp == 0) {
+        double v = 0.0;
+        for (int i = lane; i < parts; i += 32) v += part[(int64_t)blockIdx.y * parts + i];
+#pragma unroll
+        for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+        if (lane == 0) total = v;
+    }
+    __syncthreads();
+    const double norm = sqrt(total);
+    const double inv = (double)kPlaneScale / (norm < eps ? eps : norm);
+    const int64_t base = blockIdx.y * rows * cols;
+    for (int64_t r = blockIdx.x * (int64_t)(kNormThreads / 32) + warp; r < rows;
+         r += (int64_t)gridDim.x * (kNormThreads / 32))
+        for (int64_t c = lane; c < cols; c += 32)
+            put(out, blockIdx.y * out.stride + r * out.ld + c, (float)((double)io.again(base + r * cols + c) * inv));
+}
+
+// ---- longer sides: the products -----------------------------------------------------
+
+enum Mode { GRAM, POLY, UPDATE, RESULT };
+
+constexpr int BM = 128;
+constexpr int kGemmThreads = 192;
+constexpr int kStageTotal = 192 * 1024;
+
+// One K slice of the operands: 32 columns of four planes (A hi, B hi, A lo, B lo) or 64 of two.
+template <int TERMS, int BN>
+struct Cfg {
+    static constexpr int KS = TERMS == 3 ? 32 : 64;
+    static constexpr int A_BYTES = BM * KS * 2, B_BYTES = BN * KS * 2;
+    static constexpr int STAGE_BYTES = (TERMS == 3 ? 2 : 1) * (A_BYTES + B_BYTES);
+    static constexpr int STAGES = kStageTotal / STAGE_BYTES;
+    static constexpr int SMEM = STAGES * STAGE_BYTES + 1024 + 256;
+};
+
+struct Maps {
+    CUtensorMap a_hi, a_lo, b_hi, b_lo;
+};
+
+template <typename Io>
+struct Job {
+    int M, N, K;       // D [M, N] = sum over K
+    int tiles_m;       // tiles along M (symmetric modes: unused)
+    Planes out;        // GRAM, POLY, UPDATE
+    Planes g;          // POLY: the planes of G
+    float c0, c1, c2;  // POLY
+    Io io;             // RESULT
+    int* err;
+};
+
+// Shared-memory matrix descriptor.  Along K (rows of KS fp16, 64- or 128-byte swizzle): 8-row groups
+// 8 KS 2 bytes apart.  Across K (blocks of 64 columns, each KS rows of 128 bytes, 128-byte swizzle):
+// 8-row groups of K 1024 bytes apart, blocks KS 128 bytes apart.
+template <bool MN, int KS>
+__device__ __forceinline__ uint64_t operand_desc(uint32_t addr) {
+    constexpr uint32_t lbo = MN ? KS * 128 : 16, sbo = MN ? 1024 : 8 * KS * 2;
+    constexpr uint64_t swizzle = (MN || KS == 64) ? 2 : 4;
+    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(sbo >> 4) << 32) |
+           ((uint64_t)1 << 46) | (swizzle << 61);
+}
+
+template <bool A_MN, bool B_MN, int BN>
+__device__ __forceinline__ void umma_f16(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t accumulate) {
+    // A and B fp16, D fp32, each operand along K or across it
+    constexpr uint32_t desc = (1u << 4) | ((A_MN ? 1u : 0u) << 15) | ((B_MN ? 1u : 0u) << 16) |
+                              ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "l"(da), "l"(db), "r"(desc), "r"(accumulate)
+        : "memory");
+}
+
+template <bool MN, int KS, int ROWS>
+__device__ __forceinline__ void load_operand(uint32_t dst, const CUtensorMap* map, int row0, int k, int z, uint32_t bar) {
+    if constexpr (MN) {
+#pragma unroll
+        for (int b = 0; b < ROWS / 64; b++) tma_load_3d(dst + b * KS * 128, map, row0 + 64 * b, k, z, bar);
+    } else {
+        tma_load_3d(dst, map, k, row0, z, bar);
+    }
+}
+
+__device__ __forceinline__ void load_planes8(const Planes& p, int64_t i, float* v) {
+    alignas(16) __half h[8];
+    *reinterpret_cast<uint4*>(h) = *reinterpret_cast<const uint4*>(p.hi + i);
+#pragma unroll
+    for (int k = 0; k < 8; k++) v[k] = __half2float(h[k]);
+    if (p.lo) {
+        *reinterpret_cast<uint4*>(h) = *reinterpret_cast<const uint4*>(p.lo + i);
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[k] += __half2float(h[k]);
+    }
+}
+
+__device__ __forceinline__ void put8(const Planes& p, int64_t i, const float* v) {
+    alignas(16) __half h[8], l[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+        h[k] = __float2half_rn(v[k]);
+        l[k] = __float2half_rn(v[k] - __half2float(h[k]));
+    }
+    *reinterpret_cast<uint4*>(p.hi + i) = *reinterpret_cast<const uint4*>(h);
+    if (p.lo) *reinterpret_cast<uint4*>(p.lo + i) = *reinterpret_cast<const uint4*>(l);
+}
+
+// One block a BM x BN tile: warp 0 loads (TMA), one lane of warp 1 issues the MMAs, warps 2 to 5
+// take the accumulator (tensor-memory lanes 32 (w % 4) ..) through the mode's epilogue.  A wait that
+// gives up (never, in a correct run) counts itself in *err and the tile's results become NaN.
+template <int MODE, bool A_MN, bool B_MN, int TERMS, int BN, typename Io>
+__global__ void __launch_bounds__(kGemmThreads, 1) k_product(const __grid_constant__ Maps maps, const Job<Io> job) {
+    using G = Cfg<TERMS, BN>;
+    constexpr int KS = G::KS, STAGES = G::STAGES;
+    constexpr bool SYM = MODE == GRAM || MODE == POLY;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * G::STAGE_BYTES);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 1);
+    volatile uint32_t* gave_up = tmem_slot + 1;
+    const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + STAGES), acc_bar = smem_u32(bars + 2 * STAGES);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, z = blockIdx.y;
+    int m0, n0;
+    if constexpr (SYM) {  // tiles with an entry on or above the diagonal: column block b has R (b + 1)
+        constexpr int R = BN / BM;
+        int left = blockIdx.x, b = 0;
+        while (left >= R * (b + 1)) left -= R * (b + 1), b++;
+        m0 = left * BM, n0 = b * BN;
+    } else {
+        m0 = (int)(blockIdx.x % job.tiles_m) * BM, n0 = (int)(blockIdx.x / job.tiles_m) * BN;
+    }
+    const int slices = (job.K + KS - 1) / KS;
+    if (SYM && m0 >= job.M) return;  // the last column block may be wider than the matrix
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; s++) {
+            mbar_init(full0 + 8 * s, 1);
+            mbar_init(empty0 + 8 * s, 1);
+        }
+        mbar_init(acc_bar, 1);
+        *gave_up = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                     "r"((uint32_t)BN)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int i = 0;
+            bool ok = true;
+            for (; i < slices; i++) {
+                const int s = i % STAGES, round = i / STAGES;
+                if (round > 0) ok = mbar_wait(empty0 + 8 * s, (uint32_t)((round - 1) & 1), job.err);
+                if (!ok) break;
+                const uint32_t bar = full0 + 8 * s, st = smem_u32(smem + s * G::STAGE_BYTES);
+                mbar_expect_tx(bar, G::STAGE_BYTES);
+                load_operand<A_MN, KS, BM>(st, &maps.a_hi, m0, i * KS, z, bar);
+                load_operand<B_MN, KS, BN>(st + G::A_BYTES, &maps.b_hi, n0, i * KS, z, bar);
+                if constexpr (TERMS == 3) {
+                    load_operand<A_MN, KS, BM>(st + G::A_BYTES + G::B_BYTES, &maps.a_lo, m0, i * KS, z, bar);
+                    load_operand<B_MN, KS, BN>(st + 2 * G::A_BYTES + G::B_BYTES, &maps.b_lo, n0, i * KS, z, bar);
+                }
+            }
+            // every load issued into this block's shared memory has landed before it ends
+            for (int k = i > STAGES ? i - STAGES : 0; k < i; k++)
+                mbar_wait(full0 + 8 * (k % STAGES), (uint32_t)((k / STAGES) & 1), job.err);
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            for (int i = 0; i < slices; i++) {
+                const int s = i % STAGES;
+                if (!mbar_wait(full0 + 8 * s, (uint32_t)((i / STAGES) & 1), job.err)) {
+                    *gave_up = 1;
+                    __threadfence_block();
+                    break;
+                }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t a = smem_u32(smem + s * G::STAGE_BYTES), b = a + G::A_BYTES;
+                const uint32_t alo = b + G::B_BYTES, blo = alo + G::A_BYTES;
+#pragma unroll
+                for (int k = 0; k < KS / 16; k++) {  // 16 of K: 32 bytes along it, 16 rows of 128 bytes across it
+                    constexpr uint32_t sa = A_MN ? 2048 : 32, sb = B_MN ? 2048 : 32;
+                    const uint64_t ah = operand_desc<A_MN, KS>(a + sa * k), bh = operand_desc<B_MN, KS>(b + sb * k);
+                    const uint32_t first = (i > 0 || k > 0) ? 1u : 0u;
+                    if constexpr (TERMS == 3) {  // the small terms first
+                        umma_f16<A_MN, B_MN, BN>(tmem, operand_desc<A_MN, KS>(alo + sa * k), bh, first);
+                        umma_f16<A_MN, B_MN, BN>(tmem, ah, operand_desc<B_MN, KS>(blo + sb * k), 1u);
+                        umma_f16<A_MN, B_MN, BN>(tmem, ah, bh, 1u);
+                    } else {
+                        umma_f16<A_MN, B_MN, BN>(tmem, ah, bh, first);
+                    }
+                }
+                umma_commit(empty0 + 8 * s);
+            }
+            umma_commit(acc_bar);
+        }
+        __syncwarp();
+    } else {
+        const int w = warp & 3;
+        const bool ok = mbar_wait(acc_bar, 0u, job.err) && *gave_up == 0;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const int row = m0 + 32 * w + lane;
+        for (int col = 0; col < BN; col += 32) {
+            uint32_t r[32];
+            asm volatile(
+                "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+                "%14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                  "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+                  "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
+                  "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
+                  "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                : "r"(tmem + ((uint32_t)(32 * w) << 16) + (uint32_t)col));
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+            const int c0 = n0 + col;
+            if (row >= job.M || c0 >= job.N) continue;
+            float v[32];
+#pragma unroll
+            for (int j = 0; j < 32; j++) v[j] = ok ? __uint_as_float(r[j]) : __uint_as_float(0x7fc00000u);
+            if constexpr (MODE == RESULT) {
+                const int64_t at = ((int64_t)z * job.M + row) * job.N + c0;
+#pragma unroll
+                for (int j = 0; j < 32; j++)
+                    if (c0 + j < job.N) job.io.store(at + j, v[j] * (1.f / (kPlaneScale * kPlaneScale)));
+            } else {
+                // products carry the square of the planes' scale; the rows' padding (to ld) may be written
+                const int64_t at = (int64_t)z * job.out.stride + (int64_t)row * job.out.ld + c0;
+#pragma unroll
+                for (int j = 0; j < 32; j++) v[j] *= 1.f / kPlaneScale;
+                if constexpr (MODE == POLY) {
+                    const int64_t gat = (int64_t)z * job.g.stride + (int64_t)row * job.g.ld + c0;
+#pragma unroll
+                    for (int j = 0; j < 32; j += 8) {
+                        float gv[8];
+                        if (c0 + j < job.g.ld) {
+                            load_planes8(job.g, gat + j, gv);
+                        } else {
+#pragma unroll
+                            for (int k = 0; k < 8; k++) gv[k] = 0.f;
+                        }
+#pragma unroll
+                        for (int k = 0; k < 8; k++)
+                            v[j + k] = fmaf(job.c2, v[j + k], job.c1 * gv[k]) +
+                                       (c0 + j + k == row ? job.c0 * kPlaneScale : 0.f);
+                    }
+                }
+                if (!SYM || c0 > row) {
+#pragma unroll
+                    for (int j = 0; j < 32; j += 8)
+                        if (c0 + j < job.out.ld) put8(job.out, at + j, v + j);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; j++)
+                        if (c0 + j >= row && c0 + j < job.N) put(job.out, at + j, v[j]);
+                }
+                if constexpr (SYM) {  // the mirrored entries: 32 lanes store 32 neighbours of a row
+#pragma unroll
+                    for (int j = 0; j < 32; j++)
+                        if (c0 + j > row && c0 + j < job.N)
+                            put(job.out, (int64_t)z * job.out.stride + (int64_t)(c0 + j) * job.out.ld + row, v[j]);
+                }
+            }
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)BN) : "memory");
+    }
+}
+
+// ---- host ---------------------------------------------------------------------------
+
+int64_t align256(int64_t b) { return (b + 255) & ~int64_t(255); }
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+int launched() {
+    count_launches(1);
+    return cudaGetLastError() == cudaSuccess ? ENGRAM_OK : ENGRAM_ERR_CUDA;
+}
+
+bool allow_smem(const void* kernel, int bytes) {
+    return bytes <= 48 * 1024 ||
+           cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess;
+}
+
+struct Shape {
+    int64_t stack, rows, cols, side, length;  // side <= length
+    bool tall;                                // stored [length, side]
+};
+
+// Chunks of the long side, in whole tiles, for about four blocks an SM.
+int64_t small_chunk(const Shape& s) {
+    const int64_t tiles = ceil_div(s.length, KT), per = ceil_div(4 * 148, s.stack);
+    return ceil_div(tiles, per < tiles ? per : tiles) * KT;
+}
+int small_side(const Shape& s) { return s.side <= 8 ? 8 : s.side <= 16 ? 16 : s.side <= 32 ? 32 : 64; }
+
+constexpr int kNormBlocks = 592;
+int64_t norm_blocks(const Shape& s) {
+    const int64_t want = ceil_div(s.rows * s.cols, 16 * kNormThreads), most = ceil_div(kNormBlocks, s.stack);
+    return want < most ? want : most;
+}
+
+int64_t pad64(int64_t c) { return (c + 63) & ~int64_t(63); }
+
+struct Layout {
+    int64_t part, pmat;                     // small
+    int64_t err, x[2], g, b, bytes;         // planes: hi, then lo
+    int64_t x_plane, s_plane;               // bytes of one plane
+};
+
+Layout layout_of(const Shape& s, int terms) {
+    Layout l = {};
+    int64_t at = 0;
+    const auto take = [&](int64_t bytes) {
+        const int64_t here = at;
+        at += align256(bytes);
+        return here;
+    };
+    if (s.side <= kSmallSide) {
+        const int64_t rm = small_side(s), chunks = ceil_div(s.length, small_chunk(s));
+        l.part = take(s.stack * chunks * rm * rm * 8);
+        l.pmat = take(s.stack * rm * rm * 8);
+    } else {
+        l.part = take(s.stack * norm_blocks(s) * 8);
+        l.err = take(4);
+        l.x_plane = align256(s.stack * s.rows * pad64(s.cols) * 2);
+        l.s_plane = align256(s.stack * s.side * pad64(s.side) * 2);
+        const int planes = terms == 3 ? 2 : 1;
+        for (int64_t* p : {&l.x[0], &l.x[1]}) *p = take(planes * l.x_plane);
+        for (int64_t* p : {&l.g, &l.b}) *p = take(planes * l.s_plane);
+    }
+    l.bytes = at;
+    return l;
+}
+
+template <int MB, typename Io>
+int run_small(const Shape& s, const Layout& l, const Io& io, const Poly& poly, double eps, uint8_t* ws,
+              cudaStream_t st) {
+    const int64_t chunk = small_chunk(s), chunks = ceil_div(s.length, chunk);
+    double *part = (double*)(ws + l.part), *pmat = (double*)(ws + l.pmat);
+    const dim3 grid((unsigned)chunks, (unsigned)s.stack);
+    k_small_gram<MB><<<grid, kSmallThreads, 0, st>>>(io, (int)s.side, s.length, s.tall, chunk, part);
+    int e = launched();
+    if (e) return e;
+    constexpr int RM = 8 * MB, S = RM + 4, poly_smem = 4 * RM * S * 8, apply_smem = RM * S * 8 + RM * KTS * 4;
+    if (!allow_smem((const void*)k_small_poly<MB>, poly_smem)) return ENGRAM_ERR_CUDA;
+    k_small_poly<MB><<<(unsigned)s.stack, kSmallThreads, poly_smem, st>>>(part, (int)chunks, (int)s.side, poly, eps,
+                                                                         pmat);
+    e = launched();
+    if (e) return e;
+    if (!allow_smem((const void*)k_small_apply<MB, Io>, apply_smem)) return ENGRAM_ERR_CUDA;
+    k_small_apply<MB><<<grid, kSmallThreads, apply_smem, st>>>(io, (int)s.side, s.length, s.tall, chunk, pmat);
+    return launched();
+}
+
+// Map of one plane [stack, rows, ld] of which `cols` columns count, in boxes of bx columns and by rows.
+bool plane_map(CUtensorMap* map, const __half* base, int64_t rows, int64_t cols, int64_t ld, int64_t stride,
+               int64_t stack, int bx, int by) {
+    const auto fn = encode_fn();
+    if (!fn) return false;
+    const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)stack};
+    const cuuint64_t strides[2] = {(cuuint64_t)ld * 2, (cuuint64_t)stride * 2};
+    const cuuint32_t box[3] = {(cuuint32_t)bx, (cuuint32_t)by, 1}, step[3] = {1, 1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<__half*>(base), dims, strides, box, step,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, bx == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+struct Matrix {  // a plane pair and its extent
+    Planes p;
+    int64_t rows, cols;
+};
+
+struct NoIo {};
+
+template <int MODE, bool A_MN, bool B_MN, int TERMS, int BN, typename Io>
+int run_product(const Matrix& a, const Matrix& b, int64_t stack, Job<Io> job, cudaStream_t st) {
+    using G = Cfg<TERMS, BN>;
+    Maps maps;
+    memset(&maps, 0, sizeof(maps));
+    const auto make = [&](CUtensorMap* map, const __half* plane, const Matrix& x, bool mn, int tile_rows) {
+        return mn ? plane_map(map, plane, x.rows, x.cols, x.p.ld, x.p.stride, stack, 64, G::KS)
+                  : plane_map(map, plane, x.rows, x.cols, x.p.ld, x.p.stride, stack, G::KS, tile_rows);
+    };
+    if (!make(&maps.a_hi, a.p.hi, a, A_MN, BM) || !make(&maps.b_hi, b.p.hi, b, B_MN, BN)) return ENGRAM_ERR_CUDA;
+    if (TERMS == 3 && (!make(&maps.a_lo, a.p.lo, a, A_MN, BM) || !make(&maps.b_lo, b.p.lo, b, B_MN, BN)))
+        return ENGRAM_ERR_CUDA;
+    const auto kernel = k_product<MODE, A_MN, B_MN, TERMS, BN, Io>;
+    if (!allow_smem((const void*)kernel, G::SMEM)) return ENGRAM_ERR_CUDA;
+    const int64_t tn = ceil_div(job.N, BN);
+    job.tiles_m = (int)ceil_div(job.M, BM);
+    const int64_t tiles = (MODE == GRAM || MODE == POLY) ? (BN / BM) * tn * (tn + 1) / 2 : job.tiles_m * tn;
+    kernel<<<dim3((unsigned)tiles, (unsigned)stack), kGemmThreads, G::SMEM, st>>>(maps, job);
+    return launched();
+}
+
+template <int TERMS, typename Io>
+int run_planes(const Shape& s, const Layout& l, const Io& io, const Poly& poly, double eps, uint8_t* ws,
+               cudaStream_t st) {
+    constexpr int BN = 256;
+    double* part = (double*)(ws + l.part);
+    const int64_t ldx = pad64(s.cols), lds = pad64(s.side);
+    const auto planes = [&](int64_t at, int64_t plane, int64_t ld, int64_t rows) {
+        return Planes{(__half*)(ws + at), TERMS == 3 ? (__half*)(ws + at + plane) : nullptr, ld, rows * ld};
+    };
+    Matrix x[2] = {{planes(l.x[0], l.x_plane, ldx, s.rows), s.rows, s.cols},
+                   {planes(l.x[1], l.x_plane, ldx, s.rows), s.rows, s.cols}};
+    const Matrix g = {planes(l.g, l.s_plane, lds, s.side), s.side, s.side};
+    const Matrix b = {planes(l.b, l.s_plane, lds, s.side), s.side, s.side};
+    const int nb = (int)norm_blocks(s);
+    k_norm<<<dim3((unsigned)nb, (unsigned)s.stack), kNormThreads, 0, st>>>(io, s.rows * s.cols, part);
+    int e = launched();
+    if (e) return e;
+    const int64_t row_blocks = ceil_div(s.rows, kNormThreads / 32), most = ceil_div(8 * 148, s.stack);
+    k_planes<<<dim3((unsigned)(row_blocks < most ? row_blocks : most), (unsigned)s.stack), kNormThreads, 0, st>>>(
+        io, s.rows, s.cols, part, nb, eps, x[0].p);
+    e = launched();
+    Job<NoIo> job = {};
+    job.err = (int*)(ws + l.err);
+    for (int i = 0; i < poly.steps && !e; i++) {
+        const Matrix &in = x[i & 1], &next = x[(i & 1) ^ 1];
+        job.M = job.N = (int)s.side;
+        job.K = (int)s.length;
+        job.out = g.p;
+        e = s.tall ? run_product<GRAM, true, true, TERMS, BN>(in, in, s.stack, job, st)
+                   : run_product<GRAM, false, false, TERMS, BN>(in, in, s.stack, job, st);
+        if (e) break;
+        job.K = (int)s.side;
+        job.out = b.p;
+        job.g = g.p;
+        job.c0 = (float)poly.c[i][0], job.c1 = (float)poly.c[i][1], job.c2 = (float)poly.c[i][2];
+        e = run_product<POLY, false, false, TERMS, BN>(g, g, s.stack, job, st);
+        if (e) break;
+        job.M = (int)s.rows;
+        job.N = (int)s.cols;
+        job.out = next.p;
+        if (i + 1 < poly.steps) {
+            e = s.tall ? run_product<UPDATE, false, false, TERMS, BN>(in, b, s.stack, job, st)
+                       : run_product<UPDATE, false, true, TERMS, BN>(b, in, s.stack, job, st);
+        } else {
+            Job<Io> result = {};
+            result.M = job.M, result.N = job.N, result.K = job.K, result.err = job.err;
+            result.io = io;
+            e = s.tall ? run_product<RESULT, false, false, TERMS, BN>(in, b, s.stack, result, st)
+                       : run_product<RESULT, false, true, TERMS, BN>(b, in, s.stack, result, st);
+        }
+    }
+    return e;
+}
+
+template <int TERMS, typename Io>
+int run(const Shape& s, const Layout& l, const Io& io, const Poly& poly, double eps, void* ws, void* stream) {
+    uint8_t* w = (uint8_t*)ws;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (s.side <= 8) return run_small<1>(s, l, io, poly, eps, w, st);
+    if (s.side <= 16) return run_small<2>(s, l, io, poly, eps, w, st);
+    if (s.side <= 32) return run_small<4>(s, l, io, poly, eps, w, st);
+    if (s.side <= kSmallSide) return run_small<8>(s, l, io, poly, eps, w, st);
+    return run_planes<TERMS>(s, l, io, poly, eps, w, st);
+}
+
+int check_shape(int64_t stack, int64_t rows, int64_t cols, Shape* s) {
+    if (stack < 0 || rows < 1 || cols < 1) return ENGRAM_ERR_ARG;
+    if (stack > 65535 || rows > (1 << 24) || cols > (1 << 24) || (rows < cols ? rows : cols) > (1 << 15))
+        return ENGRAM_ERR_RANGE;
+    s->stack = stack, s->rows = rows, s->cols = cols;
+    s->tall = rows > cols;
+    s->side = s->tall ? cols : rows;
+    s->length = s->tall ? rows : cols;
+    return ENGRAM_OK;
+}
+
+// The iterates have to stay within what the planes hold: for every singular value in [0, 1] that the
+// first division can leave, each step's G, polynomial and result below 15.
+int check_poly(int32_t steps, const double* c, double eps, Poly* poly) {
+    if (steps < 1 || !c || !(eps > 0.0)) return ENGRAM_ERR_ARG;
+    if (steps > kMaxSteps) return ENGRAM_ERR_RANGE;
+    constexpr int kPoints = 2048;
+    for (int i = 0; i < steps; i++)
+        for (int k = 0; k < 3; k++) poly->c[i][k] = c[3 * i + k];
+    poly->steps = steps;
+    for (int p = 0; p <= kPoints; p++) {
+        double x = 1.001 * p / kPoints;
+        for (int i = 0; i < steps; i++) {
+            const double g = x * x, f = poly->c[i][0] + g * (poly->c[i][1] + g * poly->c[i][2]);
+            x *= f;
+            if (!(g < 15.0 && f < 15.0 && f > -15.0 && x < 3.8 && x > -3.8)) return ENGRAM_ERR_RANGE;
+        }
+    }
+    return ENGRAM_OK;
+}
+
+int terms_of(int32_t dtype) { return dtype == ENGRAM_DTYPE_BF16 ? 1 : 3; }
+
+bool aligned_to(const void* p, int32_t dtype) {
+    return ((uintptr_t)p & (dtype == ENGRAM_DTYPE_F32 ? 3u : 1u)) == 0;
+}
+
+}  // namespace
+
+extern "C" int64_t engram_orthogonalize_workspace_bytes(int32_t dtype, int64_t stack, int64_t rows, int64_t cols) {
+    if (dtype < ENGRAM_DTYPE_F32 || dtype > ENGRAM_DTYPE_F16) return ENGRAM_ERR_FORMAT;
+    Shape s;
+    const int e = check_shape(stack, rows, cols, &s);
+    if (e) return e;
+    return stack ? layout_of(s, terms_of(dtype)).bytes : 0;
+}
+
+extern "C" int engram_orthogonalize(int32_t dtype, const void* x, int64_t stack, int64_t rows, int64_t cols,
+                                    int32_t steps, const double* coefficients, double eps, void* out, void* workspace,
+                                    int64_t workspace_bytes, void* stream) {
+    if (dtype < ENGRAM_DTYPE_F32 || dtype > ENGRAM_DTYPE_F16) return ENGRAM_ERR_FORMAT;
+    Shape s;
+    int e = check_shape(stack, rows, cols, &s);
+    if (e) return e;
+    Poly poly;
+    e = check_poly(steps, coefficients, eps, &poly);
+    if (e) return e;
+    if (stack == 0) return ENGRAM_OK;
+    if (!x || !out || !aligned_to(x, dtype) || !aligned_to(out, dtype) || !workspace || !aligned16(workspace))
+        return ENGRAM_ERR_ARG;
+    const Layout l = layout_of(s, terms_of(dtype));
+    if (workspace_bytes < l.bytes) return ENGRAM_ERR_WORKSPACE;
+    switch (dtype) {
+        case ENGRAM_DTYPE_F32:
+            return run<3>(s, l, Plain<float>{(const float*)x, (float*)out}, poly, eps, workspace, stream);
+        case ENGRAM_DTYPE_BF16:
+            return run<1>(s, l, Plain<__nv_bfloat16>{(const __nv_bfloat16*)x, (__nv_bfloat16*)out}, poly, eps,
+                          workspace, stream);
+        default:
+            return run<3>(s, l, Plain<__half>{(const __half*)x, (__half*)out}, poly, eps, workspace, stream);
+    }
+}
+
+extern "C" int engram_muon_step(int32_t grad_dtype, const float* p, const void* grad, const float* m, float* p_out,
+                                float* m_out, int64_t stack, int64_t rows, int64_t cols, double lr, double beta,
+                                int32_t nesterov, double weight_decay, int32_t steps, const double* coefficients,
+                                double eps, void* workspace, int64_t workspace_bytes, void* stream) {
+    if (grad_dtype < ENGRAM_DTYPE_F32 || grad_dtype > ENGRAM_DTYPE_F16) return ENGRAM_ERR_FORMAT;
+    Shape s;
+    int e = check_shape(stack, rows, cols, &s);
+    if (e) return e;
+    Poly poly;
+    e = check_poly(steps, coefficients, eps, &poly);
+    if (e) return e;
+    if (stack == 0) return ENGRAM_OK;
+    if (!grad || !aligned_to(grad, grad_dtype) || !workspace || !aligned16(workspace)) return ENGRAM_ERR_ARG;
+    for (const float* f : {p, m, (const float*)p_out, (const float*)m_out})
+        if (!f || !aligned_to(f, ENGRAM_DTYPE_F32)) return ENGRAM_ERR_ARG;
+    const Layout l = layout_of(s, 3);
+    if (workspace_bytes < l.bytes) return ENGRAM_ERR_WORKSPACE;
+    const double ratio = rows > cols ? sqrt((double)rows / (double)cols) : 1.0;
+    const auto io = [&](auto* g) {
+        using T = std::remove_cv_t<std::remove_pointer_t<decltype(g)>>;
+        return MuonIo<T>{g, m, m_out, p, p_out, (float)beta, (float)(1.0 - beta), (float)(1.0 - lr * weight_decay),
+                         (float)(lr * ratio), nesterov != 0};
+    };
+    switch (grad_dtype) {
+        case ENGRAM_DTYPE_F32: return run<3>(s, l, io((const float*)grad), poly, eps, workspace, stream);
+        case ENGRAM_DTYPE_BF16: return run<3>(s, l, io((const __nv_bfloat16*)grad), poly, eps, workspace, stream);
+        default: return run<3>(s, l, io((const __half*)grad), poly, eps, workspace, stream);
+    }
+}

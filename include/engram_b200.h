@@ -705,6 +705,38 @@ ENGRAM_API int engram_adapter_backward(int32_t dtype, const void* grad, int64_t 
                                        const void* dx_base, int64_t lddx_base, void* dx, int64_t lddx, void* da,
                                        void* db, void* workspace, int64_t workspace_bytes, void* stream);
 
+/*
+ * Orthogonalising updates by Newton-Schulz products (no reference counterpart:
+ * its descent trains table rows with Adam).  For each of `stack` matrices U
+ * [rows, cols] (contiguous, one after the other):
+ *   X = U / max(|U|_F, eps);  steps times  X <- c0 X + (c1 G + c2 G G) X
+ * with G = X X^T over the shorter side (X^T X where rows > cols, the product
+ * from the right) and (c0, c1, c2) = coefficients[3 s ..] of step s (HOST
+ * doubles [steps, 3], 1 <= steps <= 32).  out (may be x) gets X.  A zero matrix
+ * stays zero.  Coefficients under which a singular value of the iterates could
+ * leave (-3.8, 3.8), or the polynomial (-15, 15), are ENGRAM_ERR_RANGE.
+ * Shorter sides up to 64 are summed in fp64; longer ones in products of split
+ * fp16 operands with fp32 accumulation (fp32-level results; for bf16 one
+ * unsplit product, within 2^-8 of the largest entries).  Shorter side <= 32768,
+ * longer <= 2^24, stack <= 65535.
+ *
+ * engram_muon_step: one optimizer step with it, per matrix,
+ *   m' = m + (1 - beta)(g - m);  u = nesterov ? g + beta (m' - g) : m'
+ *   p' = (1 - lr weight_decay) p - lr sqrt(max(1, rows / cols)) O(u)
+ * p, m, p_out (may be p), m_out (may be m): fp32; grad of type grad_dtype.
+ * workspace: 16-byte aligned device scratch of
+ * engram_orthogonalize_workspace_bytes(dtype, ...) bytes, for engram_muon_step
+ * with dtype = ENGRAM_DTYPE_F32.
+ */
+ENGRAM_API int64_t engram_orthogonalize_workspace_bytes(int32_t dtype, int64_t stack, int64_t rows, int64_t cols);
+ENGRAM_API int engram_orthogonalize(int32_t dtype, const void* x, int64_t stack, int64_t rows, int64_t cols,
+                                    int32_t steps, const double* coefficients, double eps, void* out, void* workspace,
+                                    int64_t workspace_bytes, void* stream);
+ENGRAM_API int engram_muon_step(int32_t grad_dtype, const float* p, const void* grad, const float* m, float* p_out,
+                                float* m_out, int64_t stack, int64_t rows, int64_t cols, double lr, double beta,
+                                int32_t nesterov, double weight_decay, int32_t steps, const double* coefficients,
+                                double eps, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,245 @@
+"""orthogonalize, muon_step and Muon on the GPU against the formula in 64 bits.
+
+The reference is the definition by singular values: U diag(f(s)) V^T with f the
+steps applied to each normalised singular value, from an SVD in 64 bits.
+
+Bounds.  Sides up to 64 are summed in fp64, so an element is off by half a step
+of its type and by fp64's rounding, enlarged by the steps' growth of weak
+directions squared (c0^10 = 2.4e5) and the sums' lengths: far below 2^-28 of the
+matrix' root mean square.  Longer sides round every product as fp32 does, up to
+a factor: a split product is off by at most 2^-21 of itself where fp32 rounds to
+2^-24, and the tensor cores' sums round toward zero (twice the step).  Both are
+enlarged by the steps in the same way, so the 2-norm of the error may be 16
+times that of the plain fp32 form on the same input (one product of fp16 heads,
+for bf16: operands rounded to 2^-12, 2^13 times), plus the half step of the type.
+"""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import engraft_ngram_b200 as eb
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+C = (3.4445, -4.7750, 2.0315)
+
+
+def make(stack, rows, cols, kind, dtype=F32, seed=0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    noise = torch.randn(stack, rows, cols, device=DEV, generator=g)
+    if kind == "noise":
+        x = noise
+    else:
+        k = min(6, rows, cols)
+        u = torch.randn(stack, rows, k, device=DEV, generator=g) * 0.6 ** torch.arange(k, device=DEV)
+        x = u @ torch.randn(stack, k, cols, device=DEV, generator=g)
+        if kind == "strong":
+            x = x + 0.1 * noise
+        elif kind == "tiny":
+            x = 1e-18 * (x + 0.3 * noise)
+        # "lowrank": nothing along the other directions
+    return x.to(dtype)
+
+
+def formula(x, steps=5, coefficients=C, eps=1e-7):
+    x = x.double()
+    u, s, v = torch.linalg.svd(x, full_matrices=False)
+    s = s / s.square().sum(-1, keepdim=True).sqrt().clamp_min(eps)
+    for i in range(steps):
+        c = coefficients[i] if isinstance(coefficients[0], tuple) else coefficients
+        s = s * (c[0] + c[1] * s ** 2 + c[2] * s ** 4)
+    return u @ (s.unsqueeze(-1) * v)
+
+
+def plain(x, steps=5, coefficients=C, eps=1e-7):
+    x = x.float()
+    tall = x.shape[-2] > x.shape[-1]
+    x = x.mT if tall else x
+    x = x / x.double().square().sum((-2, -1), keepdim=True).sqrt().clamp_min(eps).float()
+    for i in range(steps):
+        c = coefficients[i] if isinstance(coefficients[0], tuple) else coefficients
+        g = x @ x.mT
+        x = c[0] * x + (c[1] * g + c[2] * (g @ g)) @ x
+    return x.mT if tall else x
+
+
+def check(got, x, **kw):
+    want, dtype = formula(x, **kw), got.dtype
+    half = torch.finfo(dtype).eps / 2
+    assert torch.isfinite(got).all()
+    for i in range(want.shape[0]):
+        off, w = got[i].double() - want[i], want[i]
+        if min(w.shape) <= 64:
+            rms = float(w.square().mean().sqrt())
+            tiny = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+            bound = half * w.abs() * (1 + half) + 2.0 ** -28 * rms + tiny
+            assert float((off.abs() / bound).max()) <= 1.0, i
+        else:
+            factor = 2.0 ** 13 if dtype == BF16 else 16.0
+            own = float((plain(x[i], **kw).double() - w).norm())
+            assert float(off.norm()) <= factor * own + half * float(w.norm()), (i, float(off.norm()), own)
+
+
+SMALL = [(1, 1, 1), (3, 1, 70), (3, 70, 1), (2, 5, 7), (4, 8, 8), (5, 16, 2560), (5, 2560, 16), (3, 17, 300),
+         (3, 301, 31), (2, 64, 64), (2, 64, 1000), (2, 999, 63), (70, 4, 130), (1, 40, 12800)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=str)
+@pytest.mark.parametrize("shape", SMALL, ids=str)
+def test_short_sides_match_the_singular_values(shape, dtype):
+    for kind in ("noise", "strong"):
+        x = make(*shape, kind, dtype, seed=sum(shape))
+        check(eb.orthogonalize(x), x)
+
+
+LONG = [(1, 65, 65), (1, 128, 128), (1, 130, 257), (2, 257, 130), (1, 256, 512), (1, 512, 384), (3, 100, 90),
+        (1, 300, 1000), (1, 1001, 299), (1, 1024, 640), (2, 70, 4097)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=str)
+@pytest.mark.parametrize("shape", LONG, ids=str)
+def test_longer_sides_match_the_singular_values(shape, dtype):
+    for kind in ("noise", "strong"):
+        x = make(*shape, kind, dtype, seed=sum(shape))
+        check(eb.orthogonalize(x), x)
+
+
+@pytest.mark.parametrize("shape", [(2, 24, 200), (2, 200, 24), (1, 200, 150)], ids=str)
+def test_rank_deficient_and_tiny_updates(shape):
+    for kind in ("lowrank", "tiny"):
+        x = make(*shape, kind, seed=3)
+        check(eb.orthogonalize(x, eps=1e-30), x, eps=1e-30)
+
+
+@pytest.mark.parametrize("shape", [(4, 12, 90), (3, 90, 120)], ids=str)
+def test_zero_matrices_stay_zero_and_a_nan_stays_in_its_matrix(shape):
+    x = make(*shape, "noise", seed=4)
+    want = eb.orthogonalize(x)
+    x[1] = 0.0
+    got = eb.orthogonalize(x)
+    assert (got[1] == 0).all() and torch.equal(got[0], want[0]) and torch.equal(got[2:], want[2:])
+    x[1, 0, 0] = float("nan")
+    got = eb.orthogonalize(x)
+    assert torch.isnan(got[1]).all() and torch.equal(got[0], want[0]) and torch.equal(got[2:], want[2:])
+
+
+@pytest.mark.parametrize("shape", [(2, 20, 100), (1, 150, 100)], ids=str)
+def test_steps_and_coefficients(shape):
+    x = make(*shape, "noise", seed=5)
+    for steps, c in ((1, C), (2, (1.5, -0.5, 0.0)), (8, (1.875, -1.25, 0.375)), (3, ((3.0, -3.2, 1.2), C, (1.5, -0.5, 0.0)))):
+        check(eb.orthogonalize(x, steps=steps, coefficients=c), x, steps=steps, coefficients=c)
+    with pytest.raises(ValueError):
+        eb.orthogonalize(x, coefficients=(9.0, 9.0, 9.0))
+
+
+@pytest.mark.parametrize("shape", [(3, 10, 60), (1, 130, 70)], ids=str)
+def test_in_place_again_and_a_single_matrix(shape):
+    x = make(*shape, "strong", seed=6)
+    want = eb.orthogonalize(x)
+    assert torch.equal(eb.orthogonalize(x), want)
+    assert torch.equal(eb.orthogonalize(x[0]), want[0]) or min(shape[1:]) <= 64  # other chunks: other sums
+    version = x._version
+    y = eb.orthogonalize(x, out=x)
+    assert y is x and torch.equal(x, want) and x._version > version
+
+
+def test_nothing_to_do():
+    assert eb.orthogonalize(torch.zeros(0, 5, 7, device=DEV)).shape == (0, 5, 7)
+    assert eb.orthogonalize(torch.zeros(3, 0, 7, device=DEV)).shape == (3, 0, 7)
+
+
+def muon_formula(p, g, m, lr, beta, nesterov, wd):
+    p, g, m = p.double(), g.double(), m.double()
+    m = m + (1 - beta) * (g - m)
+    u = g + beta * (m - g) if nesterov else m
+    ratio = math.sqrt(max(1.0, p.shape[-2] / p.shape[-1]))
+    return (1 - lr * wd) * p, lr * ratio, u, m
+
+
+@pytest.mark.parametrize("grad_dtype", [F32, BF16, F16], ids=str)
+@pytest.mark.parametrize("shape", [(3, 16, 200), (2, 300, 24), (1, 200, 130), (1, 130, 300)], ids=str)
+def test_muon_step(shape, grad_dtype):
+    g = make(*shape, "strong", grad_dtype, seed=7)
+    p, m = make(*shape, "noise", seed=8), make(*shape, "strong", seed=9)
+    for nesterov, wd in ((True, 0.1), (False, 0.0)):
+        keep, step, u, m_want = muon_formula(p, g, m, 0.05, 0.9, nesterov, wd)
+        out = (torch.empty_like(p), torch.empty_like(p))
+        got = eb.muon_step(p, g, m, 0.05, 0.9, nesterov, wd, out=out)
+        assert got[0] is out[0] and got[1] is out[1]
+        # m': a subtraction, a product and a sum, each rounded once
+        assert float(((out[1].double() - m_want).abs() / (m_want.abs() + m.abs() + g.abs().float())).max()) <= 3 * 2.0 ** -24
+        o_want = formula(u)
+        # p': fp32's rounding of its two products and their sum, and step times the error of the orthogonalised
+        # update, for which u is itself rounded (2^-22 of it, enlarged by at most c0^5 = 485 and beside the plain form's)
+        own = float((plain(u.float()).double() - o_want).norm())
+        rounding = 3 * 2.0 ** -24 * float((keep.abs() + step * o_want.abs()).norm())
+        bound = rounding + step * (16 * own + 485 * 2.0 ** -22 * math.sqrt(shape[0]))
+        assert float((out[0].double() - (keep - step * o_want)).norm()) <= bound
+        p2, m2 = p.clone(), m.clone()
+        assert eb.muon_step(p2, g, m2, 0.05, 0.9, nesterov, wd)[0] is p2
+        assert torch.equal(p2, out[0]) and torch.equal(m2, out[1])
+
+
+def test_the_optimizer_is_the_step_and_saves_its_state():
+    p = [torch.nn.Parameter(make(*s, "noise", seed=i)) for i, s in enumerate(((4, 16, 100), (1, 100, 80), (2, 6, 9)))]
+    q = [x.detach().clone() for x in p]
+    m = [torch.zeros_like(x) for x in q]
+    opt = eb.Muon(p, lr=0.02, weight_decay=0.05, momentum=0.9)
+    for k in range(3):
+        for i, x in enumerate(p):
+            x.grad = make(*x.shape, "strong", seed=10 * k + i) if (i, k) != (2, 1) else None
+        if k == 2:
+            again = eb.Muon(p, lr=0.5)
+            again.load_state_dict(opt.state_dict())
+            opt = again
+        opt.step()
+        for i, x in enumerate(p):
+            if x.grad is not None:
+                eb.muon_step(q[i], x.grad, m[i], 0.02, 0.9, weight_decay=0.05)
+    assert all(torch.equal(x.detach(), y) for x, y in zip(p, q))
+    assert opt.step(lambda: torch.tensor(3.0)) == 3.0
+
+
+def test_another_stream_and_a_captured_step_replayed_on_new_gradients():
+    p, m = make(2, 150, 90, "noise", seed=1), make(2, 150, 90, "strong", seed=2)
+    f = make(8, 12, 100, "strong", seed=3)
+    grads = [make(2, 150, 90, "strong", seed=20 + k) for k in range(3)]
+    q, n = p.clone(), m.clone()
+    want = []
+    for g in grads:
+        eb.muon_step(q, g, n, 0.1)
+        want.append((q.clone(), eb.orthogonalize(f * len(want))))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = eb.orthogonalize(f)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want[1][1])
+    g, x = grads[0].clone(), torch.zeros_like(f)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        eb.muon_step(p, g, m, 0.1)
+        o = eb.orthogonalize(x)
+    for k in range(3):
+        g.copy_(grads[k])
+        x.copy_(f * k)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(p, want[k][0]) and torch.equal(o, want[k][1])
+
+
+@pytest.mark.parametrize("bad", [
+    lambda x: eb.orthogonalize(x.double()), lambda x: eb.orthogonalize(x.mT), lambda x: eb.orthogonalize(x[0, 0]),
+    lambda x: eb.orthogonalize(x, out=x.to(BF16)), lambda x: eb.orthogonalize(x, out=x[:1]),
+    lambda x: eb.orthogonalize(x, steps=0), lambda x: eb.orthogonalize(x, eps=0.0),
+    lambda x: eb.muon_step(x.to(BF16), x, x, 0.1), lambda x: eb.muon_step(x, x, x.to(BF16), 0.1),
+    lambda x: eb.muon_step(x, x[:1], x, 0.1), lambda x: eb.muon_step(x, x, x.cpu(), 0.1),
+    lambda x: eb.muon_step(x, x, x, 0.1, out=(x, x[:1]))])
+def test_refusals(bad):
+    with pytest.raises(ValueError):
+        bad(make(2, 6, 9, "noise"))
