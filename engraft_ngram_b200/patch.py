@@ -54,7 +54,8 @@ def install_ple(modules: dict | None = None) -> None:
     the name engraft.replica.model imported) to engraft_ngram_b200.ple_forward,
     with or without gradients of emb, hidden and hist (the descent's backward
     through the block); calls that need gradients of the block's own weights,
-    or whose tensors are not on a CUDA device, keep the reference's function.
+    or whose tensors are not on a CUDA device, keep the reference's function
+    (not those with adapters=, which the reference's does not take).
     modules: name -> module overrides, for tests."""
     from . import ple
     for mod_name, attr in _PLE_TARGETS:
@@ -65,7 +66,7 @@ def install_ple(modules: dict | None = None) -> None:
         original = saved[attr]
 
         def routed(emb, hidden, w, hist, hparams, *args, _orig=original, **kw):
-            if ple.weights_need_grad(w) or not emb.is_cuda:
+            if kw.get("adapters") is None and (ple.weights_need_grad(w) or not emb.is_cuda):
                 return _orig(emb, hidden, w, hist, hparams, *args, **kw)
             return ple.ple_forward(emb, hidden, w, hist, hparams, *args, **kw)
 

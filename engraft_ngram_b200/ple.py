@@ -27,6 +27,11 @@ product in closed form) and one GEMM back through both projections, d_emb =
 [d_key, d_value] @ [w_key; w_value], in the forward's arithmetic.  Gradients of
 the block's weights (frozen in the descent) are not built: such a call raises,
 and `install_ple` routes it to the reference's own function.
+
+`adapters` (a PleAdapters) adds each position's low-rank adapter to the two
+projections, on the projected rows in place, and the backward builds the
+gradients of its factors: the block is tuned, for each request on its own,
+beside frozen weights.
 """
 from __future__ import annotations
 
@@ -36,6 +41,7 @@ import ctypes as C
 import torch
 
 from . import _lib as L
+from .adapters import PleAdapters, backward_into, forward_into
 
 _GRAD_FIELDS = ("w_key", "w_value", "norm_key", "norm_query", "norm_conv", "conv1d")
 PROJECTION = "3xtf32"  # or "fp32", "tcgen05"
@@ -136,10 +142,13 @@ def project(emb: torch.Tensor, w, out: torch.Tensor, mode: str | None = None) ->
     return out
 
 
-def needs_grad(emb: torch.Tensor, hidden: torch.Tensor, w, hist: torch.Tensor) -> bool:
+def needs_grad(emb: torch.Tensor, hidden: torch.Tensor, w, hist: torch.Tensor,
+               adapters: PleAdapters | None = None) -> bool:
     if not torch.is_grad_enabled():
         return False
     ts = [emb, hidden, hist] + [getattr(w, f) for f in _GRAD_FIELDS]
+    if adapters is not None:
+        ts += [adapters.a, adapters.b]
     return any(isinstance(t, torch.Tensor) and t.requires_grad for t in ts)
 
 
@@ -173,14 +182,22 @@ def project_back(dkv: torch.Tensor, w, out: torch.Tensor, mode: str | None = Non
     return out
 
 
-def _block_forward(emb, hidden, w, hist, nk, nq, nc, cw, hc, n, K, eps, dil, want_s):
+def _project_adapted(emb, w, adapters, rows: int) -> torch.Tensor:
+    """kv [T, rows] of the projections, with each position's adapter added."""
+    kv = project(emb, w, torch.empty(emb.shape[0], rows, device=emb.device))
+    if adapters is not None:
+        forward_into(kv, kv, emb, adapters.a, adapters.b, adapters.index, adapters.scale)
+    return kv
+
+
+def _block_forward(emb, hidden, w, hist, nk, nq, nc, cw, hc, n, K, eps, dil, want_s, adapters=None):
     """kv [T, hc*n + n], gate, s, normed and out of the block (the kernels)."""
     T = emb.shape[0]
     H = hist.shape[0]
     dev = emb.device
     lib = L.load()
     stream = L.stream_of(dev)
-    kv = project(emb, w, torch.empty(T, hc * n + n, device=dev))
+    kv = _project_adapted(emb, w, adapters, hc * n + n)
     stride = hc * n + n
     value = kv[:, hc * n:]
     gate = torch.empty(T, hc, device=dev)
@@ -199,16 +216,19 @@ def _block_forward(emb, hidden, w, hist, nk, nq, nc, cw, hc, n, K, eps, dil, wan
 
 
 class _PleBlockFn(torch.autograd.Function):
-    """The block with gradients of emb, hidden and hist (weights frozen)."""
+    """The block with gradients of emb, hidden, hist and the adapters' factors a and b (weights frozen)."""
 
     @staticmethod
-    def forward(ctx, emb, hidden, hist, w, nk, nq, nc, cw, meta):
+    def forward(ctx, emb, hidden, hist, w, nk, nq, nc, cw, meta, a, b, index, scale):
         hc, n, K, eps, dil, detach_value, detach_gate = meta
-        kv, gate, s, normed, out = _block_forward(emb, hidden, w, hist, nk, nq, nc, cw, hc, n, K, eps, dil, True)
+        adapters = None if a is None else PleAdapters(a, b, index, scale)
+        kv, gate, s, normed, out = _block_forward(emb, hidden, w, hist, nk, nq, nc, cw, hc, n, K, eps, dil, True,
+                                                  adapters)
         hist_len = (K - 1) * dil
         full = torch.cat([hist, normed], dim=0) if hist.shape[0] else normed
         new_hist = full[-hist_len:].clone() if hist_len > 0 else full[:0].clone()
-        ctx.save_for_backward(hidden, hist, kv, gate, s, normed, nk, nq, nc, cw)
+        ctx.save_for_backward(hidden, hist, kv, gate, s, normed, nk, nq, nc, cw, None if a is None else emb, a, b,
+                              index, scale)
         ctx.w, ctx.meta = w, meta
         ctx.tail_len = new_hist.shape[0]
         ctx.mark_non_differentiable(gate, s)
@@ -216,7 +236,7 @@ class _PleBlockFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dout, dtail, _dgate, _ds):
-        hidden, hist, kv, gate, s, normed, nk, nq, nc, cw = ctx.saved_tensors
+        hidden, hist, kv, gate, s, normed, nk, nq, nc, cw, emb, a, b, index, scale = ctx.saved_tensors
         hc, n, K, eps, dil, detach_value, detach_gate = ctx.meta
         T, H = hidden.shape[0], hist.shape[0]
         dev = hidden.device
@@ -243,7 +263,14 @@ class _PleBlockFn(torch.autograd.Function):
         demb = None
         if ctx.needs_input_grad[0]:
             demb = project_back(dkv, ctx.w, torch.empty(T, n, device=dev))
-        return (demb, dhidden if ctx.needs_input_grad[1] else None, dhist, None, None, None, None, None, None)
+        da = db = None
+        if a is not None:
+            da = torch.empty_like(a) if ctx.needs_input_grad[9] else None
+            db = torch.empty_like(b) if ctx.needs_input_grad[10] else None
+            if demb is not None or da is not None or db is not None:
+                backward_into(dkv, emb, a, b, index, scale, demb, demb, da, db)
+        return (demb, dhidden if ctx.needs_input_grad[1] else None, dhist, None, None, None, None, None, None, da, db,
+                None, None)
 
 
 def _f32(x: torch.Tensor, name: str, shape) -> torch.Tensor:
@@ -255,10 +282,13 @@ def _f32(x: torch.Tensor, name: str, shape) -> torch.Tensor:
 
 
 def ple_forward(emb: torch.Tensor, hidden: torch.Tensor, w, hist: torch.Tensor, hparams,
-                diag: dict | None = None, detach_value: bool = False, detach_gate: bool = False):
+                diag: dict | None = None, detach_value: bool = False, detach_gate: bool = False,
+                adapters: PleAdapters | None = None):
     """(hidden + gated + silu(conv), new history tail): see the reference's
     docstring.  Differentiable in emb, hidden and hist (detach_value /
-    detach_gate as in the reference); diag receives the same five tensors."""
+    detach_gate as in the reference); diag receives the same five tensors.
+    adapters: low-rank adapters of the positions' requests, added to the key and
+    value projections; differentiable in their factors too."""
     if weights_need_grad(w):
         raise NotImplementedError("engraft_ngram_b200.ple_forward does not build gradients of the block's weights; "
                                   "install_ple routes such calls to the reference's ple_forward")
@@ -276,13 +306,19 @@ def ple_forward(emb: torch.Tensor, hidden: torch.Tensor, w, hist: torch.Tensor, 
     cw = _f32(w.conv1d.detach(), "conv1d", (hc * n, K))
     H = hist.shape[0]
     hist = _f32(hist, "hist", (H, hc, n)) if H else hist.reshape(0, hc, n)
-    if needs_grad(emb, hidden, w, hist):
+    if adapters is not None and (adapters.a.dim() != 3 or adapters.a.shape[2] != n or adapters.b.dim() != 3
+                                 or adapters.b.shape[1] != hc * n + n):
+        raise ValueError(f"adapters: a {tuple(adapters.a.shape)}, b {tuple(adapters.b.shape)}, expected "
+                         f"[adapters, rank, {n}] and [adapters, {hc * n + n}, rank]")
+    if needs_grad(emb, hidden, w, hist, adapters):
+        factors = (None,) * 4 if adapters is None else (adapters.a, adapters.b, adapters.index, adapters.scale)
         out, new_hist, gate, s = _PleBlockFn.apply(emb, hidden, hist, w, nk, nq, nc, cw,
-                                                   (hc, n, K, eps, dil, bool(detach_value), bool(detach_gate)))
+                                                   (hc, n, K, eps, dil, bool(detach_value), bool(detach_gate)),
+                                                   *factors)
         value = None
     else:
         kv, gate, s, normed, out = _block_forward(emb, hidden, w, hist, nk, nq, nc, cw, hc, n, K, eps, dil,
-                                                  diag is not None)
+                                                  diag is not None, adapters)
         value = kv[:, hc * n:]
         hist_len = (K - 1) * dil
         hist_full = torch.cat([hist.to(normed.dtype), normed], dim=0) if H else normed
@@ -290,7 +326,7 @@ def ple_forward(emb: torch.Tensor, hidden: torch.Tensor, w, hist: torch.Tensor, 
     if diag is not None:
         with torch.no_grad():
             if value is None:  # the differentiable call keeps no value: project again for the diagnostics
-                value = project(emb.detach(), w, torch.empty(T, hc * n + n, device=emb.device))[:, hc * n:]
+                value = _project_adapted(emb.detach(), w, adapters, hc * n + n)[:, hc * n:]
             diag["s"] = s.detach().clone()
             diag["gate"] = gate.detach().clone()
             diag["value_norm"] = value.norm(dim=-1)

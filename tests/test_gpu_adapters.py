@@ -10,6 +10,8 @@ own type.  k is the length of the inner sum, r of the outer one.
 """
 from __future__ import annotations
 
+import types
+
 import pytest
 import torch
 
@@ -220,3 +222,92 @@ def test_refusals(bad, text):
     c, _ = make(20, 16, 24, 8, 3, F32)
     with pytest.raises(ValueError, match=text):
         eb.adapter_add(**{**c, **bad(c)})
+
+
+PLE_WEIGHTS = ("w_key", "w_value", "norm_key", "norm_query", "norm_conv", "conv1d")
+
+
+def ple_case(T=37, n=32, hc=3, H=5, dtype=torch.float32):
+    g = torch.Generator(device=DEV).manual_seed(11)
+    r = lambda *s, std=1.0: torch.randn(*s, device=DEV, generator=g) * std  # noqa: E731
+    w = types.SimpleNamespace(w_key=r(hc * n, n, std=n ** -0.5), w_value=r(n, n, std=n ** -0.5), norm_key=r(hc, n),
+                              norm_query=r(hc, n), norm_conv=r(hc, n), conv1d=r(hc * n, 4, std=0.5))
+    hp = types.SimpleNamespace(hc_mult=hc, n_embd=n, f_norm_rms_eps=1e-6, ple_ngram_size=3)
+    ad = eb.PleAdapters(r(4, 8, n, std=n ** -0.5), r(4, hc * n + n, 8, std=0.3),
+                        torch.randint(-1, 4, (T,), device=DEV, generator=g).to(torch.int32),
+                        0.5 + torch.rand(4, device=DEV, generator=g))
+    return r(T, n), r(T, hc, n), w, r(H, hc, n), hp, ad
+
+
+def ple_formula(emb, hidden, w, hist, hp, ad):
+    """The block in plain torch, in the type of its inputs, with each position's own projection W + s b a."""
+    T, n = emb.shape
+    hc, K, dil = hp.hc_mult, w.conv1d.shape[1], hp.ple_ngram_size
+    kv = emb @ torch.cat([w.w_key, w.w_value]).T
+    live = ad.index >= 0
+    i = ad.index.clamp_min(0).long()
+    delta = torch.einsum("tfr,trk,tk->tf", ad.b[i], ad.a[i], emb) * ad.scale.to(emb.dtype)[i].unsqueeze(1)
+    kv = kv + torch.where(live.unsqueeze(1), delta, 0.0)
+    key, value = kv[:, :hc * n].reshape(T, hc, n), kv[:, hc * n:]
+
+    def rms(x, g):
+        return x * torch.rsqrt(x.square().mean(-1, keepdim=True) + hp.f_norm_rms_eps) * g.reshape(hc, n)
+
+    s = (rms(key, w.norm_key) * rms(hidden, w.norm_query)).sum(-1) / n ** 0.5
+    gated = value.unsqueeze(1) * torch.sigmoid(torch.sign(s) * s.abs().clamp_min(1e-6).sqrt()).unsqueeze(-1)
+    full = torch.cat([hist, rms(gated, w.norm_conv)]).reshape(-1, hc * n)
+    back = torch.nn.functional.pad(full, (0, 0, (K - 1) * dil, 0))
+    H = hist.shape[0]
+    conv = sum(back[H + k * dil:H + k * dil + T] * w.conv1d[:, k] for k in range(K))
+    return hidden + gated + torch.nn.functional.silu(conv).reshape(T, hc, n)
+
+
+# the block's own tests hold it to 2e-5 of the largest magnitude in fp32 (its norms and its gate enlarge the
+# projections' rounding); the adapters' rounding stands beside the projections' and is no larger
+PLE_TOL = 2e-5
+
+
+@pytest.mark.parametrize("projection", ["3xtf32", "fp32", "tcgen05"])
+def test_ple_block_with_adapters_trains_their_factors(monkeypatch, projection):
+    from engraft_ngram_b200 import ple
+    monkeypatch.setattr(ple, "PROJECTION", projection)
+    emb, hidden, w, hist, hp, ad = ple_case()
+    free, _ = eb.ple_forward(emb, hidden, w, hist, hp)
+    out, tail = eb.ple_forward(emb, hidden, w, hist, hp, adapters=ad)
+    none = ad.index < 0
+    assert not torch.equal(out, free) and none.any()
+    up = lambda v: v.double()  # noqa: E731
+    w64 = types.SimpleNamespace(**{k: up(getattr(w, k)) for k in PLE_WEIGHTS})
+    leaves = {k: up(v).requires_grad_() for k, v in (("emb", emb), ("hidden", hidden), ("hist", hist), ("a", ad.a),
+                                                    ("b", ad.b))}
+    ad64 = eb.PleAdapters(leaves["a"], leaves["b"], ad.index, ad.scale)
+    want = ple_formula(leaves["emb"], leaves["hidden"], w64, leaves["hist"], hp, ad64)
+    assert float((out.double() - want).abs().max()) <= PLE_TOL * float(want.abs().max())
+    grad = torch.randn(out.shape, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1))
+    want.backward(up(grad))
+    mine = {k: v.clone().requires_grad_() for k, v in (("emb", emb), ("hidden", hidden), ("hist", hist), ("a", ad.a),
+                                                      ("b", ad.b))}
+    diag = {}
+    got, _ = eb.ple_forward(mine["emb"], mine["hidden"], w, mine["hist"], hp, diag=diag,
+                            adapters=eb.PleAdapters(mine["a"], mine["b"], ad.index, ad.scale))
+    assert torch.equal(got.detach(), out)
+    got.backward(grad)
+    for k in mine:
+        ref = leaves[k].grad
+        assert float((mine[k].grad.double() - ref).abs().max()) <= 5 * PLE_TOL * float(ref.abs().max()), k
+    # only the factors are trained, and stepped
+    a, b = torch.nn.Parameter(ad.a.clone()), torch.nn.Parameter(ad.b.clone())
+    opt = eb.Muon([a, b], lr=0.01, weight_decay=0.0)
+    eb.ple_forward(emb, hidden, w, hist, hp, adapters=eb.PleAdapters(a, b, ad.index, ad.scale))[0].backward(grad)
+    assert torch.equal(a.grad, mine["a"].grad) and torch.equal(b.grad, mine["b"].grad)
+    opt.step()
+    want_a, _ = eb.muon_step(ad.a.clone(), mine["a"].grad, torch.zeros_like(ad.a), 0.01)
+    assert torch.equal(a.detach(), want_a) and not torch.equal(b.detach(), ad.b)
+
+
+def test_ple_block_refuses_adapters_of_other_widths():
+    emb, hidden, w, hist, hp, ad = ple_case()
+    with pytest.raises(ValueError, match="adapters"):
+        eb.ple_forward(emb, hidden, w, hist, hp, adapters=eb.PleAdapters(ad.a, ad.b[:, :-1], ad.index))
+    with pytest.raises(ValueError, match="index"):
+        eb.ple_forward(emb, hidden, w, hist, hp, adapters=eb.PleAdapters(ad.a, ad.b, ad.index[:-1]))
