@@ -2,33 +2,39 @@
 // projection: out[t] = base[t] + s_i B_i (A_i x[t]) with i = index[t], A_i
 // [rank, K] and B_i [N, rank], and the gradients of x, A and B.
 //
-// Positions are first grouped by adapter (k_plan), so that each tile of 16 or 32
-// positions reads one adapter's factors.  Three products are then needed:
-//   shrink  h[p, :] = s_i A_i x[t]          (sums over a width, rank columns out)
-//   expand  out[t, :] = base[t, :] + B_i h[p, :]   (sums over the rank)
-//   weight  G_i[f, :] = sum over i's positions of x[t, f] h[p, :]
-// p is a position's place in the grouped order, t its row.  The backward uses the
-// same three: dh = s_i B_i^T g (shrink over N), dx = A_i^T dh (expand), dA from
-// (x, dh) and dB from (g, h).
+// Positions are grouped by adapter, so that each tile of 16 or 128 positions
+// reads one adapter's factors.  Three products are then needed:
+//   shrink  h[t, :] = s_i A_i x[t]                   (a sum over a width, rank columns out)
+//   expand  out[t, :] = base[t, :] + B_i h[t, :]     (a sum over the rank)
+//   weight  G_i[f, :] = sum over i's positions of x[t, f] h[t, :]
+// The backward uses the same three: dh = s_i B_i^T g (shrink over N), dx = A_i^T dh
+// (expand), dA from (x, dh) and dB from (g, h).
 //
-// All three run on mma.sync m16n8k8 TF32 with fp32 accumulation, fragments loaded
-// from global memory straight into registers.  The tensor work is small beside
-// the bytes (2 rank flops an element of base and out), so the mma.sync rate is
-// enough, and without a staging tile in shared memory nothing waits: a fragment's
-// index inside a sum is arbitrary as long as both operands agree, so each lane
-// takes 16 consecutive bytes of its row and the four lanes of a row 64.
-//
-// Arithmetic: an fp32 operand x is split as x = hi + lo, hi = x rounded to the 11
-// significant bits of TF32, and a product is hi hi + hi lo + lo hi (the dropped
-// term is 2^-24 of it); bf16 and fp16 values are exact in TF32 and need no split.
-// h and dh, sums over a whole width, are kept in fp32 for every type.
+// What bounds them is the bytes of x, base, grad and out: 2 rank flops for each
+// of their elements is below what mma.sync gives at those bytes a second.  So
+// each block streams its rows through a ring of shared-memory stages filled by
+// cp.async (rows are gathered, and 16-byte pieces of any row will do), with two or
+// three stages in flight, and the products are mma.sync from there.  16-bit types
+// use m16n8k16 in their own type; fp32 uses m16n8k8 TF32 on split operands,
+// x = hi + lo with hi rounded to the 11 significant bits of TF32: hi hi + hi lo +
+// lo hi, the dropped term being 2^-24 of the product.
+// h and dh, sums over a whole width, are kept in fp32.  Where they are an operand
+// beside a 16-bit type they are split in it, h = hi + lo (16 bits for bf16, 22 for
+// fp16, there after scaling by a power of two that brings the largest below 2^15).
+// mma.sync adds to its accumulator with truncation, so fp32 sums are taken out of
+// it every stage and added in fp32 proper: 12800 terms were 3e-6 off without,
+// 5e-7 with it.
+#include <type_traits>
+
 #include "engram_common.cuh"
 
 using namespace engram;
 
 namespace {
 
+constexpr int kThreads = 256, kWarps = 8;
 constexpr int kPlanThreads = 1024;
+constexpr int kScanMax = 1024;       // positions up to which a block finds its tile by itself
 constexpr int kMaxAdapters = 16384;  // k_plan counts them in shared memory
 constexpr int kMaxRank = 128;
 
@@ -142,503 +148,910 @@ __global__ void __launch_bounds__(kPlanThreads) k_plan(const int32_t* __restrict
     }
 }
 
-// ---- fragments -----------------------------------------------------------------
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-template <typename T> struct Io;
-template <> struct Io<float> {
-    static constexpr bool kSplit = true;
-    static __device__ __forceinline__ float one(const float* p) { return __ldg(p); }
-    static __device__ __forceinline__ float wide(float v) { return v; }
-    static __device__ __forceinline__ float narrow(float v) { return v; }
+// Up to kScanMax positions need no plan: a block looks through all indexes itself.  List, in ascending
+// order, of the positions with adapter a (n: without one); every thread of the block calls it.
+struct Scan {
+    int32_t list[kScanMax];
+    int32_t warp_count[kWarps];
 };
-template <> struct Io<__nv_bfloat16> {
-    static constexpr bool kSplit = false;
-    static __device__ __forceinline__ float one(const __nv_bfloat16* p) {
-        return __uint_as_float((uint32_t)__ldg(reinterpret_cast<const unsigned short*>(p)) << 16);
+__device__ __forceinline__ int scan_positions(Scan& s, const int32_t* __restrict__ index, int T, int n, int a) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int total = 0;
+    for (int t0 = 0; t0 < T; t0 += kThreads) {
+        const int t = t0 + threadIdx.x;
+        const bool mine = t < T && clamp_adapter(__ldg(index + t), n) == a;
+        const uint32_t m = __ballot_sync(0xffffffffu, mine);
+        if (lane == 0) s.warp_count[warp] = __popc(m);
+        __syncthreads();
+        int before = total;
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) {
+            if (w < warp) before += s.warp_count[w];
+            total += s.warp_count[w];
+        }
+        if (mine) s.list[before + __popc(m & ((1u << lane) - 1))] = t;
+        __syncthreads();
     }
-    static __device__ __forceinline__ float wide(__nv_bfloat16 v) { return __bfloat162float(v); }
-    static __device__ __forceinline__ __nv_bfloat16 narrow(float v) { return __float2bfloat16_rn(v); }
-};
-template <> struct Io<__half> {
-    static constexpr bool kSplit = false;
-    static __device__ __forceinline__ float one(const __half* p) {
-        return half_bits_to_float(__ldg(reinterpret_cast<const unsigned short*>(p)));
-    }
-    static __device__ __forceinline__ float wide(__half v) { return __half2float(v); }
-    static __device__ __forceinline__ __half narrow(float v) { return __float2half_rn(v); }
-};
-
-__device__ __forceinline__ void widen2(uint32_t u, float* v, const __nv_bfloat16*) {
-    v[0] = __uint_as_float(u << 16);
-    v[1] = __uint_as_float(u & 0xffff0000u);
-}
-__device__ __forceinline__ void widen2(uint32_t u, float* v, const __half*) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u));
-    v[0] = f.x;
-    v[1] = f.y;
+    return total;
 }
 
-// C consecutive elements from p (a multiple of C elements past an aligned row when vec), of which
-// `left` exist; the others are zero.
-template <typename T, int C>
-__device__ __forceinline__ void load_run(const T* __restrict__ p, int64_t left, bool vec, float* v) {
+// The positions of a block's tile.  With a plan: tile blockIdx.x of it.  Without: blockIdx.x is a
+// position, and the block whose position is its adapter's 0th, BM-th, ... takes that tile.
+template <int BM>
+struct TileRows {
+    Scan scan;
+    int32_t row[BM];
+    int32_t first;
+};
+template <int BM>
+__device__ __forceinline__ bool find_tile(TileRows<BM>& r, const Plan& plan, const int32_t* __restrict__ index, int T,
+                                          int n, int& adapter, int& rows) {
+    if (plan.perm) {
+        if ((int)blockIdx.x >= __ldg(plan.tiles)) return false;
+        const Tile t = plan.tile[blockIdx.x];
+        adapter = t.adapter;
+        rows = t.rows;
+        for (int i = threadIdx.x; i < BM; i += kThreads) r.row[i] = __ldg(plan.perm + t.start + min(i, t.rows - 1));
+    } else {
+        const int t = blockIdx.x;
+        adapter = clamp_adapter(__ldg(index + t), n);
+        const int total = scan_positions(r.scan, index, T, n, adapter);
+        for (int i = threadIdx.x; i < total; i += kThreads)
+            if (r.scan.list[i] == t) r.first = i;
+        __syncthreads();
+        const int first = r.first;
+        if (first % BM) return false;
+        rows = min(BM, total - first);
+        for (int i = threadIdx.x; i < BM; i += kThreads) r.row[i] = r.scan.list[first + min(i, rows - 1)];
+    }
+    __syncthreads();
+    return true;
+}
+
+// ---- types, stages and fragments -------------------------------------------------
+
+template <typename T>
+constexpr int kE = 16 / (int)sizeof(T);  // elements of a 16-byte unit
+
+__device__ __forceinline__ uint32_t bits_of(float v) { return __float_as_uint(v); }
+__device__ __forceinline__ float wide(float v) { return v; }
+__device__ __forceinline__ float wide(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float wide(__half v) { return __half2float(v); }
+template <typename T> __device__ __forceinline__ T narrow(float v);
+template <> __device__ __forceinline__ float narrow(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 narrow(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half narrow(float v) { return __float2half_rn(v); }
+
+// Two values as one register of the 16-bit type, the first in the low half.
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t u);
+template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t u) {
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t u) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&u));
+}
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+// One 16-byte unit of a stage from src, of which `left` elements exist (the others become zero).
+// vec: src is 16-byte aligned: asynchronous; else element by element.
+template <typename T>
+__device__ __forceinline__ void stage_unit(uint8_t* dst, const T* src, const T* valid, int64_t left, bool vec) {
+    constexpr int E = kE<T>;
     if (vec) {
-        if (left <= 0) {
-#pragma unroll
-            for (int i = 0; i < C; i++) v[i] = 0.f;
-            return;
-        }
-        if constexpr (sizeof(T) == 4) {
-            if constexpr (C == 1) {
-                v[0] = __ldg(p);
-            } else if constexpr (C == 2) {
-                const float2 f = __ldg(reinterpret_cast<const float2*>(p));
-                v[0] = f.x, v[1] = f.y;
-            } else {
-#pragma unroll
-                for (int i = 0; i < C; i += 4) {
-                    const float4 f = __ldg(reinterpret_cast<const float4*>(p + i));
-                    v[i] = f.x, v[i + 1] = f.y, v[i + 2] = f.z, v[i + 3] = f.w;
-                }
-            }
-        } else {
-            if constexpr (C == 1) {
-                v[0] = Io<T>::one(p);
-            } else if constexpr (C == 2) {
-                widen2(__ldg(reinterpret_cast<const uint32_t*>(p)), v, p);
-            } else if constexpr (C == 4) {
-                const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
-                widen2(u.x, v, p);
-                widen2(u.y, v + 2, p);
-            } else {
-#pragma unroll
-                for (int i = 0; i < C; i += 8) {
-                    const uint4 u = __ldg(reinterpret_cast<const uint4*>(p + i));
-                    widen2(u.x, v + i, p);
-                    widen2(u.y, v + i + 2, p);
-                    widen2(u.z, v + i + 4, p);
-                    widen2(u.w, v + i + 6, p);
-                }
-            }
-        }
+        const int bytes = left >= E ? 16 : left > 0 ? (int)left * (int)sizeof(T) : 0;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)),
+                     "l"(bytes ? src : valid), "r"(bytes)
+                     : "memory");
     } else {
+        alignas(16) T v[E];
 #pragma unroll
-        for (int i = 0; i < C; i++) v[i] = i < left ? Io<T>::one(p + i) : 0.f;
+        for (int i = 0; i < E; i++) v[i] = i < left ? src[i] : narrow<T>(0.f);
+        *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(v);
     }
 }
+__device__ __forceinline__ void stage_done() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void stage_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// 8 consecutive elements of a row of base, which may be the output itself: plain loads, not the
-// read-only path.
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, int64_t left, bool vec, float* v) {
-    if (vec && left >= 8) {
-        if constexpr (sizeof(T) == 4) {
-            const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-        } else {
-            const uint4 u = *reinterpret_cast<const uint4*>(p);
-            widen2(u.x, v, p);
-            widen2(u.y, v + 2, p);
-            widen2(u.z, v + 4, p);
-            widen2(u.w, v + 6, p);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = i < left ? Io<T>::wide(p[i]) : 0.f;
-    }
+// Units of a row are swapped by its number, so that the rows a fragment reads fall on unlike banks:
+// neighbouring rows (a quarter warp of 16-byte reads takes two) on unlike halves of 128 bytes, eight
+// rows (ldmatrix) on eight units.
+__device__ __forceinline__ int swap_rows(int row) { return ((row & 1) << 2) | ((row >> 1) & 3); }
+
+__device__ __forceinline__ uint4 lds128(const void* p) { return *reinterpret_cast<const uint4*>(p); }
+
+__device__ __forceinline__ void ldmatrix4(uint32_t* r, const void* p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(smem_addr(p))
+                 : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t* r, const void* p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(smem_addr(p))
+                 : "memory");
 }
 
-// 8 consecutive elements of a row of the output.
-template <typename T>
-__device__ __forceinline__ void store8(T* p, int64_t left, bool vec, const float* v) {
-    if (vec && left >= 8) {
-        if constexpr (sizeof(T) == 4) {
-            *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-            *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
-        } else {
-            alignas(16) T h[8];
-#pragma unroll
-            for (int i = 0; i < 8; i++) h[i] = Io<T>::narrow(v[i]);
-            *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(h);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++)
-            if (i < left) p[i] = Io<T>::narrow(v[i]);
-    }
-}
-
-// TF32 head of x: rounded to 11 significant bits (to nearest, ties away).
-__device__ __forceinline__ float tf32_head(float x) {
-    return __uint_as_float((__float_as_uint(x) + 0x1000u) & 0xffffe000u);
-}
-
-__device__ __forceinline__ void mma_tf32(float* d, const float* a, float b0, float b1) {
+template <typename T> __device__ __forceinline__ void mma(float* d, const uint32_t* a, uint32_t b0, uint32_t b1);
+template <> __device__ __forceinline__ void mma<float>(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
     asm volatile(
         "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
         "{%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(__float_as_uint(a[0])), "r"(__float_as_uint(a[1])), "r"(__float_as_uint(a[2])),
-          "r"(__float_as_uint(a[3])), "r"(__float_as_uint(b0)), "r"(__float_as_uint(b1)));
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma<__nv_bfloat16>(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <> __device__ __forceinline__ void mma<__half>(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// An operand in TF32: its head, and its remainder where it has one.
-template <bool SPLIT>
-struct FragA {
-    float hi[4], lo[SPLIT ? 4 : 1];
-    __device__ __forceinline__ void set(int i, float x) {
-        if constexpr (SPLIT) {
-            hi[i] = tf32_head(x);
-            lo[i] = x - hi[i];
-        } else {
-            hi[i] = x;
-        }
-    }
+// x = hi + lo, hi rounded to TF32 (to nearest, ties away).
+__device__ __forceinline__ void split_tf32(uint32_t x, uint32_t& hi, uint32_t& lo) {
+    hi = (x + 0x1000u) & 0xffffe000u;
+    lo = bits_of(__uint_as_float(x) - __uint_as_float(hi));
+}
+// An A fragment in the operand type with its remainder, and d += a b, the small terms first.
+struct Split {
+    uint32_t hi[4], lo[4];
 };
-template <bool SPLIT>
-struct FragB {
-    float hi[2], lo[SPLIT ? 2 : 1];
-    __device__ __forceinline__ void set(int i, float x) {
-        if constexpr (SPLIT) {
-            hi[i] = tf32_head(x);
-            lo[i] = x - hi[i];
-        } else {
-            hi[i] = x;
-        }
-    }
-};
-// d += a b, the small terms first.
-template <bool SA, bool SB>
-__device__ __forceinline__ void mma_split(float* d, const FragA<SA>& a, const FragB<SB>& b) {
-    if constexpr (SA) mma_tf32(d, a.lo, b.hi[0], b.hi[1]);
-    if constexpr (SB) mma_tf32(d, a.hi, b.lo[0], b.lo[1]);
-    mma_tf32(d, a.hi, b.hi[0], b.hi[1]);
+__device__ __forceinline__ Split split_a(uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+    Split f;
+    split_tf32(a0, f.hi[0], f.lo[0]);
+    split_tf32(a1, f.hi[1], f.lo[1]);
+    split_tf32(a2, f.hi[2], f.lo[2]);
+    split_tf32(a3, f.hi[3], f.lo[3]);
+    return f;
+}
+__device__ __forceinline__ void mma_split(float* d, const Split& a, uint32_t b0, uint32_t b1) {
+    uint32_t h0, h1, l0, l1;
+    split_tf32(b0, h0, l0);
+    split_tf32(b1, h1, l1);
+    mma<float>(d, a.lo, h0, h1);
+    mma<float>(d, a.hi, l0, l1);
+    mma<float>(d, a.hi, h0, h1);
 }
 
 // ---- shrink --------------------------------------------------------------------
-// h[split, p, :] = scale_i * sum over this split's columns k of x[perm[p], k] W_i[:, k].
+// h[split, t, :] = scale_i * sum over this split's columns k of x[t, k] W_i[:, k].
 // TRANS = false: W_i = A_i [rank, K] (K consecutive); true: W_i = B_i [K, rank] (rank consecutive).
-// One block per (tile, split); its 8 warps take the split's chunks in turn and are summed, in
-// their order, through shared memory.  A lane holds rows g and g + 8 (g = lane / 4) and E
-// consecutive columns, E of 16 bytes; the sums' step s uses its columns 2 s and 2 s + 1.
-constexpr int kWarps = 8;
+// One block per (tile, split).  WM = 8: 128 positions, 16 a warp.  WM = 1: 16 positions, and the warps
+// share the columns and are summed, in their order, through shared memory.  A chunk is 64 bytes of a
+// row, two steps of the MMA.  fp32 fragments come as 16-byte reads: a lane holds columns 4 q ..
+// 4 q + 3 of its row, of which step s takes 2 s and 2 s + 1 (the order inside a sum is free as long as
+// both operands agree).
+template <typename T, int RB, int WM, bool TRANS>
+struct ShrinkCfg {
+    static constexpr int E = kE<T>, RP = 8 * RB, BM = 16 * WM, WK = kWarps / WM;
+    static constexpr int NCH = WM == 1 ? 8 : 4, KC = NCH * 4 * E;  // chunks and columns of a stage
+    static constexpr int X_BYTES = BM * NCH * 64;
+    // rank-consecutive rows are padded: fp32 by 16 bytes (rows 4 apart), 16-bit by 16 (8 rows of ldmatrix)
+    static constexpr int W_PITCH = TRANS ? RP * (int)sizeof(T) + 16 : NCH * 64;
+    static constexpr int W_BYTES = (TRANS ? KC : RP) * W_PITCH;
+    static constexpr int STAGE = X_BYTES + W_BYTES;
+    static constexpr int NS = 4 * STAGE <= 112 * 1024 ? 4 : 3 * STAGE <= 220 * 1024 ? 3 : 2;
+    static constexpr int RED = WM == 1 ? kWarps * BM * RP * 4 : 0;
+    static constexpr int SMEM = NS * STAGE > RED ? NS * STAGE : RED;
+    static_assert(SMEM <= 220 * 1024, "a block's shared memory");
+};
 
-template <typename T, int RB, int MT, bool TRANS>
-__global__ void __launch_bounds__(kWarps * 32) k_shrink(Plan plan, const T* __restrict__ x, int64_t ldx,
-                                                        const T* __restrict__ w, const float* __restrict__ scale,
-                                                        int n, int rank, int64_t K, int64_t k_split, int64_t T_rows,
-                                                        bool vec, bool rvec, float* __restrict__ h) {
-    constexpr int E = 16 / sizeof(T), CH = 4 * E, RP = 8 * RB, BM = 16 * MT;
-    constexpr bool SP = Io<T>::kSplit;
-    extern __shared__ float red[];  // [kWarps][BM][RP]
-    if ((int)blockIdx.x >= __ldg(plan.tiles)) return;
-    const Tile tile = plan.tile[blockIdx.x];
-    if (tile.adapter >= n) return;
+template <typename T, int RB, int WM, bool TRANS>
+__global__ void __launch_bounds__(kThreads) k_shrink(Plan plan, const int32_t* __restrict__ index,
+                                                     const T* __restrict__ x, int64_t ldx, const T* __restrict__ w,
+                                                     const float* __restrict__ scale, int n, int rank, int64_t K,
+                                                     int64_t k_split, int T_rows, bool xvec, bool wvec,
+                                                     float* __restrict__ h) {
+    using C = ShrinkCfg<T, RB, WM, TRANS>;
+    constexpr int E = C::E, RP = C::RP, BM = C::BM, WK = C::WK, NCH = C::NCH, KC = C::KC, NS = C::NS;
+    constexpr bool F32 = sizeof(T) == 4;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ TileRows<BM> tr;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
-    const T* wi = w + (int64_t)tile.adapter * rank * K;
-    const T* row[2 * MT];
-#pragma unroll
-    for (int m = 0; m < 2 * MT; m++) {
-        const int p = 8 * m + g;
-        row[m] = x + (int64_t)__ldg(plan.perm + tile.start + min(p, tile.rows - 1)) * ldx;
-    }
-    float acc[MT][RB][4];
-#pragma unroll
-    for (int m = 0; m < MT; m++)
-#pragma unroll
-        for (int b = 0; b < RB; b++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) acc[m][b][i] = 0.f;
-    const int64_t k_begin = blockIdx.y * k_split, k_end = min(K, k_begin + k_split);
-#pragma unroll 2
-    for (int64_t k0 = k_begin + warp * CH; k0 < k_end; k0 += kWarps * CH) {
-        const int64_t k = k0 + E * q;
-        float xv[2 * MT][E];
-#pragma unroll
-        for (int m = 0; m < 2 * MT; m++) load_run<T, E>(row[m] + k, k_end - k, vec, xv[m]);
+    const int wm = warp % WM, wk = warp / WM;
+    wait_for_previous();
+    let_next_start();
+    int adapter, rows;
+    if (!find_tile<BM>(tr, plan, index, T_rows, n, adapter, rows) || adapter >= n) return;
+    const T* wi = w + (int64_t)adapter * rank * K;
+    const int64_t k_begin = blockIdx.y * k_split, k_end = k_begin + k_split < K ? k_begin + k_split : K;
+    const int stages = k_begin < k_end ? (int)((k_end - k_begin + KC - 1) / KC) : 0;
+
+    const auto load = [&](int i) {
+        uint8_t* xs = smem + (i % NS) * C::STAGE;
+        uint8_t* ws = xs + C::X_BYTES;
+        const int64_t k0 = k_begin + (int64_t)i * KC;
+        for (int u = threadIdx.x; u < BM * NCH * 4; u += kThreads) {
+            const int r = u / (NCH * 4), c = u % (NCH * 4);
+            const int64_t k = k0 + c * E;
+            stage_unit<T>(xs + r * (NCH * 64) + ((c ^ swap_rows(r)) * 16), x + (int64_t)tr.row[r] * ldx + k, x,
+                          r < rows ? k_end - k : 0, xvec);
+        }
         if constexpr (!TRANS) {
-            float wv[RB][E];
-#pragma unroll
-            for (int b = 0; b < RB; b++) {
-                const int r = 8 * b + g;
-                load_run<T, E>(wi + (int64_t)r * K + k, r < rank ? k_end - k : 0, vec, wv[b]);
-            }
-#pragma unroll
-            for (int s = 0; s < E / 2; s++) {
-                FragA<SP> fa[MT];
-#pragma unroll
-                for (int m = 0; m < MT; m++) {
-                    fa[m].set(0, xv[2 * m][2 * s]);
-                    fa[m].set(1, xv[2 * m + 1][2 * s]);
-                    fa[m].set(2, xv[2 * m][2 * s + 1]);
-                    fa[m].set(3, xv[2 * m + 1][2 * s + 1]);
-                }
-#pragma unroll
-                for (int b = 0; b < RB; b++) {
-                    FragB<SP> fb;
-                    fb.set(0, wv[b][2 * s]);
-                    fb.set(1, wv[b][2 * s + 1]);
-#pragma unroll
-                    for (int m = 0; m < MT; m++) mma_split<SP, SP>(acc[m][b], fa[m], fb);
-                }
+            for (int u = threadIdx.x; u < RP * NCH * 4; u += kThreads) {
+                const int r = u / (NCH * 4), c = u % (NCH * 4);
+                const int64_t k = k0 + c * E;
+                stage_unit<T>(ws + r * C::W_PITCH + ((c ^ swap_rows(r)) * 16), wi + (int64_t)r * K + k, w,
+                              r < rank ? k_end - k : 0, wvec);
             }
         } else {
+            constexpr int U = RP / E;
+            for (int u = threadIdx.x; u < KC * U; u += kThreads) {
+                const int r = u / U, c = u % U;
+                stage_unit<T>(ws + r * C::W_PITCH + c * 16, wi + (k0 + r) * rank + c * E, w,
+                              k0 + r < k_end ? rank - c * E : 0, wvec);
+            }
+        }
+        stage_done();
+    };
+
+    float acc[RB][4], sum[F32 ? RB : 1][4];
 #pragma unroll
-            for (int s = 0; s < E / 2; s++) {
-                float wv[2][RB];  // columns k + 2 s, k + 2 s + 1; ranks RB g .. RB g + RB - 1
+    for (int b = 0; b < RB; b++)
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    const int64_t kk = k + 2 * s + j;
-                    load_run<T, RB>(wi + kk * rank + RB * g, kk < k_end ? rank - RB * g : 0, rvec, wv[j]);
+        for (int i = 0; i < 4; i++) acc[b][i] = 0.f;
+#pragma unroll
+    for (int b = 0; b < (F32 ? RB : 1); b++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) sum[b][i] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NS - 1; i++) {
+        if (i < stages) load(i);
+        else stage_done();
+    }
+    for (int i = 0; i < stages; i++) {
+        stage_wait<NS - 2>();
+        __syncthreads();
+        if (i + NS - 1 < stages) load(i + NS - 1);
+        else stage_done();
+        const uint8_t* xs = smem + (i % NS) * C::STAGE;
+        const uint8_t* ws = xs + C::X_BYTES;
+        for (int ch = wk; ch < NCH; ch += WK) {
+            if constexpr (F32) {
+                const int r0 = 16 * wm + g, c = 4 * ch + q;
+                const uint4 xa = lds128(xs + r0 * (NCH * 64) + ((c ^ swap_rows(r0)) * 16));
+                const uint4 xb = lds128(xs + (r0 + 8) * (NCH * 64) + ((c ^ swap_rows(r0 + 8)) * 16));
+                const Split f0 = split_a(xa.x, xb.x, xa.y, xb.y), f1 = split_a(xa.z, xb.z, xa.w, xb.w);
+                if constexpr (!TRANS) {
+#pragma unroll
+                    for (int b = 0; b < RB; b++) {
+                        const int r = 8 * b + g;
+                        const uint4 wv = lds128(ws + r * C::W_PITCH + ((c ^ swap_rows(r)) * 16));
+                        mma_split(acc[b], f0, wv.x, wv.y);
+                        mma_split(acc[b], f1, wv.z, wv.w);
+                    }
+                } else {  // a lane's column of block b is rank RB g + b
+#pragma unroll
+                    for (int s = 0; s < 2; s++) {
+                        const uint8_t* p = ws + (16 * ch + 4 * q + 2 * s) * C::W_PITCH + RB * g * 4;
+                        uint32_t wv[2][RB];
+#pragma unroll
+                        for (int j = 0; j < 2; j++) {
+                            if constexpr (RB == 2) {
+                                const uint2 v = *reinterpret_cast<const uint2*>(p + j * C::W_PITCH);
+                                wv[j][0] = v.x, wv[j][1] = v.y;
+                            } else {
+#pragma unroll
+                                for (int b = 0; b < RB; b += 4) {
+                                    const uint4 v = lds128(p + j * C::W_PITCH + 4 * b);
+                                    wv[j][b] = v.x, wv[j][b + 1] = v.y, wv[j][b + 2] = v.z, wv[j][b + 3] = v.w;
+                                }
+                            }
+                        }
+#pragma unroll
+                        for (int b = 0; b < RB; b++) mma_split(acc[b], s ? f1 : f0, wv[0][b], wv[1][b]);
+                    }
                 }
-                FragA<SP> fa[MT];
+            } else {
+                const int lr = lane & 7, lm = lane >> 3;  // ldmatrix: row and matrix of this lane's address
 #pragma unroll
-                for (int m = 0; m < MT; m++) {
-                    fa[m].set(0, xv[2 * m][2 * s]);
-                    fa[m].set(1, xv[2 * m + 1][2 * s]);
-                    fa[m].set(2, xv[2 * m][2 * s + 1]);
-                    fa[m].set(3, xv[2 * m + 1][2 * s + 1]);
-                }
+                for (int s = 0; s < 2; s++) {
+                    uint32_t fa[4];
+                    const int r0 = 16 * wm + lr + 8 * (lm & 1), c = 4 * ch + 2 * s + (lm >> 1);
+                    ldmatrix4(fa, xs + r0 * (NCH * 64) + ((c ^ swap_rows(r0)) * 16));
 #pragma unroll
-                for (int b = 0; b < RB; b++) {
-                    FragB<SP> fb;
-                    fb.set(0, wv[0][b]);
-                    fb.set(1, wv[1][b]);
-#pragma unroll
-                    for (int m = 0; m < MT; m++) mma_split<SP, SP>(acc[m][b], fa[m], fb);
+                    for (int b = 0; b < RB; b += 2) {
+                        uint32_t fb[4];
+                        if constexpr (!TRANS) {
+                            const int r = 8 * b + lr + 8 * (lm >> 1), cw = 4 * ch + 2 * s + (lm & 1);
+                            ldmatrix4(fb, ws + r * C::W_PITCH + ((cw ^ swap_rows(r)) * 16));
+                        } else {
+                            const int r = 32 * ch + 16 * s + lr + 8 * (lm & 1);
+                            ldmatrix4_trans(fb, ws + r * C::W_PITCH + (b + (lm >> 1)) * 16);
+                        }
+                        mma<T>(acc[b], fa, fb[0], fb[1]);
+                        mma<T>(acc[b + 1], fa, fb[2], fb[3]);
+                    }
                 }
             }
         }
-    }
-    float* mine = red + warp * BM * RP;
+        if constexpr (F32) {
 #pragma unroll
-    for (int m = 0; m < MT; m++)
+            for (int b = 0; b < RB; b++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) sum[b][k] += acc[b][k], acc[b][k] = 0.f;
+        }
+    }
+    const auto result = [&](int b, int k) { return F32 ? sum[F32 ? b : 0][k] : acc[b][k]; };
+    const auto column = [&](int b, int j) { return F32 && TRANS ? RB * (2 * q + j) + b : 8 * b + 2 * q + j; };
+    const float s = scale ? __ldg(scale + adapter) : 1.f;
+    float* dst = h + (int64_t)blockIdx.y * T_rows * RP;
+    if constexpr (WM == 1) {
+        stage_wait<0>();
+        __syncthreads();
+        float* red = reinterpret_cast<float*>(smem);  // [kWarps][BM][RP]
 #pragma unroll
         for (int b = 0; b < RB; b++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int c = 2 * q + (i & 1), r = TRANS ? RB * c + b : 8 * b + c;
-                mine[(16 * m + 8 * (i >> 1) + g) * RP + r] = acc[m][b][i];
-            }
-    __syncthreads();
-    const float s = scale ? __ldg(scale + tile.adapter) : 1.f;
-    float* dst = h + ((int64_t)blockIdx.y * T_rows + tile.start) * RP;
-    for (int e = threadIdx.x; e < tile.rows * RP; e += kWarps * 32) {
-        float v = 0.f;
+            for (int k = 0; k < 4; k++) red[(warp * BM + g + 8 * (k >> 1)) * RP + column(b, k & 1)] = result(b, k);
+        __syncthreads();
+        for (int e = threadIdx.x; e < rows * RP; e += kThreads) {
+            float v = 0.f;
 #pragma unroll
-        for (int k = 0; k < kWarps; k++) v += red[k * BM * RP + e];
-        dst[e] = s * v;
+            for (int k = 0; k < kWarps; k++) v += red[k * BM * RP + e];
+            dst[(int64_t)tr.row[e / RP] * RP + e % RP] = s * v;
+        }
+    } else {
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const int r = 16 * wm + g + 8 * u;
+            if (r < rows) {
+                float* d = dst + (int64_t)tr.row[r] * RP;
+#pragma unroll
+                for (int b = 0; b < RB; b++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++) d[column(b, j)] = s * result(b, 2 * u + j);
+            }
+        }
     }
 }
 
-// 4 consecutive ranks of a place of h, summed over the splits.
-__device__ __forceinline__ void load_h(const float* __restrict__ h, int splits, int64_t stride, float* v) {
-    float4 f = __ldg(reinterpret_cast<const float4*>(h));
+// 4 consecutive ranks of a position's h, summed over the splits.
+__device__ __forceinline__ float4 load_h(const float* h, int splits, int64_t stride) {
+    float4 f = *reinterpret_cast<const float4*>(h);
     for (int k = 1; k < splits; k++) {
-        const float4 u = __ldg(reinterpret_cast<const float4*>(h + k * stride));
+        const float4 u = *reinterpret_cast<const float4*>(h + k * stride);
         f.x += u.x, f.y += u.y, f.z += u.z, f.w += u.w;
     }
-    v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+    return f;
+}
+
+// 2^(14 - e) for m in [2^e, 2^(e + 1)): brings m into fp16 below 2^15; 1 for zero and for what is not finite.
+__device__ __forceinline__ float half_scale(float m) {
+    const int e = (int)((bits_of(m) >> 23) & 255) - 127;
+    return (e < -126 || e > 127) ? 1.f : __uint_as_float((uint32_t)(min(max(14 - e, -126), 126) + 127) << 23);
 }
 
 // ---- expand --------------------------------------------------------------------
-// out[t, f] = base[t, f] + sum over ranks of h[p, r] W_i[f, r], t = perm[p]; positions without an
-// adapter get base.  TRANS = false: W_i = B_i [F, rank]; true: W_i = A_i [rank, F].  base null: zeros.
-// A warp keeps its tile's h fragments in registers and walks over 32 columns at a time; a lane ends
-// up with 8 consecutive columns of rows g and g + 8, read and written as 16-byte pieces.
-template <typename T, int RB, int MT, bool TRANS>
-__global__ void __launch_bounds__(kWarps * 32) k_expand(Plan plan, const float* __restrict__ h, int splits,
-                                                        const T* __restrict__ w, int n, int rank, int64_t F,
-                                                        int64_t f_block, int64_t T_rows, const T* base,
-                                                        int64_t ldb, T* out, int64_t ldo, bool vec, bool wvec) {
-    constexpr int RP = 8 * RB, RC = RB / 2;  // RC chunks of 16 ranks
-    constexpr bool SP = Io<T>::kSplit;
-    if ((int)blockIdx.x >= __ldg(plan.tiles)) return;
-    const Tile tile = plan.tile[blockIdx.x];
+// out[t, f] = base[t, f] + sum over ranks of h[t, r] W_i[f, r]; positions without an adapter get base.
+// TRANS = false: W_i = B_i [F, rank]; true: W_i = A_i [rank, F].  base null: zeros.
+// WM = 8: 128 positions, 16 a warp, 64 columns a stage; WM = 1: 16 positions, 256 columns a stage, 32 a
+// warp.  A warp keeps its positions' h fragments in registers.  Columns are dealt to the MMA's so
+// that a lane ends up with whole 16-byte units of rows g and g + 8, and four lanes with 64 consecutive
+// bytes: unit 4 v + q holds, for fp32, columns 2 (b % 2) + j of blocks b = 2 v, 2 v + 1 (TRANS: columns b
+// of MMA column 2 q + v), for 16 bits columns 2 b + j (TRANS: 4 j + b).
+template <typename T, int RB, int WM, bool TRANS>
+struct ExpandCfg {
+    static constexpr int E = kE<T>, RP = 8 * RB, BM = 16 * WM, WF = kWarps / WM;
+    // columns of a stage (128 where 256 rows of fp32 factors would not fit twice)
+    static constexpr int FS = WM == 8 ? 64 : RP * (int)sizeof(T) == 512 ? 128 : 256;
+    static constexpr int FU = FS / E;                  // units of a base row
+    static constexpr int B_BYTES = BM * FS * (int)sizeof(T);
+    // B_i rows: fp32 at a pitch of 16 words beyond a multiple of 32, 16-bit dense with swapped units
+    static constexpr int W_PITCH = TRANS ? FS * (int)sizeof(T)
+                                         : sizeof(T) == 4 ? (RP == 16 ? 64 : RP * 4 + 64) : RP * 2;
+    static constexpr int W_BYTES = (TRANS ? RP : FS) * W_PITCH;
+    static constexpr int STAGE = B_BYTES + W_BYTES;
+    static constexpr int NS = 4 * STAGE <= 112 * 1024 ? 4 : 3 * STAGE <= 220 * 1024 ? 3 : 2;
+    static constexpr int SMEM = NS * STAGE;
+    static_assert(SMEM <= 220 * 1024, "a block's shared memory");
+};
+
+// Unit c of a 16-bit B_i row, swapped so that the four rows of a half warp's 8-byte reads (features 0, 1,
+// 8, 9 or 16, 17, 24, 25 apart), 32 bytes of each, fall on unlike banks.
+template <int RP>
+__device__ __forceinline__ int swap_b16(int row, int c) {
+    if constexpr (RP == 16) return ((2 * row + c) ^ (((row >> 3) & 1) << 2)) - 2 * row;
+    else if constexpr (RP == 32) return c ^ (((row >> 3) & 1) << 1);
+    else return c ^ (((row & 1) << 2) | (((row >> 3) & 1) << 1));
+}
+
+template <typename T, int RB, int WM, bool TRANS>
+__global__ void __launch_bounds__(kThreads) k_expand(Plan plan, const int32_t* __restrict__ index,
+                                                     const float* h, int splits, const T* __restrict__ w, int n,
+                                                     int rank, int64_t F, int64_t f_block, int T_rows, const T* base,
+                                                     int64_t ldb, T* out, int64_t ldo, bool bvec, bool wvec,
+                                                     bool ovec) {
+    using C = ExpandCfg<T, RB, WM, TRANS>;
+    constexpr int E = C::E, RP = C::RP, BM = C::BM, FS = C::FS, FU = C::FU, NS = C::NS;
+    constexpr bool F32 = sizeof(T) == 4;
+    constexpr int KS = F32 ? RP / 8 : RP / 16;  // MMA steps of the rank
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ TileRows<BM> tr;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
-    const bool none = tile.adapter >= n;
-    if (none && base == out) return;
-    int64_t t[2 * MT];
-    bool live[2 * MT];
-#pragma unroll
-    for (int m = 0; m < 2 * MT; m++) {
-        live[m] = 8 * m + g < tile.rows;
-        t[m] = __ldg(plan.perm + tile.start + min(8 * m + g, tile.rows - 1));
+    const int wm = warp % WM, wf = warp / WM;
+    // the plan and h come from the launch before; index, base and the factors do not
+    if (plan.perm) wait_for_previous();
+    int adapter, rows;
+    const bool found = find_tile<BM>(tr, plan, index, T_rows, n, adapter, rows);
+    const bool none = found && adapter >= n;
+    if (!found || (none && base == out)) {
+        wait_for_previous();
+        let_next_start();
+        return;
     }
-    FragA<true> fa[MT][RB];
-    if (!none) {
-#pragma unroll
-        for (int m = 0; m < MT; m++)
-#pragma unroll
-            for (int c = 0; c < RC; c++)
-#pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    const int p = min(16 * m + 8 * u + g, tile.rows - 1);
-                    float v[4];
-                    load_h(h + ((int64_t)tile.start + p) * RP + 16 * c + 4 * q, splits, T_rows * RP, v);
-                    fa[m][2 * c].set(u, v[0]);
-                    fa[m][2 * c].set(2 + u, v[1]);
-                    fa[m][2 * c + 1].set(u, v[2]);
-                    fa[m][2 * c + 1].set(2 + u, v[3]);
-                }
-    }
-    const T* wi = w + (none ? 0 : (int64_t)tile.adapter * rank * F);
-    const int64_t f_begin = blockIdx.y * f_block, f_end = min(F, f_begin + f_block);
-    for (int64_t f0 = f_begin + 32 * warp; f0 < f_end; f0 += 32 * kWarps) {
-        const int64_t f = f0 + 8 * q, left = f_end - f;
-        float acc[MT][4][4];
-#pragma unroll
-        for (int m = 0; m < MT; m++)
-#pragma unroll
-            for (int b = 0; b < 4; b++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) acc[m][b][i] = 0.f;
-        float bv[2 * MT][8];
-#pragma unroll
-        for (int m = 0; m < 2 * MT; m++) {
-            if (base && live[m]) {
-                load8<T>(base + t[m] * ldb + f, left, vec, bv[m]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; i++) bv[m][i] = 0.f;
+    const T* wi = w + (none ? 0 : (int64_t)adapter * rank * F);
+    const int64_t f_begin = blockIdx.y * f_block, f_end = f_begin + f_block < F ? f_begin + f_block : F;
+    const int stages = f_begin < f_end ? (int)((f_end - f_begin + FS - 1) / FS) : 0;
+
+    const auto load = [&](int i) {
+        uint8_t* bs = smem + (i % NS) * C::STAGE;
+        uint8_t* ws = bs + C::B_BYTES;
+        const int64_t f0 = f_begin + (int64_t)i * FS;
+        if (base) {
+            for (int u = threadIdx.x; u < BM * FU; u += kThreads) {
+                const int r = u / FU, c = u % FU;
+                const int64_t f = f0 + c * E;
+                if (r < rows)
+                    stage_unit<T>(bs + r * (FU * 16) + ((c ^ swap_rows(r)) * 16), base + (int64_t)tr.row[r] * ldb + f,
+                                  base, f_end - f, bvec);
             }
         }
         if (!none) {
+            if constexpr (!TRANS) {
+                constexpr int U = RP / E;
+                for (int u = threadIdx.x; u < FS * U; u += kThreads) {
+                    const int r = u / U, c = u % U;
+                    const int to = F32 ? c : swap_b16<RP>(r, c);
+                    stage_unit<T>(ws + r * C::W_PITCH + to * 16, wi + (f0 + r) * rank + c * E, w,
+                                  f0 + r < f_end ? rank - c * E : 0, wvec);
+                }
+            } else {
+                for (int u = threadIdx.x; u < RP * FU; u += kThreads) {
+                    const int r = u / FU, c = u % FU;
+                    const int64_t f = f0 + c * E;
+                    const int to = F32 ? c ^ ((r >> 2) & 3) : c ^ (((r >> 2) & 3) << 1);
+                    stage_unit<T>(ws + r * C::W_PITCH + to * 16, wi + (int64_t)r * F + f, w, r < rank ? f_end - f : 0,
+                                  wvec);
+                }
+            }
+        }
+        stage_done();
+    };
 #pragma unroll
-            for (int c = 0; c < RC; c++) {
-                if constexpr (!TRANS) {  // block b, column 2 q + j of the product: feature f0 + 8 q + 2 b + j
-                    float wv[4][4];
+    for (int i = 0; i < NS - 1; i++) {
+        if (i < stages) load(i);
+        else stage_done();
+    }
+    if (!plan.perm) wait_for_previous();
+    let_next_start();
+
+    // h of rows g and g + 8 of this warp's 16, split
+    uint32_t hi[KS][4], lo[KS][4];
+    float undo[2] = {1.f, 1.f};  // fp16: the rows' scales taken back
+    const int r0 = 16 * wm + g;
+    if (!none) {
+        float v[2][2 * KS * (F32 ? 1 : 2)];  // ranks: fp32 16 c + 4 q .. + 3; 16 bits 16 c + 2 q, + 1, + 8, + 9
 #pragma unroll
-                    for (int b = 0; b < 4; b++) {
-                        const int64_t fw = f0 + 8 * (g >> 1) + 2 * b + (g & 1);
-                        const int r = 16 * c + 4 * q;
-                        load_run<T, 4>(wi + fw * rank + r, fw < f_end ? rank - r : 0, wvec, wv[b]);
-                    }
+        for (int u = 0; u < 2; u++) {
+            const float* hp = h + (int64_t)tr.row[min(r0 + 8 * u, rows - 1)] * RP;
+            const int64_t stride = (int64_t)T_rows * RP;
 #pragma unroll
-                    for (int b = 0; b < 4; b++)
+            for (int c = 0; c < RP / 16; c++) {
+                const float4 f = load_h(hp + 16 * c + 4 * q, splits, stride);
+                v[u][4 * c] = f.x, v[u][4 * c + 1] = f.y, v[u][4 * c + 2] = f.z, v[u][4 * c + 3] = f.w;
+            }
+            if constexpr (sizeof(T) == 2) {
+                if constexpr (std::is_same_v<T, __half>) {
+                    float m = 0.f;
 #pragma unroll
-                        for (int s = 0; s < 2; s++) {
-                            FragB<SP> fb;
-                            fb.set(0, wv[b][2 * s]);
-                            fb.set(1, wv[b][2 * s + 1]);
+                    for (int i = 0; i < RP / 4; i++) m = fmaxf(m, fabsf(v[u][i]));
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                    const float s = half_scale(m);
+                    undo[u] = 1.f / s;
 #pragma unroll
-                            for (int m = 0; m < MT; m++) mma_split<true, SP>(acc[m][b], fa[m][2 * c + s], fb);
-                        }
-                } else {  // block b, column 2 q + j: feature f0 + 8 q + 4 j + b
-#pragma unroll
-                    for (int s = 0; s < 2; s++) {
-                        float wv[2][4];
-#pragma unroll
-                        for (int j = 0; j < 2; j++) {
-                            const int r = 16 * c + 4 * q + 2 * s + j;
-                            const int64_t fw = f0 + 4 * g;
-                            load_run<T, 4>(wi + (int64_t)r * F + fw, r < rank ? f_end - fw : 0, wvec, wv[j]);
-                        }
-#pragma unroll
-                        for (int b = 0; b < 4; b++) {
-                            FragB<SP> fb;
-                            fb.set(0, wv[0][b]);
-                            fb.set(1, wv[1][b]);
-#pragma unroll
-                            for (int m = 0; m < MT; m++) mma_split<true, SP>(acc[m][b], fa[m][2 * c + s], fb);
-                        }
-                    }
+                    for (int i = 0; i < RP / 4; i++) v[u][i] *= s;
                 }
             }
         }
 #pragma unroll
-        for (int m = 0; m < 2 * MT; m++) {
-            if (!live[m]) continue;
-            float v[8];
+        for (int s = 0; s < KS; s++)
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    if constexpr (F32) {
+                        split_tf32(bits_of(v[u][2 * s + k]), hi[s][u + 2 * k], lo[s][u + 2 * k]);
+                    } else {  // ranks 4 q + 2 k, + 1 of the step: the sum's order is the factors' below
+                        const float a = v[u][4 * s + 2 * k], b = v[u][4 * s + 2 * k + 1];
+                        const uint32_t p = pack2<T>(a, b);
+                        const float2 back = unpack2<T>(p);
+                        hi[s][u + 2 * k] = p;
+                        lo[s][u + 2 * k] = pack2<T>(a - back.x, b - back.y);
+                    }
+                }
+    }
+
+    for (int i = 0; i < stages; i++) {
+        stage_wait<NS - 2>();
+        __syncthreads();
+        if (i + NS - 1 < stages) load(i + NS - 1);
+        else stage_done();
+        const uint8_t* bs = smem + (i % NS) * C::STAGE;
+        const uint8_t* ws = bs + C::B_BYTES;
+        const int64_t f0 = f_begin + (int64_t)i * FS;
+        for (int fs = 32 * wf; fs < FS; fs += 32 * C::WF) {  // 32 columns from f0 + fs
+            if (f0 + fs >= f_end) break;
+            float acc[4][4];
 #pragma unroll
             for (int b = 0; b < 4; b++)
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    const int e = TRANS ? 4 * j + b : 2 * b + j;
-                    v[e] = bv[m][e] + acc[m >> 1][b][2 * (m & 1) + j];
+                for (int k = 0; k < 4; k++) acc[b][k] = 0.f;
+            if (!none) {
+                if constexpr (F32 && !TRANS) {
+#pragma unroll
+                    for (int b = 0; b < 4; b++) {
+                        const int r = fs + 16 * (b >> 1) + 4 * (g >> 1) + 2 * (b & 1) + (g & 1);
+#pragma unroll
+                        for (int c = 0; c < RP / 16; c++) {
+                            const uint4 wv = lds128(ws + r * C::W_PITCH + (4 * c + q) * 16);
+#pragma unroll
+                            for (int s = 0; s < 2; s++) {
+                                uint32_t h0, h1, l0, l1;
+                                split_tf32(s ? wv.z : wv.x, h0, l0);
+                                split_tf32(s ? wv.w : wv.y, h1, l1);
+                                mma<float>(acc[b], lo[2 * c + s], h0, h1);
+                                mma<float>(acc[b], hi[2 * c + s], l0, l1);
+                                mma<float>(acc[b], hi[2 * c + s], h0, h1);
+                            }
+                        }
+                    }
+                } else if constexpr (F32) {
+#pragma unroll
+                    for (int s = 0; s < KS; s++) {
+                        uint32_t wv[2][4];
+#pragma unroll
+                        for (int j = 0; j < 2; j++) {
+                            const int r = 16 * (s >> 1) + 4 * q + 2 * (s & 1) + j;
+                            const int c = (fs + 16 * (g & 1)) / 4 + (g >> 1);
+                            const uint4 v = lds128(ws + r * C::W_PITCH + ((c ^ ((r >> 2) & 3)) * 16));
+                            wv[j][0] = v.x, wv[j][1] = v.y, wv[j][2] = v.z, wv[j][3] = v.w;
+                        }
+#pragma unroll
+                        for (int b = 0; b < 4; b++) {
+                            uint32_t h0, h1, l0, l1;
+                            split_tf32(wv[0][b], h0, l0);
+                            split_tf32(wv[1][b], h1, l1);
+                            mma<float>(acc[b], lo[s], h0, h1);
+                            mma<float>(acc[b], hi[s], l0, l1);
+                            mma<float>(acc[b], hi[s], h0, h1);
+                        }
+                    }
+                } else if constexpr (!TRANS) {
+                    // a lane's four ranks 4 q .. 4 q + 3 of a step are the MMA's k = 2 q, 2 q + 1, 2 q + 8, 2 q + 9
+#pragma unroll
+                    for (int s = 0; s < KS; s++)
+#pragma unroll
+                        for (int b = 0; b < 4; b++) {
+                            const int r = fs + 8 * (g >> 1) + 2 * b + (g & 1);
+                            const uint8_t* p = ws + r * C::W_PITCH + swap_b16<RP>(r, 2 * s + (q >> 1)) * 16 + (q & 1) * 8;
+                            const uint2 wv = *reinterpret_cast<const uint2*>(p);
+                            mma<T>(acc[b], lo[s], wv.x, wv.y);
+                            mma<T>(acc[b], hi[s], wv.x, wv.y);
+                        }
+                } else {
+#pragma unroll
+                    for (int s = 0; s < KS; s++) {
+                        uint2 wv[4];  // ranks 4 q .. 4 q + 3, columns 4 g .. 4 g + 3
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            const int r = 16 * s + 4 * q + j, c = fs / 8 + (g >> 1);
+                            wv[j] = *reinterpret_cast<const uint2*>(
+                                ws + r * C::W_PITCH + ((c ^ (((r >> 2) & 3) << 1)) * 16) + (g & 1) * 8);
+                        }
+#pragma unroll
+                        for (int b = 0; b < 4; b++) {
+                            const uint32_t pick = (b & 1) ? 0x7632u : 0x5410u;
+                            const uint32_t b0 = __byte_perm(b < 2 ? wv[0].x : wv[0].y, b < 2 ? wv[1].x : wv[1].y, pick);
+                            const uint32_t b1 = __byte_perm(b < 2 ? wv[2].x : wv[2].y, b < 2 ? wv[3].x : wv[3].y, pick);
+                            mma<T>(acc[b], lo[s], b0, b1);
+                            mma<T>(acc[b], hi[s], b0, b1);
+                        }
+                    }
                 }
-            store8<T>(out + t[m] * ldo + f, left, vec, v);
+            }
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const int r = r0 + 8 * u;
+                if (r >= rows) continue;
+#pragma unroll
+                for (int v = 0; v < 8 / E; v++) {
+                    const int c = fs / E + 4 * v + q;
+                    const int64_t f = f0 + c * E;
+                    float y[E];
+#pragma unroll
+                    for (int e = 0; e < E; e++) {
+                        int b, j;
+                        if constexpr (F32) {
+                            b = TRANS ? e : 2 * v + (e >> 1);
+                            j = TRANS ? v : e & 1;
+                        } else {
+                            b = TRANS ? e & 3 : e >> 1;
+                            j = TRANS ? e >> 2 : e & 1;
+                        }
+                        y[e] = acc[b][2 * u + j] * undo[u];
+                    }
+                    alignas(16) T o[E];
+                    if (base) {
+                        alignas(16) T d[E];
+                        *reinterpret_cast<uint4*>(d) = lds128(bs + r * (FU * 16) + ((c ^ swap_rows(r)) * 16));
+#pragma unroll
+                        for (int e = 0; e < E; e++) o[e] = none ? d[e] : narrow<T>(wide(d[e]) + y[e]);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < E; e++) o[e] = narrow<T>(none ? 0.f : y[e]);
+                    }
+                    T* dst = out + (int64_t)tr.row[r] * ldo + f;
+                    if (ovec && f + E <= f_end) {
+                        *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(o);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < E; e++)
+                            if (f + e < f_end) dst[e] = o[e];
+                    }
+                }
+            }
         }
     }
 }
 
 // ---- weight gradients ------------------------------------------------------------
-// G_i = sum over adapter i's positions of x[t, f] h[p, r].  TRANS = false: G_i stored [rank, F] (dA,
-// with h = dh); true: stored [F, rank] (dB, with x = the gradient of out).  One block per (32 columns,
-// adapter); its warps take 8 positions each in turn and are summed, in their order, through shared
-// memory.  An adapter without positions gets zeros.
+// G_i = sum over adapter i's positions of x[t, f] h[t, r].  TRANS = false: G_i stored [rank, F] (dA,
+// with h = dh); true: stored [F, rank] (dB, with x = the gradient of out).  One block per (FC columns,
+// adapter), 64 positions a stage; four warps side by side along the columns, two along the positions,
+// which are summed through shared memory at the end.  An adapter without positions gets zeros.
+template <typename T, int RB>
+struct WeightCfg {
+    static constexpr int E = kE<T>, RP = 8 * RB, NB = RB == 16 ? 2 : 4;  // blocks of 8 columns a warp
+    static constexpr int FC = 4 * 8 * NB, FU = FC / E, TK = 64;
+    static constexpr int X_BYTES = TK * FC * (int)sizeof(T);
+    // h of a stage: fp32 rows at a pitch of 8 words beyond a multiple of 16; 16 bits: planes hi and lo
+    static constexpr int H_PITCH = sizeof(T) == 4 ? RP * 4 + 32 : RP * 2 + 16;
+    static constexpr int H_BYTES = TK * H_PITCH * (sizeof(T) == 4 ? 1 : 2);
+    static constexpr int NS = 3;
+    static constexpr int RED = 2 * RP * (FC + 4) * 4;
+    static constexpr int SMEM = NS * X_BYTES + 2 * H_BYTES > RED ? NS * X_BYTES + 2 * H_BYTES : RED;
+    static_assert(SMEM <= 220 * 1024, "a block's shared memory");
+};
+
 template <typename T, int RB, bool TRANS>
-__global__ void __launch_bounds__(kWarps * 32) k_weight(Plan plan, const T* __restrict__ x, int64_t ldx,
-                                                        const float* __restrict__ h, int splits, int rank, int64_t F,
-                                                        int64_t T_rows, bool vec, T* __restrict__ out) {
-    constexpr int RP = 8 * RB, RM = RB / 2;  // RM blocks of 16 ranks; lane rows g, g + 8: ranks 2 RM g + ..
-    constexpr bool SP = Io<T>::kSplit;
-    extern __shared__ float red[];  // [kWarps][RP][32]
+__global__ void __launch_bounds__(kThreads) k_weight(Plan plan, const int32_t* __restrict__ index,
+                                                     const T* __restrict__ x, int64_t ldx, const float* h, int splits,
+                                                     int n, int rank, int64_t F, int T_rows, bool xvec,
+                                                     T* __restrict__ out) {
+    using C = WeightCfg<T, RB>;
+    constexpr int E = C::E, RP = C::RP, NB = C::NB, FC = C::FC, FU = C::FU, TK = C::TK, NS = C::NS, RM = RB / 2;
+    constexpr bool F32 = sizeof(T) == 4;
+    constexpr int HV = TK * RP / 4 / kThreads;  // float4 of h a thread stages
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ Scan scan;
+    __shared__ float block_max[kWarps];
+    uint8_t* hs = smem + NS * C::X_BYTES;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
+    const int wf = warp & 3, wt = warp >> 2;
     const int a = blockIdx.y;
-    const int p0 = __ldg(plan.off + a), p1 = __ldg(plan.off + a + 1);
-    const int64_t f0 = (int64_t)blockIdx.x * 32;
-    float acc[RM][4][4];
+    const int64_t f0 = (int64_t)blockIdx.x * FC;
+    wait_for_previous();
+    let_next_start();
+    const int32_t* list;
+    int count;
+    if (plan.perm) {
+        const int p0 = __ldg(plan.off + a);
+        list = plan.perm + p0;
+        count = __ldg(plan.off + a + 1) - p0;
+    } else {
+        count = scan_positions(scan, index, T_rows, n, a);
+        list = scan.list;
+    }
+    const int stages = (count + TK - 1) / TK;
+    const int64_t stride = (int64_t)T_rows * RP;
+
+    float take = 1.f;  // fp16: h's scale
+    if constexpr (std::is_same_v<T, __half>) {
+        float m = 0.f;
+        for (int e = threadIdx.x; e < count * (RP / 4); e += kThreads) {
+            const float4 v = load_h(h + (int64_t)list[e / (RP / 4)] * RP + 4 * (e % (RP / 4)), splits, stride);
+            m = fmaxf(fmaxf(fmaxf(m, fabsf(v.x)), fmaxf(fabsf(v.y), fabsf(v.z))), fabsf(v.w));
+        }
+#pragma unroll
+        for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+        if (lane == 0) block_max[warp] = m;
+        __syncthreads();
+        for (int k = 0; k < kWarps; k++) m = fmaxf(m, block_max[k]);
+        take = half_scale(m);
+    }
+
+    const auto load_x = [&](int i) {
+        uint8_t* xs = smem + (i % NS) * C::X_BYTES;
+        for (int u = threadIdx.x; u < TK * FU; u += kThreads) {
+            const int r = u / FU, c = u % FU, p = i * TK + r;
+            const int64_t f = f0 + c * E;
+            const int to = F32 ? c ^ ((r & 3) << 1) : c ^ (r & 7);
+            stage_unit<T>(xs + r * (FU * 16) + to * 16, x + (p < count ? (int64_t)list[p] * ldx : 0) + f, x,
+                          p < count ? F - f : 0, xvec);
+        }
+        stage_done();
+    };
+    float4 hv[HV];
+    const auto load_h_regs = [&](int i) {
+#pragma unroll
+        for (int k = 0; k < HV; k++) {
+            const int e = threadIdx.x + k * kThreads, r = e / (RP / 4), c = e % (RP / 4), p = i * TK + r;
+            hv[k] = p < count ? load_h(h + (int64_t)list[p] * RP + 4 * c, splits, stride)
+                              : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+    };
+    const auto store_h = [&](int i) {
+        uint8_t* d = hs + (i & 1) * C::H_BYTES;
+#pragma unroll
+        for (int k = 0; k < HV; k++) {
+            const int e = threadIdx.x + k * kThreads, r = e / (RP / 4), c = e % (RP / 4);
+            if constexpr (F32) {
+                *reinterpret_cast<float4*>(d + r * C::H_PITCH + 16 * c) = hv[k];
+            } else {
+                const float v[4] = {hv[k].x * take, hv[k].y * take, hv[k].z * take, hv[k].w * take};
+                const uint2 p = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+                const float2 b0 = unpack2<T>(p.x), b1 = unpack2<T>(p.y);
+                *reinterpret_cast<uint2*>(d + r * C::H_PITCH + 8 * c) = p;
+                *reinterpret_cast<uint2*>(d + (TK + r) * C::H_PITCH + 8 * c) =
+                    make_uint2(pack2<T>(v[0] - b0.x, v[1] - b0.y), pack2<T>(v[2] - b1.x, v[3] - b1.y));
+            }
+        }
+    };
+
+    float acc[RM][NB][4], sum[F32 ? RM : 1][NB][4];
 #pragma unroll
     for (int m = 0; m < RM; m++)
 #pragma unroll
-        for (int b = 0; b < 4; b++)
+        for (int b = 0; b < NB; b++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) acc[m][b][i] = 0.f;
-#pragma unroll 2
-    for (int p = p0 + 8 * warp; p < p1; p += 8 * kWarps) {
-        float xv[2][4], hv[2][2 * RM];
+            for (int k = 0; k < 4; k++) {
+                acc[m][b][k] = 0.f;
+                if (F32 || m == 0) sum[F32 ? m : 0][b][k] = 0.f;
+            }
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-            const int pp = p + q + 4 * j;
-            const int64_t t = __ldg(plan.perm + min(pp, p1 - 1));
-            load_run<T, 4>(x + t * ldx + f0 + 4 * g, pp < p1 ? F - (f0 + 4 * g) : 0, vec, xv[j]);
-            const float* hp = h + (int64_t)min(pp, p1 - 1) * RP + 2 * RM * g;
+    for (int i = 0; i < NS - 1; i++) {
+        if (i < stages) load_x(i);
+        else stage_done();
+    }
+    if (stages > 0) load_h_regs(0);
+    for (int i = 0; i < stages; i++) {
+        store_h(i);  // its buffer was last read two stages ago, before the barrier of the last one
+        stage_wait<NS - 2>();
+        __syncthreads();
+        if (i + NS - 1 < stages) load_x(i + NS - 1);
+        else stage_done();
+        if (i + 1 < stages) load_h_regs(i + 1);
+        const uint8_t* xs = smem + (i % NS) * C::X_BYTES;
+        const uint8_t* hb = hs + (i & 1) * C::H_BYTES;
+        if constexpr (F32) {  // lane rows g, g + 8 of block m: ranks 2 RM g + 2 m, + 1; column 8 .. of the warp: NB g + b
 #pragma unroll
-            for (int r = 0; r < 2 * RM; r++) hv[j][r] = 0.f;
-            if (pp < p1)
-                for (int k = 0; k < splits; k++)
+            for (int s = 0; s < TK / 16; s++) {
+                const int t0 = 32 * wt + 8 * s + q;
+                uint32_t xv[2][NB], hr[2][2 * RM];
 #pragma unroll
-                    for (int r = 0; r < 2 * RM; r += 2) {
-                        const float2 u = __ldg(reinterpret_cast<const float2*>(hp + (int64_t)k * T_rows * RP + r));
-                        hv[j][r] += u.x;
-                        hv[j][r + 1] += u.y;
+                for (int j = 0; j < 2; j++) {
+                    const int t = t0 + 4 * j;
+                    if constexpr (NB == 4) {
+                        const int c = 8 * wf + g;
+                        const uint4 v = lds128(xs + t * (FU * 16) + ((c ^ ((t & 3) << 1)) * 16));
+                        xv[j][0] = v.x, xv[j][1] = v.y, xv[j][2] = v.z, xv[j][3] = v.w;
+                    } else {
+                        const int c = 4 * wf + (g >> 1);
+                        const uint2 v = *reinterpret_cast<const uint2*>(
+                            xs + t * (FU * 16) + ((c ^ ((t & 3) << 1)) * 16) + (g & 1) * 8);
+                        xv[j][0] = v.x, xv[j][1] = v.y;
                     }
-        }
-        FragB<SP> fb[4];
+                    const uint8_t* hp = hb + t * C::H_PITCH + 8 * RM * g;
+                    if constexpr (RM == 1) {
+                        const uint2 v = *reinterpret_cast<const uint2*>(hp);
+                        hr[j][0] = v.x, hr[j][1] = v.y;
+                    } else {
 #pragma unroll
-        for (int b = 0; b < 4; b++) {
-            fb[b].set(0, xv[0][b]);
-            fb[b].set(1, xv[1][b]);
-        }
+                        for (int r = 0; r < 2 * RM; r += 4) {
+                            const uint4 v = lds128(hp + 4 * r);
+                            hr[j][r] = v.x, hr[j][r + 1] = v.y, hr[j][r + 2] = v.z, hr[j][r + 3] = v.w;
+                        }
+                    }
+                }
 #pragma unroll
-        for (int m = 0; m < RM; m++) {
-            FragA<true> fa;
-            fa.set(0, hv[0][2 * m]);
-            fa.set(1, hv[0][2 * m + 1]);
-            fa.set(2, hv[1][2 * m]);
-            fa.set(3, hv[1][2 * m + 1]);
+                for (int m = 0; m < RM; m++) {
+                    const Split fa = split_a(hr[0][2 * m], hr[0][2 * m + 1], hr[1][2 * m], hr[1][2 * m + 1]);
 #pragma unroll
-            for (int b = 0; b < 4; b++) mma_split<true, SP>(acc[m][b], fa, fb[b]);
+                    for (int b = 0; b < NB; b++) mma_split(acc[m][b], fa, xv[0][b], xv[1][b]);
+                }
+            }
+#pragma unroll
+            for (int m = 0; m < RM; m++)
+#pragma unroll
+                for (int b = 0; b < NB; b++)
+#pragma unroll
+                    for (int k = 0; k < 4; k++) sum[m][b][k] += acc[m][b][k], acc[m][b][k] = 0.f;
+        } else {
+            const int lr = lane & 7, lm = lane >> 3;
+#pragma unroll
+            for (int s = 0; s < TK / 32; s++) {
+                const int t0 = 32 * wt + 16 * s;
+                uint32_t fb[NB][2];
+#pragma unroll
+                for (int b = 0; b < NB; b += 2) {
+                    uint32_t v[4];
+                    const int t = t0 + lr + 8 * (lm & 1), c = NB * wf + b + (lm >> 1);
+                    ldmatrix4_trans(v, xs + t * (FU * 16) + ((c ^ (t & 7)) * 16));
+                    fb[b][0] = v[0], fb[b][1] = v[1], fb[b + 1][0] = v[2], fb[b + 1][1] = v[3];
+                }
+#pragma unroll
+                for (int m = 0; m < RM; m++) {
+                    uint32_t fh[4], fl[4];
+                    const uint8_t* p = hb + (t0 + lr + 8 * (lm >> 1)) * C::H_PITCH + (2 * m + (lm & 1)) * 16;
+                    ldmatrix4_trans(fh, p);
+                    ldmatrix4_trans(fl, p + TK * C::H_PITCH);
+#pragma unroll
+                    for (int b = 0; b < NB; b++) {
+                        mma<T>(acc[m][b], fl, fb[b][0], fb[b][1]);
+                        mma<T>(acc[m][b], fh, fb[b][0], fb[b][1]);
+                    }
+                }
+            }
         }
     }
-    float* mine = red + warp * RP * 32;
+    stage_wait<0>();
+    __syncthreads();
+    constexpr int RS = FC + 4;
+    float* red = reinterpret_cast<float*>(smem);  // [2][RP][RS]
+    const float undo = 1.f / take;
 #pragma unroll
     for (int m = 0; m < RM; m++)
 #pragma unroll
-        for (int b = 0; b < 4; b++)
+        for (int b = 0; b < NB; b++)
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                mine[(2 * RM * g + 2 * m + (i >> 1)) * 32 + 4 * (2 * q + (i & 1)) + b] = acc[m][b][i];
+            for (int k = 0; k < 4; k++) {
+                const int c = 2 * q + (k & 1);
+                const int r = F32 ? 2 * RM * g + 2 * m + (k >> 1) : 16 * m + g + 8 * (k >> 1);
+                const int f = 8 * NB * wf + (F32 ? NB * c + b : 8 * b + c);
+                if constexpr (F32) red[(wt * RP + r) * RS + f] = sum[m][b][k];
+                else red[(wt * RP + r) * RS + f] = acc[m][b][k] * undo;
+            }
     __syncthreads();
     T* dst = out + (int64_t)a * rank * F;
-    for (int e = threadIdx.x; e < 32 * rank; e += kWarps * 32) {
-        const int r = TRANS ? e % rank : e / 32, c = TRANS ? e / rank : e % 32;
+    for (int e = threadIdx.x; e < FC * rank; e += kThreads) {
+        const int r = TRANS ? e % rank : e / FC, c = TRANS ? e / rank : e % FC;
         if (f0 + c >= F) continue;
-        float v = 0.f;
-#pragma unroll
-        for (int k = 0; k < kWarps; k++) v += red[(k * RP + r) * 32 + c];
-        dst[TRANS ? (f0 + c) * rank + r : (int64_t)r * F + f0 + c] = Io<T>::narrow(v);
+        dst[TRANS ? (f0 + c) * rank + r : (int64_t)r * F + f0 + c] =
+            narrow<T>(red[r * RS + c] + red[(RP + r) * RS + c]);
     }
 }
 
@@ -646,12 +1059,14 @@ __global__ void __launch_bounds__(kWarps * 32) k_weight(Plan plan, const T* __re
 
 struct Shape {
     int64_t T, K, N;
-    int n, rank, rb, mt;
-    int64_t tiles_max;
+    int n, rank, rb, wm;
+    bool planned;            // by k_plan; else each block finds its tile
+    int64_t tiles;           // blocks along x: at least the tiles there are
     int splits_k, splits_n;  // blocks per tile that share the sum over K, over N
 };
 
 int64_t align256(int64_t b) { return (b + 255) & ~int64_t(255); }
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Places of the workspace; bytes = its size.
 struct Layout {
@@ -666,17 +1081,21 @@ int check_shape(int64_t T, int32_t n, int32_t rank, int64_t K, int64_t N) {
     return ENGRAM_OK;
 }
 
+constexpr int kSms = 148;
+
 Shape shape_of(int64_t T, int n, int rank, int64_t K, int64_t N) {
     Shape s;
     s.T = T, s.K = K, s.N = N, s.n = n, s.rank = rank;
     s.rb = rank_blocks(rank);
     const int64_t groups = T < (int64_t)n + 1 ? T : (int64_t)n + 1;
-    s.mt = (s.rb < 16 && groups > 0 && T / groups >= 64) ? 2 : 1;
-    const int bm = 16 * s.mt;
-    s.tiles_max = (T + (bm - 1) * groups) / bm;
+    s.wm = groups > 0 && T / groups >= 32 ? 8 : 1;
+    const int bm = 16 * s.wm;
+    s.planned = T > kScanMax;
+    const int64_t most = (T + (bm - 1) * groups) / bm;  // tiles there can be
+    s.tiles = s.planned ? most : T;
     const auto splits = [&](int64_t width) {
-        const int64_t want = s.tiles_max > 0 ? (2 * 148) / s.tiles_max : 1, most = (width + 255) / 256;
-        const int64_t k = want < most ? want : most;
+        const int64_t want = most > 0 ? ceil_div(2 * kSms, most) : 1, can = ceil_div(width, 512);
+        const int64_t k = want < can ? want : can;
         return (int)(k < 1 ? 1 : k > 16 ? 16 : k);
     };
     s.splits_k = splits(K);
@@ -685,89 +1104,94 @@ Shape shape_of(int64_t T, int n, int rank, int64_t K, int64_t N) {
 }
 
 Layout layout_of(const Shape& s, bool backward) {
-    Layout l;
+    Layout l = {};
     int64_t at = 0;
     const auto take = [&](int64_t bytes) {
         const int64_t here = at;
         at += align256(bytes);
         return here;
     };
-    l.off = take((int64_t)(s.n + 2) * 4);
-    l.perm = take(s.T * 4);
-    l.tiles = take(4);
-    l.tile = take(s.tiles_max * (int64_t)sizeof(Tile));
+    if (s.planned) {
+        l.off = take((int64_t)(s.n + 2) * 4);
+        l.perm = take(s.T * 4);
+        l.tiles = take(4);
+        l.tile = take(s.tiles * (int64_t)sizeof(Tile));
+    }
     l.h = take((int64_t)s.splits_k * s.T * 8 * s.rb * 4);
-    l.dh = backward ? take((int64_t)s.splits_n * s.T * 8 * s.rb * 4) : 0;
+    if (backward) l.dh = take((int64_t)s.splits_n * s.T * 8 * s.rb * 4);
     l.bytes = at;
     return l;
 }
 
-Plan plan_at(uint8_t* ws, const Layout& l) {
+Plan plan_at(uint8_t* ws, const Shape& s, const Layout& l) {
+    if (!s.planned) return Plan{};
     return Plan{reinterpret_cast<int32_t*>(ws + l.off), reinterpret_cast<int32_t*>(ws + l.perm),
                 reinterpret_cast<int32_t*>(ws + l.tiles), reinterpret_cast<Tile*>(ws + l.tile)};
 }
 
-// Raises the kernel's limit of dynamic shared memory where the launch needs it.
-bool allow_smem(const void* kernel, int bytes) {
-    return bytes <= 48 * 1024 ||
-           cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess;
-}
-
-int launched() {
+// Starts a kernel; after = true: it may start while the launch before it still runs (it waits for that
+// one's results itself, griddepcontrol.wait), which hides the start and its first loads.
+template <typename... P, typename... A>
+int start(void (*kernel)(P...), dim3 grid, int threads, int smem, bool after, cudaStream_t st, A... args) {
+    if (smem > 48 * 1024 &&
+        cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+        return ENGRAM_ERR_CUDA;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = after ? 1 : 0;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, P(args)...);
     count_launches(1);
-    return cudaGetLastError() == cudaSuccess ? ENGRAM_OK : ENGRAM_ERR_CUDA;
+    return e == cudaSuccess && cudaGetLastError() == cudaSuccess ? ENGRAM_OK : ENGRAM_ERR_CUDA;
 }
 
 int run_plan(const Shape& s, const int32_t* index, const Plan& plan, cudaStream_t st) {
-    const int64_t per = (s.T + 127) / 128;
-    const int chunk = (int)((per + kPlanThreads - 1) / kPlanThreads) * kPlanThreads;
-    const int smem = (3 * s.n + 4) * 4;
-    if (!allow_smem((const void*)k_plan, smem)) return ENGRAM_ERR_CUDA;
-    k_plan<<<(unsigned)((s.T + chunk - 1) / chunk), kPlanThreads, smem, st>>>(index, (int)s.T, s.n, chunk, 16 * s.mt,
-                                                                              plan);
-    return launched();
+    if (!s.planned) return ENGRAM_OK;
+    const int chunk = (int)ceil_div(ceil_div(s.T, 128), kPlanThreads) * kPlanThreads;
+    return start(k_plan, dim3((unsigned)ceil_div(s.T, chunk)), kPlanThreads, (3 * s.n + 4) * 4, false, st, index,
+                 (int)s.T, s.n, chunk, 16 * s.wm, plan);
 }
 
-template <typename T, int RB, int MT, bool TRANS>
-int run_shrink(const Shape& s, const Plan& plan, const T* x, int64_t ldx, const T* w, const float* scale, int64_t K,
-               int splits, float* h, cudaStream_t st) {
-    constexpr int E = 16 / sizeof(T), CH = 4 * E;
-    const int64_t step = kWarps * CH, k_split = ((K + splits - 1) / splits + step - 1) / step * step;
-    const bool vec = aligned16(x) && ldx % E == 0 && K % E == 0 && (TRANS || aligned16(w));
-    const bool rvec = TRANS && aligned16(w) && s.rank % RB == 0;
-    const int smem = kWarps * 16 * MT * 8 * RB * 4;
-    if (!allow_smem((const void*)k_shrink<T, RB, MT, TRANS>, smem)) return ENGRAM_ERR_CUDA;
-    k_shrink<T, RB, MT, TRANS><<<dim3((unsigned)s.tiles_max, splits), kWarps * 32, smem, st>>>(
-        plan, x, ldx, w, scale, s.n, s.rank, K, k_split, s.T, vec, rvec, h);
-    return launched();
+template <typename T>
+bool row_units(const T* p, int64_t ld) {  // every row starts on 16 bytes
+    return aligned16(p) && ld % kE<T> == 0;
 }
 
-template <typename T, int RB, int MT, bool TRANS>
-int run_expand(const Shape& s, const Plan& plan, const float* h, int splits, const T* w, int64_t F, const T* base,
-               int64_t ldb, T* out, int64_t ldo, cudaStream_t st) {
-    constexpr int E = 16 / sizeof(T);
-    // columns of a block: whole passes of its warps, about four blocks an SM
-    const int64_t step = 32 * kWarps;
-    const int64_t passes = (F + step - 1) / step, want = s.tiles_max > 0 ? (4 * 148 + s.tiles_max - 1) / s.tiles_max : 1;
-    const int64_t blocks = want < passes ? want : passes;
-    const int64_t f_block = (passes + blocks - 1) / blocks * step;
-    const bool vec = (!base || (aligned16(base) && ldb % E == 0)) && aligned16(out) && ldo % E == 0 && F % 8 == 0;
-    const bool wvec = aligned16(w) && (TRANS ? F % 4 == 0 : s.rank % 4 == 0);
-    k_expand<T, RB, MT, TRANS><<<dim3((unsigned)s.tiles_max, (unsigned)((F + f_block - 1) / f_block)), kWarps * 32, 0,
-                                 st>>>(plan, h, splits, w, s.n, s.rank, F, f_block, s.T, base, ldb, out, ldo, vec,
-                                       wvec);
-    return launched();
+template <typename T, int RB, int WM, bool TRANS>
+int run_shrink(const Shape& s, const Plan& plan, const int32_t* index, const T* x, int64_t ldx, const T* w,
+               const float* scale, int64_t K, int splits, float* h, bool after, cudaStream_t st) {
+    using C = ShrinkCfg<T, RB, WM, TRANS>;
+    const int64_t k_split = ceil_div(ceil_div(K, splits), C::KC) * C::KC;
+    return start(k_shrink<T, RB, WM, TRANS>, dim3((unsigned)s.tiles, (unsigned)splits), kThreads, C::SMEM, after, st,
+                 plan, index, x, ldx, w, scale, s.n, s.rank, K, k_split, (int)s.T, row_units(x, ldx),
+                 row_units(w, TRANS ? s.rank : K), h);
+}
+
+template <typename T, int RB, int WM, bool TRANS>
+int run_expand(const Shape& s, const Plan& plan, const int32_t* index, const float* h, int splits, const T* w,
+               int64_t F, const T* base, int64_t ldb, T* out, int64_t ldo, cudaStream_t st) {
+    using C = ExpandCfg<T, RB, WM, TRANS>;
+    // columns of a block: whole stages, for about four blocks an SM
+    const int64_t passes = ceil_div(F, C::FS), tiles = s.planned ? s.tiles : ceil_div(s.T, 16 * WM);
+    const int64_t want = ceil_div(4 * kSms, tiles), blocks = want < passes ? want : passes;
+    const int64_t f_block = ceil_div(passes, blocks) * C::FS;
+    return start(k_expand<T, RB, WM, TRANS>, dim3((unsigned)s.tiles, (unsigned)ceil_div(F, f_block)), kThreads, C::SMEM,
+                 true, st, plan, index, h, splits, w, s.n, s.rank, F, f_block, (int)s.T, base, ldb, out, ldo,
+                 base && row_units(base, ldb), row_units(w, TRANS ? F : s.rank), row_units((const T*)out, ldo));
 }
 
 template <typename T, int RB, bool TRANS>
-int run_weight(const Shape& s, const Plan& plan, const T* x, int64_t ldx, const float* h, int splits, int64_t F,
-               T* out, cudaStream_t st) {
-    const bool vec = aligned16(x) && ldx % 4 == 0 && F % 4 == 0;
-    const int smem = kWarps * 8 * RB * 32 * 4;
-    if (!allow_smem((const void*)k_weight<T, RB, TRANS>, smem)) return ENGRAM_ERR_CUDA;
-    k_weight<T, RB, TRANS><<<dim3((unsigned)((F + 31) / 32), s.n), kWarps * 32, smem, st>>>(
-        plan, x, ldx, h, splits, s.rank, F, s.T, vec, out);
-    return launched();
+int run_weight(const Shape& s, const Plan& plan, const int32_t* index, const T* x, int64_t ldx, const float* h,
+               int splits, int64_t F, T* out, cudaStream_t st) {
+    using C = WeightCfg<T, RB>;
+    return start(k_weight<T, RB, TRANS>, dim3((unsigned)ceil_div(F, C::FC), (unsigned)s.n), kThreads, C::SMEM, true, st,
+                 plan, index, x, ldx, h, splits, s.n, s.rank, F, (int)s.T, row_units(x, ldx), out);
 }
 
 struct Args {
@@ -780,52 +1204,56 @@ struct Args {
     cudaStream_t st;
 };
 
-template <typename T, int RB, int MT>
+template <typename T, int RB, int WM>
 int forward(const Shape& s, const Layout& l, const Args& g) {
-    const Plan plan = plan_at(g.ws, l);
+    const Plan plan = plan_at(g.ws, s, l);
     float* h = reinterpret_cast<float*>(g.ws + l.h);
     int e = run_plan(s, g.index, plan, g.st);
     if (!e)
-        e = run_shrink<T, RB, MT, false>(s, plan, (const T*)g.x, g.ldx, (const T*)g.a, g.scale, s.K, s.splits_k, h,
-                                         g.st);
+        e = run_shrink<T, RB, WM, false>(s, plan, g.index, (const T*)g.x, g.ldx, (const T*)g.a, g.scale, s.K,
+                                         s.splits_k, h, s.planned, g.st);
     if (!e)
-        e = run_expand<T, RB, MT, false>(s, plan, h, s.splits_k, (const T*)g.b, s.N, (const T*)g.base, g.ldbase,
-                                         (T*)g.out, g.ldout, g.st);
+        e = run_expand<T, RB, WM, false>(s, plan, g.index, h, s.splits_k, (const T*)g.b, s.N, (const T*)g.base,
+                                         g.ldbase, (T*)g.out, g.ldout, g.st);
     return e;
 }
 
-template <typename T, int RB, int MT>
+template <typename T, int RB, int WM>
 int backward(const Shape& s, const Layout& l, const Args& g) {
-    const Plan plan = plan_at(g.ws, l);
+    const Plan plan = plan_at(g.ws, s, l);
     float *h = reinterpret_cast<float*>(g.ws + l.h), *dh = reinterpret_cast<float*>(g.ws + l.dh);
     int e = run_plan(s, g.index, plan, g.st);
-    if (!e && (g.dx || g.da))
-        e = run_shrink<T, RB, MT, true>(s, plan, (const T*)g.grad, g.ldgrad, (const T*)g.b, g.scale, s.N, s.splits_n,
-                                        dh, g.st);
+    bool after = s.planned;
+    if (!e && (g.dx || g.da)) {
+        e = run_shrink<T, RB, WM, true>(s, plan, g.index, (const T*)g.grad, g.ldgrad, (const T*)g.b, g.scale, s.N,
+                                        s.splits_n, dh, after, g.st);
+        after = true;
+    }
     if (!e && g.dx)
-        e = run_expand<T, RB, MT, true>(s, plan, dh, s.splits_n, (const T*)g.a, s.K, (const T*)g.base, g.ldbase,
-                                        (T*)g.dx, g.lddx, g.st);
+        e = run_expand<T, RB, WM, true>(s, plan, g.index, dh, s.splits_n, (const T*)g.a, s.K, (const T*)g.base,
+                                        g.ldbase, (T*)g.dx, g.lddx, g.st);
     if (!e && g.da)
-        e = run_weight<T, RB, false>(s, plan, (const T*)g.x, g.ldx, dh, s.splits_n, s.K, (T*)g.da, g.st);
+        e = run_weight<T, RB, false>(s, plan, g.index, (const T*)g.x, g.ldx, dh, s.splits_n, s.K, (T*)g.da, g.st);
     if (!e && g.db)
-        e = run_shrink<T, RB, MT, false>(s, plan, (const T*)g.x, g.ldx, (const T*)g.a, g.scale, s.K, s.splits_k, h,
-                                         g.st);
+        e = run_shrink<T, RB, WM, false>(s, plan, g.index, (const T*)g.x, g.ldx, (const T*)g.a, g.scale, s.K,
+                                         s.splits_k, h, after, g.st);
     if (!e && g.db)
-        e = run_weight<T, RB, true>(s, plan, (const T*)g.grad, g.ldgrad, h, s.splits_k, s.N, (T*)g.db, g.st);
+        e = run_weight<T, RB, true>(s, plan, g.index, (const T*)g.grad, g.ldgrad, h, s.splits_k, s.N, (T*)g.db, g.st);
     return e;
 }
 
 template <typename T>
 int by_rank(const Shape& s, const Layout& l, const Args& g, bool back) {
-#define ENGRAM_CASE(RB, MT) \
-    if (s.rb == RB && s.mt == MT) return back ? backward<T, RB, MT>(s, l, g) : forward<T, RB, MT>(s, l, g);
+#define ENGRAM_CASE(RB, WM) \
+    if (s.rb == RB && s.wm == WM) return back ? backward<T, RB, WM>(s, l, g) : forward<T, RB, WM>(s, l, g);
     ENGRAM_CASE(2, 1)
-    ENGRAM_CASE(2, 2)
+    ENGRAM_CASE(2, 8)
     ENGRAM_CASE(4, 1)
-    ENGRAM_CASE(4, 2)
+    ENGRAM_CASE(4, 8)
     ENGRAM_CASE(8, 1)
-    ENGRAM_CASE(8, 2)
+    ENGRAM_CASE(8, 8)
     ENGRAM_CASE(16, 1)
+    ENGRAM_CASE(16, 8)
 #undef ENGRAM_CASE
     return ENGRAM_ERR_RANGE;
 }
