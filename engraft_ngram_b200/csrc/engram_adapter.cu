@@ -13,8 +13,10 @@
 // What bounds them is the bytes of x, base, grad and out: 2 rank flops for each
 // of their elements is below what mma.sync gives at those bytes a second.  So
 // each block streams its rows through a ring of shared-memory stages filled by
-// cp.async (rows are gathered, and 16-byte pieces of any row will do), with two or
-// three stages in flight, and the products are mma.sync from there.  16-bit types
+// cp.async, 16 bytes a thread from addresses held in registers (bulk copies of whole
+// row pieces are issued one lane at a time, and cost more instructions than that);
+// rows that do not start on 16 bytes, and the last stage, take a slower loop.  The
+// products are mma.sync from there.  16-bit types
 // use m16n8k16 in their own type; fp32 uses m16n8k8 TF32 on split operands,
 // x = hi + lo with hi rounded to the 11 significant bits of TF32: hi hi + hi lo +
 // lo hi, the dropped term being 2^-24 of the product.
@@ -26,6 +28,8 @@
 // 5e-7 with it.
 #include <type_traits>
 
+#include <cooperative_groups.h>
+
 #include "engram_common.cuh"
 
 using namespace engram;
@@ -34,21 +38,23 @@ namespace {
 
 constexpr int kThreads = 256, kWarps = 8;
 constexpr int kPlanThreads = 1024;
-constexpr int kScanMax = 1024;       // positions up to which a block finds its tile by itself
+constexpr int kScanMax = 1024;       // positions and
+constexpr int kScanAdapters = 2048;  // adapters up to which a block finds its tile by itself
 constexpr int kMaxAdapters = 16384;  // k_plan counts them in shared memory
 constexpr int kMaxRank = 128;
 
 // ---- the plan ----------------------------------------------------------------
 // int32 arrays in the workspace.  off[i] = first place of adapter i in the grouped
 // order, off[n] = first place of the positions without an adapter, off[n+1] = T;
-// perm[p] = position; tile k covers places [start, start + rows) of one adapter.
+// perm[p] = position; tile k covers places [start, start + rows) of one adapter.  Without k_plan (few
+// positions) there is no off and no count: tile k has its own places, from k BM on, and may be empty.
 struct Tile {
     int32_t adapter, start, rows, pad;
 };
 struct Plan {
     int32_t* off;    // [n + 2]
     int32_t* perm;   // [T]
-    int32_t* tiles;  // [1]: number of tiles
+    int32_t* tiles;  // [1]: number of tiles; null: as many as blocks
     Tile* tile;      // [max tiles]
 };
 
@@ -151,8 +157,9 @@ __global__ void __launch_bounds__(kPlanThreads) k_plan(const int32_t* __restrict
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-// Up to kScanMax positions need no plan: a block looks through all indexes itself.  List, in ascending
-// order, of the positions with adapter a (n: without one); every thread of the block calls it.
+// Few positions need no launch for the plan: each block of the first launch looks through all indexes
+// itself, and writes its tile down for the launches after it.  List, in ascending order, of the positions
+// with adapter a (n: without one); every thread of the block calls it.
 struct Scan {
     int32_t list[kScanMax];
     int32_t warp_count[kWarps];
@@ -178,35 +185,65 @@ __device__ __forceinline__ int scan_positions(Scan& s, const int32_t* __restrict
     return total;
 }
 
-// The positions of a block's tile.  With a plan: tile blockIdx.x of it.  Without: blockIdx.x is a
-// position, and the block whose position is its adapter's 0th, BM-th, ... takes that tile.
+// The positions of a block's tile.
 template <int BM>
 struct TileRows {
-    Scan scan;
     int32_t row[BM];
-    int32_t first;
+    int32_t adapter, first, rows;
 };
+struct FindTile {  // used by the first launch only, where its stages come to stand later
+    Scan scan;
+    int32_t tiles[kScanAdapters + 1];
+    int32_t warp_sum[kWarps];
+};
+
+// Tile blockIdx.x in the order of the adapters, found without a plan.
 template <int BM>
-__device__ __forceinline__ bool find_tile(TileRows<BM>& r, const Plan& plan, const int32_t* __restrict__ index, int T,
-                                          int n, int& adapter, int& rows) {
-    if (plan.perm) {
-        if ((int)blockIdx.x >= __ldg(plan.tiles)) return false;
-        const Tile t = plan.tile[blockIdx.x];
-        adapter = t.adapter;
-        rows = t.rows;
-        for (int i = threadIdx.x; i < BM; i += kThreads) r.row[i] = __ldg(plan.perm + t.start + min(i, t.rows - 1));
-    } else {
-        const int t = blockIdx.x;
-        adapter = clamp_adapter(__ldg(index + t), n);
-        const int total = scan_positions(r.scan, index, T, n, adapter);
-        for (int i = threadIdx.x; i < total; i += kThreads)
-            if (r.scan.list[i] == t) r.first = i;
+__device__ __forceinline__ void find_tile(FindTile& f, TileRows<BM>& r, const int32_t* __restrict__ index, int T, int n) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, k = blockIdx.x;
+    for (int i = tid; i <= n; i += kThreads) f.tiles[i] = 0;
+    if (tid == 0) r.adapter = -1, r.first = r.rows = 0;
+    __syncthreads();
+    for (int t = tid; t < T; t += kThreads) atomicAdd(f.tiles + clamp_adapter(__ldg(index + t), n), 1);
+    __syncthreads();
+    int before = 0;  // tiles of the adapters so far
+    for (int i0 = 0; i0 <= n; i0 += kThreads) {
+        const int i = i0 + tid, count = i <= n ? f.tiles[i] : 0, mine = (count + BM - 1) / BM;
+        int sum = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, sum, d);
+            if (lane >= d) sum += u;
+        }
+        if (lane == 31) f.warp_sum[warp] = sum;
         __syncthreads();
-        const int first = r.first;
-        if (first % BM) return false;
-        rows = min(BM, total - first);
-        for (int i = threadIdx.x; i < BM; i += kThreads) r.row[i] = r.scan.list[first + min(i, rows - 1)];
+        int at = before + sum - mine;
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) {
+            if (w < warp) at += f.warp_sum[w];
+            before += f.warp_sum[w];
+        }
+        if (k >= at && k < at + mine) {
+            r.adapter = i;
+            r.first = (k - at) * BM;
+            r.rows = min(BM, count - r.first);
+        }
+        __syncthreads();
     }
+    if (r.adapter < 0) return;
+    scan_positions(f.scan, index, T, n, r.adapter);
+    for (int i = tid; i < BM; i += kThreads) r.row[i] = f.scan.list[r.first + min(i, r.rows - 1)];
+    __syncthreads();
+}
+
+// The block's tile from the plan; false: there is none.
+template <int BM>
+__device__ __forceinline__ bool read_tile(TileRows<BM>& r, const Plan& plan) {
+    if (plan.tiles && (int)blockIdx.x >= *plan.tiles) return false;
+    const Tile t = plan.tile[blockIdx.x];
+    if (t.rows == 0) return false;
+    for (int i = threadIdx.x; i < BM; i += kThreads) r.row[i] = plan.perm[t.start + min(i, t.rows - 1)];
+    if (threadIdx.x == 0) r.adapter = t.adapter, r.rows = t.rows;
     __syncthreads();
     return true;
 }
@@ -243,7 +280,7 @@ template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t u) {
     return __half22float2(*reinterpret_cast<const __half2*>(&u));
 }
 
-__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
 // One 16-byte unit of a stage from src, of which `left` elements exist (the others become zero).
 // vec: src is 16-byte aligned: asynchronous; else element by element.
@@ -252,7 +289,7 @@ __device__ __forceinline__ void stage_unit(uint8_t* dst, const T* src, const T* 
     constexpr int E = kE<T>;
     if (vec) {
         const int bytes = left >= E ? 16 : left > 0 ? (int)left * (int)sizeof(T) : 0;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)),
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)),
                      "l"(bytes ? src : valid), "r"(bytes)
                      : "memory");
     } else {
@@ -265,23 +302,34 @@ __device__ __forceinline__ void stage_unit(uint8_t* dst, const T* src, const T* 
 __device__ __forceinline__ void stage_done() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void stage_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// Units of a row are swapped by its number, so that the rows a fragment reads fall on unlike banks:
-// neighbouring rows (a quarter warp of 16-byte reads takes two) on unlike halves of 128 bytes, eight
-// rows (ldmatrix) on eight units.
-__device__ __forceinline__ int swap_rows(int row) { return ((row & 1) << 2) | ((row >> 1) & 3); }
+// The units of a stage's ROWS x U that a thread copies: a fixed column, and rows 256 / U apart.
+template <typename T, int ROWS, int U>
+struct Units {
+    static constexpr int N = (ROWS * U + kThreads - 1) / kThreads, STEP = kThreads / U;
+    static_assert(kThreads % U == 0, "a thread keeps its column");
+    const T* src[N];
+    uint32_t bytes[N];  // 16, or 0: the unit becomes zero
+    static __device__ __forceinline__ int row(int k) { return (int)threadIdx.x / U + k * STEP; }
+    static __device__ __forceinline__ int column() { return (int)threadIdx.x % U; }
+    static __device__ __forceinline__ bool mine(int k) { return ROWS % STEP == 0 || row(k) < ROWS; }
+    __device__ __forceinline__ void copy(int k, uint32_t dst, int64_t offset) const {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src[k] + offset), "r"(bytes[k])
+                     : "memory");
+    }
+};
 
 __device__ __forceinline__ uint4 lds128(const void* p) { return *reinterpret_cast<const uint4*>(p); }
 
 __device__ __forceinline__ void ldmatrix4(uint32_t* r, const void* p) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(smem_addr(p))
+                 : "r"(smem_u32(p))
                  : "memory");
 }
 __device__ __forceinline__ void ldmatrix4_trans(uint32_t* r, const void* p) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(smem_addr(p))
+                 : "r"(smem_u32(p))
                  : "memory");
 }
 
@@ -342,24 +390,28 @@ __device__ __forceinline__ void mma_split(float* d, const Split& a, uint32_t b0,
 // share the columns and are summed, in their order, through shared memory.  A chunk is 64 bytes of a
 // row, two steps of the MMA.  fp32 fragments come as 16-byte reads: a lane holds columns 4 q ..
 // 4 q + 3 of its row, of which step s takes 2 s and 2 s + 1 (the order inside a sum is free as long as
-// both operands agree).
+// both operands agree).  Rows are padded so that those reads (two rows of 64 bytes a quarter warp: 64
+// bytes) and ldmatrix (eight rows of 16: 16 bytes) meet no bank twice.
 template <typename T, int RB, int WM, bool TRANS>
 struct ShrinkCfg {
-    static constexpr int E = kE<T>, RP = 8 * RB, BM = 16 * WM, WK = kWarps / WM;
+    static constexpr int E = kE<T>, RP = 8 * RB, BM = 16 * WM, WK = kWarps / WM, PAD = sizeof(T) == 4 ? 64 : 16;
     static constexpr int NCH = WM == 1 ? 8 : 4, KC = NCH * 4 * E;  // chunks and columns of a stage
-    static constexpr int X_BYTES = BM * NCH * 64;
-    // rank-consecutive rows are padded: fp32 by 16 bytes (rows 4 apart), 16-bit by 16 (8 rows of ldmatrix)
-    static constexpr int W_PITCH = TRANS ? RP * (int)sizeof(T) + 16 : NCH * 64;
+    static constexpr int X_PITCH = NCH * 64 + PAD, X_BYTES = BM * X_PITCH;
+    static constexpr int W_PITCH = TRANS ? RP * (int)sizeof(T) + 16 : X_PITCH;
     static constexpr int W_BYTES = (TRANS ? KC : RP) * W_PITCH;
     static constexpr int STAGE = X_BYTES + W_BYTES;
-    static constexpr int NS = 4 * STAGE <= 112 * 1024 ? 4 : 3 * STAGE <= 220 * 1024 ? 3 : 2;
+    static constexpr int NS = 3 * STAGE <= 108 * 1024 ? 3 : 2 * STAGE <= 108 * 1024 ? 2 : 3 * STAGE <= 216 * 1024 ? 3 : 2;
     static constexpr int RED = WM == 1 ? kWarps * BM * RP * 4 : 0;
-    static constexpr int SMEM = NS * STAGE > RED ? NS * STAGE : RED;
+    static constexpr int MOST = NS * STAGE > RED ? NS * STAGE : RED;
+    static constexpr int SMEM = MOST > (int)sizeof(FindTile) ? MOST : (int)sizeof(FindTile);
     static_assert(SMEM <= 220 * 1024, "a block's shared memory");
 };
 
+// Where a block finds its tile: k_plan's, found here and written to `plan`, or written by a launch before.
+enum Tiles { PLANNED, FIND };
+
 template <typename T, int RB, int WM, bool TRANS>
-__global__ void __launch_bounds__(kThreads) k_shrink(Plan plan, const int32_t* __restrict__ index,
+__global__ void __launch_bounds__(kThreads) k_shrink(Plan plan, int tiles, const int32_t* __restrict__ index,
                                                      const T* __restrict__ x, int64_t ldx, const T* __restrict__ w,
                                                      const float* __restrict__ scale, int n, int rank, int64_t K,
                                                      int64_t k_split, int T_rows, bool xvec, bool wvec,
@@ -371,37 +423,72 @@ __global__ void __launch_bounds__(kThreads) k_shrink(Plan plan, const int32_t* _
     __shared__ TileRows<BM> tr;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
     const int wm = warp % WM, wk = warp / WM;
-    wait_for_previous();
-    let_next_start();
-    int adapter, rows;
-    if (!find_tile<BM>(tr, plan, index, T_rows, n, adapter, rows) || adapter >= n) return;
+    if (tiles == FIND) {
+        let_next_start();
+        find_tile<BM>(*reinterpret_cast<FindTile*>(smem), tr, index, T_rows, n);
+        if (blockIdx.y == 0) {
+            for (int i = threadIdx.x; i < tr.rows; i += kThreads) plan.perm[blockIdx.x * BM + i] = tr.row[i];
+            if (threadIdx.x == 0) plan.tile[blockIdx.x] = Tile{tr.adapter, (int)blockIdx.x * BM, tr.rows, 0};
+        }
+        if (tr.rows == 0 || tr.adapter >= n) return;
+        __syncthreads();  // the scan's memory becomes the stages'
+    } else {
+        wait_for_previous();
+        let_next_start();
+        if (!read_tile<BM>(tr, plan) || tr.adapter >= n) return;
+    }
+    const int adapter = tr.adapter, rows = tr.rows;
     const T* wi = w + (int64_t)adapter * rank * K;
     const int64_t k_begin = blockIdx.y * k_split, k_end = k_begin + k_split < K ? k_begin + k_split : K;
     const int stages = k_begin < k_end ? (int)((k_end - k_begin + KC - 1) / KC) : 0;
 
+    constexpr int XU = NCH * 4, WU = TRANS ? RP / E : NCH * 4, WR = TRANS ? KC : RP;
+    Units<T, BM, XU> ux;
+    Units<T, WR, WU> uw;
+#pragma unroll
+    for (int k = 0; k < ux.N; k++) {
+        const int r = ux.row(k);
+        ux.src[k] = x + (int64_t)tr.row[min(r, BM - 1)] * ldx + k_begin + ux.column() * E;
+        ux.bytes[k] = r < rows ? 16 : 0;
+    }
+#pragma unroll
+    for (int k = 0; k < uw.N; k++) {
+        const int r = uw.row(k), c = uw.column() * E;
+        const bool real = TRANS ? c < rank : r < rank;
+        uw.src[k] = !real ? w : TRANS ? wi + (k_begin + r) * rank + c : wi + (int64_t)r * K + k_begin + c;
+        uw.bytes[k] = real ? 16 : 0;
+    }
     const auto load = [&](int i) {
         uint8_t* xs = smem + (i % NS) * C::STAGE;
         uint8_t* ws = xs + C::X_BYTES;
-        const int64_t k0 = k_begin + (int64_t)i * KC;
-        for (int u = threadIdx.x; u < BM * NCH * 4; u += kThreads) {
-            const int r = u / (NCH * 4), c = u % (NCH * 4);
-            const int64_t k = k0 + c * E;
-            stage_unit<T>(xs + r * (NCH * 64) + ((c ^ swap_rows(r)) * 16), x + (int64_t)tr.row[r] * ldx + k, x,
-                          r < rows ? k_end - k : 0, xvec);
-        }
-        if constexpr (!TRANS) {
-            for (int u = threadIdx.x; u < RP * NCH * 4; u += kThreads) {
-                const int r = u / (NCH * 4), c = u % (NCH * 4);
-                const int64_t k = k0 + c * E;
-                stage_unit<T>(ws + r * C::W_PITCH + ((c ^ swap_rows(r)) * 16), wi + (int64_t)r * K + k, w,
-                              r < rank ? k_end - k : 0, wvec);
-            }
+        const int64_t k0 = k_begin + (int64_t)i * KC, left = k_end - k0;
+        if (xvec && left >= KC) {
+            const uint32_t to = smem_u32(xs) + ux.row(0) * C::X_PITCH + ux.column() * 16;
+#pragma unroll
+            for (int k = 0; k < ux.N; k++)
+                if (ux.mine(k)) ux.copy(k, to + k * ux.STEP * C::X_PITCH, (int64_t)i * KC);
         } else {
-            constexpr int U = RP / E;
-            for (int u = threadIdx.x; u < KC * U; u += kThreads) {
-                const int r = u / U, c = u % U;
-                stage_unit<T>(ws + r * C::W_PITCH + c * 16, wi + (k0 + r) * rank + c * E, w,
-                              k0 + r < k_end ? rank - c * E : 0, wvec);
+            for (int u = threadIdx.x; u < BM * XU; u += kThreads) {
+                const int r = u / XU, c = u % XU;
+                stage_unit<T>(xs + r * C::X_PITCH + c * 16, x + (int64_t)tr.row[r] * ldx + k0 + c * E, x,
+                              r < rows ? left - c * E : 0, xvec);
+            }
+        }
+        if (wvec && left >= KC) {
+            const uint32_t to = smem_u32(ws) + uw.row(0) * C::W_PITCH + uw.column() * 16;
+#pragma unroll
+            for (int k = 0; k < uw.N; k++)
+                if (uw.mine(k))
+                    uw.copy(k, to + k * uw.STEP * C::W_PITCH, uw.bytes[k] ? (int64_t)i * KC * (TRANS ? rank : 1) : 0);
+        } else {
+            for (int u = threadIdx.x; u < WR * WU; u += kThreads) {
+                const int r = u / WU, c = u % WU;
+                if constexpr (TRANS)
+                    stage_unit<T>(ws + r * C::W_PITCH + c * 16, wi + (k0 + r) * rank + c * E, w,
+                                  r < left ? rank - c * E : 0, wvec);
+                else
+                    stage_unit<T>(ws + r * C::W_PITCH + c * 16, wi + (int64_t)r * K + k0 + c * E, w,
+                                  r < rank ? left - c * E : 0, wvec);
             }
         }
         stage_done();
@@ -428,17 +515,17 @@ __global__ void __launch_bounds__(kThreads) k_shrink(Plan plan, const int32_t* _
         else stage_done();
         const uint8_t* xs = smem + (i % NS) * C::STAGE;
         const uint8_t* ws = xs + C::X_BYTES;
-        for (int ch = wk; ch < NCH; ch += WK) {
+#pragma unroll
+        for (int cc = 0; cc < NCH / WK; cc++) {
+            const int ch = wk + WK * cc;
             if constexpr (F32) {
-                const int r0 = 16 * wm + g, c = 4 * ch + q;
-                const uint4 xa = lds128(xs + r0 * (NCH * 64) + ((c ^ swap_rows(r0)) * 16));
-                const uint4 xb = lds128(xs + (r0 + 8) * (NCH * 64) + ((c ^ swap_rows(r0 + 8)) * 16));
+                const uint8_t* xp = xs + (16 * wm + g) * C::X_PITCH + (4 * ch + q) * 16;
+                const uint4 xa = lds128(xp), xb = lds128(xp + 8 * C::X_PITCH);
                 const Split f0 = split_a(xa.x, xb.x, xa.y, xb.y), f1 = split_a(xa.z, xb.z, xa.w, xb.w);
                 if constexpr (!TRANS) {
 #pragma unroll
                     for (int b = 0; b < RB; b++) {
-                        const int r = 8 * b + g;
-                        const uint4 wv = lds128(ws + r * C::W_PITCH + ((c ^ swap_rows(r)) * 16));
+                        const uint4 wv = lds128(ws + (8 * b + g) * C::W_PITCH + (4 * ch + q) * 16);
                         mma_split(acc[b], f0, wv.x, wv.y);
                         mma_split(acc[b], f1, wv.z, wv.w);
                     }
@@ -469,18 +556,16 @@ __global__ void __launch_bounds__(kThreads) k_shrink(Plan plan, const int32_t* _
 #pragma unroll
                 for (int s = 0; s < 2; s++) {
                     uint32_t fa[4];
-                    const int r0 = 16 * wm + lr + 8 * (lm & 1), c = 4 * ch + 2 * s + (lm >> 1);
-                    ldmatrix4(fa, xs + r0 * (NCH * 64) + ((c ^ swap_rows(r0)) * 16));
+                    ldmatrix4(fa, xs + (16 * wm + lr + 8 * (lm & 1)) * C::X_PITCH + (4 * ch + 2 * s + (lm >> 1)) * 16);
 #pragma unroll
                     for (int b = 0; b < RB; b += 2) {
                         uint32_t fb[4];
-                        if constexpr (!TRANS) {
-                            const int r = 8 * b + lr + 8 * (lm >> 1), cw = 4 * ch + 2 * s + (lm & 1);
-                            ldmatrix4(fb, ws + r * C::W_PITCH + ((cw ^ swap_rows(r)) * 16));
-                        } else {
-                            const int r = 32 * ch + 16 * s + lr + 8 * (lm & 1);
-                            ldmatrix4_trans(fb, ws + r * C::W_PITCH + (b + (lm >> 1)) * 16);
-                        }
+                        if constexpr (!TRANS)
+                            ldmatrix4(fb, ws + (8 * b + lr + 8 * (lm >> 1)) * C::W_PITCH +
+                                              (4 * ch + 2 * s + (lm & 1)) * 16);
+                        else
+                            ldmatrix4_trans(fb, ws + (32 * ch + 16 * s + lr + 8 * (lm & 1)) * C::W_PITCH +
+                                                    (b + (lm >> 1)) * 16);
                         mma<T>(acc[b], fa, fb[0], fb[1]);
                         mma<T>(acc[b + 1], fa, fb[2], fb[3]);
                     }
@@ -538,6 +623,25 @@ __device__ __forceinline__ float4 load_h(const float* h, int splits, int64_t str
     return f;
 }
 
+// The splits' sums into the first, of two arrays, for the launches that read them often.  Rows without an
+// adapter hold nothing and are summed like the others.
+__global__ void __launch_bounds__(kThreads) k_sum_splits(float4* h, int h_splits, float4* dh, int dh_splits,
+                                                         int64_t count4) {
+    wait_for_previous();
+    let_next_start();
+    const int64_t i = blockIdx.x * (int64_t)kThreads + threadIdx.x;
+    float4* p = blockIdx.y ? dh : h;
+    const int splits = blockIdx.y ? dh_splits : h_splits;
+    if (i >= count4 || splits < 2) return;
+    float4 f = p[i];
+#pragma unroll 4
+    for (int k = 1; k < splits; k++) {
+        const float4 u = p[k * count4 + i];
+        f.x += u.x, f.y += u.y, f.z += u.z, f.w += u.w;
+    }
+    p[i] = f;
+}
+
 // 2^(14 - e) for m in [2^e, 2^(e + 1)): brings m into fp16 below 2^15; 1 for zero and for what is not finite.
 __device__ __forceinline__ float half_scale(float m) {
     const int e = (int)((bits_of(m) >> 23) & 255) - 127;
@@ -547,95 +651,139 @@ __device__ __forceinline__ float half_scale(float m) {
 // ---- expand --------------------------------------------------------------------
 // out[t, f] = base[t, f] + sum over ranks of h[t, r] W_i[f, r]; positions without an adapter get base.
 // TRANS = false: W_i = B_i [F, rank]; true: W_i = A_i [rank, F].  base null: zeros.
-// WM = 8: 128 positions, 16 a warp, 64 columns a stage; WM = 1: 16 positions, 256 columns a stage, 32 a
-// warp.  A warp keeps its positions' h fragments in registers.  Columns are dealt to the MMA's so
-// that a lane ends up with whole 16-byte units of rows g and g + 8, and four lanes with 64 consecutive
-// bytes: unit 4 v + q holds, for fp32, columns 2 (b % 2) + j of blocks b = 2 v, 2 v + 1 (TRANS: columns b
-// of MMA column 2 q + v), for 16 bits columns 2 b + j (TRANS: 4 j + b).
-template <typename T, int RB, int WM, bool TRANS>
+// BIG: 128 positions; four warps of 32 along them, two along the columns (fp32 at rank 128, whose h
+// fragments fill the registers: eight of 16).  Else 16 positions and all warps along the columns.  A
+// warp keeps its positions' h fragments in registers and takes 32 columns at a time, dealt to the MMAs
+// so that a lane ends up with whole 16-byte units of its rows and four lanes with 64 consecutive bytes:
+// unit 4 v + q holds, for fp32, columns 2 (b % 2) + j of blocks b = 2 v, 2 v + 1 (TRANS: columns b of MMA
+// column 2 q + v), for 16 bits columns 2 b + j (TRANS: 4 j + b).
+template <typename T, int RB, bool BIG, bool TRANS>
 struct ExpandCfg {
-    static constexpr int E = kE<T>, RP = 8 * RB, BM = 16 * WM, WF = kWarps / WM;
-    // columns of a stage (128 where 256 rows of fp32 factors would not fit twice)
-    static constexpr int FS = WM == 8 ? 64 : RP * (int)sizeof(T) == 512 ? 128 : 256;
-    static constexpr int FU = FS / E;                  // units of a base row
-    static constexpr int B_BYTES = BM * FS * (int)sizeof(T);
-    // B_i rows: fp32 at a pitch of 16 words beyond a multiple of 32, 16-bit dense with swapped units
-    static constexpr int W_PITCH = TRANS ? FS * (int)sizeof(T)
-                                         : sizeof(T) == 4 ? (RP == 16 ? 64 : RP * 4 + 64) : RP * 2;
+    static constexpr int E = kE<T>, RP = 8 * RB, SIZE = sizeof(T), BM = BIG ? 128 : 16;
+    static constexpr int MT = BIG && RP * SIZE < 512 ? 2 : 1, WM = BM / (16 * MT), WF = kWarps / WM;
+    // columns of a stage
+    static constexpr int FS = BIG ? (SIZE == 2 && RB <= 4 ? 128 : 64) : RP * SIZE == 512 ? 128 : 256;
+    static constexpr int FU = FS / E;  // units of a row
+    static constexpr int B_PITCH = FS * SIZE + 64, B_BYTES = BM * B_PITCH;
+    // B_i rows lie in the order in which the lanes of an MMA read them (row_slot), at a pitch that puts the
+    // two rows of a quarter warp's 16-byte reads 64 bytes apart (fp32), the four of a half warp's 8-byte
+    // reads 32 (16 bits).  A_i rows are dense, their units swapped by row number.
+    static constexpr int W_PITCH = TRANS ? FS * SIZE
+                                         : SIZE == 4 ? (RP == 16 ? 64 : RP * 4 + 64) : (RP == 16 ? 32 : RP * 2 + 32);
     static constexpr int W_BYTES = (TRANS ? RP : FS) * W_PITCH;
     static constexpr int STAGE = B_BYTES + W_BYTES;
-    static constexpr int NS = 4 * STAGE <= 112 * 1024 ? 4 : 3 * STAGE <= 220 * 1024 ? 3 : 2;
+    static constexpr int NS = 3 * STAGE <= 108 * 1024 ? 3 : 2 * STAGE <= 108 * 1024 ? 2 : 3 * STAGE <= 216 * 1024 ? 3 : 2;
     static constexpr int SMEM = NS * STAGE;
     static_assert(SMEM <= 220 * 1024, "a block's shared memory");
 };
 
-// Unit c of a 16-bit B_i row, swapped so that the four rows of a half warp's 8-byte reads (features 0, 1,
-// 8, 9 or 16, 17, 24, 25 apart), 32 bytes of each, fall on unlike banks.
-template <int RP>
-__device__ __forceinline__ int swap_b16(int row, int c) {
-    if constexpr (RP == 16) return ((2 * row + c) ^ (((row >> 3) & 1) << 2)) - 2 * row;
-    else if constexpr (RP == 32) return c ^ (((row >> 3) & 1) << 1);
-    else return c ^ (((row & 1) << 2) | (((row >> 3) & 1) << 1));
+// Place of feature f (of each 32) of B_i in a stage: block b's eight rows follow one another.
+template <typename T>
+__device__ __forceinline__ int row_slot(int f) {
+    if constexpr (sizeof(T) == 4)  // f = 16 v + 4 q + 2 (b % 2) + j, b = 2 v + b % 2
+        return (f & ~31) + 8 * (2 * ((f >> 4) & 1) + ((f >> 1) & 1)) + 2 * ((f >> 2) & 3) + (f & 1);
+    else  // f = 8 q + 2 b + j
+        return (f & ~31) + 8 * ((f >> 1) & 3) + 2 * ((f >> 3) & 3) + (f & 1);
 }
 
-template <typename T, int RB, int WM, bool TRANS>
-__global__ void __launch_bounds__(kThreads) k_expand(Plan plan, const int32_t* __restrict__ index,
-                                                     const float* h, int splits, const T* __restrict__ w, int n,
-                                                     int rank, int64_t F, int64_t f_block, int T_rows, const T* base,
-                                                     int64_t ldb, T* out, int64_t ldo, bool bvec, bool wvec,
-                                                     bool ovec) {
-    using C = ExpandCfg<T, RB, WM, TRANS>;
-    constexpr int E = C::E, RP = C::RP, BM = C::BM, FS = C::FS, FU = C::FU, NS = C::NS;
+// Columns [f, f_end) of the rows: out = base (null: zeros).
+template <typename T>
+__device__ __forceinline__ void copy_rows(const int32_t* row, int rows, const T* base, int64_t ldb, T* out, int64_t ldo,
+                                          int64_t f, int64_t f_end, bool vec) {
+    constexpr int E = kE<T>;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int r = warp; r < rows; r += kWarps) {
+        const T* src = base ? base + (int64_t)row[r] * ldb : nullptr;
+        T* dst = out + (int64_t)row[r] * ldo;
+        for (int64_t c = f + lane * E; c < f_end; c += 32 * E) {
+            if (base && vec && c + E <= f_end) {
+                *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<const uint4*>(src + c);
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; e++)
+                    if (c + e < f_end) dst[c + e] = base ? src[c + e] : narrow<T>(0.f);
+            }
+        }
+    }
+}
+
+template <typename T, int RB, bool BIG, bool TRANS>
+__global__ void __launch_bounds__(kThreads) k_expand(Plan plan, const float* h, int splits, const T* __restrict__ w,
+                                                     int n, int rank, int64_t F, int64_t f_block, int T_rows,
+                                                     const T* base, int64_t ldb, T* out, int64_t ldo, bool bvec,
+                                                     bool wvec, bool ovec) {
+    using C = ExpandCfg<T, RB, BIG, TRANS>;
+    constexpr int E = C::E, RP = C::RP, BM = C::BM, MT = C::MT, FS = C::FS, FU = C::FU, NS = C::NS;
     constexpr bool F32 = sizeof(T) == 4;
     constexpr int KS = F32 ? RP / 8 : RP / 16;  // MMA steps of the rank
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ TileRows<BM> tr;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
-    const int wm = warp % WM, wf = warp / WM;
-    // the plan and h come from the launch before; index, base and the factors do not
-    if (plan.perm) wait_for_previous();
-    int adapter, rows;
-    const bool found = find_tile<BM>(tr, plan, index, T_rows, n, adapter, rows);
-    const bool none = found && adapter >= n;
-    if (!found || (none && base == out)) {
-        wait_for_previous();
-        let_next_start();
+    const int wm = warp % C::WM, wf = warp / C::WM;
+    wait_for_previous();
+    let_next_start();
+    if (!read_tile<BM>(tr, plan)) return;
+    const int adapter = tr.adapter, rows = tr.rows;
+    const int64_t f_begin = blockIdx.y * f_block, f_end = f_begin + f_block < F ? f_begin + f_block : F;
+    if (adapter >= n) {  // no adapter: base, or zeros
+        if (base != out) copy_rows<T>(tr.row, rows, base, ldb, out, ldo, f_begin, f_end, bvec && ovec);
         return;
     }
-    const T* wi = w + (none ? 0 : (int64_t)adapter * rank * F);
-    const int64_t f_begin = blockIdx.y * f_block, f_end = f_begin + f_block < F ? f_begin + f_block : F;
+    const T* wi = w + (int64_t)adapter * rank * F;
     const int stages = f_begin < f_end ? (int)((f_end - f_begin + FS - 1) / FS) : 0;
 
+    constexpr int WU = TRANS ? FU : RP / E, WR = TRANS ? RP : FS;
+    const auto w_place = [](int r, int c) {  // where a unit of the factors stands
+        if constexpr (!TRANS) return row_slot<T>(r) * C::W_PITCH + c * 16;
+        else return r * C::W_PITCH + (F32 ? c ^ ((r >> 2) & 3) : c ^ (((r >> 2) & 3) << 1)) * 16;
+    };
+    Units<T, BM, FU> ub;
+    Units<T, WR, WU> uw;
+#pragma unroll
+    for (int k = 0; k < ub.N; k++) {
+        const int r = ub.row(k);
+        ub.src[k] = base + (int64_t)tr.row[min(r, BM - 1)] * ldb + f_begin + ub.column() * E;
+        ub.bytes[k] = r < rows ? 16 : 0;
+    }
+#pragma unroll
+    for (int k = 0; k < uw.N; k++) {
+        const int r = uw.row(k), c = uw.column() * E;
+        const bool real = TRANS ? r < rank : c < rank;
+        uw.src[k] = !real ? w : TRANS ? wi + (int64_t)r * F + f_begin + c : wi + (f_begin + r) * rank + c;
+        uw.bytes[k] = real ? 16 : 0;
+    }
     const auto load = [&](int i) {
         uint8_t* bs = smem + (i % NS) * C::STAGE;
         uint8_t* ws = bs + C::B_BYTES;
-        const int64_t f0 = f_begin + (int64_t)i * FS;
-        if (base) {
+        const int64_t f0 = f_begin + (int64_t)i * FS, left = f_end - f0;
+        if (bvec && left >= FS) {
+            const uint32_t to = smem_u32(bs) + ub.row(0) * C::B_PITCH + ub.column() * 16;
+#pragma unroll
+            for (int k = 0; k < ub.N; k++)
+                if (ub.mine(k)) ub.copy(k, to + k * ub.STEP * C::B_PITCH, (int64_t)i * FS);
+        } else if (base) {
             for (int u = threadIdx.x; u < BM * FU; u += kThreads) {
                 const int r = u / FU, c = u % FU;
-                const int64_t f = f0 + c * E;
                 if (r < rows)
-                    stage_unit<T>(bs + r * (FU * 16) + ((c ^ swap_rows(r)) * 16), base + (int64_t)tr.row[r] * ldb + f,
-                                  base, f_end - f, bvec);
+                    stage_unit<T>(bs + r * C::B_PITCH + c * 16, base + (int64_t)tr.row[r] * ldb + f0 + c * E, base,
+                                  left - c * E, bvec);
             }
         }
-        if (!none) {
-            if constexpr (!TRANS) {
-                constexpr int U = RP / E;
-                for (int u = threadIdx.x; u < FS * U; u += kThreads) {
-                    const int r = u / U, c = u % U;
-                    const int to = F32 ? c : swap_b16<RP>(r, c);
-                    stage_unit<T>(ws + r * C::W_PITCH + to * 16, wi + (f0 + r) * rank + c * E, w,
-                                  f0 + r < f_end ? rank - c * E : 0, wvec);
-                }
-            } else {
-                for (int u = threadIdx.x; u < RP * FU; u += kThreads) {
-                    const int r = u / FU, c = u % FU;
-                    const int64_t f = f0 + c * E;
-                    const int to = F32 ? c ^ ((r >> 2) & 3) : c ^ (((r >> 2) & 3) << 1);
-                    stage_unit<T>(ws + r * C::W_PITCH + to * 16, wi + (int64_t)r * F + f, w, r < rank ? f_end - f : 0,
+        if (wvec && left >= FS) {
+#pragma unroll
+            for (int k = 0; k < uw.N; k++)
+                if (uw.mine(k))
+                    uw.copy(k, smem_u32(ws) + w_place(uw.row(k), uw.column()),
+                            uw.bytes[k] ? (int64_t)i * FS * (TRANS ? 1 : rank) : 0);
+        } else {
+            for (int u = threadIdx.x; u < WR * WU; u += kThreads) {
+                const int r = u / WU, c = u % WU;
+                if constexpr (TRANS)
+                    stage_unit<T>(ws + w_place(r, c), wi + (int64_t)r * F + f0 + c * E, w, r < rank ? left - c * E : 0,
                                   wvec);
-                }
+                else
+                    stage_unit<T>(ws + w_place(r, c), wi + (f0 + r) * rank + c * E, w, r < left ? rank - c * E : 0,
+                                  wvec);
             }
         }
         stage_done();
@@ -645,54 +793,50 @@ __global__ void __launch_bounds__(kThreads) k_expand(Plan plan, const int32_t* _
         if (i < stages) load(i);
         else stage_done();
     }
-    if (!plan.perm) wait_for_previous();
-    let_next_start();
 
-    // h of rows g and g + 8 of this warp's 16, split
-    uint32_t hi[KS][4], lo[KS][4];
-    float undo[2] = {1.f, 1.f};  // fp16: the rows' scales taken back
-    const int r0 = 16 * wm + g;
-    if (!none) {
-        float v[2][2 * KS * (F32 ? 1 : 2)];  // ranks: fp32 16 c + 4 q .. + 3; 16 bits 16 c + 2 q, + 1, + 8, + 9
+    // h of the warp's rows, split, and where they go
+    uint32_t hi[MT][KS][4], lo[MT][KS][4];
+    T* dst[2 * MT];
+    float undo[2 * MT];  // fp16: the rows' scales taken back
+    bool live[2 * MT];
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
-            const float* hp = h + (int64_t)tr.row[min(r0 + 8 * u, rows - 1)] * RP;
-            const int64_t stride = (int64_t)T_rows * RP;
+    for (int m = 0; m < 2 * MT; m++) {
+        const int r = 16 * MT * wm + 8 * m + g, t = tr.row[min(r, rows - 1)];
+        live[m] = r < rows;
+        dst[m] = out + (int64_t)t * ldo;
+        undo[m] = 1.f;
+        float v[RP / 4];  // ranks 16 c + 4 q .. + 3
+        const float* hp = h + (int64_t)t * RP + 4 * q;
 #pragma unroll
-            for (int c = 0; c < RP / 16; c++) {
-                const float4 f = load_h(hp + 16 * c + 4 * q, splits, stride);
-                v[u][4 * c] = f.x, v[u][4 * c + 1] = f.y, v[u][4 * c + 2] = f.z, v[u][4 * c + 3] = f.w;
-            }
-            if constexpr (sizeof(T) == 2) {
-                if constexpr (std::is_same_v<T, __half>) {
-                    float m = 0.f;
+        for (int c = 0; c < RP / 16; c++) {
+            const float4 f = load_h(hp + 16 * c, splits, (int64_t)T_rows * RP);
+            v[4 * c] = f.x, v[4 * c + 1] = f.y, v[4 * c + 2] = f.z, v[4 * c + 3] = f.w;
+        }
+        if constexpr (std::is_same_v<T, __half>) {
+            float most = 0.f;
 #pragma unroll
-                    for (int i = 0; i < RP / 4; i++) m = fmaxf(m, fabsf(v[u][i]));
-                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-                    const float s = half_scale(m);
-                    undo[u] = 1.f / s;
+            for (int i = 0; i < RP / 4; i++) most = fmaxf(most, fabsf(v[i]));
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+            const float s = half_scale(most);
+            undo[m] = 1.f / s;
 #pragma unroll
-                    for (int i = 0; i < RP / 4; i++) v[u][i] *= s;
-                }
-            }
+            for (int i = 0; i < RP / 4; i++) v[i] *= s;
         }
 #pragma unroll
         for (int s = 0; s < KS; s++)
 #pragma unroll
-            for (int u = 0; u < 2; u++)
-#pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    if constexpr (F32) {
-                        split_tf32(bits_of(v[u][2 * s + k]), hi[s][u + 2 * k], lo[s][u + 2 * k]);
-                    } else {  // ranks 4 q + 2 k, + 1 of the step: the sum's order is the factors' below
-                        const float a = v[u][4 * s + 2 * k], b = v[u][4 * s + 2 * k + 1];
-                        const uint32_t p = pack2<T>(a, b);
-                        const float2 back = unpack2<T>(p);
-                        hi[s][u + 2 * k] = p;
-                        lo[s][u + 2 * k] = pack2<T>(a - back.x, b - back.y);
-                    }
+            for (int k = 0; k < 2; k++) {
+                uint32_t &a = hi[m >> 1][s][(m & 1) + 2 * k], &b = lo[m >> 1][s][(m & 1) + 2 * k];
+                if constexpr (F32) {
+                    split_tf32(bits_of(v[2 * s + k]), a, b);
+                } else {  // ranks 4 q + 2 k, + 1 of the step: the sum's order is the factors' below
+                    const float v0 = v[4 * s + 2 * k], v1 = v[4 * s + 2 * k + 1];
+                    a = pack2<T>(v0, v1);
+                    const float2 back = unpack2<T>(a);
+                    b = pack2<T>(v0 - back.x, v1 - back.y);
                 }
+            }
     }
 
     for (int i = 0; i < stages; i++) {
@@ -703,124 +847,116 @@ __global__ void __launch_bounds__(kThreads) k_expand(Plan plan, const int32_t* _
         const uint8_t* bs = smem + (i % NS) * C::STAGE;
         const uint8_t* ws = bs + C::B_BYTES;
         const int64_t f0 = f_begin + (int64_t)i * FS;
+#pragma unroll 1
         for (int fs = 32 * wf; fs < FS; fs += 32 * C::WF) {  // 32 columns from f0 + fs
-            if (f0 + fs >= f_end) break;
-            float acc[4][4];
+            const int left = f_end - f0 - fs < 32 ? (int)(f_end - f0 - fs) : 32;
+            if (left <= 0) break;
+            float acc[MT][4][4];
 #pragma unroll
-            for (int b = 0; b < 4; b++)
+            for (int m = 0; m < MT; m++)
 #pragma unroll
-                for (int k = 0; k < 4; k++) acc[b][k] = 0.f;
-            if (!none) {
-                if constexpr (F32 && !TRANS) {
+                for (int b = 0; b < 4; b++)
+#pragma unroll
+                    for (int k = 0; k < 4; k++) acc[m][b][k] = 0.f;
+            if constexpr (F32 && !TRANS) {
+#pragma unroll
+                for (int b = 0; b < 4; b++)
+#pragma unroll
+                    for (int c = 0; c < RP / 16; c++) {
+                        const uint4 wv = lds128(ws + (fs + 8 * b + g) * C::W_PITCH + (4 * c + q) * 16);
+#pragma unroll
+                        for (int s = 0; s < 2; s++) {
+                            uint32_t h0, h1, l0, l1;
+                            split_tf32(s ? wv.z : wv.x, h0, l0);
+                            split_tf32(s ? wv.w : wv.y, h1, l1);
+#pragma unroll
+                            for (int m = 0; m < MT; m++) mma<float>(acc[m][b], lo[m][2 * c + s], h0, h1);
+#pragma unroll
+                            for (int m = 0; m < MT; m++) mma<float>(acc[m][b], hi[m][2 * c + s], l0, l1);
+#pragma unroll
+                            for (int m = 0; m < MT; m++) mma<float>(acc[m][b], hi[m][2 * c + s], h0, h1);
+                        }
+                    }
+            } else if constexpr (F32) {
+#pragma unroll
+                for (int s = 0; s < KS; s++) {
+                    uint32_t wv[2][4];
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        const int r = 16 * (s >> 1) + 4 * q + 2 * (s & 1) + j;
+                        const int c = (fs + 16 * (g & 1)) / 4 + (g >> 1);
+                        const uint4 v = lds128(ws + r * C::W_PITCH + ((c ^ q) * 16));
+                        wv[j][0] = v.x, wv[j][1] = v.y, wv[j][2] = v.z, wv[j][3] = v.w;
+                    }
 #pragma unroll
                     for (int b = 0; b < 4; b++) {
-                        const int r = fs + 16 * (b >> 1) + 4 * (g >> 1) + 2 * (b & 1) + (g & 1);
+                        uint32_t h0, h1, l0, l1;
+                        split_tf32(wv[0][b], h0, l0);
+                        split_tf32(wv[1][b], h1, l1);
 #pragma unroll
-                        for (int c = 0; c < RP / 16; c++) {
-                            const uint4 wv = lds128(ws + r * C::W_PITCH + (4 * c + q) * 16);
+                        for (int m = 0; m < MT; m++) mma<float>(acc[m][b], lo[m][s], h0, h1);
 #pragma unroll
-                            for (int s = 0; s < 2; s++) {
-                                uint32_t h0, h1, l0, l1;
-                                split_tf32(s ? wv.z : wv.x, h0, l0);
-                                split_tf32(s ? wv.w : wv.y, h1, l1);
-                                mma<float>(acc[b], lo[2 * c + s], h0, h1);
-                                mma<float>(acc[b], hi[2 * c + s], l0, l1);
-                                mma<float>(acc[b], hi[2 * c + s], h0, h1);
-                            }
-                        }
+                        for (int m = 0; m < MT; m++) mma<float>(acc[m][b], hi[m][s], l0, l1);
+#pragma unroll
+                        for (int m = 0; m < MT; m++) mma<float>(acc[m][b], hi[m][s], h0, h1);
                     }
-                } else if constexpr (F32) {
+                }
+            } else if constexpr (!TRANS) {
+                // a lane's four ranks 4 q .. 4 q + 3 of a step are the MMA's k = 2 q, 2 q + 1, 2 q + 8, 2 q + 9
 #pragma unroll
-                    for (int s = 0; s < KS; s++) {
-                        uint32_t wv[2][4];
+                for (int s = 0; s < KS; s++)
 #pragma unroll
-                        for (int j = 0; j < 2; j++) {
-                            const int r = 16 * (s >> 1) + 4 * q + 2 * (s & 1) + j;
-                            const int c = (fs + 16 * (g & 1)) / 4 + (g >> 1);
-                            const uint4 v = lds128(ws + r * C::W_PITCH + ((c ^ ((r >> 2) & 3)) * 16));
-                            wv[j][0] = v.x, wv[j][1] = v.y, wv[j][2] = v.z, wv[j][3] = v.w;
-                        }
+                    for (int b = 0; b < 4; b++) {
+                        const uint2 wv = *reinterpret_cast<const uint2*>(ws + (fs + 8 * b + g) * C::W_PITCH + 32 * s + 8 * q);
 #pragma unroll
-                        for (int b = 0; b < 4; b++) {
-                            uint32_t h0, h1, l0, l1;
-                            split_tf32(wv[0][b], h0, l0);
-                            split_tf32(wv[1][b], h1, l1);
-                            mma<float>(acc[b], lo[s], h0, h1);
-                            mma<float>(acc[b], hi[s], l0, l1);
-                            mma<float>(acc[b], hi[s], h0, h1);
-                        }
+                        for (int m = 0; m < MT; m++) mma<T>(acc[m][b], lo[m][s], wv.x, wv.y);
+#pragma unroll
+                        for (int m = 0; m < MT; m++) mma<T>(acc[m][b], hi[m][s], wv.x, wv.y);
                     }
-                } else if constexpr (!TRANS) {
-                    // a lane's four ranks 4 q .. 4 q + 3 of a step are the MMA's k = 2 q, 2 q + 1, 2 q + 8, 2 q + 9
+            } else {
 #pragma unroll
-                    for (int s = 0; s < KS; s++)
+                for (int s = 0; s < KS; s++) {
+                    uint2 wv[4];  // ranks 4 q .. 4 q + 3, columns 4 g .. 4 g + 3
 #pragma unroll
-                        for (int b = 0; b < 4; b++) {
-                            const int r = fs + 8 * (g >> 1) + 2 * b + (g & 1);
-                            const uint8_t* p = ws + r * C::W_PITCH + swap_b16<RP>(r, 2 * s + (q >> 1)) * 16 + (q & 1) * 8;
-                            const uint2 wv = *reinterpret_cast<const uint2*>(p);
-                            mma<T>(acc[b], lo[s], wv.x, wv.y);
-                            mma<T>(acc[b], hi[s], wv.x, wv.y);
-                        }
-                } else {
+                    for (int j = 0; j < 4; j++)
+                        wv[j] = *reinterpret_cast<const uint2*>(ws + (16 * s + 4 * q + j) * C::W_PITCH +
+                                                                (((fs / 8 + (g >> 1)) ^ (q << 1)) * 16) + (g & 1) * 8);
 #pragma unroll
-                    for (int s = 0; s < KS; s++) {
-                        uint2 wv[4];  // ranks 4 q .. 4 q + 3, columns 4 g .. 4 g + 3
+                    for (int b = 0; b < 4; b++) {
+                        const uint32_t pick = (b & 1) ? 0x7632u : 0x5410u;
+                        const uint32_t b0 = __byte_perm(b < 2 ? wv[0].x : wv[0].y, b < 2 ? wv[1].x : wv[1].y, pick);
+                        const uint32_t b1 = __byte_perm(b < 2 ? wv[2].x : wv[2].y, b < 2 ? wv[3].x : wv[3].y, pick);
 #pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            const int r = 16 * s + 4 * q + j, c = fs / 8 + (g >> 1);
-                            wv[j] = *reinterpret_cast<const uint2*>(
-                                ws + r * C::W_PITCH + ((c ^ (((r >> 2) & 3) << 1)) * 16) + (g & 1) * 8);
-                        }
+                        for (int m = 0; m < MT; m++) mma<T>(acc[m][b], lo[m][s], b0, b1);
 #pragma unroll
-                        for (int b = 0; b < 4; b++) {
-                            const uint32_t pick = (b & 1) ? 0x7632u : 0x5410u;
-                            const uint32_t b0 = __byte_perm(b < 2 ? wv[0].x : wv[0].y, b < 2 ? wv[1].x : wv[1].y, pick);
-                            const uint32_t b1 = __byte_perm(b < 2 ? wv[2].x : wv[2].y, b < 2 ? wv[3].x : wv[3].y, pick);
-                            mma<T>(acc[b], lo[s], b0, b1);
-                            mma<T>(acc[b], hi[s], b0, b1);
-                        }
+                        for (int m = 0; m < MT; m++) mma<T>(acc[m][b], hi[m][s], b0, b1);
                     }
                 }
             }
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const int r = r0 + 8 * u;
-                if (r >= rows) continue;
+            for (int m = 0; m < 2 * MT; m++) {
+                if (!live[m]) continue;
+                const uint8_t* bp = bs + (16 * MT * wm + 8 * m + g) * C::B_PITCH + fs * (int)sizeof(T) + 16 * q;
+                T* to = dst[m] + f0 + fs;
 #pragma unroll
                 for (int v = 0; v < 8 / E; v++) {
-                    const int c = fs / E + 4 * v + q;
-                    const int64_t f = f0 + c * E;
-                    float y[E];
+                    alignas(16) T o[E], d[E];
+                    if (base) *reinterpret_cast<uint4*>(d) = lds128(bp + 64 * v);
 #pragma unroll
                     for (int e = 0; e < E; e++) {
-                        int b, j;
-                        if constexpr (F32) {
-                            b = TRANS ? e : 2 * v + (e >> 1);
-                            j = TRANS ? v : e & 1;
-                        } else {
-                            b = TRANS ? e & 3 : e >> 1;
-                            j = TRANS ? e >> 2 : e & 1;
-                        }
-                        y[e] = acc[b][2 * u + j] * undo[u];
+                        const int b = F32 ? (TRANS ? e : 2 * v + (e >> 1)) : TRANS ? e & 3 : e >> 1;
+                        const int j = F32 ? (TRANS ? v : e & 1) : TRANS ? e >> 2 : e & 1;
+                        float y = acc[m >> 1][b][2 * (m & 1) + j];
+                        if constexpr (std::is_same_v<T, __half>) y *= undo[m];
+                        o[e] = narrow<T>(base ? wide(d[e]) + y : y);
                     }
-                    alignas(16) T o[E];
-                    if (base) {
-                        alignas(16) T d[E];
-                        *reinterpret_cast<uint4*>(d) = lds128(bs + r * (FU * 16) + ((c ^ swap_rows(r)) * 16));
-#pragma unroll
-                        for (int e = 0; e < E; e++) o[e] = none ? d[e] : narrow<T>(wide(d[e]) + y[e]);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < E; e++) o[e] = narrow<T>(none ? 0.f : y[e]);
-                    }
-                    T* dst = out + (int64_t)tr.row[r] * ldo + f;
-                    if (ovec && f + E <= f_end) {
-                        *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(o);
+                    const int f = (4 * v + q) * E;
+                    if (ovec && f + E <= left) {
+                        *reinterpret_cast<uint4*>(to + f) = *reinterpret_cast<const uint4*>(o);
                     } else {
 #pragma unroll
                         for (int e = 0; e < E; e++)
-                            if (f + e < f_end) dst[e] = o[e];
+                            if (f + e < left) to[f + e] = o[e];
                     }
                 }
             }
@@ -830,9 +966,20 @@ __global__ void __launch_bounds__(kThreads) k_expand(Plan plan, const int32_t* _
 
 // ---- weight gradients ------------------------------------------------------------
 // G_i = sum over adapter i's positions of x[t, f] h[t, r].  TRANS = false: G_i stored [rank, F] (dA,
-// with h = dh); true: stored [F, rank] (dB, with x = the gradient of out).  One block per (FC columns,
-// adapter), 64 positions a stage; four warps side by side along the columns, two along the positions,
-// which are summed through shared memory at the end.  An adapter without positions gets zeros.
+// with h = dh); true: stored [F, rank] (dB, with x = the gradient of out).  Both in one launch: blocks up
+// to `first` along x take the first side.  A cluster of blocks per (FC columns, adapter) shares its
+// positions, 64 a stage; four warps side by side along the columns, two along the positions.  All are
+// summed, in their order, through (distributed) shared memory at the end.  An adapter without positions
+// gets zeros.
+template <typename T>
+struct Side {
+    const T* x;
+    int64_t ldx;
+    const float* h;
+    int64_t F;
+    T* out;
+    bool trans, vec;
+};
 template <typename T, int RB>
 struct WeightCfg {
     static constexpr int E = kE<T>, RP = 8 * RB, NB = RB == 16 ? 2 : 4;  // blocks of 8 columns a warp
@@ -847,11 +994,9 @@ struct WeightCfg {
     static_assert(SMEM <= 220 * 1024, "a block's shared memory");
 };
 
-template <typename T, int RB, bool TRANS>
-__global__ void __launch_bounds__(kThreads) k_weight(Plan plan, const int32_t* __restrict__ index,
-                                                     const T* __restrict__ x, int64_t ldx, const float* h, int splits,
-                                                     int n, int rank, int64_t F, int T_rows, bool xvec,
-                                                     T* __restrict__ out) {
+template <typename T, int RB>
+__global__ void __launch_bounds__(kThreads) k_weight(Plan plan, const int32_t* __restrict__ index, Side<T> side_a,
+                                                     Side<T> side_b, int first, int n, int rank, int T_rows) {
     using C = WeightCfg<T, RB>;
     constexpr int E = C::E, RP = C::RP, NB = C::NB, FC = C::FC, FU = C::FU, TK = C::TK, NS = C::NS, RM = RB / 2;
     constexpr bool F32 = sizeof(T) == 4;
@@ -862,13 +1007,18 @@ __global__ void __launch_bounds__(kThreads) k_weight(Plan plan, const int32_t* _
     uint8_t* hs = smem + NS * C::X_BYTES;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
     const int wf = warp & 3, wt = warp >> 2;
-    const int a = blockIdx.y;
-    const int64_t f0 = (int64_t)blockIdx.x * FC;
+    const int a = blockIdx.y, part = blockIdx.z, parts = gridDim.z;  // the cluster is (1, 1, parts)
+    const bool second = (int)blockIdx.x >= first;
+    const Side<T>& side = second ? side_b : side_a;
+    const T* __restrict__ x = side.x;
+    const float* h = side.h;
+    const int64_t ldx = side.ldx, F = side.F, f0 = (int64_t)((int)blockIdx.x - (second ? first : 0)) * FC;
+    const bool xvec = side.vec;
     wait_for_previous();
     let_next_start();
     const int32_t* list;
     int count;
-    if (plan.perm) {
+    if (plan.off) {
         const int p0 = __ldg(plan.off + a);
         list = plan.perm + p0;
         count = __ldg(plan.off + a + 1) - p0;
@@ -876,14 +1026,14 @@ __global__ void __launch_bounds__(kThreads) k_weight(Plan plan, const int32_t* _
         count = scan_positions(scan, index, T_rows, n, a);
         list = scan.list;
     }
-    const int stages = (count + TK - 1) / TK;
-    const int64_t stride = (int64_t)T_rows * RP;
+    const int all = (count + TK - 1) / TK;  // stages; this block takes part, part + parts, ..
+    const int stages = part < all ? (all - part + parts - 1) / parts : 0;
 
     float take = 1.f;  // fp16: h's scale
     if constexpr (std::is_same_v<T, __half>) {
         float m = 0.f;
         for (int e = threadIdx.x; e < count * (RP / 4); e += kThreads) {
-            const float4 v = load_h(h + (int64_t)list[e / (RP / 4)] * RP + 4 * (e % (RP / 4)), splits, stride);
+            const float4 v = load_h(h + (int64_t)list[e / (RP / 4)] * RP + 4 * (e % (RP / 4)), 1, 0);
             m = fmaxf(fmaxf(fmaxf(m, fabsf(v.x)), fmaxf(fabsf(v.y), fabsf(v.z))), fabsf(v.w));
         }
 #pragma unroll
@@ -896,12 +1046,13 @@ __global__ void __launch_bounds__(kThreads) k_weight(Plan plan, const int32_t* _
 
     const auto load_x = [&](int i) {
         uint8_t* xs = smem + (i % NS) * C::X_BYTES;
-        for (int u = threadIdx.x; u < TK * FU; u += kThreads) {
-            const int r = u / FU, c = u % FU, p = i * TK + r;
-            const int64_t f = f0 + c * E;
+        const int p0 = (part + i * parts) * TK;
+#pragma unroll
+        for (int k = 0; k < TK * FU / kThreads; k++) {
+            const int u = threadIdx.x + k * kThreads, r = u / FU, c = u % FU, p = p0 + r;
             const int to = F32 ? c ^ ((r & 3) << 1) : c ^ (r & 7);
-            stage_unit<T>(xs + r * (FU * 16) + to * 16, x + (p < count ? (int64_t)list[p] * ldx : 0) + f, x,
-                          p < count ? F - f : 0, xvec);
+            stage_unit<T>(xs + r * (FU * 16) + to * 16, x + (p < count ? (int64_t)list[p] * ldx : 0) + f0 + c * E, x,
+                          p < count ? F - f0 - c * E : 0, xvec);
         }
         stage_done();
     };
@@ -909,8 +1060,8 @@ __global__ void __launch_bounds__(kThreads) k_weight(Plan plan, const int32_t* _
     const auto load_h_regs = [&](int i) {
 #pragma unroll
         for (int k = 0; k < HV; k++) {
-            const int e = threadIdx.x + k * kThreads, r = e / (RP / 4), c = e % (RP / 4), p = i * TK + r;
-            hv[k] = p < count ? load_h(h + (int64_t)list[p] * RP + 4 * c, splits, stride)
+            const int e = threadIdx.x + k * kThreads, r = e / (RP / 4), c = e % (RP / 4), p = (part + i * parts) * TK + r;
+            hv[k] = p < count ? load_h(h + (int64_t)list[p] * RP + 4 * c, 1, 0)
                               : make_float4(0.f, 0.f, 0.f, 0.f);
         }
     };
@@ -1045,14 +1196,22 @@ __global__ void __launch_bounds__(kThreads) k_weight(Plan plan, const int32_t* _
                 if constexpr (F32) red[(wt * RP + r) * RS + f] = sum[m][b][k];
                 else red[(wt * RP + r) * RS + f] = acc[m][b][k] * undo;
             }
-    __syncthreads();
-    T* dst = out + (int64_t)a * rank * F;
-    for (int e = threadIdx.x; e < FC * rank; e += kThreads) {
-        const int r = TRANS ? e % rank : e / FC, c = TRANS ? e / rank : e % FC;
+    // each block of the cluster finishes its share of the elements, from all blocks' sums
+    const cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+    if (parts > 1) cluster.sync();
+    else __syncthreads();
+    T* dst = side.out + (int64_t)a * rank * F;
+    for (int e = threadIdx.x + part * kThreads; e < FC * rank; e += parts * kThreads) {
+        const int r = side.trans ? e % rank : e / FC, c = side.trans ? e / rank : e % FC;
         if (f0 + c >= F) continue;
-        dst[TRANS ? (f0 + c) * rank + r : (int64_t)r * F + f0 + c] =
-            narrow<T>(red[r * RS + c] + red[(RP + r) * RS + c]);
+        float v = 0.f;
+        for (int k = 0; k < parts; k++) {
+            const float* from = parts > 1 ? cluster.map_shared_rank(red, k) : red;
+            v += from[r * RS + c] + from[(RP + r) * RS + c];
+        }
+        dst[side.trans ? (f0 + c) * rank + r : (int64_t)r * F + f0 + c] = narrow<T>(v);
     }
+    if (parts > 1) cluster.sync();  // its shared memory is read until here
 }
 
 // ---- host ------------------------------------------------------------------------
@@ -1060,7 +1219,7 @@ __global__ void __launch_bounds__(kThreads) k_weight(Plan plan, const int32_t* _
 struct Shape {
     int64_t T, K, N;
     int n, rank, rb, wm;
-    bool planned;            // by k_plan; else each block finds its tile
+    bool planned;            // by k_plan; else the first launch's blocks find their tiles
     int64_t tiles;           // blocks along x: at least the tiles there are
     int splits_k, splits_n;  // blocks per tile that share the sum over K, over N
 };
@@ -1090,11 +1249,10 @@ Shape shape_of(int64_t T, int n, int rank, int64_t K, int64_t N) {
     const int64_t groups = T < (int64_t)n + 1 ? T : (int64_t)n + 1;
     s.wm = groups > 0 && T / groups >= 32 ? 8 : 1;
     const int bm = 16 * s.wm;
-    s.planned = T > kScanMax;
-    const int64_t most = (T + (bm - 1) * groups) / bm;  // tiles there can be
-    s.tiles = s.planned ? most : T;
+    s.planned = T > kScanMax || n > kScanAdapters;
+    s.tiles = (T + (bm - 1) * groups) / bm;  // as many as there can be
     const auto splits = [&](int64_t width) {
-        const int64_t want = most > 0 ? ceil_div(2 * kSms, most) : 1, can = ceil_div(width, 512);
+        const int64_t want = s.tiles > 0 ? ceil_div(2 * kSms, s.tiles) : 1, can = ceil_div(width, 512);
         const int64_t k = want < can ? want : can;
         return (int)(k < 1 ? 1 : k > 16 ? 16 : k);
     };
@@ -1111,12 +1269,10 @@ Layout layout_of(const Shape& s, bool backward) {
         at += align256(bytes);
         return here;
     };
-    if (s.planned) {
-        l.off = take((int64_t)(s.n + 2) * 4);
-        l.perm = take(s.T * 4);
-        l.tiles = take(4);
-        l.tile = take(s.tiles * (int64_t)sizeof(Tile));
-    }
+    l.off = take((int64_t)(s.n + 2) * 4);
+    l.perm = take(s.planned ? s.T * 4 : s.tiles * 16 * s.wm * 4);
+    l.tiles = take(4);
+    l.tile = take(s.tiles * (int64_t)sizeof(Tile));
     l.h = take((int64_t)s.splits_k * s.T * 8 * s.rb * 4);
     if (backward) l.dh = take((int64_t)s.splits_n * s.T * 8 * s.rb * 4);
     l.bytes = at;
@@ -1124,9 +1280,9 @@ Layout layout_of(const Shape& s, bool backward) {
 }
 
 Plan plan_at(uint8_t* ws, const Shape& s, const Layout& l) {
-    if (!s.planned) return Plan{};
-    return Plan{reinterpret_cast<int32_t*>(ws + l.off), reinterpret_cast<int32_t*>(ws + l.perm),
-                reinterpret_cast<int32_t*>(ws + l.tiles), reinterpret_cast<Tile*>(ws + l.tile)};
+    return Plan{s.planned ? reinterpret_cast<int32_t*>(ws + l.off) : nullptr,
+                reinterpret_cast<int32_t*>(ws + l.perm),
+                s.planned ? reinterpret_cast<int32_t*>(ws + l.tiles) : nullptr, reinterpret_cast<Tile*>(ws + l.tile)};
 }
 
 // Starts a kernel; after = true: it may start while the launch before it still runs (it waits for that
@@ -1141,12 +1297,17 @@ int start(void (*kernel)(P...), dim3 grid, int threads, int smem, bool after, cu
     cfg.blockDim = dim3((unsigned)threads);
     cfg.dynamicSmemBytes = (size_t)smem;
     cfg.stream = st;
-    cudaLaunchAttribute attr = {};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = after ? 1 : 0;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+    cudaLaunchAttribute attr[2] = {};
+    if (after) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (grid.z > 1) {  // a cluster shares its grid's third dimension
+        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attr[cfg.numAttrs++].val.clusterDim = {1, 1, grid.z};
+    }
+    cfg.attrs = attr;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
     count_launches(1);
     return e == cudaSuccess && cudaGetLastError() == cudaSuccess ? ENGRAM_OK : ENGRAM_ERR_CUDA;
 }
@@ -1165,33 +1326,46 @@ bool row_units(const T* p, int64_t ld) {  // every row starts on 16 bytes
 
 template <typename T, int RB, int WM, bool TRANS>
 int run_shrink(const Shape& s, const Plan& plan, const int32_t* index, const T* x, int64_t ldx, const T* w,
-               const float* scale, int64_t K, int splits, float* h, bool after, cudaStream_t st) {
+               const float* scale, int64_t K, int splits, float* h, bool first, cudaStream_t st) {
     using C = ShrinkCfg<T, RB, WM, TRANS>;
     const int64_t k_split = ceil_div(ceil_div(K, splits), C::KC) * C::KC;
-    return start(k_shrink<T, RB, WM, TRANS>, dim3((unsigned)s.tiles, (unsigned)splits), kThreads, C::SMEM, after, st,
-                 plan, index, x, ldx, w, scale, s.n, s.rank, K, k_split, (int)s.T, row_units(x, ldx),
-                 row_units(w, TRANS ? s.rank : K), h);
+    const bool find = first && !s.planned;
+    return start(k_shrink<T, RB, WM, TRANS>, dim3((unsigned)s.tiles, (unsigned)splits), kThreads, C::SMEM, !find, st,
+                 plan, (int)(find ? FIND : PLANNED), index, x, ldx, w, scale, s.n, s.rank, K, k_split, (int)s.T,
+                 row_units(x, ldx), row_units(w, TRANS ? s.rank : K), h);
+}
+
+int run_sum(const Shape& s, float* h, int h_splits, float* dh, int dh_splits, cudaStream_t st) {
+    if (h_splits == 1 && dh_splits == 1) return ENGRAM_OK;
+    const int64_t count4 = s.T * 2 * s.rb;
+    return start(k_sum_splits, dim3((unsigned)ceil_div(count4, kThreads), 2), kThreads, 0, true, st,
+                 reinterpret_cast<float4*>(h), h_splits, reinterpret_cast<float4*>(dh), dh_splits, count4);
 }
 
 template <typename T, int RB, int WM, bool TRANS>
-int run_expand(const Shape& s, const Plan& plan, const int32_t* index, const float* h, int splits, const T* w,
-               int64_t F, const T* base, int64_t ldb, T* out, int64_t ldo, cudaStream_t st) {
-    using C = ExpandCfg<T, RB, WM, TRANS>;
+int run_expand(const Shape& s, const Plan& plan, const float* h, int splits, const T* w, int64_t F, const T* base,
+               int64_t ldb, T* out, int64_t ldo, cudaStream_t st) {
+    using C = ExpandCfg<T, RB, WM == 8, TRANS>;
     // columns of a block: whole stages, for about four blocks an SM
-    const int64_t passes = ceil_div(F, C::FS), tiles = s.planned ? s.tiles : ceil_div(s.T, 16 * WM);
-    const int64_t want = ceil_div(4 * kSms, tiles), blocks = want < passes ? want : passes;
-    const int64_t f_block = ceil_div(passes, blocks) * C::FS;
-    return start(k_expand<T, RB, WM, TRANS>, dim3((unsigned)s.tiles, (unsigned)ceil_div(F, f_block)), kThreads, C::SMEM,
-                 true, st, plan, index, h, splits, w, s.n, s.rank, F, f_block, (int)s.T, base, ldb, out, ldo,
+    const int64_t passes = ceil_div(F, C::FS), want = ceil_div(4 * kSms, s.tiles);
+    const int64_t f_block = ceil_div(passes, want < passes ? want : passes) * C::FS;
+    return start(k_expand<T, RB, WM == 8, TRANS>, dim3((unsigned)s.tiles, (unsigned)ceil_div(F, f_block)), kThreads,
+                 C::SMEM, true, st, plan, h, splits, w, s.n, s.rank, F, f_block, (int)s.T, base, ldb, out, ldo,
                  base && row_units(base, ldb), row_units(w, TRANS ? F : s.rank), row_units((const T*)out, ldo));
 }
 
-template <typename T, int RB, bool TRANS>
-int run_weight(const Shape& s, const Plan& plan, const int32_t* index, const T* x, int64_t ldx, const float* h,
-               int splits, int64_t F, T* out, cudaStream_t st) {
+// Either side may be missing (out null).
+template <typename T, int RB>
+int run_weight(const Shape& s, const Plan& plan, const int32_t* index, const Side<T>& a, const Side<T>& b,
+               cudaStream_t st) {
     using C = WeightCfg<T, RB>;
-    return start(k_weight<T, RB, TRANS>, dim3((unsigned)ceil_div(F, C::FC), (unsigned)s.n), kThreads, C::SMEM, true, st,
-                 plan, index, x, ldx, h, splits, s.n, s.rank, F, (int)s.T, row_units(x, ldx), out);
+    const int64_t blocks_a = a.out ? ceil_div(a.F, C::FC) : 0, blocks_b = b.out ? ceil_div(b.F, C::FC) : 0;
+    // blocks of a cluster: about two blocks an SM, while an adapter's usual share of positions has stages for them
+    const int64_t want = ceil_div(2 * kSms, (blocks_a + blocks_b) * s.n), can = ceil_div(s.T, (int64_t)s.n * C::TK);
+    const int64_t most = want < can ? want : can;
+    const unsigned parts = most >= 8 ? 8 : most >= 4 ? 4 : most >= 2 ? 2 : 1;
+    return start(k_weight<T, RB>, dim3((unsigned)(blocks_a + blocks_b), (unsigned)s.n, parts), kThreads, C::SMEM, true, st,
+                 plan, index, a, b, (int)blocks_a, s.n, s.rank, (int)s.T);
 }
 
 struct Args {
@@ -1211,10 +1385,10 @@ int forward(const Shape& s, const Layout& l, const Args& g) {
     int e = run_plan(s, g.index, plan, g.st);
     if (!e)
         e = run_shrink<T, RB, WM, false>(s, plan, g.index, (const T*)g.x, g.ldx, (const T*)g.a, g.scale, s.K,
-                                         s.splits_k, h, s.planned, g.st);
+                                         s.splits_k, h, true, g.st);
     if (!e)
-        e = run_expand<T, RB, WM, false>(s, plan, g.index, h, s.splits_k, (const T*)g.b, s.N, (const T*)g.base,
-                                         g.ldbase, (T*)g.out, g.ldout, g.st);
+        e = run_expand<T, RB, WM, false>(s, plan, h, s.splits_k, (const T*)g.b, s.N, (const T*)g.base, g.ldbase,
+                                         (T*)g.out, g.ldout, g.st);
     return e;
 }
 
@@ -1222,23 +1396,23 @@ template <typename T, int RB, int WM>
 int backward(const Shape& s, const Layout& l, const Args& g) {
     const Plan plan = plan_at(g.ws, s, l);
     float *h = reinterpret_cast<float*>(g.ws + l.h), *dh = reinterpret_cast<float*>(g.ws + l.dh);
+    const bool inner = g.dx || g.da;
     int e = run_plan(s, g.index, plan, g.st);
-    bool after = s.planned;
-    if (!e && (g.dx || g.da)) {
+    if (!e && inner)
         e = run_shrink<T, RB, WM, true>(s, plan, g.index, (const T*)g.grad, g.ldgrad, (const T*)g.b, g.scale, s.N,
-                                        s.splits_n, dh, after, g.st);
-        after = true;
-    }
-    if (!e && g.dx)
-        e = run_expand<T, RB, WM, true>(s, plan, g.index, dh, s.splits_n, (const T*)g.a, s.K, (const T*)g.base,
-                                        g.ldbase, (T*)g.dx, g.lddx, g.st);
-    if (!e && g.da)
-        e = run_weight<T, RB, false>(s, plan, g.index, (const T*)g.x, g.ldx, dh, s.splits_n, s.K, (T*)g.da, g.st);
+                                        s.splits_n, dh, true, g.st);
     if (!e && g.db)
         e = run_shrink<T, RB, WM, false>(s, plan, g.index, (const T*)g.x, g.ldx, (const T*)g.a, g.scale, s.K,
-                                         s.splits_k, h, after, g.st);
-    if (!e && g.db)
-        e = run_weight<T, RB, true>(s, plan, g.index, (const T*)g.grad, g.ldgrad, h, s.splits_k, s.N, (T*)g.db, g.st);
+                                         s.splits_k, h, !inner, g.st);
+    if (!e) e = run_sum(s, h, g.db ? s.splits_k : 1, dh, inner ? s.splits_n : 1, g.st);
+    if (!e && g.dx)
+        e = run_expand<T, RB, WM, true>(s, plan, dh, 1, (const T*)g.a, s.K, (const T*)g.base, g.ldbase, (T*)g.dx,
+                                        g.lddx, g.st);
+    if (!e && (g.da || g.db)) {
+        const Side<T> da = {(const T*)g.x, g.ldx, dh, s.K, (T*)g.da, false, row_units((const T*)g.x, g.ldx)};
+        const Side<T> db = {(const T*)g.grad, g.ldgrad, h, s.N, (T*)g.db, true, row_units((const T*)g.grad, g.ldgrad)};
+        e = run_weight<T, RB>(s, plan, g.index, da, db, g.st);
+    }
     return e;
 }
 
