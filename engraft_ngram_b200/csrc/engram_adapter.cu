@@ -236,14 +236,16 @@ __device__ __forceinline__ void find_tile(FindTile& f, TileRows<BM>& r, const in
     __syncthreads();
 }
 
-// The block's tile from the plan; false: there is none.
-template <int BM>
+// The block's tile, or its BM positions of one shared by PARTS blocks, from the plan; false: there are none.
+template <int BM, int PARTS = 1>
 __device__ __forceinline__ bool read_tile(TileRows<BM>& r, const Plan& plan) {
-    if (plan.tiles && (int)blockIdx.x >= *plan.tiles) return false;
-    const Tile t = plan.tile[blockIdx.x];
-    if (t.rows == 0) return false;
-    for (int i = threadIdx.x; i < BM; i += kThreads) r.row[i] = plan.perm[t.start + min(i, t.rows - 1)];
-    if (threadIdx.x == 0) r.adapter = t.adapter, r.rows = t.rows;
+    const int k = blockIdx.x / PARTS, from = (int)(blockIdx.x % PARTS) * BM;
+    if (plan.tiles && k >= *plan.tiles) return false;
+    const Tile t = plan.tile[k];
+    const int rows = min(BM, t.rows - from);
+    if (rows <= 0) return false;
+    for (int i = threadIdx.x; i < BM; i += kThreads) r.row[i] = plan.perm[t.start + from + min(i, rows - 1)];
+    if (threadIdx.x == 0) r.adapter = t.adapter, r.rows = rows;
     __syncthreads();
     return true;
 }
@@ -335,7 +337,7 @@ __device__ __forceinline__ void ldmatrix4_trans(uint32_t* r, const void* p) {
 
 template <typename T> __device__ __forceinline__ void mma(float* d, const uint32_t* a, uint32_t b0, uint32_t b1);
 template <> __device__ __forceinline__ void mma<float>(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
         "{%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -343,14 +345,14 @@ template <> __device__ __forceinline__ void mma<float>(float* d, const uint32_t*
 }
 template <>
 __device__ __forceinline__ void mma<__nv_bfloat16>(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
         "{%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 template <> __device__ __forceinline__ void mma<__half>(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
         "{%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -374,13 +376,26 @@ __device__ __forceinline__ Split split_a(uint32_t a0, uint32_t a1, uint32_t a2, 
     split_tf32(a3, f.hi[3], f.lo[3]);
     return f;
 }
-__device__ __forceinline__ void mma_split(float* d, const Split& a, uint32_t b0, uint32_t b1) {
-    uint32_t h0, h1, l0, l1;
-    split_tf32(b0, h0, l0);
-    split_tf32(b1, h1, l1);
-    mma<float>(d, a.lo, h0, h1);
-    mma<float>(d, a.hi, l0, l1);
-    mma<float>(d, a.hi, h0, h1);
+// Two blocks of columns at a time: a step on one accumulator waits for the step before it.
+__device__ __forceinline__ void mma_split2(float* d, float* e, const Split& a, uint32_t b0, uint32_t b1, uint32_t c0,
+                                           uint32_t c1) {
+    uint32_t bh[2], bl[2], ch[2], cl[2];
+    split_tf32(b0, bh[0], bl[0]);
+    split_tf32(b1, bh[1], bl[1]);
+    split_tf32(c0, ch[0], cl[0]);
+    split_tf32(c1, ch[1], cl[1]);
+    mma<float>(d, a.lo, bh[0], bh[1]);
+    mma<float>(e, a.lo, ch[0], ch[1]);
+    mma<float>(d, a.hi, bl[0], bl[1]);
+    mma<float>(e, a.hi, cl[0], cl[1]);
+    mma<float>(d, a.hi, bh[0], bh[1]);
+    mma<float>(e, a.hi, ch[0], ch[1]);
+}
+
+// Stages of a ring: three where that leaves room for three blocks an SM, four or three for two.
+constexpr int fit_stages(int bytes) {
+    return 3 * bytes <= 74 * 1024 ? 3 : 4 * bytes <= 108 * 1024 ? 4 : 3 * bytes <= 108 * 1024 ? 3
+           : 2 * bytes <= 108 * 1024 ? 2 : 3 * bytes <= 216 * 1024 ? 3 : 2;
 }
 
 // ---- shrink --------------------------------------------------------------------
@@ -400,7 +415,7 @@ struct ShrinkCfg {
     static constexpr int W_PITCH = TRANS ? RP * (int)sizeof(T) + 16 : X_PITCH;
     static constexpr int W_BYTES = (TRANS ? KC : RP) * W_PITCH;
     static constexpr int STAGE = X_BYTES + W_BYTES;
-    static constexpr int NS = 3 * STAGE <= 108 * 1024 ? 3 : 2 * STAGE <= 108 * 1024 ? 2 : 3 * STAGE <= 216 * 1024 ? 3 : 2;
+    static constexpr int NS = fit_stages(STAGE);
     static constexpr int RED = WM == 1 ? kWarps * BM * RP * 4 : 0;
     static constexpr int MOST = NS * STAGE > RED ? NS * STAGE : RED;
     static constexpr int SMEM = MOST > (int)sizeof(FindTile) ? MOST : (int)sizeof(FindTile);
@@ -524,10 +539,11 @@ __global__ void __launch_bounds__(kThreads) k_shrink(Plan plan, int tiles, const
                 const Split f0 = split_a(xa.x, xb.x, xa.y, xb.y), f1 = split_a(xa.z, xb.z, xa.w, xb.w);
                 if constexpr (!TRANS) {
 #pragma unroll
-                    for (int b = 0; b < RB; b++) {
-                        const uint4 wv = lds128(ws + (8 * b + g) * C::W_PITCH + (4 * ch + q) * 16);
-                        mma_split(acc[b], f0, wv.x, wv.y);
-                        mma_split(acc[b], f1, wv.z, wv.w);
+                    for (int b = 0; b < RB; b += 2) {
+                        const uint4 wa = lds128(ws + (8 * b + g) * C::W_PITCH + (4 * ch + q) * 16);
+                        const uint4 wb = lds128(ws + (8 * b + 8 + g) * C::W_PITCH + (4 * ch + q) * 16);
+                        mma_split2(acc[b], acc[b + 1], f0, wa.x, wa.y, wb.x, wb.y);
+                        mma_split2(acc[b], acc[b + 1], f1, wa.z, wa.w, wb.z, wb.w);
                     }
                 } else {  // a lane's column of block b is rank RB g + b
 #pragma unroll
@@ -548,7 +564,8 @@ __global__ void __launch_bounds__(kThreads) k_shrink(Plan plan, int tiles, const
                             }
                         }
 #pragma unroll
-                        for (int b = 0; b < RB; b++) mma_split(acc[b], s ? f1 : f0, wv[0][b], wv[1][b]);
+                        for (int b = 0; b < RB; b += 2)
+                            mma_split2(acc[b], acc[b + 1], s ? f1 : f0, wv[0][b], wv[1][b], wv[0][b + 1], wv[1][b + 1]);
                     }
                 }
             } else {
@@ -651,16 +668,18 @@ __device__ __forceinline__ float half_scale(float m) {
 // ---- expand --------------------------------------------------------------------
 // out[t, f] = base[t, f] + sum over ranks of h[t, r] W_i[f, r]; positions without an adapter get base.
 // TRANS = false: W_i = B_i [F, rank]; true: W_i = A_i [rank, F].  base null: zeros.
-// BIG: 128 positions; four warps of 32 along them, two along the columns (fp32 at rank 128, whose h
-// fragments fill the registers: eight of 16).  Else 16 positions and all warps along the columns.  A
+// BIG: 64 positions, half a tile, four warps of 16 along them and two along the columns (16 bits at ranks
+// over 32: the whole tile, warps of 32, which halves the reads of the factors).  Else 16 positions and
+// all warps along the columns.  A
 // warp keeps its positions' h fragments in registers and takes 32 columns at a time, dealt to the MMAs
 // so that a lane ends up with whole 16-byte units of its rows and four lanes with 64 consecutive bytes:
 // unit 4 v + q holds, for fp32, columns 2 (b % 2) + j of blocks b = 2 v, 2 v + 1 (TRANS: columns b of MMA
 // column 2 q + v), for 16 bits columns 2 b + j (TRANS: 4 j + b).
 template <typename T, int RB, bool BIG, bool TRANS>
 struct ExpandCfg {
-    static constexpr int E = kE<T>, RP = 8 * RB, SIZE = sizeof(T), BM = BIG ? 128 : 16;
-    static constexpr int MT = BIG && RP * SIZE < 512 ? 2 : 1, WM = BM / (16 * MT), WF = kWarps / WM;
+    static constexpr int E = kE<T>, RP = 8 * RB, SIZE = sizeof(T);
+    static constexpr int MT = BIG && SIZE == 2 && RB >= 8 ? 2 : 1, WM = BIG ? 4 : 1, WF = kWarps / WM;
+    static constexpr int BM = 16 * MT * WM, PARTS = BIG ? 128 / BM : 1;  // blocks of a tile
     // columns of a stage
     static constexpr int FS = BIG ? (SIZE == 2 && RB <= 4 ? 128 : 64) : RP * SIZE == 512 ? 128 : 256;
     static constexpr int FU = FS / E;  // units of a row
@@ -672,7 +691,7 @@ struct ExpandCfg {
                                          : SIZE == 4 ? (RP == 16 ? 64 : RP * 4 + 64) : (RP == 16 ? 32 : RP * 2 + 32);
     static constexpr int W_BYTES = (TRANS ? RP : FS) * W_PITCH;
     static constexpr int STAGE = B_BYTES + W_BYTES;
-    static constexpr int NS = 3 * STAGE <= 108 * 1024 ? 3 : 2 * STAGE <= 108 * 1024 ? 2 : 3 * STAGE <= 216 * 1024 ? 3 : 2;
+    static constexpr int NS = fit_stages(STAGE);
     static constexpr int SMEM = NS * STAGE;
     static_assert(SMEM <= 220 * 1024, "a block's shared memory");
 };
@@ -708,7 +727,7 @@ __device__ __forceinline__ void copy_rows(const int32_t* row, int rows, const T*
 }
 
 template <typename T, int RB, bool BIG, bool TRANS>
-__global__ void __launch_bounds__(kThreads) k_expand(Plan plan, const float* h, int splits, const T* __restrict__ w,
+__global__ void __launch_bounds__(kThreads, RB * (int)sizeof(T) <= 8 ? 3 : RB * (int)sizeof(T) <= 16 ? 2 : 1) k_expand(Plan plan, const float* h, int splits, const T* __restrict__ w,
                                                      int n, int rank, int64_t F, int64_t f_block, int T_rows,
                                                      const T* base, int64_t ldb, T* out, int64_t ldo, bool bvec,
                                                      bool wvec, bool ovec) {
@@ -722,7 +741,7 @@ __global__ void __launch_bounds__(kThreads) k_expand(Plan plan, const float* h, 
     const int wm = warp % C::WM, wf = warp / C::WM;
     wait_for_previous();
     let_next_start();
-    if (!read_tile<BM>(tr, plan)) return;
+    if (!read_tile<BM, C::PARTS>(tr, plan)) return;
     const int adapter = tr.adapter, rows = tr.rows;
     const int64_t f_begin = blockIdx.y * f_block, f_end = f_begin + f_block < F ? f_begin + f_block : F;
     if (adapter >= n) {  // no adapter: base, or zeros
@@ -858,79 +877,73 @@ __global__ void __launch_bounds__(kThreads) k_expand(Plan plan, const float* h, 
                 for (int b = 0; b < 4; b++)
 #pragma unroll
                     for (int k = 0; k < 4; k++) acc[m][b][k] = 0.f;
-            if constexpr (F32 && !TRANS) {
+            if constexpr (F32) {
 #pragma unroll
-                for (int b = 0; b < 4; b++)
+                for (int c = 0; c < RP / 16; c++) {
+                    uint32_t wv[2][2][4];  // step, rank of the pair, block
+                    if constexpr (!TRANS) {
 #pragma unroll
-                    for (int c = 0; c < RP / 16; c++) {
-                        const uint4 wv = lds128(ws + (fs + 8 * b + g) * C::W_PITCH + (4 * c + q) * 16);
+                        for (int b = 0; b < 4; b++) {
+                            const uint4 v = lds128(ws + (fs + 8 * b + g) * C::W_PITCH + (4 * c + q) * 16);
+                            wv[0][0][b] = v.x, wv[0][1][b] = v.y, wv[1][0][b] = v.z, wv[1][1][b] = v.w;
+                        }
+                    } else {
 #pragma unroll
-                        for (int s = 0; s < 2; s++) {
-                            uint32_t h0, h1, l0, l1;
-                            split_tf32(s ? wv.z : wv.x, h0, l0);
-                            split_tf32(s ? wv.w : wv.y, h1, l1);
-#pragma unroll
-                            for (int m = 0; m < MT; m++) mma<float>(acc[m][b], lo[m][2 * c + s], h0, h1);
-#pragma unroll
-                            for (int m = 0; m < MT; m++) mma<float>(acc[m][b], hi[m][2 * c + s], l0, l1);
-#pragma unroll
-                            for (int m = 0; m < MT; m++) mma<float>(acc[m][b], hi[m][2 * c + s], h0, h1);
+                        for (int r = 0; r < 4; r++) {
+                            const int u = (fs + 16 * (g & 1)) / 4 + (g >> 1);
+                            const uint4 v = lds128(ws + (16 * c + 4 * q + r) * C::W_PITCH + ((u ^ q) * 16));
+                            wv[r >> 1][r & 1][0] = v.x, wv[r >> 1][r & 1][1] = v.y;
+                            wv[r >> 1][r & 1][2] = v.z, wv[r >> 1][r & 1][3] = v.w;
                         }
                     }
-            } else if constexpr (F32) {
 #pragma unroll
-                for (int s = 0; s < KS; s++) {
-                    uint32_t wv[2][4];
+                    for (int s = 0; s < 2; s++) {
+                        uint32_t wh[2][4], wl[2][4];
 #pragma unroll
-                    for (int j = 0; j < 2; j++) {
-                        const int r = 16 * (s >> 1) + 4 * q + 2 * (s & 1) + j;
-                        const int c = (fs + 16 * (g & 1)) / 4 + (g >> 1);
-                        const uint4 v = lds128(ws + r * C::W_PITCH + ((c ^ q) * 16));
-                        wv[j][0] = v.x, wv[j][1] = v.y, wv[j][2] = v.z, wv[j][3] = v.w;
-                    }
+                        for (int b = 0; b < 4; b++) {
+                            split_tf32(wv[s][0][b], wh[0][b], wl[0][b]);
+                            split_tf32(wv[s][1][b], wh[1][b], wl[1][b]);
+                        }
 #pragma unroll
-                    for (int b = 0; b < 4; b++) {
-                        uint32_t h0, h1, l0, l1;
-                        split_tf32(wv[0][b], h0, l0);
-                        split_tf32(wv[1][b], h1, l1);
+                        for (int b = 0; b < 4; b++) mma<float>(acc[0][b], lo[0][2 * c + s], wh[0][b], wh[1][b]);
 #pragma unroll
-                        for (int m = 0; m < MT; m++) mma<float>(acc[m][b], lo[m][s], h0, h1);
+                        for (int b = 0; b < 4; b++) mma<float>(acc[0][b], hi[0][2 * c + s], wl[0][b], wl[1][b]);
 #pragma unroll
-                        for (int m = 0; m < MT; m++) mma<float>(acc[m][b], hi[m][s], l0, l1);
-#pragma unroll
-                        for (int m = 0; m < MT; m++) mma<float>(acc[m][b], hi[m][s], h0, h1);
+                        for (int b = 0; b < 4; b++) mma<float>(acc[0][b], hi[0][2 * c + s], wh[0][b], wh[1][b]);
                     }
                 }
-            } else if constexpr (!TRANS) {
-                // a lane's four ranks 4 q .. 4 q + 3 of a step are the MMA's k = 2 q, 2 q + 1, 2 q + 8, 2 q + 9
-#pragma unroll
-                for (int s = 0; s < KS; s++)
-#pragma unroll
-                    for (int b = 0; b < 4; b++) {
-                        const uint2 wv = *reinterpret_cast<const uint2*>(ws + (fs + 8 * b + g) * C::W_PITCH + 32 * s + 8 * q);
-#pragma unroll
-                        for (int m = 0; m < MT; m++) mma<T>(acc[m][b], lo[m][s], wv.x, wv.y);
-#pragma unroll
-                        for (int m = 0; m < MT; m++) mma<T>(acc[m][b], hi[m][s], wv.x, wv.y);
-                    }
             } else {
 #pragma unroll
                 for (int s = 0; s < KS; s++) {
-                    uint2 wv[4];  // ranks 4 q .. 4 q + 3, columns 4 g .. 4 g + 3
+                    uint32_t w0[4], w1[4];
+                    if constexpr (!TRANS) {
+                        // a lane's four ranks 4 q .. 4 q + 3 of a step are the MMA's k = 2 q, 2 q + 1, 2 q + 8, 2 q + 9
 #pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        wv[j] = *reinterpret_cast<const uint2*>(ws + (16 * s + 4 * q + j) * C::W_PITCH +
-                                                                (((fs / 8 + (g >> 1)) ^ (q << 1)) * 16) + (g & 1) * 8);
+                        for (int b = 0; b < 4; b++) {
+                            const uint2 v = *reinterpret_cast<const uint2*>(ws + (fs + 8 * b + g) * C::W_PITCH + 32 * s + 8 * q);
+                            w0[b] = v.x, w1[b] = v.y;
+                        }
+                    } else {
+                        uint2 v[4];  // ranks 4 q .. 4 q + 3, columns 4 g .. 4 g + 3
 #pragma unroll
-                    for (int b = 0; b < 4; b++) {
-                        const uint32_t pick = (b & 1) ? 0x7632u : 0x5410u;
-                        const uint32_t b0 = __byte_perm(b < 2 ? wv[0].x : wv[0].y, b < 2 ? wv[1].x : wv[1].y, pick);
-                        const uint32_t b1 = __byte_perm(b < 2 ? wv[2].x : wv[2].y, b < 2 ? wv[3].x : wv[3].y, pick);
+                        for (int j = 0; j < 4; j++)
+                            v[j] = *reinterpret_cast<const uint2*>(ws + (16 * s + 4 * q + j) * C::W_PITCH +
+                                                                   (((fs / 8 + (g >> 1)) ^ (q << 1)) * 16) + (g & 1) * 8);
 #pragma unroll
-                        for (int m = 0; m < MT; m++) mma<T>(acc[m][b], lo[m][s], b0, b1);
-#pragma unroll
-                        for (int m = 0; m < MT; m++) mma<T>(acc[m][b], hi[m][s], b0, b1);
+                        for (int b = 0; b < 4; b++) {
+                            const uint32_t pick = (b & 1) ? 0x7632u : 0x5410u;
+                            w0[b] = __byte_perm(b < 2 ? v[0].x : v[0].y, b < 2 ? v[1].x : v[1].y, pick);
+                            w1[b] = __byte_perm(b < 2 ? v[2].x : v[2].y, b < 2 ? v[3].x : v[3].y, pick);
+                        }
                     }
+#pragma unroll
+                    for (int b = 0; b < 4; b++)
+#pragma unroll
+                        for (int m = 0; m < MT; m++) mma<T>(acc[m][b], lo[m][s], w0[b], w1[b]);
+#pragma unroll
+                    for (int b = 0; b < 4; b++)
+#pragma unroll
+                        for (int m = 0; m < MT; m++) mma<T>(acc[m][b], hi[m][s], w0[b], w1[b]);
                 }
             }
 #pragma unroll
@@ -1142,7 +1155,8 @@ __global__ void __launch_bounds__(kThreads) k_weight(Plan plan, const int32_t* _
                 for (int m = 0; m < RM; m++) {
                     const Split fa = split_a(hr[0][2 * m], hr[0][2 * m + 1], hr[1][2 * m], hr[1][2 * m + 1]);
 #pragma unroll
-                    for (int b = 0; b < NB; b++) mma_split(acc[m][b], fa, xv[0][b], xv[1][b]);
+                    for (int b = 0; b < NB; b += 2)
+                        mma_split2(acc[m][b], acc[m][b + 1], fa, xv[0][b], xv[1][b], xv[0][b + 1], xv[1][b + 1]);
                 }
             }
 #pragma unroll
@@ -1171,10 +1185,9 @@ __global__ void __launch_bounds__(kThreads) k_weight(Plan plan, const int32_t* _
                     ldmatrix4_trans(fh, p);
                     ldmatrix4_trans(fl, p + TK * C::H_PITCH);
 #pragma unroll
-                    for (int b = 0; b < NB; b++) {
-                        mma<T>(acc[m][b], fl, fb[b][0], fb[b][1]);
-                        mma<T>(acc[m][b], fh, fb[b][0], fb[b][1]);
-                    }
+                    for (int b = 0; b < NB; b++) mma<T>(acc[m][b], fl, fb[b][0], fb[b][1]);
+#pragma unroll
+                    for (int b = 0; b < NB; b++) mma<T>(acc[m][b], fh, fb[b][0], fb[b][1]);
                 }
             }
         }
@@ -1346,10 +1359,10 @@ template <typename T, int RB, int WM, bool TRANS>
 int run_expand(const Shape& s, const Plan& plan, const float* h, int splits, const T* w, int64_t F, const T* base,
                int64_t ldb, T* out, int64_t ldo, cudaStream_t st) {
     using C = ExpandCfg<T, RB, WM == 8, TRANS>;
-    // columns of a block: whole stages, for about four blocks an SM
-    const int64_t passes = ceil_div(F, C::FS), want = ceil_div(4 * kSms, s.tiles);
+    // columns of a block: whole stages, for about eight blocks an SM
+    const int64_t passes = ceil_div(F, C::FS), want = ceil_div(8 * kSms, s.tiles * C::PARTS);
     const int64_t f_block = ceil_div(passes, want < passes ? want : passes) * C::FS;
-    return start(k_expand<T, RB, WM == 8, TRANS>, dim3((unsigned)s.tiles, (unsigned)ceil_div(F, f_block)), kThreads,
+    return start(k_expand<T, RB, WM == 8, TRANS>, dim3((unsigned)(s.tiles * C::PARTS), (unsigned)ceil_div(F, f_block)), kThreads,
                  C::SMEM, true, st, plan, h, splits, w, s.n, s.rank, F, f_block, (int)s.T, base, ldb, out, ldo,
                  base && row_units(base, ldb), row_units(w, TRANS ? F : s.rank), row_units((const T*)out, ldo));
 }
