@@ -30,7 +30,7 @@
 
 #include <cooperative_groups.h>
 
-#include "engram_common.cuh"
+#include "engram_tensor.cuh"
 
 using namespace engram;
 
@@ -54,7 +54,7 @@ struct Tile {
 struct Plan {
     int32_t* off;    // [n + 2]
     int32_t* perm;   // [T]
-    int32_t* tiles;  // [1]: number of tiles; null: as many as blocks
+    int32_t* tiles;  // [2]: number of tiles, of those with an adapter (they come first); null: as many as blocks
     Tile* tile;      // [max tiles]
 };
 
@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_plan(const int32_t* __restrict
     __syncthreads();
     if (blockIdx.x == 0) {
         for (int i = tid; i <= n; i += kPlanThreads) plan.off[i] = cnt[i];
-        if (tid == 0) plan.off[n + 1] = T, *plan.tiles = n_tiles;
+        if (tid == 0) plan.off[n + 1] = T, plan.tiles[0] = n_tiles, plan.tiles[1] = tile0[n];
     }
     for (int k = blockIdx.x * kPlanThreads + tid; k < n_tiles; k += gridDim.x * kPlanThreads) {
         int lo = 0, hi = n + 1;  // the adapter with tile0[a] <= k < tile0[a + 1]
@@ -281,8 +281,6 @@ template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t u)
 template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t u) {
     return __half22float2(*reinterpret_cast<const __half2*>(&u));
 }
-
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
 // One 16-byte unit of a stage from src, of which `left` elements exist (the others become zero).
 // vec: src is 16-byte aligned: asynchronous; else element by element.
@@ -977,6 +975,434 @@ __global__ void __launch_bounds__(kThreads, RB * (int)sizeof(T) <= 8 ? 3 : RB * 
     }
 }
 
+// ---- expand on the tcgen05 tensor cores -------------------------------------------
+// The same product, TRANS = false, for many positions, rows of base and out that start on 16 bytes and whole
+// groups of 32 columns (fp32: 16).  What the kernel above spends its time on is instructions, 400 to 500 a
+// 32 x 32 piece; here the products and the factors' way to them cost the streaming warps nothing:
+//   warps 0-15  out = base + accumulator, from shared memory and tensor memory straight to memory (out's
+//               way through shared memory and TMA added three hops of barriers a stage: half the rate);
+//   warp 20     base's rows, NB stages of 32 KB ahead: by TMA for each 32 positions that follow one another
+//               in memory, else by cp.async (gathered by TMA, tile::gather4, 512 bytes took 32 ns);
+//   warp 16     the factors' tiles by TMA, NS stages ahead;
+//   warp 17     one lane issues the MMAs, D [128 positions, FS columns] = H_hi W^T + H_lo W^T (fp32: in TF32,
+//               H_lo W^T + H_hi W_lo^T + H_hi W^T; the tensor cores read W as its head), into four
+//               accumulators in turn;
+//   warp 18     h of a new tile, split, into the A operand's layout;
+//   warp 19     fp32: the factors' remainders W_lo.
+// An accumulator is read in the 16x256b form: a lane gets columns 2 q, 2 q + 1 of each 8 of rows g and g + 8.
+// The factors' rows are loaded in an order (a five-dimensional tensor map) that makes a lane's columns of 32
+// (fp32: 16) one 16-byte unit of the row: column 8 k + 2 q + j of the product is feature 8 q + 2 k + j (fp32: 4 q
+// + 2 k + j).  Blocks are persistent, one an SM, and share all (tile, stage) pairs evenly in their order.
+// Every wait is bounded: one that gives up ends its warp's loop (results stay unwritten).
+template <typename T, int RB>
+struct WideCfg {
+    static constexpr int SIZE = sizeof(T), RP = 8 * RB, BM = 128;
+    static constexpr bool F32 = SIZE == 4;
+    static constexpr int GROUP = F32 ? 16 : 32, FS = 4 * GROUP, BLOCKS = GROUP / 8;  // columns of a warp, of a stage
+    // the rank's extent in the operands: rows of SPAN bytes (the swizzle), in blocks of all rows
+    static constexpr int SPAN = RP * SIZE < 128 ? RP * SIZE : 128, KB = RP * SIZE / SPAN;
+    static constexpr int H_BYTES = BM * RP * SIZE, W_BYTES = FS * RP * SIZE;
+    static constexpr int STAGE = W_BYTES * (F32 ? 2 : 1), NS = RP * SIZE >= 256 ? 2 : 3;
+    static constexpr int BLOCK = BM * 128, B_BYTES = 2 * BLOCK;  // base: 256 bytes of each row, in two blocks
+    static constexpr int NB = (220 * 1024 - 2 * H_BYTES - NS * STAGE) / B_BYTES;
+    static constexpr int SMEM = 2 * H_BYTES + NS * STAGE + NB * B_BYTES + 1024;
+    static constexpr bool OK = NB >= 2;
+    static constexpr uint32_t SWIZZLE = SPAN == 128 ? 2 : SPAN == 64 ? 4 : 6;
+};
+
+constexpr int kWideThreads = 672;
+constexpr long long kWideSpins = 1 << 20;  // polls of a barrier before a wait gives up: over ten milliseconds
+
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %3, %3, %4}], "
+        "[%5];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(0), "r"(y), "r"(bar)
+        : "memory");
+}
+
+// Arrives once this thread's cp.async copies so far have landed.
+__device__ __forceinline__ void mbar_arrive_copies(uint32_t bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+// Descriptor of a tile of rows of SPAN bytes along K: 8-row groups 8 SPAN apart.
+template <typename C>
+__device__ __forceinline__ uint64_t wide_desc(uint32_t addr) {
+    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)1 << 16) | ((uint64_t)(8 * C::SPAN >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)C::SWIZZLE << 61);
+}
+
+template <typename T>
+__device__ __forceinline__ void wide_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t desc, uint32_t accumulate) {
+    if constexpr (sizeof(T) == 4)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::tf32 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+            "l"(a), "l"(b), "r"(desc), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+            "l"(a), "l"(b), "r"(desc), "r"(accumulate)
+            : "memory");
+}
+
+// The place in the (tile, stage) order, and the tile's adapter.
+struct WideStep {
+    int tile, stage, per_tile, n;
+    bool real;
+    __device__ __forceinline__ bool start(const Plan& plan, int64_t at, int per, int adapters) {
+        tile = (int)(at / per), stage = (int)(at % per), per_tile = per, n = adapters;
+        return true;
+    }
+    // Called at step i; true where a tile begins.
+    __device__ __forceinline__ bool next(int i) {
+        if (i && ++stage == per_tile) {
+            tile++, stage = 0;
+            return true;
+        }
+        return i == 0;
+    }
+};
+
+template <typename T, int RB>
+__global__ void __launch_bounds__(kWideThreads, 1) k_expand_wide(const __grid_constant__ CUtensorMap w_map,
+                                                                 const __grid_constant__ CUtensorMap b_map, Plan plan,
+                                                                 const float* h, int splits, int n, int64_t F,
+                                                                 int T_rows, const T* base, int64_t ldb, T* out,
+                                                                 int64_t ldo) {
+    using C = WideCfg<T, RB>;
+    constexpr int RP = C::RP, FS = C::FS, NS = C::NS, NB = C::NB, SPAN = C::SPAN, KB = C::KB, SIZE = C::SIZE, BM = C::BM;
+    constexpr bool F32 = SIZE == 4;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* planes = smem + NS * C::STAGE;     // H_hi, H_lo
+    uint8_t* rows_at = planes + 2 * C::H_BYTES;  // base's stages
+    __shared__ uint64_t bars[3 * NS + 2 * NB + 10];
+    __shared__ uint32_t tmem_slot;
+    __shared__ float undo[6][BM];  // fp16: the rows' scales taken back, of the tiles that can be in flight
+    const uint32_t full = smem_u32(bars), low = full + 8 * NS, empty = low + 8 * NS, acc_full = empty + 8 * NS;
+    const uint32_t acc_empty = acc_full + 32, h_full = acc_empty + 32, h_empty = h_full + 8;
+    const uint32_t b_full = h_empty + 8, b_empty = b_full + 8 * NB;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < NS; i++) {
+            mbar_init(full + 8 * i, 1);
+            mbar_init(low + 8 * i, 1);
+            mbar_init(empty + 8 * i, 1);
+        }
+        for (int i = 0; i < 4; i++) {
+            mbar_init(acc_full + 8 * i, 1);
+            mbar_init(acc_empty + 8 * i, 16);
+        }
+        mbar_init(h_full, 1);
+        mbar_init(h_empty, 1);
+        for (int i = 0; i < NB; i++) {
+            mbar_init(b_full + 8 * i, 33);  // warp 20's lanes, and its bytes
+            mbar_init(b_empty + 8 * i, 16);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 17) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
+                     "r"((uint32_t)(4 * FS))
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = tmem_slot;
+    wait_for_previous();
+    let_next_start();
+
+    // this block's share of the (tile, stage) pairs; in place, positions without an adapter stay as they are
+    const int per_tile = (int)((F + FS - 1) / FS);
+    const int64_t total = (int64_t)(base == out ? plan.tiles[1] : plan.tiles[0]) * per_tile;
+    const int64_t begin = total * blockIdx.x / gridDim.x, end = total * (blockIdx.x + 1) / gridDim.x;
+    const int steps = (int)(end - begin);
+    const int real_tiles = plan.tiles[1];  // the tiles with an adapter come first
+    WideStep at;
+    at.start(plan, begin, per_tile, n);
+
+    if (warp < 16) {
+        // rows g, g + 8, g + 16, g + 24 of the warp's 32; unit q of its columns
+        const int quarter = warp & 3, part = warp >> 2, g = lane >> 2, q = lane & 3;
+        int row[4], tiles = 0, made = 0;
+        bool ok = true;
+        for (int i = 0; i < steps && ok; i++) {
+            if (at.next(i)) {
+                const Tile t = plan.tile[at.tile];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const int p = 32 * quarter + 8 * k + g;
+                    row[k] = p < t.rows ? plan.perm[t.start + p] : -1;
+                }
+                tiles += at.tile < real_tiles;
+            }
+            const int64_t f = (int64_t)at.stage * FS + part * C::GROUP;
+            const bool real = at.tile < real_tiles;
+            const int a = made & 3;
+            uint32_t r[2][4 * C::BLOCKS];  // columns 2 b + j of unit q: r[4 b + j], rows 8 below: r[4 b + 2 + j]
+            if (real) {
+                ok = mbar_wait(acc_full + 8 * a, (uint32_t)((made >> 2) & 1), nullptr, kWideSpins);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+                for (int m = 0; m < 2; m++) {
+                    const uint32_t from =
+                        tmem + ((uint32_t)(32 * quarter + 16 * m) << 16) + (uint32_t)(a * FS + part * C::GROUP);
+                    if constexpr (F32)
+                        asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                                     : "=r"(r[m][0]), "=r"(r[m][1]), "=r"(r[m][2]), "=r"(r[m][3]), "=r"(r[m][4]),
+                                       "=r"(r[m][5]), "=r"(r[m][6]), "=r"(r[m][7])
+                                     : "r"(from));
+                    else
+                        asm volatile(
+                            "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+                            "%12, %13, %14, %15}, [%16];"
+                            : "=r"(r[m][0]), "=r"(r[m][1]), "=r"(r[m][2]), "=r"(r[m][3]), "=r"(r[m][4]), "=r"(r[m][5]),
+                              "=r"(r[m][6]), "=r"(r[m][7]), "=r"(r[m][8]), "=r"(r[m][9]), "=r"(r[m][10]),
+                              "=r"(r[m][11]), "=r"(r[m][12]), "=r"(r[m][13]), "=r"(r[m][14]), "=r"(r[m][15])
+                            : "r"(from));
+                }
+            }
+            uint4 v[4];
+            if (base) {
+                const int s = i % NB;
+                ok = ok && mbar_wait(b_full + 8 * s, (uint32_t)((i / NB) & 1), nullptr, kWideSpins);
+                const uint8_t* from = rows_at + s * C::B_BYTES + (part >> 1) * C::BLOCK;
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const int m = 32 * quarter + 8 * k + g;
+                    v[k] = lds128(from + m * 128 + (((4 * (part & 1) + q) ^ g) << 4));
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; k++) v[k] = make_uint4(0, 0, 0, 0);
+            }
+            float back[4] = {1.f, 1.f, 1.f, 1.f};
+            if (real) {
+                if constexpr (std::is_same_v<T, __half>) {
+#pragma unroll
+                    for (int k = 0; k < 4; k++) back[k] = undo[(tiles - 1) % 6][32 * quarter + 8 * k + g];
+                }
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    uint32_t* w = reinterpret_cast<uint32_t*>(&v[k]);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        if constexpr (F32) {
+                            w[e] = bits_of(__uint_as_float(w[e]) +
+                                           __uint_as_float(r[k >> 1][4 * (e >> 1) + 2 * (k & 1) + (e & 1)]));
+                        } else {
+                            const float2 b = unpack2<T>(w[e]);
+                            w[e] = pack2<T>(fmaf(back[k], __uint_as_float(r[k >> 1][4 * e + 2 * (k & 1)]), b.x),
+                                            fmaf(back[k], __uint_as_float(r[k >> 1][4 * e + 2 * (k & 1) + 1]), b.y));
+                        }
+                    }
+                }
+            }
+            __syncwarp();  // the lanes have read base's stage and the accumulator
+            if (lane == 0) {
+                if (base) mbar_arrive(b_empty + 8 * (i % NB));
+                if (real) mbar_arrive(acc_empty + 8 * a);
+            }
+            made += real;
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if (ok && row[k] >= 0 && f < F)
+                    *reinterpret_cast<uint4*>(out + (int64_t)row[k] * ldo + f + q * (16 / SIZE)) = v[k];
+        }
+    } else if (warp == 20) {
+        int row[4], first[4], count = 0, i = 0;
+        bool run[4];
+        for (; base && i < steps; i++) {
+            if (at.next(i)) {
+                const Tile t = plan.tile[at.tile];
+                count = t.rows;
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const int p = 32 * k + lane;
+                    row[k] = plan.perm[t.start + min(p, t.rows - 1)];
+                    first[k] = __shfl_sync(0xffffffffu, row[k], 0);
+                    run[k] = __all_sync(0xffffffffu, p < t.rows && row[k] == first[k] + lane);
+                }
+            }
+            const int s = i % NB;
+            if (i >= NB && !mbar_wait(b_empty + 8 * s, (uint32_t)((i / NB - 1) & 1), nullptr, kWideSpins)) break;
+            const uint32_t bar = b_full + 8 * s, to = smem_u32(rows_at + s * C::B_BYTES);
+            if (lane == 0) mbar_expect_tx(bar, (run[0] + run[1] + run[2] + run[3]) * 8192);
+            __syncwarp();
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+#pragma unroll
+                for (int b = 0; b < 2; b++) {
+                    const int x = at.stage * FS + b * (128 / SIZE);
+                    const uint32_t dst = to + b * C::BLOCK + k * 4096;
+                    if (run[k]) {
+                        if (lane == 0) tma_load_2d(dst, &b_map, x, first[k], bar);
+                    } else if (32 * k < count) {
+                        const int64_t f = x + (lane & 7) * (16 / SIZE);
+                        const int bytes = f < F ? 16 : 0;
+#pragma unroll
+                        for (int j = 0; j < 8; j++) {
+                            const int m = 4 * j + (lane >> 3), t = __shfl_sync(0xffffffffu, row[k], m);
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                                             dst + m * 128 + (((lane & 7) ^ (m & 7)) << 4)),
+                                         "l"(bytes ? base + (int64_t)t * ldb + f : base), "r"(bytes)
+                                         : "memory");
+                        }
+                    }
+                }
+            }
+            mbar_arrive_copies(bar);
+        }
+        for (int k = i > NB ? i - NB : 0; k < i; k++)
+            mbar_wait(b_full + 8 * (k % NB), (uint32_t)((k / NB) & 1), nullptr, kWideSpins);
+    } else if (warp == 16) {
+        if (lane == 0) {
+            int made = 0;
+            int adapter = 0;
+            for (int i = 0; i < steps; i++) {
+                if (at.next(i) && at.tile < real_tiles) adapter = plan.tile[at.tile].adapter;
+                if (at.tile >= real_tiles) break;
+                const int s = made % NS;
+                if (made >= NS && !mbar_wait(empty + 8 * s, (uint32_t)((made / NS - 1) & 1), nullptr, kWideSpins)) break;
+                const uint32_t bar = full + 8 * s, to = smem_u32(smem + s * C::STAGE);
+                mbar_expect_tx(bar, C::W_BYTES);
+                const int y = (int)(((int64_t)adapter * F + (int64_t)at.stage * FS) / C::GROUP);
+#pragma unroll
+                for (int b = 0; b < KB; b++) tma_load_5d(to + b * FS * SPAN, &w_map, b * (SPAN / SIZE), y, bar);
+                made++;
+            }
+            for (int k = made > NS ? made - NS : 0; k < made; k++)
+                mbar_wait(full + 8 * (k % NS), (uint32_t)((k / NS) & 1), nullptr, kWideSpins);
+        }
+    } else if (warp == 17) {
+        if (lane == 0) {
+            constexpr uint32_t type = F32 ? 2u : std::is_same_v<T, __nv_bfloat16> ? 1u : 0u;
+            constexpr uint32_t desc =
+                (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)(FS >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+            int tiles = 0, made = 0;
+            bool ok = true;
+            for (int i = 0; i < steps && ok; i++) {
+                const bool first = at.next(i);
+                if (at.tile >= real_tiles) break;
+                if (first) ok = mbar_wait(h_full, (uint32_t)(tiles++ & 1), nullptr, kWideSpins);
+                const int s = made % NS, a = made & 3;
+                ok = ok && mbar_wait((F32 ? low : full) + 8 * s, (uint32_t)((made / NS) & 1), nullptr, kWideSpins);
+                if (made >= 4) ok = ok && mbar_wait(acc_empty + 8 * a, (uint32_t)((made / 4 - 1) & 1), nullptr, kWideSpins);
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t hh = smem_u32(planes), hl = hh + C::H_BYTES;
+                const uint32_t w = smem_u32(smem + s * C::STAGE), wl = w + C::W_BYTES, d = tmem + a * FS;
+#pragma unroll
+                for (int k = 0; k < RP * SIZE / 32; k++) {  // 32 bytes of the rank a step, the small terms first
+                    constexpr int PER = SPAN / 32;
+                    const uint32_t ho = (k / PER) * BM * SPAN + (k % PER) * 32, wo = (k / PER) * FS * SPAN + (k % PER) * 32;
+                    wide_mma<T>(d, wide_desc<C>(hl + ho), wide_desc<C>(w + wo), desc, k > 0);
+                    if (F32) wide_mma<T>(d, wide_desc<C>(hh + ho), wide_desc<C>(wl + wo), desc, 1);
+                    wide_mma<T>(d, wide_desc<C>(hh + ho), wide_desc<C>(w + wo), desc, 1);
+                }
+                umma_commit(acc_full + 8 * a);
+                umma_commit(empty + 8 * s);
+                if (i + 1 == steps || at.stage + 1 == per_tile) umma_commit(h_empty);  // h's planes have been read
+                made++;
+            }
+        }
+        __syncwarp();
+    } else if (warp == 18) {
+        int tiles = 0;
+        for (int i = 0; i < steps; i++) {
+            if (!at.next(i)) continue;
+            if (at.tile >= real_tiles) break;
+            const Tile t = plan.tile[at.tile];
+            if (tiles && !mbar_wait(h_empty, (uint32_t)((tiles - 1) & 1), nullptr, kWideSpins)) break;
+#pragma unroll 1
+            for (int m = 0; m < BM; m += 32) {  // a row a lane
+                const int r = m + lane;
+                const float* hp = h + (int64_t)plan.perm[t.start + min(r, t.rows - 1)] * RP;
+                float s = 1.f;
+                if constexpr (std::is_same_v<T, __half>) {
+                    float most = 0.f;
+                    for (int c = 0; c < RP; c += 4) {
+                        const float4 f = load_h(hp + c, splits, (int64_t)T_rows * RP);
+                        most = fmaxf(fmaxf(fmaxf(most, fabsf(f.x)), fmaxf(fabsf(f.y), fabsf(f.z))), fabsf(f.w));
+                    }
+                    s = half_scale(most);
+                    undo[tiles % 6][r] = 1.f / s;
+                }
+#pragma unroll 4
+                for (int c = 0; c < RP; c += 16 / SIZE) {
+                    uint4 hi, lo;
+                    uint32_t *ph = reinterpret_cast<uint32_t*>(&hi), *pl = reinterpret_cast<uint32_t*>(&lo);
+                    const float4 f = load_h(hp + c, splits, (int64_t)T_rows * RP);
+                    if constexpr (F32) {
+                        split_tf32(bits_of(f.x), ph[0], pl[0]);
+                        split_tf32(bits_of(f.y), ph[1], pl[1]);
+                        split_tf32(bits_of(f.z), ph[2], pl[2]);
+                        split_tf32(bits_of(f.w), ph[3], pl[3]);
+                    } else {
+                        const float4 e = load_h(hp + c + 4, splits, (int64_t)T_rows * RP);
+                        const float v[8] = {f.x * s, f.y * s, f.z * s, f.w * s, e.x * s, e.y * s, e.z * s, e.w * s};
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            ph[k] = pack2<T>(v[2 * k], v[2 * k + 1]);
+                            const float2 b = unpack2<T>(ph[k]);
+                            pl[k] = pack2<T>(v[2 * k] - b.x, v[2 * k + 1] - b.y);
+                        }
+                    }
+                    const int byte = c * SIZE, unit = (byte % SPAN) >> 4;
+                    const int turn = SPAN == 128 ? r & 7 : SPAN == 64 ? (r >> 1) & 3 : (r >> 2) & 1;
+                    uint8_t* to = planes + (byte / SPAN) * BM * SPAN + r * SPAN + ((unit ^ turn) << 4);
+                    *reinterpret_cast<uint4*>(to) = hi;
+                    *reinterpret_cast<uint4*>(to + C::H_BYTES) = lo;
+                }
+            }
+            fence_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(h_full);
+            tiles++;
+        }
+    } else if (warp == 19 && F32) {
+        int made = 0;
+        for (int i = 0; i < steps; i++) {
+            at.next(i);
+            if (at.tile >= real_tiles) break;
+            const int s = made % NS;
+            if (!mbar_wait(full + 8 * s, (uint32_t)((made / NS) & 1), nullptr, kWideSpins)) break;
+            uint8_t* w = smem + s * C::STAGE;
+#pragma unroll 4
+            for (int u = lane; u < C::W_BYTES / 16; u += 32) {
+                uint4 v = *reinterpret_cast<const uint4*>(w + 16 * u);
+                uint32_t* p = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+                for (int k = 0; k < 4; k++) p[k] = bits_of(__uint_as_float(p[k]) - __uint_as_float(p[k] & 0xffffe000u));
+                *reinterpret_cast<uint4*>(w + C::W_BYTES + 16 * u) = v;
+            }
+            fence_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(low + 8 * s);
+            made++;
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 17) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)(4 * FS))
+                     : "memory");
+    }
+}
+
 // ---- weight gradients ------------------------------------------------------------
 // G_i = sum over adapter i's positions of x[t, f] h[t, r].  TRANS = false: G_i stored [rank, F] (dA,
 // with h = dh); true: stored [F, rank] (dB, with x = the gradient of out).  Both in one launch: blocks up
@@ -1284,7 +1710,7 @@ Layout layout_of(const Shape& s, bool backward) {
     };
     l.off = take((int64_t)(s.n + 2) * 4);
     l.perm = take(s.planned ? s.T * 4 : s.tiles * 16 * s.wm * 4);
-    l.tiles = take(4);
+    l.tiles = take(8);
     l.tile = take(s.tiles * (int64_t)sizeof(Tile));
     l.h = take((int64_t)s.splits_k * s.T * 8 * s.rb * 4);
     if (backward) l.dh = take((int64_t)s.splits_n * s.T * 8 * s.rb * 4);
@@ -1355,10 +1781,47 @@ int run_sum(const Shape& s, float* h, int h_splits, float* dh, int dh_splits, cu
                  reinterpret_cast<float4*>(h), h_splits, reinterpret_cast<float4*>(dh), dh_splits, count4);
 }
 
+template <typename T, int RB>
+int run_expand_wide(const Shape& s, const Plan& plan, const float* h, int splits, const T* w, int64_t F, const T* base,
+                    int64_t ldb, T* out, int64_t ldo, cudaStream_t st) {
+    using C = WideCfg<T, RB>;
+    constexpr CUtensorMapSwizzle span = C::SPAN == 128 ? CU_TENSOR_MAP_SWIZZLE_128B
+                                        : C::SPAN == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B;
+    const auto fn = encode_fn();
+    if (!fn) return ENGRAM_ERR_CUDA;
+    constexpr CUtensorMapDataType type = C::F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                         : std::is_same_v<T, __half> ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                     : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    // feature of a group = BLOCKS 2 q + 2 k + j, in the order (j, q, k)
+    const cuuint64_t row = (cuuint64_t)s.rank * sizeof(T);
+    const cuuint64_t dims[5] = {(cuuint64_t)s.rank, 2, 4, C::BLOCKS, (cuuint64_t)(s.n * F / C::GROUP)};
+    const cuuint64_t strides[4] = {row, 2 * C::BLOCKS * row, 2 * row, C::GROUP * row};
+    const cuuint32_t box[5] = {C::SPAN / C::SIZE, 2, 4, C::BLOCKS, 4}, step[5] = {1, 1, 1, 1, 1};
+    CUtensorMap map;
+    if (fn(&map, type, 5, const_cast<T*>(w), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, span,
+           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        return ENGRAM_ERR_CUDA;
+    CUtensorMap rows;
+    memset(&rows, 0, sizeof(rows));
+    const cuuint64_t row_dims[2] = {(cuuint64_t)F, (cuuint64_t)s.T}, row_strides[1] = {(cuuint64_t)ldb * sizeof(T)};
+    const cuuint32_t row_box[2] = {128 / C::SIZE, 32};
+    if (base && fn(&rows, type, 2, const_cast<T*>(base), row_dims, row_strides, row_box, step,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        return ENGRAM_ERR_CUDA;
+    return start(k_expand_wide<T, RB>, dim3((unsigned)sm_count()), kWideThreads, C::SMEM, true, st, map, rows, plan, h,
+                 splits, s.n, F, (int)s.T, base, ldb, out, ldo);
+}
+
 template <typename T, int RB, int WM, bool TRANS>
 int run_expand(const Shape& s, const Plan& plan, const float* h, int splits, const T* w, int64_t F, const T* base,
                int64_t ldb, T* out, int64_t ldo, cudaStream_t st) {
     using C = ExpandCfg<T, RB, WM == 8, TRANS>;
+    if constexpr (WM == 8 && !TRANS && WideCfg<T, RB>::OK) {
+        if (s.planned && s.n > 0 && F % WideCfg<T, RB>::GROUP == 0 && s.n * F / WideCfg<T, RB>::GROUP < (1ll << 31) &&
+            (!base || row_units(base, ldb)) && row_units((const T*)out, ldo) && row_units(w, s.rank))
+            return run_expand_wide<T, RB>(s, plan, h, splits, w, F, base, ldb, out, ldo, st);
+    }
     // columns of a block: whole stages, for about eight blocks an SM
     const int64_t passes = ceil_div(F, C::FS), want = ceil_div(8 * kSms, s.tiles * C::PARTS);
     const int64_t f_block = ceil_div(passes, want < passes ? want : passes) * C::FS;

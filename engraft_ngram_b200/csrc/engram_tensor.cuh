@@ -33,8 +33,8 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
     return ok != 0;
 }
 // Bounded wait for the phase with the given parity; false (and *err raised) on timeout.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int* err) {
-    for (long long it = 0; it < kSpinLimit; it++)
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int* err, long long limit = kSpinLimit) {
+    for (long long it = 0; it < limit; it++)
         if (mbar_try_wait(bar, parity)) return true;
     if (err) atomicAdd(err, 1);
     return false;

@@ -98,6 +98,42 @@ def test_forward_and_gradients_match_the_formula(case):
         grad, c["x"], c["a"], c["b"], c["index"], c["scale"])))
 
 
+# many positions and rows on 16 bytes: the tensor-memory kernel, at each of its operand layouts (rows of 32, 64,
+# 128 and more bytes of the rank), ranks that end inside one, widths that end inside a stage and inside 128 bytes
+WIDE = [(1500, 96, 264, 16, 3, F32, "random"), (1300, 64, 520, 12, 2, F32, "segments"), (1200, 128, 100, 32, 4, F32, "random"),
+        (1100, 64, 1300, 64, 3, F32, "random"), (1400, 72, 264, 128, 2, F32, "random"),
+        (1500, 128, 264, 16, 3, BF16, "random"), (1300, 64, 520, 8, 2, BF16, "segments"), (1200, 136, 104, 32, 4, BF16, "random"),
+        (1100, 64, 1304, 64, 3, BF16, "random"), (1400, 72, 264, 128, 2, BF16, "segments"), (1030, 64, 264, 24, 1, BF16, "0"),
+        (1500, 128, 264, 16, 3, F16, "random"), (1200, 136, 104, 40, 4, F16, "segments"), (1100, 64, 776, 128, 3, F16, "random"),
+        (20000, 64, 136, 16, 5, BF16, "segments"), (9000, 64, 72, 16, 2, F32, "random"), (1100, 64, 264, 16, 2, F32, "none")]
+
+
+@pytest.mark.parametrize("case", WIDE, ids=str)
+def test_many_positions(case):
+    test_forward_and_gradients_match_the_formula(case)
+    c, _ = make(*case)
+    want = eb.adapter_add(**c)
+    held = c["base"].clone()
+    assert torch.equal(eb.adapter_add(held, *list(c.values())[1:], out=held), want)
+    wide = torch.full((case[0], case[2] + 24), 7.0, dtype=case[5], device=DEV)
+    eb.adapter_add(**c, out=wide[:, 8:8 + case[2]])
+    assert torch.equal(wide[:, 8:8 + case[2]], want) and (wide[:, :8] == 7).all() and (wide[:, 8 + case[2]:] == 7).all()
+    zeros = {**c, "base": torch.zeros_like(c["base"])}
+    assert torch.equal(eb.adapter_add(None, *list(c.values())[1:]), eb.adapter_add(**zeros))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=str)
+def test_large_and_small_positions_side_by_side(dtype):
+    """One position's values 1e4 times another's: each keeps its own accuracy."""
+    c, grad = make(1200, 64, 256, 16, 2, dtype, "random", seed=12)
+    c["x"][::5] *= 100 if dtype == F16 else 1e4
+    c["x"][1::5] /= 100 if dtype == F16 else 1e4
+    c["base"].zero_()
+    if dtype == F16:
+        c["b"] /= 64  # keeps the results inside the type
+    check(eb.adapter_add(**c), formula(c, grad)[0], formula(c, grad, mag=True)[0], 80, dtype)
+
+
 def test_rows_without_an_adapter_keep_base_bit_for_bit_and_their_inputs_are_not_read():
     c, grad = make(100, 64, 48, 8, 4, F32, "random", seed=3)
     c["index"][::3] = -1
