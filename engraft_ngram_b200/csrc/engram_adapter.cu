@@ -979,10 +979,10 @@ __global__ void __launch_bounds__(kThreads, RB * (int)sizeof(T) <= 8 ? 3 : RB * 
 // The same product, TRANS = false, for many positions, rows of base and out that start on 16 bytes and whole
 // groups of 32 columns (fp32: 16).  What the kernel above spends its time on is instructions, 400 to 500 a
 // 32 x 32 piece; here the products and the factors' way to them cost the streaming warps nothing:
-//   warps 0-15  out = base + accumulator, from shared memory and tensor memory straight to memory (out's
-//               way through shared memory and TMA added three hops of barriers a stage: half the rate);
-//   warp 20     base's rows, NB stages of 32 KB ahead: by TMA for each 32 positions that follow one another
-//               in memory, else by cp.async (gathered by TMA, tile::gather4, 512 bytes took 32 ns);
+//   warps 0-15  out = base + accumulator, 16 positions x 256 bytes a warp and stage, eight warps a stage in
+//               turn.  A lane fetches the units of base that it will add to by cp.async into a place of
+//               its own, DEPTH of its stages ahead (64 KB in flight an SM each), so base needs no barriers;
+//               with base and out on TMA and mbarriers this took 1.5 to 2 times as long;
 //   warp 16     the factors' tiles by TMA, NS stages ahead;
 //   warp 17     one lane issues the MMAs, D [128 positions, FS columns] = H_hi W^T + H_lo W^T (fp32: in TF32,
 //               H_lo W^T + H_hi W_lo^T + H_hi W^T; the tensor cores read W as its head), into four
@@ -1003,14 +1003,14 @@ struct WideCfg {
     static constexpr int SPAN = RP * SIZE < 128 ? RP * SIZE : 128, KB = RP * SIZE / SPAN;
     static constexpr int H_BYTES = BM * RP * SIZE, W_BYTES = FS * RP * SIZE;
     static constexpr int STAGE = W_BYTES * (F32 ? 2 : 1), NS = RP * SIZE >= 256 ? 2 : 3;
-    static constexpr int BLOCK = BM * 128, B_BYTES = 2 * BLOCK;  // base: 256 bytes of each row, in two blocks
-    static constexpr int NB = (220 * 1024 - 2 * H_BYTES - NS * STAGE) / B_BYTES;
-    static constexpr int SMEM = 2 * H_BYTES + NS * STAGE + NB * B_BYTES + 1024;
-    static constexpr bool OK = NB >= 2;
+    static constexpr int FETCH = 16 * 4096;  // a stage of all sixteen warps
+    static constexpr int FIT = (220 * 1024 - 2 * H_BYTES - NS * STAGE) / FETCH, DEPTH = FIT > 2 ? 2 : FIT;
+    static constexpr int SMEM = 2 * H_BYTES + NS * STAGE + DEPTH * FETCH + 1024;
+    static constexpr bool OK = DEPTH >= 1;
     static constexpr uint32_t SWIZZLE = SPAN == 128 ? 2 : SPAN == 64 ? 4 : 6;
 };
 
-constexpr int kWideThreads = 672;
+constexpr int kWideThreads = 640;
 constexpr long long kWideSpins = 1 << 20;  // polls of a barrier before a wait gives up: over ten milliseconds
 
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
@@ -1023,11 +1023,6 @@ __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map
         "[%5];" ::"r"(dst),
         "l"(map), "r"(x), "r"(0), "r"(y), "r"(bar)
         : "memory");
-}
-
-// Arrives once this thread's cp.async copies so far have landed.
-__device__ __forceinline__ void mbar_arrive_copies(uint32_t bar) {
-    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 
 // Descriptor of a tile of rows of SPAN bytes along K: 8-row groups 8 SPAN apart.
@@ -1053,43 +1048,40 @@ __device__ __forceinline__ void wide_mma(uint32_t d, uint64_t a, uint64_t b, uin
             : "memory");
 }
 
-// The place in the (tile, stage) order, and the tile's adapter.
+// The place in the (tile, stage) order.
 struct WideStep {
-    int tile, stage, per_tile, n;
-    bool real;
-    __device__ __forceinline__ bool start(const Plan& plan, int64_t at, int per, int adapters) {
-        tile = (int)(at / per), stage = (int)(at % per), per_tile = per, n = adapters;
-        return true;
+    int tile, stage, per_tile;
+    __device__ __forceinline__ void start(int64_t at, int per) {
+        tile = (int)(at / per), stage = (int)(at % per), per_tile = per;
     }
-    // Called at step i; true where a tile begins.
-    __device__ __forceinline__ bool next(int i) {
-        if (i && ++stage == per_tile) {
-            tile++, stage = 0;
-            return true;
-        }
-        return i == 0;
+    // k steps on; true where that is another tile.
+    __device__ __forceinline__ bool move(int k) {
+        stage += k;
+        bool other = false;
+        while (stage >= per_tile) stage -= per_tile, tile++, other = true;
+        return other;
     }
+    // Called at step i, one by one; true where a tile begins.
+    __device__ __forceinline__ bool next(int i) { return i ? move(1) : true; }
 };
 
 template <typename T, int RB>
-__global__ void __launch_bounds__(kWideThreads, 1) k_expand_wide(const __grid_constant__ CUtensorMap w_map,
-                                                                 const __grid_constant__ CUtensorMap b_map, Plan plan,
+__global__ void __launch_bounds__(kWideThreads, 1) k_expand_wide(const __grid_constant__ CUtensorMap w_map, Plan plan,
                                                                  const float* h, int splits, int n, int64_t F,
                                                                  int T_rows, const T* base, int64_t ldb, T* out,
                                                                  int64_t ldo) {
     using C = WideCfg<T, RB>;
-    constexpr int RP = C::RP, FS = C::FS, NS = C::NS, NB = C::NB, SPAN = C::SPAN, KB = C::KB, SIZE = C::SIZE, BM = C::BM;
+    constexpr int RP = C::RP, FS = C::FS, NS = C::NS, SPAN = C::SPAN, KB = C::KB, SIZE = C::SIZE, BM = C::BM;
     constexpr bool F32 = SIZE == 4;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* planes = smem + NS * C::STAGE;     // H_hi, H_lo
-    uint8_t* rows_at = planes + 2 * C::H_BYTES;  // base's stages
-    __shared__ uint64_t bars[3 * NS + 2 * NB + 10];
+    uint8_t* fetched = planes + 2 * C::H_BYTES;  // base: [DEPTH][warp][8][lane] units
+    __shared__ uint64_t bars[3 * NS + 10];
     __shared__ uint32_t tmem_slot;
     __shared__ float undo[6][BM];  // fp16: the rows' scales taken back, of the tiles that can be in flight
     const uint32_t full = smem_u32(bars), low = full + 8 * NS, empty = low + 8 * NS, acc_full = empty + 8 * NS;
     const uint32_t acc_empty = acc_full + 32, h_full = acc_empty + 32, h_empty = h_full + 8;
-    const uint32_t b_full = h_empty + 8, b_empty = b_full + 8 * NB;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < NS; i++) {
@@ -1099,14 +1091,10 @@ __global__ void __launch_bounds__(kWideThreads, 1) k_expand_wide(const __grid_co
         }
         for (int i = 0; i < 4; i++) {
             mbar_init(acc_full + 8 * i, 1);
-            mbar_init(acc_empty + 8 * i, 16);
+            mbar_init(acc_empty + 8 * i, 8);
         }
         mbar_init(h_full, 1);
         mbar_init(h_empty, 1);
-        for (int i = 0; i < NB; i++) {
-            mbar_init(b_full + 8 * i, 33);  // warp 20's lanes, and its bytes
-            mbar_init(b_empty + 8 * i, 16);
-        }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 17) {
@@ -1129,144 +1117,124 @@ __global__ void __launch_bounds__(kWideThreads, 1) k_expand_wide(const __grid_co
     const int steps = (int)(end - begin);
     const int real_tiles = plan.tiles[1];  // the tiles with an adapter come first
     WideStep at;
-    at.start(plan, begin, per_tile, n);
+    at.start(begin, per_tile);
 
     if (warp < 16) {
-        // rows g, g + 8, g + 16, g + 24 of the warp's 32; unit q of its columns
-        const int quarter = warp & 3, part = warp >> 2, g = lane >> 2, q = lane & 3;
-        int row[4], tiles = 0, made = 0;
-        bool ok = true;
-        for (int i = 0; i < steps && ok; i++) {
-            if (at.next(i)) {
-                const Tile t = plan.tile[at.tile];
+        // rows g and g + 8 of the warp's 16, units 4 c + q of their 256 bytes; steps first, first + 2, ..
+        const int quarter = warp & 3, half = (warp >> 2) & 1, first = warp >> 3, g = lane >> 2, q = lane & 3;
+        constexpr int E = 16 / SIZE;
+        const uint32_t place = smem_u32(fetched) + warp * 4096 + lane * 16;
+        int row[2], row_ahead[2];
+        const auto read_rows = [&](int (&r)[2], int tile) {
+            const Tile t = plan.tile[tile];
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const int p = 32 * quarter + 8 * k + g;
-                    row[k] = p < t.rows ? plan.perm[t.start + p] : -1;
-                }
-                tiles += at.tile < real_tiles;
+            for (int k = 0; k < 2; k++) {
+                const int p = 32 * quarter + 16 * half + 8 * k + g;
+                r[k] = p < t.rows ? plan.perm[t.start + p] : -1;
             }
-            const int64_t f = (int64_t)at.stage * FS + part * C::GROUP;
-            const bool real = at.tile < real_tiles;
-            const int a = made & 3;
-            uint32_t r[2][4 * C::BLOCKS];  // columns 2 b + j of unit q: r[4 b + j], rows 8 below: r[4 b + 2 + j]
-            if (real) {
-                ok = mbar_wait(acc_full + 8 * a, (uint32_t)((made >> 2) & 1), nullptr, kWideSpins);
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        };
+        WideStep ahead = at;
+        bool there = false;  // row_ahead is ahead.tile's
+        ahead.move(first);
+        const auto fetch = [&](int i, int slot) {
+            if (i < steps && base) {
+                if (!there) read_rows(row_ahead, ahead.tile);
 #pragma unroll
-                for (int m = 0; m < 2; m++) {
-                    const uint32_t from =
-                        tmem + ((uint32_t)(32 * quarter + 16 * m) << 16) + (uint32_t)(a * FS + part * C::GROUP);
-                    if constexpr (F32)
-                        asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                                     : "=r"(r[m][0]), "=r"(r[m][1]), "=r"(r[m][2]), "=r"(r[m][3]), "=r"(r[m][4]),
-                                       "=r"(r[m][5]), "=r"(r[m][6]), "=r"(r[m][7])
-                                     : "r"(from));
-                    else
-                        asm volatile(
-                            "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
-                            "%12, %13, %14, %15}, [%16];"
-                            : "=r"(r[m][0]), "=r"(r[m][1]), "=r"(r[m][2]), "=r"(r[m][3]), "=r"(r[m][4]), "=r"(r[m][5]),
-                              "=r"(r[m][6]), "=r"(r[m][7]), "=r"(r[m][8]), "=r"(r[m][9]), "=r"(r[m][10]),
-                              "=r"(r[m][11]), "=r"(r[m][12]), "=r"(r[m][13]), "=r"(r[m][14]), "=r"(r[m][15])
-                            : "r"(from));
-                }
-            }
-            uint4 v[4];
-            if (base) {
-                const int s = i % NB;
-                ok = ok && mbar_wait(b_full + 8 * s, (uint32_t)((i / NB) & 1), nullptr, kWideSpins);
-                const uint8_t* from = rows_at + s * C::B_BYTES + (part >> 1) * C::BLOCK;
+                for (int k = 0; k < 2; k++)
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const int m = 32 * quarter + 8 * k + g;
-                    v[k] = lds128(from + m * 128 + (((4 * (part & 1) + q) ^ g) << 4));
-                }
-            } else {
-#pragma unroll
-                for (int k = 0; k < 4; k++) v[k] = make_uint4(0, 0, 0, 0);
-            }
-            float back[4] = {1.f, 1.f, 1.f, 1.f};
-            if (real) {
-                if constexpr (std::is_same_v<T, __half>) {
-#pragma unroll
-                    for (int k = 0; k < 4; k++) back[k] = undo[(tiles - 1) % 6][32 * quarter + 8 * k + g];
-                }
-                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    uint32_t* w = reinterpret_cast<uint32_t*>(&v[k]);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        if constexpr (F32) {
-                            w[e] = bits_of(__uint_as_float(w[e]) +
-                                           __uint_as_float(r[k >> 1][4 * (e >> 1) + 2 * (k & 1) + (e & 1)]));
-                        } else {
-                            const float2 b = unpack2<T>(w[e]);
-                            w[e] = pack2<T>(fmaf(back[k], __uint_as_float(r[k >> 1][4 * e + 2 * (k & 1)]), b.x),
-                                            fmaf(back[k], __uint_as_float(r[k >> 1][4 * e + 2 * (k & 1) + 1]), b.y));
-                        }
-                    }
-                }
-            }
-            __syncwarp();  // the lanes have read base's stage and the accumulator
-            if (lane == 0) {
-                if (base) mbar_arrive(b_empty + 8 * (i % NB));
-                if (real) mbar_arrive(acc_empty + 8 * a);
-            }
-            made += real;
-#pragma unroll
-            for (int k = 0; k < 4; k++)
-                if (ok && row[k] >= 0 && f < F)
-                    *reinterpret_cast<uint4*>(out + (int64_t)row[k] * ldo + f + q * (16 / SIZE)) = v[k];
-        }
-    } else if (warp == 20) {
-        int row[4], first[4], count = 0, i = 0;
-        bool run[4];
-        for (; base && i < steps; i++) {
-            if (at.next(i)) {
-                const Tile t = plan.tile[at.tile];
-                count = t.rows;
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const int p = 32 * k + lane;
-                    row[k] = plan.perm[t.start + min(p, t.rows - 1)];
-                    first[k] = __shfl_sync(0xffffffffu, row[k], 0);
-                    run[k] = __all_sync(0xffffffffu, p < t.rows && row[k] == first[k] + lane);
-                }
-            }
-            const int s = i % NB;
-            if (i >= NB && !mbar_wait(b_empty + 8 * s, (uint32_t)((i / NB - 1) & 1), nullptr, kWideSpins)) break;
-            const uint32_t bar = b_full + 8 * s, to = smem_u32(rows_at + s * C::B_BYTES);
-            if (lane == 0) mbar_expect_tx(bar, (run[0] + run[1] + run[2] + run[3]) * 8192);
-            __syncwarp();
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-#pragma unroll
-                for (int b = 0; b < 2; b++) {
-                    const int x = at.stage * FS + b * (128 / SIZE);
-                    const uint32_t dst = to + b * C::BLOCK + k * 4096;
-                    if (run[k]) {
-                        if (lane == 0) tma_load_2d(dst, &b_map, x, first[k], bar);
-                    } else if (32 * k < count) {
-                        const int64_t f = x + (lane & 7) * (16 / SIZE);
-                        const int bytes = f < F ? 16 : 0;
-#pragma unroll
-                        for (int j = 0; j < 8; j++) {
-                            const int m = 4 * j + (lane >> 3), t = __shfl_sync(0xffffffffu, row[k], m);
-                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
-                                             dst + m * 128 + (((lane & 7) ^ (m & 7)) << 4)),
-                                         "l"(bytes ? base + (int64_t)t * ldb + f : base), "r"(bytes)
+                    for (int c = 0; c < 4; c++) {
+                        const int64_t f = (int64_t)ahead.stage * FS + c * C::GROUP + q * E;
+                        if (row_ahead[k] >= 0 && f < F)
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                                             place + slot * C::FETCH + (4 * k + c) * 512),
+                                         "l"(base + (int64_t)row_ahead[k] * ldb + f)
                                          : "memory");
-                        }
+                    }
+                there = !ahead.move(2);
+            }
+            stage_done();
+        };
+#pragma unroll
+        for (int d = 0; d < C::DEPTH; d++) fetch(first + 2 * d, d);
+        at.move(first);
+        bool ok = true, fresh = true;
+        int slot = 0;
+        const int tile_first = (int)(begin / per_tile);
+        for (int i = first; i < steps && ok; i += 2) {
+            if (fresh) read_rows(row, at.tile);
+            const bool real = at.tile < real_tiles;
+            const int a = i & 3;
+            if (real) {
+                ok = mbar_wait(acc_full + 8 * a, (uint32_t)((i >> 2) & 1), nullptr, kWideSpins);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            }
+            stage_wait<C::DEPTH - 1>();
+            float back[2] = {1.f, 1.f};
+            if constexpr (std::is_same_v<T, __half>) {
+                if (real)
+#pragma unroll
+                    for (int k = 0; k < 2; k++)
+                        back[k] = undo[(at.tile - tile_first) % 6][32 * quarter + 16 * half + 8 * k + g];
+            }
+#pragma unroll
+            for (int c2 = 0; c2 < 4; c2 += 2) {
+                uint32_t r[2][4 * C::BLOCKS];  // columns 2 b + j of unit q: r[4 b + j], rows 8 below: r[4 b + 2 + j]
+                if (real) {
+#pragma unroll
+                    for (int m = 0; m < 2; m++) {
+                        const uint32_t from = tmem + ((uint32_t)(32 * quarter + 16 * half) << 16) +
+                                              (uint32_t)(a * FS + (c2 + m) * C::GROUP);
+                        if constexpr (F32)
+                            asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                                         : "=r"(r[m][0]), "=r"(r[m][1]), "=r"(r[m][2]), "=r"(r[m][3]), "=r"(r[m][4]),
+                                           "=r"(r[m][5]), "=r"(r[m][6]), "=r"(r[m][7])
+                                         : "r"(from));
+                        else
+                            asm volatile(
+                                "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+                                "%11, %12, %13, %14, %15}, [%16];"
+                                : "=r"(r[m][0]), "=r"(r[m][1]), "=r"(r[m][2]), "=r"(r[m][3]), "=r"(r[m][4]),
+                                  "=r"(r[m][5]), "=r"(r[m][6]), "=r"(r[m][7]), "=r"(r[m][8]), "=r"(r[m][9]),
+                                  "=r"(r[m][10]), "=r"(r[m][11]), "=r"(r[m][12]), "=r"(r[m][13]), "=r"(r[m][14]),
+                                  "=r"(r[m][15])
+                                : "r"(from));
+                    }
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    if (c2 == 2) {  // the accumulator, and the rows' scales, have been read
+                        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(acc_empty + 8 * a);
                     }
                 }
+#pragma unroll
+                for (int m = 0; m < 2; m++)
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        const int c = c2 + m;
+                        const int64_t f = (int64_t)at.stage * FS + c * C::GROUP + q * E;
+                        uint4 v = make_uint4(0, 0, 0, 0);
+                        if (base) v = lds128(fetched + warp * 4096 + lane * 16 + slot * C::FETCH + (4 * k + c) * 512);
+                        uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+                        if (real) {
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                if constexpr (F32) {
+                                    w[e] = bits_of(__uint_as_float(w[e]) +
+                                                   __uint_as_float(r[m][4 * (e >> 1) + 2 * k + (e & 1)]));
+                                } else {
+                                    const float2 b = unpack2<T>(w[e]);
+                                    w[e] = pack2<T>(fmaf(back[k], __uint_as_float(r[m][4 * e + 2 * k]), b.x),
+                                                    fmaf(back[k], __uint_as_float(r[m][4 * e + 2 * k + 1]), b.y));
+                                }
+                            }
+                        }
+                        if (ok && row[k] >= 0 && f < F) *reinterpret_cast<uint4*>(out + (int64_t)row[k] * ldo + f) = v;
+                    }
             }
-            mbar_arrive_copies(bar);
+            fetch(i + 2 * C::DEPTH, slot);
+            slot = slot + 1 == C::DEPTH ? 0 : slot + 1;
+            fresh = at.move(2);
         }
-        for (int k = i > NB ? i - NB : 0; k < i; k++)
-            mbar_wait(b_full + 8 * (k % NB), (uint32_t)((k / NB) & 1), nullptr, kWideSpins);
     } else if (warp == 16) {
         if (lane == 0) {
             int made = 0;
@@ -1801,15 +1769,7 @@ int run_expand_wide(const Shape& s, const Plan& plan, const float* h, int splits
     if (fn(&map, type, 5, const_cast<T*>(w), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, span,
            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return ENGRAM_ERR_CUDA;
-    CUtensorMap rows;
-    memset(&rows, 0, sizeof(rows));
-    const cuuint64_t row_dims[2] = {(cuuint64_t)F, (cuuint64_t)s.T}, row_strides[1] = {(cuuint64_t)ldb * sizeof(T)};
-    const cuuint32_t row_box[2] = {128 / C::SIZE, 32};
-    if (base && fn(&rows, type, 2, const_cast<T*>(base), row_dims, row_strides, row_box, step,
-                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-        return ENGRAM_ERR_CUDA;
-    return start(k_expand_wide<T, RB>, dim3((unsigned)sm_count()), kWideThreads, C::SMEM, true, st, map, rows, plan, h,
+    return start(k_expand_wide<T, RB>, dim3((unsigned)sm_count()), kWideThreads, C::SMEM, true, st, map, plan, h,
                  splits, s.n, F, (int)s.T, base, ldb, out, ldo);
 }
 
