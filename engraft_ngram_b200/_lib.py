@@ -220,5 +220,14 @@ def stream_of(device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def on_device(device, call):
+    """call(stream) with the device current (a launch goes to the current device) and its current stream."""
+    import torch
+    if device.index == torch.cuda.current_device():
+        return call(torch.cuda.current_stream().cuda_stream)
+    with torch.cuda.device(device):
+        return call(torch.cuda.current_stream().cuda_stream)
+
+
 def ptr(t) -> int | None:
     return None if t is None else t.data_ptr()

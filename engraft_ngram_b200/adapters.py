@@ -19,6 +19,7 @@ same inputs, the same bits.
 """
 from __future__ import annotations
 
+import functools
 from dataclasses import dataclass
 
 import torch
@@ -46,85 +47,90 @@ def _rows(x: torch.Tensor, name: str, T: int, width: int, like: torch.Tensor) ->
     """The row stride of a [T, width] operand (its elements of a row consecutive)."""
     if x.dtype != like.dtype or x.device != like.device:
         raise ValueError(f"{name}: {x.dtype} on {x.device}, but x is {like.dtype} on {like.device}")
-    if x.dim() != 2 or x.shape[0] != T or x.shape[1] != width:
+    if x.shape != (T, width):
         raise ValueError(f"{name}: shape {tuple(x.shape)}, expected {(T, width)}")
-    ld = x.stride(0) if T > 1 else width
-    if (width > 1 and x.stride(1) != 1) or ld < width:
-        raise ValueError(f"{name}: strides {tuple(x.stride())}: the elements of a row have to be consecutive "
+    rows, columns = x.stride()
+    ld = rows if T > 1 else width
+    if (width > 1 and columns != 1) or ld < width:
+        raise ValueError(f"{name}: strides {(rows, columns)}: the elements of a row have to be consecutive "
                          "and its rows apart")
     return ld
 
 
-def _check(x, a, b, index, scale) -> tuple[int, int, int, int, int, int]:
-    """(dtype code, T, K, N, rank, adapters) of a call."""
-    code = _DTYPES.get(x.dtype)
-    if code is None or not x.is_cuda or x.dim() != 2:
-        raise ValueError(f"x: needs a [T, K] float32, bfloat16 or float16 CUDA tensor (got {x.dtype} "
-                         f"{tuple(x.shape)} on {x.device})")
-    if a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2]:
-        raise ValueError(f"a {tuple(a.shape)}, b {tuple(b.shape)}: expected [adapters, rank, K] and "
-                         "[adapters, N, rank]")
-    T, K = x.shape
-    n, rank, N = a.shape[0], a.shape[1], b.shape[1]
-    if a.shape[2] != K:
-        raise ValueError(f"a {tuple(a.shape)}: its last dimension has to be x's {K}")
+@functools.lru_cache(maxsize=256)
+def _plan(dtype, x_shape, a_shape, b_shape, backward: int):
+    """(dtype code, T, K, N, rank, adapters, workspace bytes) of a call's types and shapes."""
+    code = _DTYPES.get(dtype)
+    if code is None or len(x_shape) != 2:
+        raise ValueError(f"x: needs a [T, K] float32, bfloat16 or float16 CUDA tensor (got {dtype} {tuple(x_shape)})")
+    if len(a_shape) != 3 or len(b_shape) != 3 or a_shape[0] != b_shape[0] or a_shape[1] != b_shape[2]:
+        raise ValueError(f"a {tuple(a_shape)}, b {tuple(b_shape)}: expected [adapters, rank, K] and [adapters, N, rank]")
+    T, K = x_shape
+    n, rank, N = a_shape[0], a_shape[1], b_shape[1]
+    if a_shape[2] != K:
+        raise ValueError(f"a {tuple(a_shape)}: its last dimension has to be x's {K}")
     if not 1 <= rank <= MAX_RANK or n > MAX_ADAPTERS or K < 1 or N < 1:
         raise ValueError(f"rank {rank}, {n} adapters, {K} -> {N}: ranks are 1 to {MAX_RANK}, at most {MAX_ADAPTERS} "
                          "adapters, widths at least 1")
-    for name, f in (("a", a), ("b", b)):
-        if f.dtype != x.dtype or f.device != x.device or not f.is_contiguous():
-            raise ValueError(f"{name}: needs a contiguous {x.dtype} tensor on {x.device} (got {f.dtype} on {f.device}, "
-                             f"strides {tuple(f.stride())})")
-    if index.dtype != torch.int32 or index.device != x.device or index.shape != (T,) or not index.is_contiguous():
-        raise ValueError(f"index: needs a contiguous int32 [{T}] tensor on {x.device} (got {index.dtype} "
-                         f"{tuple(index.shape)} on {index.device})")
-    if scale is not None and (scale.dtype != torch.float32 or scale.device != x.device or scale.shape != (n,)
-                              or not scale.is_contiguous()):
-        raise ValueError(f"scale: needs a contiguous float32 [{n}] tensor on {x.device} (got {scale.dtype} "
-                         f"{tuple(scale.shape)} on {scale.device})")
-    return code, T, K, N, rank, n
-
-
-def _workspace(lib, T, n, rank, K, N, backward, device) -> torch.Tensor:
-    size = lib.engram_adapter_workspace_bytes(T, n, rank, K, N, backward)
+    size = L.load().engram_adapter_workspace_bytes(T, n, rank, K, N, backward)
     L.check(min(size, 0), "engram_adapter_workspace_bytes")
-    return torch.empty(max(size, 1), dtype=torch.uint8, device=device)
+    return code, T, K, N, rank, n, max(size, 1)
+
+
+def _check(x, a, b, index, scale, backward: int):
+    if not x.is_cuda:
+        raise ValueError(f"x: needs a CUDA tensor (got {x.dtype} on {x.device})")
+    plan = _plan(x.dtype, x.shape, a.shape, b.shape, backward)
+    dtype, dev = x.dtype, x.device
+    if a.dtype != dtype or b.dtype != dtype or a.device != dev or b.device != dev or not a.is_contiguous() \
+            or not b.is_contiguous():
+        for name, f in (("a", a), ("b", b)):
+            if f.dtype != dtype or f.device != dev or not f.is_contiguous():
+                raise ValueError(f"{name}: needs a contiguous {dtype} tensor on {dev} (got {f.dtype} on {f.device}, "
+                                 f"strides {tuple(f.stride())})")
+    if index.dtype != torch.int32 or index.device != dev or index.shape != (plan[1],) or not index.is_contiguous():
+        raise ValueError(f"index: needs a contiguous int32 [{plan[1]}] tensor on {dev} (got {index.dtype} "
+                         f"{tuple(index.shape)} on {index.device})")
+    if scale is not None and (scale.dtype != torch.float32 or scale.device != dev or scale.shape != (plan[5],)
+                              or not scale.is_contiguous()):
+        raise ValueError(f"scale: needs a contiguous float32 [{plan[5]}] tensor on {dev} (got {scale.dtype} "
+                         f"{tuple(scale.shape)} on {scale.device})")
+    return plan
 
 
 def forward_into(out, base, x, a, b, index, scale) -> torch.Tensor:
     """out (None: a new tensor) = base (None: zeros) + the adapters' product; no autograd.  out may be base."""
-    code, T, K, N, rank, n = _check(x, a, b, index, scale)
+    code, T, K, N, rank, n, ws_bytes = _check(x, a, b, index, scale, 0)
     dev = x.device
-    if out is None:
-        out = torch.empty(T, N, dtype=x.dtype, device=dev)
-    ldx, ldout = _rows(x, "x", T, K, x), _rows(out, "out", T, N, x)
+    given = out is not None
+    if not given:
+        out = x.new_empty((T, N))
+    ldx = _rows(x, "x", T, K, x)
+    ldout = _rows(out, "out", T, N, x) if given else N
     ldbase = _rows(base, "base", T, N, x) if base is not None else 0
-    lib = L.load()
-    with torch.cuda.device(dev):
-        ws = _workspace(lib, T, n, rank, K, N, 0, dev)
-        st = lib.engram_adapter_forward(code, x.data_ptr(), ldx, a.data_ptr(), b.data_ptr(), index.data_ptr(),
-                                        L.ptr(scale), T, n, rank, K, N, L.ptr(base), ldbase, out.data_ptr(), ldout,
-                                        ws.data_ptr(), ws.numel(), L.stream_of(dev))
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    st = L.on_device(dev, lambda stream: L.load().engram_adapter_forward(
+        code, x.data_ptr(), ldx, a.data_ptr(), b.data_ptr(), index.data_ptr(), None if scale is None else scale.data_ptr(),
+        T, n, rank, K, N, None if base is None else base.data_ptr(), ldbase, out.data_ptr(), ldout, ws.data_ptr(),
+        ws_bytes, stream))
     L.check(st, "engram_adapter_forward")
-    torch.autograd.graph.increment_version(out)
+    if given:
+        torch.autograd.graph.increment_version(out)
     return out
 
 
 def backward_into(grad, x, a, b, index, scale, dx=None, dx_base=None, da=None, db=None) -> None:
     """The gradients wanted (dx, da, db given) of the adapters' product; dx = dx_base (None: zeros) + its own
     part, and dx_base may be dx."""
-    code, T, K, N, rank, n = _check(x, a, b, index, scale)
+    code, T, K, N, rank, n, ws_bytes = _check(x, a, b, index, scale, 1)
     dev = x.device
     ldx, ldg = _rows(x, "x", T, K, x), _rows(grad, "grad", T, N, x)
     lddx = _rows(dx, "dx", T, K, x) if dx is not None else 0
     ldbase = _rows(dx_base, "dx_base", T, K, x) if dx_base is not None else 0
-    lib = L.load()
-    with torch.cuda.device(dev):
-        ws = _workspace(lib, T, n, rank, K, N, 1, dev)
-        st = lib.engram_adapter_backward(code, grad.data_ptr(), ldg, x.data_ptr(), ldx, a.data_ptr(), b.data_ptr(),
-                                         index.data_ptr(), L.ptr(scale), T, n, rank, K, N, L.ptr(dx_base), ldbase,
-                                         L.ptr(dx), lddx, L.ptr(da), L.ptr(db), ws.data_ptr(), ws.numel(),
-                                         L.stream_of(dev))
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    st = L.on_device(dev, lambda stream: L.load().engram_adapter_backward(
+        code, grad.data_ptr(), ldg, x.data_ptr(), ldx, a.data_ptr(), b.data_ptr(), index.data_ptr(), L.ptr(scale), T, n,
+        rank, K, N, L.ptr(dx_base), ldbase, L.ptr(dx), lddx, L.ptr(da), L.ptr(db), ws.data_ptr(), ws_bytes, stream))
     L.check(st, "engram_adapter_backward")
 
 

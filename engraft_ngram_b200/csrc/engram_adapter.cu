@@ -1692,13 +1692,27 @@ Plan plan_at(uint8_t* ws, const Shape& s, const Layout& l) {
                 s.planned ? reinterpret_cast<int32_t*>(ws + l.tiles) : nullptr, reinterpret_cast<Tile*>(ws + l.tile)};
 }
 
+template <typename... P, typename... A>
+cudaError_t launch(void (*kernel)(P...), const cudaLaunchConfig_t& cfg, A... args) {
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
 // Starts a kernel; after = true: it may start while the launch before it still runs (it waits for that
 // one's results itself, griddepcontrol.wait), which hides the start and its first loads.
-template <typename... P, typename... A>
-int start(void (*kernel)(P...), dim3 grid, int threads, int smem, bool after, cudaStream_t st, A... args) {
-    if (smem > 48 * 1024 &&
-        cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-        return ENGRAM_ERR_CUDA;
+// MOST: the most dynamic shared memory a launch of the kernel takes (0: always `smem`).
+template <auto KERNEL, int MOST = 0, typename... A>
+int start(dim3 grid, int threads, int smem, bool after, cudaStream_t st, A... args) {
+    if (smem > 48 * 1024 || MOST > 48 * 1024) {
+        static bool allowed[64] = {false};
+        int dev = 0;
+        cudaGetDevice(&dev);
+        if (dev < 0 || dev >= 64 || !allowed[dev]) {
+            if (cudaFuncSetAttribute((const void*)KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     MOST ? MOST : smem) != cudaSuccess)
+                return ENGRAM_ERR_CUDA;
+            if (dev >= 0 && dev < 64) allowed[dev] = true;
+        }
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3((unsigned)threads);
@@ -1714,7 +1728,7 @@ int start(void (*kernel)(P...), dim3 grid, int threads, int smem, bool after, cu
         attr[cfg.numAttrs++].val.clusterDim = {1, 1, grid.z};
     }
     cfg.attrs = attr;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+    const cudaError_t e = launch(KERNEL, cfg, args...);
     count_launches(1);
     return e == cudaSuccess && cudaGetLastError() == cudaSuccess ? ENGRAM_OK : ENGRAM_ERR_CUDA;
 }
@@ -1722,7 +1736,7 @@ int start(void (*kernel)(P...), dim3 grid, int threads, int smem, bool after, cu
 int run_plan(const Shape& s, const int32_t* index, const Plan& plan, cudaStream_t st) {
     if (!s.planned) return ENGRAM_OK;
     const int chunk = (int)ceil_div(ceil_div(s.T, 128), kPlanThreads) * kPlanThreads;
-    return start(k_plan, dim3((unsigned)ceil_div(s.T, chunk)), kPlanThreads, (3 * s.n + 4) * 4, false, st, index,
+    return start<k_plan, (3 * kMaxAdapters + 4) * 4>(dim3((unsigned)ceil_div(s.T, chunk)), kPlanThreads, (3 * s.n + 4) * 4, false, st, index,
                  (int)s.T, s.n, chunk, 16 * s.wm, plan);
 }
 
@@ -1737,7 +1751,7 @@ int run_shrink(const Shape& s, const Plan& plan, const int32_t* index, const T* 
     using C = ShrinkCfg<T, RB, WM, TRANS>;
     const int64_t k_split = ceil_div(ceil_div(K, splits), C::KC) * C::KC;
     const bool find = first && !s.planned;
-    return start(k_shrink<T, RB, WM, TRANS>, dim3((unsigned)s.tiles, (unsigned)splits), kThreads, C::SMEM, !find, st,
+    return start<k_shrink<T, RB, WM, TRANS>>(dim3((unsigned)s.tiles, (unsigned)splits), kThreads, C::SMEM, !find, st,
                  plan, (int)(find ? FIND : PLANNED), index, x, ldx, w, scale, s.n, s.rank, K, k_split, (int)s.T,
                  row_units(x, ldx), row_units(w, TRANS ? s.rank : K), h);
 }
@@ -1745,7 +1759,7 @@ int run_shrink(const Shape& s, const Plan& plan, const int32_t* index, const T* 
 int run_sum(const Shape& s, float* h, int h_splits, float* dh, int dh_splits, cudaStream_t st) {
     if (h_splits == 1 && dh_splits == 1) return ENGRAM_OK;
     const int64_t count4 = s.T * 2 * s.rb;
-    return start(k_sum_splits, dim3((unsigned)ceil_div(count4, kThreads), 2), kThreads, 0, true, st,
+    return start<k_sum_splits>(dim3((unsigned)ceil_div(count4, kThreads), 2), kThreads, 0, true, st,
                  reinterpret_cast<float4*>(h), h_splits, reinterpret_cast<float4*>(dh), dh_splits, count4);
 }
 
@@ -1769,7 +1783,7 @@ int run_expand_wide(const Shape& s, const Plan& plan, const float* h, int splits
     if (fn(&map, type, 5, const_cast<T*>(w), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, span,
            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return ENGRAM_ERR_CUDA;
-    return start(k_expand_wide<T, RB>, dim3((unsigned)sm_count()), kWideThreads, C::SMEM, true, st, map, plan, h,
+    return start<k_expand_wide<T, RB>>(dim3((unsigned)sm_count()), kWideThreads, C::SMEM, true, st, map, plan, h,
                  splits, s.n, F, (int)s.T, base, ldb, out, ldo);
 }
 
@@ -1785,7 +1799,7 @@ int run_expand(const Shape& s, const Plan& plan, const float* h, int splits, con
     // columns of a block: whole stages, for about eight blocks an SM
     const int64_t passes = ceil_div(F, C::FS), want = ceil_div(8 * kSms, s.tiles * C::PARTS);
     const int64_t f_block = ceil_div(passes, want < passes ? want : passes) * C::FS;
-    return start(k_expand<T, RB, WM == 8, TRANS>, dim3((unsigned)(s.tiles * C::PARTS), (unsigned)ceil_div(F, f_block)), kThreads,
+    return start<k_expand<T, RB, WM == 8, TRANS>>(dim3((unsigned)(s.tiles * C::PARTS), (unsigned)ceil_div(F, f_block)), kThreads,
                  C::SMEM, true, st, plan, h, splits, w, s.n, s.rank, F, f_block, (int)s.T, base, ldb, out, ldo,
                  base && row_units(base, ldb), row_units(w, TRANS ? F : s.rank), row_units((const T*)out, ldo));
 }
@@ -1800,7 +1814,7 @@ int run_weight(const Shape& s, const Plan& plan, const int32_t* index, const Sid
     const int64_t want = ceil_div(2 * kSms, (blocks_a + blocks_b) * s.n), can = ceil_div(s.T, (int64_t)s.n * C::TK);
     const int64_t most = want < can ? want : can;
     const unsigned parts = most >= 8 ? 8 : most >= 4 ? 4 : most >= 2 ? 2 : 1;
-    return start(k_weight<T, RB>, dim3((unsigned)(blocks_a + blocks_b), (unsigned)s.n, parts), kThreads, C::SMEM, true, st,
+    return start<k_weight<T, RB>>(dim3((unsigned)(blocks_a + blocks_b), (unsigned)s.n, parts), kThreads, C::SMEM, true, st,
                  plan, index, a, b, (int)blocks_a, s.n, s.rank, (int)s.T);
 }
 

@@ -23,6 +23,8 @@
 // the polynomial, so X' is one product.  The planes are read in the layout in which
 // U was given: tall matrices use U^T U and X P, so nothing is transposed in memory;
 // the descriptors take each operand along K or across it.
+#include <type_traits>
+
 #include "engram_tensor.cuh"
 
 using namespace engram;
@@ -46,37 +48,113 @@ template <> __device__ __forceinline__ float from_f32(float v) { return v; }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_f32(float v) { return __float2half_rn(v); }
 
+// Four elements from i on; vec: as one load (i a multiple of 4 from an aligned array), else `left` of them.
+__device__ __forceinline__ float4 load4(const float* p, int64_t i, int left, bool vec) {
+    if (vec) return *reinterpret_cast<const float4*>(p + i);
+    return make_float4(p[i], left > 1 ? p[i + 1] : 0.f, left > 2 ? p[i + 2] : 0.f, left > 3 ? p[i + 3] : 0.f);
+}
+template <typename T>
+__device__ __forceinline__ float4 load4(const T* p, int64_t i, int left, bool vec) {
+    if (vec) {
+        alignas(8) T v[4];
+        *reinterpret_cast<uint2*>(v) = *reinterpret_cast<const uint2*>(p + i);
+        return make_float4(to_f32(v[0]), to_f32(v[1]), to_f32(v[2]), to_f32(v[3]));
+    }
+    return make_float4(to_f32(p[i]), left > 1 ? to_f32(p[i + 1]) : 0.f, left > 2 ? to_f32(p[i + 2]) : 0.f,
+                       left > 3 ? to_f32(p[i + 3]) : 0.f);
+}
+template <typename T>
+__device__ __forceinline__ void store4(T* p, int64_t i, int left, bool vec, float4 v) {
+    if (vec) {
+        if constexpr (sizeof(T) == 4) {
+            *reinterpret_cast<float4*>(p + i) = v;
+        } else {
+            alignas(8) T o[4] = {from_f32<T>(v.x), from_f32<T>(v.y), from_f32<T>(v.z), from_f32<T>(v.w)};
+            *reinterpret_cast<uint2*>(p + i) = *reinterpret_cast<const uint2*>(o);
+        }
+        return;
+    }
+    p[i] = from_f32<T>(v.x);
+    if (left > 1) p[i + 1] = from_f32<T>(v.y);
+    if (left > 2) p[i + 2] = from_f32<T>(v.z);
+    if (left > 3) p[i + 3] = from_f32<T>(v.w);
+}
+
 // Where U comes from and where the result goes.  Plain: U = x, the result is out.
 // Muon: m' = m + (1 - beta)(g - m), U = g + beta (m' - g) (Nesterov) or m'; the first
 // pass writes m', the later one reads it; the result O gives p' = decay p - step O.
+// fetch() only loads, so that the next elements are under way while others are worked
+// on; the value follows from what it loaded.
 template <typename T>
 struct Plain {
+    struct Raw {
+        float4 x;
+    };
     const T* x;
     T* out;
+    bool aligned;  // both on four elements
     __device__ __forceinline__ float first(int64_t i) const { return to_f32(x[i]); }
     __device__ __forceinline__ float again(int64_t i) const { return to_f32(x[i]); }
     __device__ __forceinline__ void store(int64_t i, float o) const { out[i] = from_f32<T>(o); }
+    template <bool FIRST>
+    __device__ __forceinline__ void fetch(Raw& r, int64_t i, int left, bool vec) const {
+        r.x = load4(x, i, left, vec);
+    }
+    template <bool FIRST>
+    __device__ __forceinline__ float4 value(const Raw& r, int64_t, int, bool) const {
+        return r.x;
+    }
+    __device__ __forceinline__ void put(const Raw&, int64_t i, int left, bool vec, float4 o) const {
+        store4(out, i, left, vec, o);
+    }
 };
 template <typename T>
 struct MuonIo {
+    struct Raw {
+        float4 g, m, p;
+    };
     const T* g;
     const float* m;
     float* m_out;
     const float* p;
     float* p_out;
     float beta, rest, decay, step;
-    bool nesterov;
+    bool nesterov, aligned;
     __device__ __forceinline__ float update(float gv, float mv) const {
         return nesterov ? __fmaf_rn(beta, mv - gv, gv) : mv;
     }
+    __device__ __forceinline__ float moved(float gv, float mv) const { return __fmaf_rn(rest, gv - mv, mv); }
     __device__ __forceinline__ float first(int64_t i) const {
-        const float gv = to_f32(g[i]), mv = m[i], mn = __fmaf_rn(rest, gv - mv, mv);
+        const float gv = to_f32(g[i]), mn = moved(gv, m[i]);
         m_out[i] = mn;
         return update(gv, mn);
     }
     __device__ __forceinline__ float again(int64_t i) const { return update(to_f32(g[i]), m_out[i]); }
     __device__ __forceinline__ void store(int64_t i, float o) const { p_out[i] = __fmaf_rn(-step, o, decay * p[i]); }
+    template <bool FIRST>
+    __device__ __forceinline__ void fetch(Raw& r, int64_t i, int left, bool vec) const {
+        r.g = load4(g, i, left, vec);
+        r.m = load4(FIRST ? m : m_out, i, left, vec);
+        if (!FIRST) r.p = load4(p, i, left, vec);
+    }
+    template <bool FIRST>
+    __device__ __forceinline__ float4 value(const Raw& r, int64_t i, int left, bool vec) const {
+        float4 n = r.m;
+        if (FIRST) {
+            n = make_float4(moved(r.g.x, r.m.x), moved(r.g.y, r.m.y), moved(r.g.z, r.m.z), moved(r.g.w, r.m.w));
+            store4(m_out, i, left, vec, n);
+        }
+        return make_float4(update(r.g.x, n.x), update(r.g.y, n.y), update(r.g.z, n.z), update(r.g.w, n.w));
+    }
+    __device__ __forceinline__ void put(const Raw& r, int64_t i, int left, bool vec, float4 o) const {
+        store4(p_out, i, left, vec,
+               make_float4(__fmaf_rn(-step, o.x, decay * r.p.x), __fmaf_rn(-step, o.y, decay * r.p.y),
+                           __fmaf_rn(-step, o.z, decay * r.p.z), __fmaf_rn(-step, o.w, decay * r.p.w)));
+    }
 };
+
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // ---- short sides up to 64 -------------------------------------------------------
 
@@ -87,53 +165,93 @@ __device__ __forceinline__ void dmma(double* d, double a, double b) {
 }
 
 constexpr int kSmallThreads = 256;
-constexpr int KT = 64;        // long-side columns of a tile in shared memory
-constexpr int KTS = KT + 4;   // its row stride: rows 8 apart in a quarter fall on unlike banks
 
-// Columns k0 .. k0 + KT - 1 (below k_end) of the m x L matrix from element base on into tile
-// [8 MB][KTS], zeros outside.  tall: stored [L][m], else [m][L].
-template <int MB, typename F>
-__device__ __forceinline__ void load_tile(float* tile, int64_t base, int m, int64_t L, int64_t k0, int64_t k_end,
-                                          bool tall, F value) {
-    if (tall) {
-        const int64_t left = k_end - k0;
-        const int cols = left < KT ? (int)left : KT;
-        for (int e = threadIdx.x; e < KT * 8 * MB; e += kSmallThreads) {
-            const int k = e / (8 * MB), i = e % (8 * MB);
-            tile[i * KTS + k] = (i < m && k < cols) ? value(base + (k0 + k) * m + i) : 0.f;
-        }
-    } else {
-        for (int e = threadIdx.x; e < KT * 8 * MB; e += kSmallThreads) {
-            const int k = e % KT, i = e / KT;
-            tile[i * KTS + k] = (i < m && k0 + k < k_end) ? value(base + (int64_t)i * L + k0 + k) : 0.f;
-        }
+// A tile of the m x L matrix in shared memory: KT columns of its long side, rows padded to 8 MB.  It lies as the
+// matrix does, so both are copied four elements at a time: TALL (stored [L][m]) column by column, else row by row;
+// the padding keeps the fragments' reads (8 rows x 4 columns) on unlike banks.
+template <int MB, bool TALL>
+struct SmallTile {
+    static constexpr int RM = 8 * MB, KT = MB <= 2 ? 128 : 64;
+    static constexpr int PITCH = TALL ? RM + 8 : KT + 4, SIZE = TALL ? KT * PITCH : RM * PITCH;
+    static constexpr int N = RM * KT / 4 / kSmallThreads;  // pieces of four a thread copies
+    static_assert(N >= 1 && RM * KT % (4 * kSmallThreads) == 0, "whole pieces a thread");
+    static __device__ __forceinline__ int at(int i, int k) { return TALL ? k * PITCH + i : i * PITCH + k; }
+    // Piece n of this thread: its first row and column, and its place in the matrix
+    static __device__ __forceinline__ void piece(int n, int& i, int& k) {
+        const int e = (int)threadIdx.x + n * kSmallThreads;
+        if (TALL) i = e % (RM / 4) * 4, k = e / (RM / 4);
+        else k = e % (KT / 4) * 4, i = e / (KT / 4);
+    }
+    static __device__ __forceinline__ int64_t place(int64_t base, int m, int64_t L, int64_t k0, int i, int k) {
+        return TALL ? base + (k0 + k) * m + i : base + (int64_t)i * L + k0 + k;
+    }
+    // elements of the piece that exist
+    static __device__ __forceinline__ int left(int m, int64_t cols, int i, int k) {
+        if (i >= m || k >= cols) return 0;
+        const int64_t n = TALL ? (int64_t)m - i : cols - k;
+        return n < 4 ? (int)n : 4;
+    }
+};
+
+template <bool FIRST, typename S, typename Io>
+__device__ __forceinline__ void fetch_tile(const Io& io, typename Io::Raw (&raw)[S::N], int64_t base, int m, int64_t L,
+                                           int64_t k0, int64_t k_end, bool vec) {
+#pragma unroll
+    for (int n = 0; n < S::N; n++) {
+        int i, k;
+        S::piece(n, i, k);
+        const int left = S::left(m, k_end - k0, i, k);
+        if (left) io.template fetch<FIRST>(raw[n], S::place(base, m, L, k0, i, k), left, vec && left == 4);
+    }
+}
+template <bool FIRST, typename S, typename Io>
+__device__ __forceinline__ void store_tile(const Io& io, const typename Io::Raw (&raw)[S::N], float* tile, int64_t base,
+                                           int m, int64_t L, int64_t k0, int64_t k_end, bool vec) {
+#pragma unroll
+    for (int n = 0; n < S::N; n++) {
+        int i, k;
+        S::piece(n, i, k);
+        const int left = S::left(m, k_end - k0, i, k);
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (left) v = io.template value<FIRST>(raw[n], S::place(base, m, L, k0, i, k), left, vec && left == 4);
+        if (left < 2) v.y = 0.f;
+        if (left < 3) v.z = 0.f;
+        if (left < 4) v.w = 0.f;
+        *reinterpret_cast<float4*>(tile + S::at(i, k)) = v;
     }
 }
 
 // part[s, chunk] = U U^T over the chunk's columns, fp64, [8 MB][8 MB] (blocks of 8 on and above the
-// diagonal).  Warp w sums columns 8 w .. 8 w + 7 of each tile; the warps are added in their order.
-template <int MB, typename Io>
-__global__ void __launch_bounds__(kSmallThreads) k_small_gram(Io io, int m, int64_t L, bool tall, int64_t chunk,
+// diagonal).  Warp w sums columns 8 w .. 8 w + 7 (and 64 further) of each tile; the warps are added in
+// their order.
+template <int MB, bool TALL, typename Io>
+__global__ void __launch_bounds__(kSmallThreads) k_small_gram(Io io, int m, int64_t L, int64_t chunk, bool vec,
                                                               double* __restrict__ part) {
+    using S = SmallTile<MB, TALL>;
     constexpr int RM = 8 * MB, NT = MB * (MB + 1) / 2;
     // the tile, and after the last one the sums
-    __shared__ __align__(16) double sum[RM * RM > RM * KTS / 2 ? RM * RM : RM * KTS / 2];
+    __shared__ __align__(16) double sum[RM * RM > S::SIZE / 2 ? RM * RM : S::SIZE / 2];
     float* tile = reinterpret_cast<float*>(sum);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
     const int64_t base = (int64_t)blockIdx.y * m * L, k_begin = blockIdx.x * chunk;
     const int64_t k_end = k_begin + chunk < L ? k_begin + chunk : L;
+    let_next_start();
     double acc[NT][2];
 #pragma unroll
     for (int i = 0; i < NT; i++) acc[i][0] = acc[i][1] = 0.0;
-    for (int64_t k0 = k_begin; k0 < k_end; k0 += KT) {
+    typename Io::Raw raw[S::N];
+    fetch_tile<true, S>(io, raw, base, m, L, k_begin, k_end, vec);
+    for (int64_t k0 = k_begin; k0 < k_end; k0 += S::KT) {
         __syncthreads();
-        load_tile<MB>(tile, base, m, L, k0, k_end, tall, [&](int64_t i) { return io.first(i); });
+        store_tile<true, S>(io, raw, tile, base, m, L, k0, k_end, vec);
         __syncthreads();
+        if (k0 + S::KT < k_end) fetch_tile<true, S>(io, raw, base, m, L, k0 + S::KT, k_end, vec);
 #pragma unroll
-        for (int s = 0; s < 2; s++) {
+        for (int s = 0; s < S::KT / 32; s++) {
             double f[MB];
 #pragma unroll
-            for (int i = 0; i < MB; i++) f[i] = (double)tile[(8 * i + g) * KTS + 8 * warp + 4 * s + q];
+            for (int i = 0; i < MB; i++)
+                f[i] = (double)tile[S::at(8 * i + g, 64 * (s >> 1) + 8 * warp + 4 * (s & 1) + q)];
             int at = 0;
 #pragma unroll
             for (int i = 0; i < MB; i++)
@@ -168,7 +286,7 @@ template <int MB, typename F>
 __device__ __forceinline__ void small_product(const double* x, const double* y, double* z, F f) {
     constexpr int S = 8 * MB + 4, NT = MB * (MB + 1) / 2;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
-    for (int at = warp; at < NT; at += kSmallThreads / 32) {
+    for (int at = warp; at < NT; at += (int)blockDim.x / 32) {
         int i = 0, left = at;
         while (left >= MB - i) left -= MB - i, i++;
         const int j = i + left;
@@ -196,10 +314,13 @@ __global__ void __launch_bounds__(kSmallThreads) k_small_poly(const double* __re
     double *A = sd, *B = A + RM * S, *P = B + RM * S, *Q = P + RM * S;
     __shared__ double inv_norm;
     const double* src = part + (int64_t)blockIdx.x * chunks * RM * RM;
-    for (int e = threadIdx.x; e < RM * RM; e += kSmallThreads) {
+    wait_for_previous();
+    let_next_start();
+    for (int e = threadIdx.x; e < RM * RM; e += blockDim.x) {
         const int i = e / RM, j = e % RM;
         if (j < (i & ~7)) continue;
         double v = 0.0;
+#pragma unroll 8
         for (int c = 0; c < chunks; c++) v += src[(int64_t)c * RM * RM + e];
         A[i * S + j] = v;
         if (j / 8 != i / 8) A[j * S + i] = v;
@@ -213,7 +334,7 @@ __global__ void __launch_bounds__(kSmallThreads) k_small_poly(const double* __re
     }
     __syncthreads();
     const double inv = inv_norm;
-    for (int e = threadIdx.x; e < RM * RM; e += kSmallThreads) {
+    for (int e = threadIdx.x; e < RM * RM; e += blockDim.x) {
         const int i = e / RM, j = e % RM;
         A[i * S + j] *= inv * inv;
         P[i * S + j] = i == j ? inv : 0.0;
@@ -231,55 +352,64 @@ __global__ void __launch_bounds__(kSmallThreads) k_small_poly(const double* __re
             small_product<MB>(B, Q, A, [](int, int, double v) { return v; });
         }
     }
-    for (int e = threadIdx.x; e < RM * RM; e += kSmallThreads)
+    for (int e = threadIdx.x; e < RM * RM; e += blockDim.x)
         pmat[(int64_t)blockIdx.x * RM * RM + e] = P[(e / RM) * S + e % RM];
 }
 
 // The result P U, tile by tile.
-template <int MB, typename Io>
-__global__ void __launch_bounds__(kSmallThreads) k_small_apply(Io io, int m, int64_t L, bool tall, int64_t chunk,
+template <int MB, bool TALL, typename Io>
+__global__ void __launch_bounds__(kSmallThreads) k_small_apply(Io io, int m, int64_t L, int64_t chunk, bool vec,
                                                                const double* __restrict__ pmat) {
-    constexpr int RM = 8 * MB, S = RM + 4;
+    using S = SmallTile<MB, TALL>;
+    constexpr int RM = 8 * MB, SP = RM + 4;
     extern __shared__ double sd[];
     double* P = sd;
-    float* tile = reinterpret_cast<float*>(P + RM * S);
+    float* tile = reinterpret_cast<float*>(P + RM * SP);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
     const int64_t base = (int64_t)blockIdx.y * m * L, k_begin = blockIdx.x * chunk;
     const int64_t k_end = k_begin + chunk < L ? k_begin + chunk : L;
+    typename Io::Raw raw[S::N];
+    wait_for_previous();  // P, and what the first pass wrote
+    let_next_start();
+    fetch_tile<false, S>(io, raw, base, m, L, k_begin, k_end, vec);
     for (int e = threadIdx.x; e < RM * RM; e += kSmallThreads)
-        P[(e / RM) * S + e % RM] = pmat[(int64_t)blockIdx.y * RM * RM + e];
-    for (int64_t k0 = k_begin; k0 < k_end; k0 += KT) {
+        P[(e / RM) * SP + e % RM] = pmat[(int64_t)blockIdx.y * RM * RM + e];
+    for (int64_t k0 = k_begin; k0 < k_end; k0 += S::KT) {
+        typename Io::Raw now[S::N];
+#pragma unroll
+        for (int n = 0; n < S::N; n++) now[n] = raw[n];
         __syncthreads();
-        load_tile<MB>(tile, base, m, L, k0, k_end, tall, [&](int64_t i) { return io.again(i); });
+        store_tile<false, S>(io, now, tile, base, m, L, k0, k_end, vec);
         __syncthreads();
-        double acc[MB][2];
+        if (k0 + S::KT < k_end) fetch_tile<false, S>(io, raw, base, m, L, k0 + S::KT, k_end, vec);
 #pragma unroll
-        for (int i = 0; i < MB; i++) acc[i][0] = acc[i][1] = 0.0;
+        for (int part = 0; part < S::KT / 64; part++) {  // warp w: columns 8 w .. 8 w + 7, and 64 further
+            double acc[MB][2];
 #pragma unroll
-        for (int s = 0; s < 2 * MB; s++) {  // warp w: columns 8 w .. 8 w + 7
-            const double b = (double)tile[(4 * s + q) * KTS + 8 * warp + g];
+            for (int i = 0; i < MB; i++) acc[i][0] = acc[i][1] = 0.0;
+            const int k = 64 * part + 8 * warp;
 #pragma unroll
-            for (int i = 0; i < MB; i++) dmma(acc[i], P[(8 * i + g) * S + 4 * s + q], b);
-        }
-        __syncwarp();
+            for (int s = 0; s < 2 * MB; s++) {
+                const double b = (double)tile[S::at(4 * s + q, k + g)];
 #pragma unroll
-        for (int i = 0; i < MB; i++) {
-            tile[(8 * i + g) * KTS + 8 * warp + 2 * q] = (float)acc[i][0];
-            tile[(8 * i + g) * KTS + 8 * warp + 2 * q + 1] = (float)acc[i][1];
-        }
-        __syncthreads();
-        const int64_t left = k_end - k0;
-        const int cols = left < KT ? (int)left : KT;
-        if (tall) {
-            for (int e = threadIdx.x; e < cols * RM; e += kSmallThreads) {
-                const int k = e / RM, i = e % RM;
-                if (i < m) io.store(base + (k0 + k) * m + i, tile[i * KTS + k]);
+                for (int i = 0; i < MB; i++) dmma(acc[i], P[(8 * i + g) * SP + 4 * s + q], b);
             }
-        } else {
-            for (int e = threadIdx.x; e < KT * m; e += kSmallThreads) {
-                const int k = e % KT, i = e / KT;
-                if (k < cols) io.store(base + (int64_t)i * L + k0 + k, tile[i * KTS + k]);
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < MB; i++) {
+                tile[S::at(8 * i + g, k + 2 * q)] = (float)acc[i][0];
+                tile[S::at(8 * i + g, k + 2 * q + 1)] = (float)acc[i][1];
             }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < S::N; n++) {
+            int i, kk;
+            S::piece(n, i, kk);
+            const int left = S::left(m, k_end - k0, i, kk);
+            if (left)
+                io.put(now[n], S::place(base, m, L, k0, i, kk), left, vec && left == 4,
+                       *reinterpret_cast<const float4*>(tile + S::at(i, kk)));
         }
     }
 }
@@ -612,14 +742,38 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_product(const __grid_consta
 int64_t align256(int64_t b) { return (b + 255) & ~int64_t(255); }
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-int launched() {
-    count_launches(1);
-    return cudaGetLastError() == cudaSuccess ? ENGRAM_OK : ENGRAM_ERR_CUDA;
+template <typename... P, typename... A>
+cudaError_t launch(void (*kernel)(P...), const cudaLaunchConfig_t& cfg, A... args) {
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
 }
 
-bool allow_smem(const void* kernel, int bytes) {
-    return bytes <= 48 * 1024 ||
-           cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess;
+// Starts a kernel; after = true: it may start while the launch before it still runs (it waits for that
+// one's results itself, griddepcontrol.wait).
+template <auto KERNEL, typename... A>
+int start(dim3 grid, int threads, int smem, bool after, cudaStream_t st, A... args) {
+    if (smem > 48 * 1024) {
+        static bool allowed[64] = {false};
+        int dev = 0;
+        cudaGetDevice(&dev);
+        if (dev < 0 || dev >= 64 || !allowed[dev]) {
+            if (cudaFuncSetAttribute((const void*)KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+                return ENGRAM_ERR_CUDA;
+            if (dev >= 0 && dev < 64) allowed[dev] = true;
+        }
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = after ? 1 : 0;
+    const cudaError_t e = launch(KERNEL, cfg, args...);
+    count_launches(1);
+    return e == cudaSuccess && cudaGetLastError() == cudaSuccess ? ENGRAM_OK : ENGRAM_ERR_CUDA;
 }
 
 struct Shape {
@@ -629,8 +783,8 @@ struct Shape {
 
 // Chunks of the long side, in whole tiles, for about four blocks an SM.
 int64_t small_chunk(const Shape& s) {
-    const int64_t tiles = ceil_div(s.length, KT), per = ceil_div(4 * 148, s.stack);
-    return ceil_div(tiles, per < tiles ? per : tiles) * KT;
+    const int64_t kt = s.side <= 16 ? 128 : 64, tiles = ceil_div(s.length, kt), per = ceil_div(4 * 148, s.stack);
+    return ceil_div(tiles, per < tiles ? per : tiles) * kt;
 }
 int small_side(const Shape& s) { return s.side <= 8 ? 8 : s.side <= 16 ? 16 : s.side <= 32 ? 32 : 64; }
 
@@ -673,24 +827,24 @@ Layout layout_of(const Shape& s, int terms) {
     return l;
 }
 
-template <int MB, typename Io>
+template <int MB, bool TALL, typename Io>
 int run_small(const Shape& s, const Layout& l, const Io& io, const Poly& poly, double eps, uint8_t* ws,
               cudaStream_t st) {
+    using S = SmallTile<MB, TALL>;
     const int64_t chunk = small_chunk(s), chunks = ceil_div(s.length, chunk);
     double *part = (double*)(ws + l.part), *pmat = (double*)(ws + l.pmat);
     const dim3 grid((unsigned)chunks, (unsigned)s.stack);
-    k_small_gram<MB><<<grid, kSmallThreads, 0, st>>>(io, (int)s.side, s.length, s.tall, chunk, part);
-    int e = launched();
-    if (e) return e;
-    constexpr int RM = 8 * MB, S = RM + 4, poly_smem = 4 * RM * S * 8, apply_smem = RM * S * 8 + RM * KTS * 4;
-    if (!allow_smem((const void*)k_small_poly<MB>, poly_smem)) return ENGRAM_ERR_CUDA;
-    k_small_poly<MB><<<(unsigned)s.stack, kSmallThreads, poly_smem, st>>>(part, (int)chunks, (int)s.side, poly, eps,
-                                                                         pmat);
-    e = launched();
-    if (e) return e;
-    if (!allow_smem((const void*)k_small_apply<MB, Io>, apply_smem)) return ENGRAM_ERR_CUDA;
-    k_small_apply<MB><<<grid, kSmallThreads, apply_smem, st>>>(io, (int)s.side, s.length, s.tall, chunk, pmat);
-    return launched();
+    const bool vec = io.aligned && (TALL ? s.side : s.length) % 4 == 0;
+    constexpr int RM = 8 * MB, SP = RM + 4, NT = MB * (MB + 1) / 2;
+    int e = start<k_small_gram<MB, TALL, Io>>(grid, kSmallThreads, 0, false, st, io, (int)s.side, s.length, chunk, vec,
+                                              part);
+    if (!e)
+        e = start<k_small_poly<MB>>(dim3((unsigned)s.stack), NT >= 8 ? kSmallThreads : 32 * NT, 4 * RM * SP * 8, true, st,
+                                    part, (int)chunks, (int)s.side, poly, eps, pmat);
+    if (!e)
+        e = start<k_small_apply<MB, TALL, Io>>(grid, kSmallThreads, RM * SP * 8 + S::SIZE * 4, true, st, io, (int)s.side,
+                                               s.length, chunk, vec, pmat);
+    return e;
 }
 
 // Map of one plane [stack, rows, ld] of which `cols` columns count, in boxes of bx columns and by rows.
@@ -725,13 +879,11 @@ int run_product(const Matrix& a, const Matrix& b, int64_t stack, Job<Io> job, cu
     if (!make(&maps.a_hi, a.p.hi, a, A_MN, BM) || !make(&maps.b_hi, b.p.hi, b, B_MN, BN)) return ENGRAM_ERR_CUDA;
     if (TERMS == 3 && (!make(&maps.a_lo, a.p.lo, a, A_MN, BM) || !make(&maps.b_lo, b.p.lo, b, B_MN, BN)))
         return ENGRAM_ERR_CUDA;
-    const auto kernel = k_product<MODE, A_MN, B_MN, TERMS, BN, Io>;
-    if (!allow_smem((const void*)kernel, G::SMEM)) return ENGRAM_ERR_CUDA;
     const int64_t tn = ceil_div(job.N, BN);
     job.tiles_m = (int)ceil_div(job.M, BM);
     const int64_t tiles = (MODE == GRAM || MODE == POLY) ? (BN / BM) * tn * (tn + 1) / 2 : job.tiles_m * tn;
-    kernel<<<dim3((unsigned)tiles, (unsigned)stack), kGemmThreads, G::SMEM, st>>>(maps, job);
-    return launched();
+    return start<k_product<MODE, A_MN, B_MN, TERMS, BN, Io>>(dim3((unsigned)tiles, (unsigned)stack), kGemmThreads,
+                                                             G::SMEM, false, st, maps, job);
 }
 
 template <int TERMS, typename Io>
@@ -748,13 +900,12 @@ int run_planes(const Shape& s, const Layout& l, const Io& io, const Poly& poly, 
     const Matrix g = {planes(l.g, l.s_plane, lds, s.side), s.side, s.side};
     const Matrix b = {planes(l.b, l.s_plane, lds, s.side), s.side, s.side};
     const int nb = (int)norm_blocks(s);
-    k_norm<<<dim3((unsigned)nb, (unsigned)s.stack), kNormThreads, 0, st>>>(io, s.rows * s.cols, part);
-    int e = launched();
+    int e = start<k_norm<Io>>(dim3((unsigned)nb, (unsigned)s.stack), kNormThreads, 0, false, st, io, s.rows * s.cols,
+                              part);
     if (e) return e;
     const int64_t row_blocks = ceil_div(s.rows, kNormThreads / 32), most = ceil_div(8 * 148, s.stack);
-    k_planes<<<dim3((unsigned)(row_blocks < most ? row_blocks : most), (unsigned)s.stack), kNormThreads, 0, st>>>(
-        io, s.rows, s.cols, part, nb, eps, x[0].p);
-    e = launched();
+    e = start<k_planes<Io>>(dim3((unsigned)(row_blocks < most ? row_blocks : most), (unsigned)s.stack), kNormThreads, 0,
+                            false, st, io, s.rows, s.cols, part, nb, eps, x[0].p);
     Job<NoIo> job = {};
     job.err = (int*)(ws + l.err);
     for (int i = 0; i < poly.steps && !e; i++) {
@@ -792,10 +943,14 @@ template <int TERMS, typename Io>
 int run(const Shape& s, const Layout& l, const Io& io, const Poly& poly, double eps, void* ws, void* stream) {
     uint8_t* w = (uint8_t*)ws;
     cudaStream_t st = (cudaStream_t)stream;
-    if (s.side <= 8) return run_small<1>(s, l, io, poly, eps, w, st);
-    if (s.side <= 16) return run_small<2>(s, l, io, poly, eps, w, st);
-    if (s.side <= 32) return run_small<4>(s, l, io, poly, eps, w, st);
-    if (s.side <= kSmallSide) return run_small<8>(s, l, io, poly, eps, w, st);
+    const auto small = [&](auto mb) {
+        constexpr int MB = decltype(mb)::value;
+        return s.tall ? run_small<MB, true>(s, l, io, poly, eps, w, st) : run_small<MB, false>(s, l, io, poly, eps, w, st);
+    };
+    if (s.side <= 8) return small(std::integral_constant<int, 1>{});
+    if (s.side <= 16) return small(std::integral_constant<int, 2>{});
+    if (s.side <= 32) return small(std::integral_constant<int, 4>{});
+    if (s.side <= kSmallSide) return small(std::integral_constant<int, 8>{});
     return run_planes<TERMS>(s, l, io, poly, eps, w, st);
 }
 
@@ -810,22 +965,28 @@ int check_shape(int64_t stack, int64_t rows, int64_t cols, Shape* s) {
     return ENGRAM_OK;
 }
 
-// The iterates have to stay within what the planes hold: for every singular value in [0, 1] that the
-// first division can leave, each step's G, polynomial and result below 15.
+// The iterates have to stay within what the planes hold: from singular values in [0, 1] on, each step's
+// G, polynomial and result below 15.  `top` is the largest singular value that a step can meet, found on a
+// grid over all that the step before can leave.
 int check_poly(int32_t steps, const double* c, double eps, Poly* poly) {
     if (steps < 1 || !c || !(eps > 0.0)) return ENGRAM_ERR_ARG;
     if (steps > kMaxSteps) return ENGRAM_ERR_RANGE;
-    constexpr int kPoints = 2048;
-    for (int i = 0; i < steps; i++)
-        for (int k = 0; k < 3; k++) poly->c[i][k] = c[3 * i + k];
     poly->steps = steps;
-    for (int p = 0; p <= kPoints; p++) {
-        double x = 1.001 * p / kPoints;
-        for (int i = 0; i < steps; i++) {
-            const double g = x * x, f = poly->c[i][0] + g * (poly->c[i][1] + g * poly->c[i][2]);
-            x *= f;
-            if (!(g < 15.0 && f < 15.0 && f > -15.0 && x < 3.8 && x > -3.8)) return ENGRAM_ERR_RANGE;
+    constexpr int kPoints = 128;
+    double top = 1.0;
+    for (int i = 0; i < steps; i++) {
+        const double c0 = c[3 * i], c1 = c[3 * i + 1], c2 = c[3 * i + 2];
+        poly->c[i][0] = c0, poly->c[i][1] = c1, poly->c[i][2] = c2;
+        double f_most = 0.0, x_most = 0.0;
+        bool number = true;
+        for (int p = 0; p <= kPoints; p++) {
+            const double x = top * p / kPoints, g = x * x, f = fabs(c0 + g * (c1 + g * c2)), y = x * f;
+            number = number && f < 1e30;
+            f_most = f > f_most ? f : f_most;
+            x_most = y > x_most ? y : x_most;
         }
+        if (!number || !(top * top < 15.0) || !(f_most < 15.0) || !(x_most < 3.8)) return ENGRAM_ERR_RANGE;
+        top = x_most;
     }
     return ENGRAM_OK;
 }
@@ -861,14 +1022,15 @@ extern "C" int engram_orthogonalize(int32_t dtype, const void* x, int64_t stack,
         return ENGRAM_ERR_ARG;
     const Layout l = layout_of(s, terms_of(dtype));
     if (workspace_bytes < l.bytes) return ENGRAM_ERR_WORKSPACE;
+    const bool four = aligned16(x) && aligned16(out);
     switch (dtype) {
         case ENGRAM_DTYPE_F32:
-            return run<3>(s, l, Plain<float>{(const float*)x, (float*)out}, poly, eps, workspace, stream);
+            return run<3>(s, l, Plain<float>{(const float*)x, (float*)out, four}, poly, eps, workspace, stream);
         case ENGRAM_DTYPE_BF16:
-            return run<1>(s, l, Plain<__nv_bfloat16>{(const __nv_bfloat16*)x, (__nv_bfloat16*)out}, poly, eps,
-                          workspace, stream);
+            return run<1>(s, l, Plain<__nv_bfloat16>{(const __nv_bfloat16*)x, (__nv_bfloat16*)out, four}, poly,
+                          eps, workspace, stream);
         default:
-            return run<3>(s, l, Plain<__half>{(const __half*)x, (__half*)out}, poly, eps, workspace, stream);
+            return run<3>(s, l, Plain<__half>{(const __half*)x, (__half*)out, four}, poly, eps, workspace, stream);
     }
 }
 
@@ -890,10 +1052,11 @@ extern "C" int engram_muon_step(int32_t grad_dtype, const float* p, const void* 
     const Layout l = layout_of(s, 3);
     if (workspace_bytes < l.bytes) return ENGRAM_ERR_WORKSPACE;
     const double ratio = rows > cols ? sqrt((double)rows / (double)cols) : 1.0;
+    const bool four = aligned16(p) && aligned16(grad) && aligned16(m) && aligned16(p_out) && aligned16(m_out);
     const auto io = [&](auto* g) {
         using T = std::remove_cv_t<std::remove_pointer_t<decltype(g)>>;
         return MuonIo<T>{g, m, m_out, p, p_out, (float)beta, (float)(1.0 - beta), (float)(1.0 - lr * weight_decay),
-                         (float)(lr * ratio), nesterov != 0};
+                         (float)(lr * ratio), nesterov != 0, four};
     };
     switch (grad_dtype) {
         case ENGRAM_DTYPE_F32: return run<3>(s, l, io((const float*)grad), poly, eps, workspace, stream);

@@ -34,6 +34,8 @@ def _table(coefficients: tuple, steps: int):
 def _coefficients(coefficients, steps: int):
     if not 1 <= steps <= 32:
         raise ValueError(f"steps: {steps}, expected 1 to 32")
+    if coefficients is COEFFICIENTS:
+        return _table(coefficients, steps)
     return _table(tuple(tuple(c) if isinstance(c, (tuple, list)) else float(c) for c in coefficients), int(steps))
 
 
@@ -52,10 +54,11 @@ def _same(x: torch.Tensor, like: torch.Tensor, name: str, dtype=None) -> None:
                          f"(got {x.dtype} {tuple(x.shape)}, strides {tuple(x.stride())}, on {x.device})")
 
 
-def _workspace(lib, code, stack, rows, cols, device) -> torch.Tensor:
-    size = lib.engram_orthogonalize_workspace_bytes(code, stack, rows, cols)
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(code, stack, rows, cols) -> int:
+    size = L.load().engram_orthogonalize_workspace_bytes(code, stack, rows, cols)
     L.check(min(size, 0), "engram_orthogonalize_workspace_bytes")
-    return torch.empty(max(size, 1), dtype=torch.uint8, device=device)
+    return max(size, 1)
 
 
 @torch.no_grad()
@@ -72,11 +75,11 @@ def orthogonalize(update: torch.Tensor, steps: int = 5, coefficients=COEFFICIENT
         out = torch.empty_like(update)
     else:
         _same(out, update, "out")
-    lib, code = L.load(), _DTYPES[update.dtype]
-    with torch.cuda.device(update.device):
-        ws = _workspace(lib, code, stack, rows, cols, update.device)
-        st = lib.engram_orthogonalize(code, update.data_ptr(), stack, rows, cols, steps, table, eps, out.data_ptr(),
-                                      ws.data_ptr(), ws.numel(), L.stream_of(update.device))
+    code = _DTYPES[update.dtype]
+    size = _workspace_bytes(code, stack, rows, cols)
+    ws = torch.empty(size, dtype=torch.uint8, device=update.device)
+    st = L.on_device(update.device, lambda stream: L.load().engram_orthogonalize(
+        code, update.data_ptr(), stack, rows, cols, steps, table, eps, out.data_ptr(), ws.data_ptr(), size, stream))
     L.check(st, "engram_orthogonalize")
     torch.autograd.graph.increment_version(out)
     return out
@@ -100,13 +103,11 @@ def muon_step(param: torch.Tensor, grad: torch.Tensor, momentum: torch.Tensor, l
     if out is not None:
         _same(p_out, grad, "out[0]", torch.float32)
         _same(m_out, grad, "out[1]", torch.float32)
-    lib = L.load()
-    with torch.cuda.device(grad.device):
-        ws = _workspace(lib, L.DTYPE_F32, stack, rows, cols, grad.device)
-        st = lib.engram_muon_step(_DTYPES[grad.dtype], param.data_ptr(), grad.data_ptr(), momentum.data_ptr(),
-                                  p_out.data_ptr(), m_out.data_ptr(), stack, rows, cols, lr, beta, int(nesterov),
-                                  weight_decay, steps, table, eps, ws.data_ptr(), ws.numel(),
-                                  L.stream_of(grad.device))
+    size = _workspace_bytes(L.DTYPE_F32, stack, rows, cols)
+    ws = torch.empty(size, dtype=torch.uint8, device=grad.device)
+    st = L.on_device(grad.device, lambda stream: L.load().engram_muon_step(
+        _DTYPES[grad.dtype], param.data_ptr(), grad.data_ptr(), momentum.data_ptr(), p_out.data_ptr(), m_out.data_ptr(),
+        stack, rows, cols, lr, beta, int(nesterov), weight_decay, steps, table, eps, ws.data_ptr(), size, stream))
     L.check(st, "engram_muon_step")
     torch.autograd.graph.increment_version((p_out, m_out))
     return p_out, m_out
