@@ -1426,9 +1426,9 @@ __global__ void __launch_bounds__(kThreads) k_weight(Plan plan, const int32_t* _
     const int32_t* list;
     int count;
     if (plan.off) {
-        const int p0 = __ldg(plan.off + a);
+        const int p0 = plan.off[a];
         list = plan.perm + p0;
-        count = __ldg(plan.off + a + 1) - p0;
+        count = plan.off[a + 1] - p0;
     } else {
         count = scan_positions(scan, index, T_rows, n, a);
         list = scan.list;

@@ -16,11 +16,14 @@
 // kept as y = 2^12 x = hi + lo, two fp16 (22 significant bits); a product is
 // hi hi + hi lo + lo hi in fp32 accumulators in tensor memory.  Every iterate has
 // entries below 16 (checked for the coefficients on the host), so hi is far from
-// fp16's limits, and lo's steps of 2^-24 are 2^-36 of x.  Results rounded to bf16
-// take one product of the hi planes: 2^-12 a rounding, eight times finer than
-// the result's own.  G and G G are symmetric: only tiles that reach the diagonal
-// or lie above it are computed and stored twice.  c0 is added to the diagonal of
-// the polynomial, so X' is one product.  The planes are read in the layout in which
+// fp16's limits, and lo's steps of 2^-24 are 2^-36 of x.  c0 is added to the
+// diagonal of the polynomial, so X' is one product.  Results rounded to bf16 take
+// one product of the hi planes, operands rounded to 2^-12; there X keeps its lo
+// plane all the same and c0 X is added to the product from both, since an X rounded
+// at each step drowns the weak directions (1.5e-2 off on updates whose noise is 1/50
+// of their signal, against 2e-4 so; 1.8e-3 at most on any spectrum tried, beside
+// 1.7e-3 of bf16 itself).  G and G G are symmetric: only tiles that reach the diagonal
+// or lie above it are computed and stored twice.  The planes are read in the layout in which
 // U was given: tall matrices use U^T U and X P, so nothing is transposed in memory;
 // the descriptors take each operand along K or across it.
 #include <type_traits>
@@ -93,9 +96,6 @@ struct Plain {
     const T* x;
     T* out;
     bool aligned;  // both on four elements
-    __device__ __forceinline__ float first(int64_t i) const { return to_f32(x[i]); }
-    __device__ __forceinline__ float again(int64_t i) const { return to_f32(x[i]); }
-    __device__ __forceinline__ void store(int64_t i, float o) const { out[i] = from_f32<T>(o); }
     template <bool FIRST>
     __device__ __forceinline__ void fetch(Raw& r, int64_t i, int left, bool vec) const {
         r.x = load4(x, i, left, vec);
@@ -107,6 +107,7 @@ struct Plain {
     __device__ __forceinline__ void put(const Raw&, int64_t i, int left, bool vec, float4 o) const {
         store4(out, i, left, vec, o);
     }
+    __device__ __forceinline__ void finish(int64_t i, int left, bool vec, float4 o) const { store4(out, i, left, vec, o); }
 };
 template <typename T>
 struct MuonIo {
@@ -124,13 +125,6 @@ struct MuonIo {
         return nesterov ? __fmaf_rn(beta, mv - gv, gv) : mv;
     }
     __device__ __forceinline__ float moved(float gv, float mv) const { return __fmaf_rn(rest, gv - mv, mv); }
-    __device__ __forceinline__ float first(int64_t i) const {
-        const float gv = to_f32(g[i]), mn = moved(gv, m[i]);
-        m_out[i] = mn;
-        return update(gv, mn);
-    }
-    __device__ __forceinline__ float again(int64_t i) const { return update(to_f32(g[i]), m_out[i]); }
-    __device__ __forceinline__ void store(int64_t i, float o) const { p_out[i] = __fmaf_rn(-step, o, decay * p[i]); }
     template <bool FIRST>
     __device__ __forceinline__ void fetch(Raw& r, int64_t i, int left, bool vec) const {
         r.g = load4(g, i, left, vec);
@@ -150,6 +144,11 @@ struct MuonIo {
         store4(p_out, i, left, vec,
                make_float4(__fmaf_rn(-step, o.x, decay * r.p.x), __fmaf_rn(-step, o.y, decay * r.p.y),
                            __fmaf_rn(-step, o.z, decay * r.p.z), __fmaf_rn(-step, o.w, decay * r.p.w)));
+    }
+    __device__ __forceinline__ void finish(int64_t i, int left, bool vec, float4 o) const {
+        Raw r;
+        r.p = load4(p, i, left, vec);
+        put(r, i, left, vec, o);
     }
 };
 
@@ -307,7 +306,7 @@ __device__ __forceinline__ void small_product(const double* x, const double* y, 
 
 // The steps on the small matrices: pmat[s] = P / max(|U|, eps).
 template <int MB>
-__global__ void __launch_bounds__(kSmallThreads) k_small_poly(const double* __restrict__ part, int chunks, int m,
+__global__ void __launch_bounds__(kSmallThreads) k_small_poly(const double* part, int chunks, int m,
                                                               Poly poly, double eps, double* __restrict__ pmat) {
     constexpr int RM = 8 * MB, S = RM + 4;
     extern __shared__ double sd[];
@@ -359,7 +358,7 @@ __global__ void __launch_bounds__(kSmallThreads) k_small_poly(const double* __re
 // The result P U, tile by tile.
 template <int MB, bool TALL, typename Io>
 __global__ void __launch_bounds__(kSmallThreads) k_small_apply(Io io, int m, int64_t L, int64_t chunk, bool vec,
-                                                               const double* __restrict__ pmat) {
+                                                               const double* pmat) {
     using S = SmallTile<MB, TALL>;
     constexpr int RM = 8 * MB, SP = RM + 4;
     extern __shared__ double sd[];
@@ -421,13 +420,28 @@ constexpr int kNormThreads = 256;
 
 // part[s, block] = the block's share of |U|^2, fp64 (updates of 1e-20 and of 1e20 alike).
 template <typename Io>
-__global__ void __launch_bounds__(kNormThreads) k_norm(Io io, int64_t size, double* __restrict__ part) {
+__global__ void __launch_bounds__(kNormThreads) k_norm(Io io, int64_t size, bool vec, double* __restrict__ part) {
     __shared__ double warp_sum[kNormThreads / 32];
-    const int64_t base = blockIdx.y * size;
+    const int64_t base = blockIdx.y * size, pieces = (size + 3) / 4, step = (int64_t)gridDim.x * kNormThreads;
     double v = 0.0;
-    for (int64_t i = blockIdx.x * (int64_t)kNormThreads + threadIdx.x; i < size; i += (int64_t)gridDim.x * kNormThreads) {
-        const double u = (double)io.first(base + i);
-        v += u * u;
+    constexpr int N = 4;  // pieces under way a thread
+    for (int64_t i0 = blockIdx.x * (int64_t)kNormThreads + threadIdx.x; i0 < pieces; i0 += N * step) {
+        typename Io::Raw raw[N];
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            const int64_t i = 4 * (i0 + k * step), left = size - i;
+            if (left > 0) io.template fetch<true>(raw[k], base + i, (int)(left < 4 ? left : 4), vec);
+        }
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            const int64_t i = 4 * (i0 + k * step), left = size - i;
+            if (left <= 0) continue;
+            const float4 u = io.template value<true>(raw[k], base + i, (int)(left < 4 ? left : 4), vec);
+            v += (double)u.x * u.x;
+            if (left > 1) v += (double)u.y * u.y;
+            if (left > 2) v += (double)u.z * u.z;
+            if (left > 3) v += (double)u.w * u.w;
+        }
     }
 #pragma unroll
     for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
@@ -452,9 +466,8 @@ __device__ __forceinline__ void put(const Planes& p, int64_t i, float y) {
 
 // planes = 2^12 U / max(|U|, eps); a warp takes a row at a time.
 template <typename Io>
-__global__ void __launch_bounds__(kNormThreads) k_planes(Io io, int64_t rows, int64_t cols,
-                                                         const double* __restrict__ part, int parts, double eps,
-                                                         Planes out) {
+__global__ void __launch_bounds__(kNormThreads) k_planes(Io io, int64_t rows, int64_t cols, bool vec,
+                                                         const double* part, int parts, double eps, Planes out) {
     __shared__ double total;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (warp == 0) {
@@ -469,9 +482,34 @@ __global__ void __launch_bounds__(kNormThreads) k_planes(Io io, int64_t rows, in
     const double inv = (double)kPlaneScale / (norm < eps ? eps : norm);
     const int64_t base = blockIdx.y * rows * cols;
     for (int64_t r = blockIdx.x * (int64_t)(kNormThreads / 32) + warp; r < rows;
-         r += (int64_t)gridDim.x * (kNormThreads / 32))
-        for (int64_t c = lane; c < cols; c += 32)
-            put(out, blockIdx.y * out.stride + r * out.ld + c, (float)((double)io.again(base + r * cols + c) * inv));
+         r += (int64_t)gridDim.x * (kNormThreads / 32)) {
+        constexpr int N = 4;  // pieces of four under way a lane
+        for (int64_t c0 = 4 * lane; c0 < cols; c0 += N * 128) {
+            typename Io::Raw raw[N];
+#pragma unroll
+            for (int k = 0; k < N; k++) {
+                const int64_t c = c0 + 128 * k, left = cols - c;
+                if (left > 0) io.template fetch<false>(raw[k], base + r * cols + c, (int)(left < 4 ? left : 4), vec);
+            }
+#pragma unroll
+            for (int k = 0; k < N; k++) {
+                const int64_t c = c0 + 128 * k, left = cols - c;
+                if (left <= 0) continue;
+                const float4 u = io.template value<false>(raw[k], base + r * cols + c, (int)(left < 4 ? left : 4), vec);
+                const float v[4] = {u.x, u.y, u.z, u.w};
+                alignas(8) __half hi[4], lo[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {  // the padding (to a multiple of 64) may be written
+                    const float y = e < left ? (float)((double)v[e] * inv) : 0.f;
+                    hi[e] = __float2half_rn(y);
+                    lo[e] = __float2half_rn(y - __half2float(hi[e]));
+                }
+                const int64_t at = blockIdx.y * out.stride + r * out.ld + c;
+                *reinterpret_cast<uint2*>(out.hi + at) = *reinterpret_cast<const uint2*>(hi);
+                *reinterpret_cast<uint2*>(out.lo + at) = *reinterpret_cast<const uint2*>(lo);
+            }
+        }
+    }
 }
 
 // ---- longer sides: the products -----------------------------------------------------
@@ -501,9 +539,10 @@ struct Job {
     int M, N, K;       // D [M, N] = sum over K
     int tiles_m;       // tiles along M (symmetric modes: unused)
     Planes out;        // GRAM, POLY, UPDATE
-    Planes g;          // POLY: the planes of G
+    Planes g;          // POLY: the planes of G; UPDATE, RESULT of one term: those of X
     float c0, c1, c2;  // POLY
     Io io;             // RESULT
+    bool vec;          // RESULT: rows of whole, aligned fours
     int* err;
 };
 
@@ -684,11 +723,27 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_product(const __grid_consta
             float v[32];
 #pragma unroll
             for (int j = 0; j < 32; j++) v[j] = ok ? __uint_as_float(r[j]) : __uint_as_float(0x7fc00000u);
+            if constexpr (TERMS == 1 && !SYM) {  // c0 X, at the product's scale
+                const int64_t xat = (int64_t)z * job.g.stride + (int64_t)row * job.g.ld + c0;
+#pragma unroll
+                for (int j = 0; j < 32; j += 8) {
+                    if (c0 + j >= job.g.ld) continue;
+                    float xv[8];
+                    load_planes8(job.g, xat + j, xv);
+#pragma unroll
+                    for (int k = 0; k < 8; k++) v[j + k] = fmaf(job.c0 * kPlaneScale, xv[k], v[j + k]);
+                }
+            }
             if constexpr (MODE == RESULT) {
                 const int64_t at = ((int64_t)z * job.M + row) * job.N + c0;
+                constexpr float one = 1.f / (kPlaneScale * kPlaneScale);
 #pragma unroll
-                for (int j = 0; j < 32; j++)
-                    if (c0 + j < job.N) job.io.store(at + j, v[j] * (1.f / (kPlaneScale * kPlaneScale)));
+                for (int j = 0; j < 32; j += 4) {
+                    const int left = job.N - c0 - j;
+                    if (left > 0)
+                        job.io.finish(at + j, left < 4 ? left : 4, job.vec && left >= 4,
+                                      make_float4(v[j] * one, v[j + 1] * one, v[j + 2] * one, v[j + 3] * one));
+                }
             } else {
                 // products carry the square of the planes' scale; the rows' padding (to ld) may be written
                 const int64_t at = (int64_t)z * job.out.stride + (int64_t)row * job.out.ld + c0;
@@ -708,7 +763,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_product(const __grid_consta
 #pragma unroll
                         for (int k = 0; k < 8; k++)
                             v[j + k] = fmaf(job.c2, v[j + k], job.c1 * gv[k]) +
-                                       (c0 + j + k == row ? job.c0 * kPlaneScale : 0.f);
+                                       (TERMS == 3 && c0 + j + k == row ? job.c0 * kPlaneScale : 0.f);
                     }
                 }
                 if (!SYM || c0 > row) {
@@ -820,7 +875,7 @@ Layout layout_of(const Shape& s, int terms) {
         l.x_plane = align256(s.stack * s.rows * pad64(s.cols) * 2);
         l.s_plane = align256(s.stack * s.side * pad64(s.side) * 2);
         const int planes = terms == 3 ? 2 : 1;
-        for (int64_t* p : {&l.x[0], &l.x[1]}) *p = take(planes * l.x_plane);
+        for (int64_t* p : {&l.x[0], &l.x[1]}) *p = take(2 * l.x_plane);
         for (int64_t* p : {&l.g, &l.b}) *p = take(planes * l.s_plane);
     }
     l.bytes = at;
@@ -839,7 +894,7 @@ int run_small(const Shape& s, const Layout& l, const Io& io, const Poly& poly, d
     int e = start<k_small_gram<MB, TALL, Io>>(grid, kSmallThreads, 0, false, st, io, (int)s.side, s.length, chunk, vec,
                                               part);
     if (!e)
-        e = start<k_small_poly<MB>>(dim3((unsigned)s.stack), NT >= 8 ? kSmallThreads : 32 * NT, 4 * RM * SP * 8, true, st,
+        e = start<k_small_poly<MB>>(dim3((unsigned)s.stack), kSmallThreads, 4 * RM * SP * 8, true, st,
                                     part, (int)chunks, (int)s.side, poly, eps, pmat);
     if (!e)
         e = start<k_small_apply<MB, TALL, Io>>(grid, kSmallThreads, RM * SP * 8 + S::SIZE * 4, true, st, io, (int)s.side,
@@ -892,20 +947,21 @@ int run_planes(const Shape& s, const Layout& l, const Io& io, const Poly& poly, 
     constexpr int BN = 256;
     double* part = (double*)(ws + l.part);
     const int64_t ldx = pad64(s.cols), lds = pad64(s.side);
-    const auto planes = [&](int64_t at, int64_t plane, int64_t ld, int64_t rows) {
-        return Planes{(__half*)(ws + at), TERMS == 3 ? (__half*)(ws + at + plane) : nullptr, ld, rows * ld};
+    const auto planes = [&](int64_t at, int64_t plane, int64_t ld, int64_t rows, bool two) {
+        return Planes{(__half*)(ws + at), two ? (__half*)(ws + at + plane) : nullptr, ld, rows * ld};
     };
-    Matrix x[2] = {{planes(l.x[0], l.x_plane, ldx, s.rows), s.rows, s.cols},
-                   {planes(l.x[1], l.x_plane, ldx, s.rows), s.rows, s.cols}};
-    const Matrix g = {planes(l.g, l.s_plane, lds, s.side), s.side, s.side};
-    const Matrix b = {planes(l.b, l.s_plane, lds, s.side), s.side, s.side};
+    const Matrix x[2] = {{planes(l.x[0], l.x_plane, ldx, s.rows, true), s.rows, s.cols},
+                         {planes(l.x[1], l.x_plane, ldx, s.rows, true), s.rows, s.cols}};
+    const Matrix g = {planes(l.g, l.s_plane, lds, s.side, TERMS == 3), s.side, s.side};
+    const Matrix b = {planes(l.b, l.s_plane, lds, s.side, TERMS == 3), s.side, s.side};
+    const bool vec = io.aligned && s.cols % 4 == 0;
     const int nb = (int)norm_blocks(s);
     int e = start<k_norm<Io>>(dim3((unsigned)nb, (unsigned)s.stack), kNormThreads, 0, false, st, io, s.rows * s.cols,
-                              part);
+                              io.aligned && s.rows * s.cols % 4 == 0, part);
     if (e) return e;
     const int64_t row_blocks = ceil_div(s.rows, kNormThreads / 32), most = ceil_div(8 * 148, s.stack);
     e = start<k_planes<Io>>(dim3((unsigned)(row_blocks < most ? row_blocks : most), (unsigned)s.stack), kNormThreads, 0,
-                            false, st, io, s.rows, s.cols, part, nb, eps, x[0].p);
+                            false, st, io, s.rows, s.cols, vec, part, nb, eps, x[0].p);
     Job<NoIo> job = {};
     job.err = (int*)(ws + l.err);
     for (int i = 0; i < poly.steps && !e; i++) {
@@ -925,6 +981,7 @@ int run_planes(const Shape& s, const Layout& l, const Io& io, const Poly& poly, 
         job.M = (int)s.rows;
         job.N = (int)s.cols;
         job.out = next.p;
+        job.g = in.p;
         if (i + 1 < poly.steps) {
             e = s.tall ? run_product<UPDATE, false, false, TERMS, BN>(in, b, s.stack, job, st)
                        : run_product<UPDATE, false, true, TERMS, BN>(b, in, s.stack, job, st);
@@ -932,6 +989,8 @@ int run_planes(const Shape& s, const Layout& l, const Io& io, const Poly& poly, 
             Job<Io> result = {};
             result.M = job.M, result.N = job.N, result.K = job.K, result.err = job.err;
             result.io = io;
+            result.vec = vec;
+            result.g = in.p, result.c0 = job.c0;
             e = s.tall ? run_product<RESULT, false, false, TERMS, BN>(in, b, s.stack, result, st)
                        : run_product<RESULT, false, true, TERMS, BN>(b, in, s.stack, result, st);
         }

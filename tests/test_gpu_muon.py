@@ -10,8 +10,10 @@ matrix' root mean square.  Longer sides round every product as fp32 does, up to
 a factor: a split product is off by at most 2^-21 of itself where fp32 rounds to
 2^-24, and the tensor cores' sums round toward zero (twice the step).  Both are
 enlarged by the steps in the same way, so the 2-norm of the error may be 16
-times that of the plain fp32 form on the same input (one product of fp16 heads,
-for bf16: operands rounded to 2^-12, 2^13 times), plus the half step of the type.
+times that of the plain fp32 form on the same input, plus the half step of the
+type.  bf16 takes one product of operands rounded to 2^-12: a step is off by about
+2^-11 of its sums, whose magnitudes are at most 3.5 times its result, and the steps
+after it enlarge an error as they do the result: 2^-8 of the result's norm in all.
 """
 from __future__ import annotations
 
@@ -39,6 +41,8 @@ def make(stack, rows, cols, kind, dtype=F32, seed=0):
         x = u @ torch.randn(stack, k, cols, device=DEV, generator=g)
         if kind == "strong":
             x = x + 0.1 * noise
+        elif kind == "weak":
+            x = x + 0.003 * noise
         elif kind == "tiny":
             x = 1e-18 * (x + 0.3 * noise)
         # "lowrank": nothing along the other directions
@@ -79,9 +83,9 @@ def check(got, x, **kw):
             bound = half * w.abs() * (1 + half) + 2.0 ** -28 * rms + tiny
             assert float((off.abs() / bound).max()) <= 1.0, i
         else:
-            factor = 2.0 ** 13 if dtype == BF16 else 16.0
             own = float((plain(x[i], **kw).double() - w).norm())
-            assert float(off.norm()) <= factor * own + half * float(w.norm()), (i, float(off.norm()), own)
+            bound = 2.0 ** -8 * float(w.norm()) if dtype == BF16 else 16.0 * own
+            assert float(off.norm()) <= bound + half * float(w.norm()), (i, float(off.norm()), own)
 
 
 SMALL = [(1, 1, 1), (3, 1, 70), (3, 70, 1), (2, 5, 7), (4, 8, 8), (5, 16, 2560), (5, 2560, 16), (3, 17, 300),
@@ -103,7 +107,7 @@ LONG = [(1, 65, 65), (1, 128, 128), (1, 130, 257), (2, 257, 130), (1, 256, 512),
 @pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=str)
 @pytest.mark.parametrize("shape", LONG, ids=str)
 def test_longer_sides_match_the_singular_values(shape, dtype):
-    for kind in ("noise", "strong"):
+    for kind in ("noise", "strong", "weak"):
         x = make(*shape, kind, dtype, seed=sum(shape))
         check(eb.orthogonalize(x), x)
 
