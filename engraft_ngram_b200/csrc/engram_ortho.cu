@@ -26,6 +26,7 @@
 // or lie above it are computed and stored twice.  The planes are read in the layout in which
 // U was given: tall matrices use U^T U and X P, so nothing is transposed in memory;
 // the descriptors take each operand along K or across it.
+#include <algorithm>
 #include <type_traits>
 
 #include "engram_tensor.cuh"
@@ -422,6 +423,7 @@ constexpr int kNormThreads = 256;
 template <typename Io>
 __global__ void __launch_bounds__(kNormThreads) k_norm(Io io, int64_t size, bool vec, double* __restrict__ part) {
     __shared__ double warp_sum[kNormThreads / 32];
+    let_next_start();
     const int64_t base = blockIdx.y * size, pieces = (size + 3) / 4, step = (int64_t)gridDim.x * kNormThreads;
     double v = 0.0;
     constexpr int N = 4;  // pieces under way a thread
@@ -469,6 +471,8 @@ template <typename Io>
 __global__ void __launch_bounds__(kNormThreads) k_planes(Io io, int64_t rows, int64_t cols, bool vec,
                                                          const double* part, int parts, double eps, Planes out) {
     __shared__ double total;
+    wait_for_previous();
+    let_next_start();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (warp == 0) {
         double v = 0.0;
@@ -517,7 +521,7 @@ __global__ void __launch_bounds__(kNormThreads) k_planes(Io io, int64_t rows, in
 enum Mode { GRAM, POLY, UPDATE, RESULT };
 
 constexpr int BM = 128;
-constexpr int kGemmThreads = 192;
+constexpr int kGemmThreads = 320, kEpilogueWarps = 8;
 constexpr int kStageTotal = 192 * 1024;
 
 // One K slice of the operands: 32 columns of four planes (A hi, B hi, A lo, B lo) or 64 of two.
@@ -537,7 +541,8 @@ struct Maps {
 template <typename Io>
 struct Job {
     int M, N, K;       // D [M, N] = sum over K
-    int tiles_m;       // tiles along M (symmetric modes: unused)
+    int tiles_m, tiles_n, tiles;  // tiles along M, along N, of a matrix
+    int total;                    // tiles of the stack
     Planes out;        // GRAM, POLY, UPDATE
     Planes g;          // POLY: the planes of G; UPDATE, RESULT of one term: those of X
     float c0, c1, c2;  // POLY
@@ -555,6 +560,10 @@ __device__ __forceinline__ uint64_t operand_desc(uint32_t addr) {
     constexpr uint64_t swizzle = (MN || KS == 64) ? 2 : 4;
     return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(sbo >> 4) << 32) |
            ((uint64_t)1 << 46) | (swizzle << 61);
+}
+
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 template <bool A_MN, bool B_MN, int BN>
@@ -603,9 +612,27 @@ __device__ __forceinline__ void put8(const Planes& p, int64_t i, const float* v)
     if (p.lo) *reinterpret_cast<uint4*>(p.lo + i) = *reinterpret_cast<const uint4*>(l);
 }
 
-// One block a BM x BN tile: warp 0 loads (TMA), one lane of warp 1 issues the MMAs, warps 2 to 5
-// take the accumulator (tensor-memory lanes 32 (w % 4) ..) through the mode's epilogue.  A wait that
-// gives up (never, in a correct run) counts itself in *err and the tile's results become NaN.
+// Tile t of the stack.  Symmetric modes have those with an entry on or above the diagonal: column block b has
+// the first R (b + 1) row blocks, as far as there are any.
+template <bool SYM, int BN, typename J>
+__device__ __forceinline__ void tile_at(const J& job, int t, int& z, int& m0, int& n0) {
+    z = t / job.tiles;
+    int left = t - z * job.tiles;
+    if constexpr (SYM) {
+        constexpr int R = BN / BM;
+        int b = 0, rows = min(R, job.tiles_m);
+        while (left >= rows) left -= rows, b++, rows = min(R * (b + 1), job.tiles_m);
+        m0 = left * BM, n0 = b * BN;
+    } else {
+        m0 = left % job.tiles_m * BM, n0 = left / job.tiles_m * BN;
+    }
+}
+
+// BM x BN tiles on persistent blocks, one an SM: warp 0 loads (TMA), one lane of warp 1 issues the MMAs into
+// two accumulators in turn, and warps 2 to 9 take each through the mode's epilogue (tensor-memory lanes 32
+// (w % 4) .., half of the columns) while the next one is made: the epilogue, up to 8 us a tile beside 11 us
+// of products, costs time only after a block's last tile.  A wait that gives up (never, in a correct run)
+// counts itself in *err and the tile's results become NaN.
 template <int MODE, bool A_MN, bool B_MN, int TERMS, int BN, typename Io>
 __global__ void __launch_bounds__(kGemmThreads, 1) k_product(const __grid_constant__ Maps maps, const Job<Io> job) {
     using G = Cfg<TERMS, BN>;
@@ -614,34 +641,28 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_product(const __grid_consta
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * G::STAGE_BYTES);
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 1);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 4);
     volatile uint32_t* gave_up = tmem_slot + 1;
-    const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + STAGES), acc_bar = smem_u32(bars + 2 * STAGES);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, z = blockIdx.y;
-    int m0, n0;
-    if constexpr (SYM) {  // tiles with an entry on or above the diagonal: column block b has R (b + 1)
-        constexpr int R = BN / BM;
-        int left = blockIdx.x, b = 0;
-        while (left >= R * (b + 1)) left -= R * (b + 1), b++;
-        m0 = left * BM, n0 = b * BN;
-    } else {
-        m0 = (int)(blockIdx.x % job.tiles_m) * BM, n0 = (int)(blockIdx.x / job.tiles_m) * BN;
-    }
+    const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + STAGES), acc_full = smem_u32(bars + 2 * STAGES);
+    const uint32_t acc_empty = acc_full + 16;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int slices = (job.K + KS - 1) / KS;
-    if (SYM && m0 >= job.M) return;  // the last column block may be wider than the matrix
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; s++) {
             mbar_init(full0 + 8 * s, 1);
             mbar_init(empty0 + 8 * s, 1);
         }
-        mbar_init(acc_bar, 1);
+        for (int a = 0; a < 2; a++) {
+            mbar_init(acc_full + 8 * a, 1);
+            mbar_init(acc_empty + 8 * a, kEpilogueWarps);
+        }
         *gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                     "r"((uint32_t)BN)
+                     "r"((uint32_t)(2 * BN))
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -649,22 +670,28 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_product(const __grid_consta
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *tmem_slot;
+    wait_for_previous();
+    let_next_start();
 
     if (warp == 0) {
         if (lane == 0) {
             int i = 0;
             bool ok = true;
-            for (; i < slices; i++) {
-                const int s = i % STAGES, round = i / STAGES;
-                if (round > 0) ok = mbar_wait(empty0 + 8 * s, (uint32_t)((round - 1) & 1), job.err);
-                if (!ok) break;
-                const uint32_t bar = full0 + 8 * s, st = smem_u32(smem + s * G::STAGE_BYTES);
-                mbar_expect_tx(bar, G::STAGE_BYTES);
-                load_operand<A_MN, KS, BM>(st, &maps.a_hi, m0, i * KS, z, bar);
-                load_operand<B_MN, KS, BN>(st + G::A_BYTES, &maps.b_hi, n0, i * KS, z, bar);
-                if constexpr (TERMS == 3) {
-                    load_operand<A_MN, KS, BM>(st + G::A_BYTES + G::B_BYTES, &maps.a_lo, m0, i * KS, z, bar);
-                    load_operand<B_MN, KS, BN>(st + 2 * G::A_BYTES + G::B_BYTES, &maps.b_lo, n0, i * KS, z, bar);
+            for (int t = blockIdx.x; t < job.total && ok; t += gridDim.x) {
+                int z, m0, n0;
+                tile_at<SYM, BN>(job, t, z, m0, n0);
+                for (int k = 0; k < slices; k++, i++) {
+                    const int s = i % STAGES, round = i / STAGES;
+                    if (round > 0) ok = mbar_wait(empty0 + 8 * s, (uint32_t)((round - 1) & 1), job.err);
+                    if (!ok) break;
+                    const uint32_t bar = full0 + 8 * s, st = smem_u32(smem + s * G::STAGE_BYTES);
+                    mbar_expect_tx(bar, G::STAGE_BYTES);
+                    load_operand<A_MN, KS, BM>(st, &maps.a_hi, m0, k * KS, z, bar);
+                    load_operand<B_MN, KS, BN>(st + G::A_BYTES, &maps.b_hi, n0, k * KS, z, bar);
+                    if constexpr (TERMS == 3) {
+                        load_operand<A_MN, KS, BM>(st + G::A_BYTES + G::B_BYTES, &maps.a_lo, m0, k * KS, z, bar);
+                        load_operand<B_MN, KS, BN>(st + 2 * G::A_BYTES + G::B_BYTES, &maps.b_lo, n0, k * KS, z, bar);
+                    }
                 }
             }
             // every load issued into this block's shared memory has landed before it ends
@@ -673,40 +700,54 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_product(const __grid_consta
         }
     } else if (warp == 1) {
         if (lane == 0) {
-            for (int i = 0; i < slices; i++) {
-                const int s = i % STAGES;
-                if (!mbar_wait(full0 + 8 * s, (uint32_t)((i / STAGES) & 1), job.err)) {
+            int i = 0, made = 0;
+            bool ok = true;
+            for (int t = blockIdx.x; t < job.total; t += gridDim.x, made++) {
+                const int acc = made & 1;
+                if (made >= 2) ok = ok && mbar_wait(acc_empty + 8 * acc, (uint32_t)((made / 2 - 1) & 1), job.err);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t d = tmem + acc * BN;
+                for (int n = 0; n < slices && ok; n++, i++) {
+                    const int s = i % STAGES;
+                    ok = mbar_wait(full0 + 8 * s, (uint32_t)((i / STAGES) & 1), job.err);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t a = smem_u32(smem + s * G::STAGE_BYTES), b = a + G::A_BYTES;
+                    const uint32_t alo = b + G::B_BYTES, blo = alo + G::A_BYTES;
+#pragma unroll
+                    for (int k = 0; k < KS / 16; k++) {  // 16 of K: 32 bytes along it, 16 rows of 128 bytes across it
+                        constexpr uint32_t sa = A_MN ? 2048 : 32, sb = B_MN ? 2048 : 32;
+                        const uint64_t ah = operand_desc<A_MN, KS>(a + sa * k), bh = operand_desc<B_MN, KS>(b + sb * k);
+                        const uint32_t first = (n > 0 || k > 0) ? 1u : 0u;
+                        if constexpr (TERMS == 3) {  // the small terms first
+                            umma_f16<A_MN, B_MN, BN>(d, operand_desc<A_MN, KS>(alo + sa * k), bh, first);
+                            umma_f16<A_MN, B_MN, BN>(d, ah, operand_desc<B_MN, KS>(blo + sb * k), 1u);
+                            umma_f16<A_MN, B_MN, BN>(d, ah, bh, 1u);
+                        } else {
+                            umma_f16<A_MN, B_MN, BN>(d, ah, bh, first);
+                        }
+                    }
+                    umma_commit(empty0 + 8 * s);
+                }
+                if (!ok) {
                     *gave_up = 1;
                     __threadfence_block();
-                    break;
                 }
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t a = smem_u32(smem + s * G::STAGE_BYTES), b = a + G::A_BYTES;
-                const uint32_t alo = b + G::B_BYTES, blo = alo + G::A_BYTES;
-#pragma unroll
-                for (int k = 0; k < KS / 16; k++) {  // 16 of K: 32 bytes along it, 16 rows of 128 bytes across it
-                    constexpr uint32_t sa = A_MN ? 2048 : 32, sb = B_MN ? 2048 : 32;
-                    const uint64_t ah = operand_desc<A_MN, KS>(a + sa * k), bh = operand_desc<B_MN, KS>(b + sb * k);
-                    const uint32_t first = (i > 0 || k > 0) ? 1u : 0u;
-                    if constexpr (TERMS == 3) {  // the small terms first
-                        umma_f16<A_MN, B_MN, BN>(tmem, operand_desc<A_MN, KS>(alo + sa * k), bh, first);
-                        umma_f16<A_MN, B_MN, BN>(tmem, ah, operand_desc<B_MN, KS>(blo + sb * k), 1u);
-                        umma_f16<A_MN, B_MN, BN>(tmem, ah, bh, 1u);
-                    } else {
-                        umma_f16<A_MN, B_MN, BN>(tmem, ah, bh, first);
-                    }
-                }
-                umma_commit(empty0 + 8 * s);
+                umma_commit(acc_full + 8 * acc);
             }
-            umma_commit(acc_bar);
         }
         __syncwarp();
     } else {
-        const int w = warp & 3;
-        const bool ok = mbar_wait(acc_bar, 0u, job.err) && *gave_up == 0;
+        const int w = warp & 3, part = (warp - 2) >> 2;
+        int made = 0;
+        for (int t = blockIdx.x; t < job.total; t += gridDim.x, made++) {
+        int z, m0, n0;
+        tile_at<SYM, BN>(job, t, z, m0, n0);
+        const int acc = made & 1;
+        const bool ok = mbar_wait(acc_full + 8 * acc, (uint32_t)((made / 2) & 1), job.err) && *gave_up == 0;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const int row = m0 + 32 * w + lane;
-        for (int col = 0; col < BN; col += 32) {
+        for (int col = part * (BN / 2); col < (part + 1) * (BN / 2); col += 32) {
             uint32_t r[32];
             asm volatile(
                 "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
@@ -716,8 +757,13 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_product(const __grid_consta
                   "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
                   "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
                   "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-                : "r"(tmem + ((uint32_t)(32 * w) << 16) + (uint32_t)col));
+                : "r"(tmem + ((uint32_t)(32 * w) << 16) + (uint32_t)(acc * BN + col)));
             asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+            if (col + 32 == (part + 1) * (BN / 2)) {  // this warp's part of the accumulator has been read
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(acc_empty + 8 * acc);
+            }
             const int c0 = n0 + col;
             if (row >= job.M || c0 >= job.N) continue;
             float v[32];
@@ -783,12 +829,14 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_product(const __grid_consta
                 }
             }
         }
+        }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)BN) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)(2 * BN))
+                     : "memory");
     }
 }
 
@@ -934,11 +982,16 @@ int run_product(const Matrix& a, const Matrix& b, int64_t stack, Job<Io> job, cu
     if (!make(&maps.a_hi, a.p.hi, a, A_MN, BM) || !make(&maps.b_hi, b.p.hi, b, B_MN, BN)) return ENGRAM_ERR_CUDA;
     if (TERMS == 3 && (!make(&maps.a_lo, a.p.lo, a, A_MN, BM) || !make(&maps.b_lo, b.p.lo, b, B_MN, BN)))
         return ENGRAM_ERR_CUDA;
-    const int64_t tn = ceil_div(job.N, BN);
-    job.tiles_m = (int)ceil_div(job.M, BM);
-    const int64_t tiles = (MODE == GRAM || MODE == POLY) ? (BN / BM) * tn * (tn + 1) / 2 : job.tiles_m * tn;
-    return start<k_product<MODE, A_MN, B_MN, TERMS, BN, Io>>(dim3((unsigned)tiles, (unsigned)stack), kGemmThreads,
-                                                             G::SMEM, false, st, maps, job);
+    job.tiles_m = (int)ceil_div(job.M, BM), job.tiles_n = (int)ceil_div(job.N, BN);
+    job.tiles = job.tiles_m * job.tiles_n;
+    if (MODE == GRAM || MODE == POLY) {
+        job.tiles = 0;
+        for (int b = 0; b < job.tiles_n; b++) job.tiles += std::min(BN / BM * (b + 1), job.tiles_m);
+    }
+    if (job.tiles * stack > INT32_MAX) return ENGRAM_ERR_RANGE;
+    job.total = (int)(job.tiles * stack);
+    return start<k_product<MODE, A_MN, B_MN, TERMS, BN, Io>>(dim3((unsigned)std::min(job.total, sm_count())),
+                                                             kGemmThreads, G::SMEM, true, st, maps, job);
 }
 
 template <int TERMS, typename Io>
@@ -961,7 +1014,7 @@ int run_planes(const Shape& s, const Layout& l, const Io& io, const Poly& poly, 
     if (e) return e;
     const int64_t row_blocks = ceil_div(s.rows, kNormThreads / 32), most = ceil_div(8 * 148, s.stack);
     e = start<k_planes<Io>>(dim3((unsigned)(row_blocks < most ? row_blocks : most), (unsigned)s.stack), kNormThreads, 0,
-                            false, st, io, s.rows, s.cols, vec, part, nb, eps, x[0].p);
+                            true, st, io, s.rows, s.cols, vec, part, nb, eps, x[0].p);
     Job<NoIo> job = {};
     job.err = (int*)(ws + l.err);
     for (int i = 0; i < poly.steps && !e; i++) {
