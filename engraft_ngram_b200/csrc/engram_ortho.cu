@@ -531,7 +531,7 @@ struct Cfg {
     static constexpr int A_BYTES = BM * KS * 2, B_BYTES = BN * KS * 2;
     static constexpr int STAGE_BYTES = (TERMS == 3 ? 2 : 1) * (A_BYTES + B_BYTES);
     static constexpr int STAGES = kStageTotal / STAGE_BYTES;
-    static constexpr int SMEM = STAGES * STAGE_BYTES + 1024 + 256;
+    static constexpr int SMEM = STAGES * STAGE_BYTES + kEpilogueWarps * 4096 + 1024 + 256;
 };
 
 struct Maps {
@@ -640,7 +640,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_product(const __grid_consta
     constexpr bool SYM = MODE == GRAM || MODE == POLY;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * G::STAGE_BYTES);
+    uint8_t* turned = smem + STAGES * G::STAGE_BYTES;  // a 32 x 32 piece of each epilogue warp
+    uint64_t* bars = reinterpret_cast<uint64_t*>(turned + kEpilogueWarps * 4096);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 4);
     volatile uint32_t* gave_up = tmem_slot + 1;
     const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + STAGES), acc_full = smem_u32(bars + 2 * STAGES);
@@ -746,7 +747,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_product(const __grid_consta
         const int acc = made & 1;
         const bool ok = mbar_wait(acc_full + 8 * acc, (uint32_t)((made / 2) & 1), job.err) && *gave_up == 0;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const int row = m0 + 32 * w + lane;
+        uint8_t* tile = turned + (warp - 2) * 4096;
         for (int col = part * (BN / 2); col < (part + 1) * (BN / 2); col += 32) {
             uint32_t r[32];
             asm volatile(
@@ -764,68 +765,95 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_product(const __grid_consta
                 __syncwarp();
                 if (lane == 0) mbar_arrive(acc_empty + 8 * acc);
             }
-            const int c0 = n0 + col;
-            if (row >= job.M || c0 >= job.N) continue;
-            float v[32];
+            const int r0 = m0 + 32 * w, c0 = n0 + col;
+            if (r0 >= job.M || c0 >= job.N) continue;
+            if constexpr (SYM)
+                if (c0 + 31 < r0) continue;  // below the diagonal: its mirror image is computed
+            // Through shared memory, so that four lanes take 64 consecutive bytes of a row: a lane has a row of
+            // the accumulator, and 16 bytes of each of 32 rows a store are half a sector each, at a fifth of
+            // the rate.  Units of 16 bytes are swapped by row: no bank twice.
+            __syncwarp();
 #pragma unroll
-            for (int j = 0; j < 32; j++) v[j] = ok ? __uint_as_float(r[j]) : __uint_as_float(0x7fc00000u);
-            if constexpr (TERMS == 1 && !SYM) {  // c0 X, at the product's scale
-                const int64_t xat = (int64_t)z * job.g.stride + (int64_t)row * job.g.ld + c0;
+            for (int u = 0; u < 8; u++)
+                *reinterpret_cast<uint4*>(tile + lane * 128 + ((u ^ (lane & 7)) << 4)) =
+                    make_uint4(r[4 * u], r[4 * u + 1], r[4 * u + 2], r[4 * u + 3]);
+            __syncwarp();
 #pragma unroll
-                for (int j = 0; j < 32; j += 8) {
-                    if (c0 + j >= job.g.ld) continue;
-                    float xv[8];
-                    load_planes8(job.g, xat + j, xv);
+            for (int it = 0; it < 4; it++) {
+                const int lr = 8 * it + (lane >> 2), u = 2 * (lane & 3), row = r0 + lr, c = c0 + 4 * u;
+                float* lo4 = reinterpret_cast<float*>(tile + lr * 128 + ((u ^ (lr & 7)) << 4));
+                float* hi4 = reinterpret_cast<float*>(tile + lr * 128 + (((u + 1) ^ (lr & 7)) << 4));
+                float v[8];
+                *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(lo4);
+                *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(hi4);
+                if (!ok)
 #pragma unroll
-                    for (int k = 0; k < 8; k++) v[j + k] = fmaf(job.c0 * kPlaneScale, xv[k], v[j + k]);
-                }
-            }
-            if constexpr (MODE == RESULT) {
-                const int64_t at = ((int64_t)z * job.M + row) * job.N + c0;
-                constexpr float one = 1.f / (kPlaneScale * kPlaneScale);
+                    for (int j = 0; j < 8; j++) v[j] = __uint_as_float(0x7fc00000u);
+                const bool in = row < job.M && c < job.N;
+                if constexpr (TERMS == 1 && !SYM) {  // c0 X, at the product's scale
+                    if (in) {
+                        float xv[8];
+                        load_planes8(job.g, (int64_t)z * job.g.stride + (int64_t)row * job.g.ld + c, xv);
 #pragma unroll
-                for (int j = 0; j < 32; j += 4) {
-                    const int left = job.N - c0 - j;
-                    if (left > 0)
-                        job.io.finish(at + j, left < 4 ? left : 4, job.vec && left >= 4,
-                                      make_float4(v[j] * one, v[j + 1] * one, v[j + 2] * one, v[j + 3] * one));
-                }
-            } else {
-                // products carry the square of the planes' scale; the rows' padding (to ld) may be written
-                const int64_t at = (int64_t)z * job.out.stride + (int64_t)row * job.out.ld + c0;
-#pragma unroll
-                for (int j = 0; j < 32; j++) v[j] *= 1.f / kPlaneScale;
-                if constexpr (MODE == POLY) {
-                    const int64_t gat = (int64_t)z * job.g.stride + (int64_t)row * job.g.ld + c0;
-#pragma unroll
-                    for (int j = 0; j < 32; j += 8) {
-                        float gv[8];
-                        if (c0 + j < job.g.ld) {
-                            load_planes8(job.g, gat + j, gv);
-                        } else {
-#pragma unroll
-                            for (int k = 0; k < 8; k++) gv[k] = 0.f;
-                        }
-#pragma unroll
-                        for (int k = 0; k < 8; k++)
-                            v[j + k] = fmaf(job.c2, v[j + k], job.c1 * gv[k]) +
-                                       (TERMS == 3 && c0 + j + k == row ? job.c0 * kPlaneScale : 0.f);
+                        for (int j = 0; j < 8; j++) v[j] = fmaf(job.c0 * kPlaneScale, xv[j], v[j]);
                     }
                 }
-                if (!SYM || c0 > row) {
+                if constexpr (MODE == RESULT) {
+                    const int64_t at = ((int64_t)z * job.M + row) * job.N + c;
+                    constexpr float one = 1.f / (kPlaneScale * kPlaneScale);
 #pragma unroll
-                    for (int j = 0; j < 32; j += 8)
-                        if (c0 + j < job.out.ld) put8(job.out, at + j, v + j);
+                    for (int j = 0; j < 8; j += 4) {
+                        const int left = job.N - c - j;
+                        if (in && left > 0)
+                            job.io.finish(at + j, left < 4 ? left : 4, job.vec && left >= 4,
+                                          make_float4(v[j] * one, v[j + 1] * one, v[j + 2] * one, v[j + 3] * one));
+                    }
                 } else {
+                    // products carry the square of the planes' scale; the rows' padding (to ld) may be written
+                    const int64_t at = (int64_t)z * job.out.stride + (int64_t)row * job.out.ld + c;
 #pragma unroll
-                    for (int j = 0; j < 32; j++)
-                        if (c0 + j >= row && c0 + j < job.N) put(job.out, at + j, v[j]);
+                    for (int j = 0; j < 8; j++) v[j] *= 1.f / kPlaneScale;
+                    if constexpr (MODE == POLY) {
+                        if (in) {
+                            float gv[8];
+                            load_planes8(job.g, (int64_t)z * job.g.stride + (int64_t)row * job.g.ld + c, gv);
+#pragma unroll
+                            for (int j = 0; j < 8; j++)
+                                v[j] = fmaf(job.c2, v[j], job.c1 * gv[j]) +
+                                       (TERMS == 3 && c + j == row ? job.c0 * kPlaneScale : 0.f);
+                        }
+                    }
+                    if (in && (!SYM || c > row)) {
+                        put8(job.out, at, v);
+                    } else if (in) {
+#pragma unroll
+                        for (int j = 0; j < 8; j++)
+                            if (c + j >= row && c + j < job.N) put(job.out, at + j, v[j]);
+                    }
+                    if constexpr (SYM) {
+                        *reinterpret_cast<float4*>(lo4) = *reinterpret_cast<const float4*>(v);
+                        *reinterpret_cast<float4*>(hi4) = *reinterpret_cast<const float4*>(v + 4);
+                    }
                 }
-                if constexpr (SYM) {  // the mirrored entries: 32 lanes store 32 neighbours of a row
+            }
+            if constexpr (SYM) {  // the mirrored entries: row c0 + ., eight columns of it a lane
+                __syncwarp();
 #pragma unroll
-                    for (int j = 0; j < 32; j++)
-                        if (c0 + j > row && c0 + j < job.N)
-                            put(job.out, (int64_t)z * job.out.stride + (int64_t)(c0 + j) * job.out.ld + row, v[j]);
+                for (int it = 0; it < 4; it++) {
+                    const int lc = 8 * it + (lane >> 2), lr = 8 * (lane & 3), row = c0 + lc, c = r0 + lr;
+                    float v[8];
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        v[j] = *reinterpret_cast<const float*>(tile + (lr + j) * 128 + (((lc >> 2) ^ j) << 4) + 4 * (lc & 3));
+                    if (row >= job.N || c >= job.M) continue;
+                    const int64_t at = (int64_t)z * job.out.stride + (int64_t)row * job.out.ld + c;
+                    if (c + 7 < row && c + 7 < job.M) {
+                        put8(job.out, at, v);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 8; j++)
+                            if (c + j < row && c + j < job.M) put(job.out, at + j, v[j]);
+                    }
                 }
             }
         }
