@@ -197,10 +197,11 @@ struct FindTile {  // used by the first launch only, where its stages come to st
     int32_t warp_sum[kWarps];
 };
 
-// Tile blockIdx.x in the order of the adapters, found without a plan.
+// Tile k in the order of the adapters, found without a plan.
 template <int BM>
-__device__ __forceinline__ void find_tile(FindTile& f, TileRows<BM>& r, const int32_t* __restrict__ index, int T, int n) {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, k = blockIdx.x;
+__device__ __forceinline__ void find_tile(FindTile& f, TileRows<BM>& r, const int32_t* __restrict__ index, int T, int n,
+                                          int k) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     for (int i = tid; i <= n; i += kThreads) f.tiles[i] = 0;
     if (tid == 0) r.adapter = -1, r.first = r.rows = 0;
     __syncthreads();
@@ -237,8 +238,8 @@ __device__ __forceinline__ void find_tile(FindTile& f, TileRows<BM>& r, const in
 }
 
 // The block's tile, or its BM positions of one shared by PARTS blocks, from the plan; false: there are none.
-template <int BM, int PARTS = 1>
-__device__ __forceinline__ bool read_tile(TileRows<BM>& r, const Plan& plan) {
+template <int BM, int PARTS = 1, int ROWS>
+__device__ __forceinline__ bool read_tile(TileRows<ROWS>& r, const Plan& plan) {
     const int k = blockIdx.x / PARTS, from = (int)(blockIdx.x % PARTS) * BM;
     if (plan.tiles && k >= *plan.tiles) return false;
     const Tile t = plan.tile[k];
@@ -399,22 +400,24 @@ constexpr int fit_stages(int bytes) {
 // ---- shrink --------------------------------------------------------------------
 // h[split, t, :] = scale_i * sum over this split's columns k of x[t, k] W_i[:, k].
 // TRANS = false: W_i = A_i [rank, K] (K consecutive); true: W_i = B_i [K, rank] (rank consecutive).
-// One block per (tile, split).  WM = 8: 128 positions, 16 a warp.  WM = 1: 16 positions, and the warps
-// share the columns and are summed, in their order, through shared memory.  A chunk is 64 bytes of a
+// WM = 8: 64 positions of a tile of 128 a block, four warps of 16 along them; WM = 1: 16 positions.  The other
+// warps share the columns and are summed, in their order, through shared memory.  (128 positions a block
+// left two stages of a ring: 30 us where this takes 22 for 2048 x 12800 in fp32.)  A chunk is 64 bytes of a
 // row, two steps of the MMA.  fp32 fragments come as 16-byte reads: a lane holds columns 4 q ..
 // 4 q + 3 of its row, of which step s takes 2 s and 2 s + 1 (the order inside a sum is free as long as
 // both operands agree).  Rows are padded so that those reads (two rows of 64 bytes a quarter warp: 64
 // bytes) and ldmatrix (eight rows of 16: 16 bytes) meet no bank twice.
 template <typename T, int RB, int WM, bool TRANS>
 struct ShrinkCfg {
-    static constexpr int E = kE<T>, RP = 8 * RB, BM = 16 * WM, WK = kWarps / WM, PAD = sizeof(T) == 4 ? 64 : 16;
+    static constexpr int E = kE<T>, RP = 8 * RB, TILE = 16 * WM, PAD = sizeof(T) == 4 ? 64 : 16;
+    static constexpr int WR = WM == 8 ? 4 : 1, BM = 16 * WR, PARTS = TILE / BM, WK = kWarps / WR;  // warps along rows, columns
     static constexpr int NCH = WM == 1 ? 8 : 4, KC = NCH * 4 * E;  // chunks and columns of a stage
     static constexpr int X_PITCH = NCH * 64 + PAD, X_BYTES = BM * X_PITCH;
     static constexpr int W_PITCH = TRANS ? RP * (int)sizeof(T) + 16 : X_PITCH;
     static constexpr int W_BYTES = (TRANS ? KC : RP) * W_PITCH;
     static constexpr int STAGE = X_BYTES + W_BYTES;
     static constexpr int NS = fit_stages(STAGE);
-    static constexpr int RED = WM == 1 ? kWarps * BM * RP * 4 : 0;
+    static constexpr int RED = WK * BM * RP * 4;
     static constexpr int MOST = NS * STAGE > RED ? NS * STAGE : RED;
     static constexpr int SMEM = MOST > (int)sizeof(FindTile) ? MOST : (int)sizeof(FindTile);
     static_assert(SMEM <= 220 * 1024, "a block's shared memory");
@@ -424,7 +427,7 @@ struct ShrinkCfg {
 enum Tiles { PLANNED, FIND };
 
 template <typename T, int RB, int WM, bool TRANS>
-__global__ void __launch_bounds__(kThreads) k_shrink(Plan plan, int tiles, const int32_t* __restrict__ index,
+__global__ void __launch_bounds__(kThreads, RB <= 4 ? 3 : 1) k_shrink(Plan plan, int tiles, const int32_t* __restrict__ index,
                                                      const T* __restrict__ x, int64_t ldx, const T* __restrict__ w,
                                                      const float* __restrict__ scale, int n, int rank, int64_t K,
                                                      int64_t k_split, int T_rows, bool xvec, bool wvec,
@@ -433,24 +436,28 @@ __global__ void __launch_bounds__(kThreads) k_shrink(Plan plan, int tiles, const
     constexpr int E = C::E, RP = C::RP, BM = C::BM, WK = C::WK, NCH = C::NCH, KC = C::KC, NS = C::NS;
     constexpr bool F32 = sizeof(T) == 4;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ TileRows<BM> tr;
+    __shared__ TileRows<C::TILE> tr;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
-    const int wm = warp % WM, wk = warp / WM;
+    const int wm = warp % C::WR, wk = warp / C::WR;
+    int from = 0;  // this block's first position of the tile
     if (tiles == FIND) {
         let_next_start();
-        find_tile<BM>(*reinterpret_cast<FindTile*>(smem), tr, index, T_rows, n);
-        if (blockIdx.y == 0) {
-            for (int i = threadIdx.x; i < tr.rows; i += kThreads) plan.perm[blockIdx.x * BM + i] = tr.row[i];
-            if (threadIdx.x == 0) plan.tile[blockIdx.x] = Tile{tr.adapter, (int)blockIdx.x * BM, tr.rows, 0};
+        const int k = blockIdx.x / C::PARTS;
+        find_tile<C::TILE>(*reinterpret_cast<FindTile*>(smem), tr, index, T_rows, n, k);
+        from = (int)(blockIdx.x % C::PARTS) * BM;
+        if (blockIdx.y == 0 && from == 0) {
+            for (int i = threadIdx.x; i < tr.rows; i += kThreads) plan.perm[k * C::TILE + i] = tr.row[i];
+            if (threadIdx.x == 0) plan.tile[k] = Tile{tr.adapter, k * C::TILE, tr.rows, 0};
         }
-        if (tr.rows == 0 || tr.adapter >= n) return;
+        if (tr.rows <= from || tr.adapter >= n) return;
         __syncthreads();  // the scan's memory becomes the stages'
     } else {
         wait_for_previous();
         let_next_start();
-        if (!read_tile<BM>(tr, plan) || tr.adapter >= n) return;
+        if (!read_tile<BM, C::PARTS>(tr, plan) || tr.adapter >= n) return;
     }
-    const int adapter = tr.adapter, rows = tr.rows;
+    const int adapter = tr.adapter, rows = min(BM, tr.rows - from);
+    const int32_t* row_of = tr.row + from;
     const T* wi = w + (int64_t)adapter * rank * K;
     const int64_t k_begin = blockIdx.y * k_split, k_end = k_begin + k_split < K ? k_begin + k_split : K;
     const int stages = k_begin < k_end ? (int)((k_end - k_begin + KC - 1) / KC) : 0;
@@ -461,7 +468,7 @@ __global__ void __launch_bounds__(kThreads) k_shrink(Plan plan, int tiles, const
 #pragma unroll
     for (int k = 0; k < ux.N; k++) {
         const int r = ux.row(k);
-        ux.src[k] = x + (int64_t)tr.row[min(r, BM - 1)] * ldx + k_begin + ux.column() * E;
+        ux.src[k] = x + (int64_t)row_of[min(r, BM - 1)] * ldx + k_begin + ux.column() * E;
         ux.bytes[k] = r < rows ? 16 : 0;
     }
 #pragma unroll
@@ -483,7 +490,7 @@ __global__ void __launch_bounds__(kThreads) k_shrink(Plan plan, int tiles, const
         } else {
             for (int u = threadIdx.x; u < BM * XU; u += kThreads) {
                 const int r = u / XU, c = u % XU;
-                stage_unit<T>(xs + r * C::X_PITCH + c * 16, x + (int64_t)tr.row[r] * ldx + k0 + c * E, x,
+                stage_unit<T>(xs + r * C::X_PITCH + c * 16, x + (int64_t)row_of[r] * ldx + k0 + c * E, x,
                               r < rows ? left - c * E : 0, xvec);
             }
         }
@@ -598,33 +605,19 @@ __global__ void __launch_bounds__(kThreads) k_shrink(Plan plan, int tiles, const
     const auto column = [&](int b, int j) { return F32 && TRANS ? RB * (2 * q + j) + b : 8 * b + 2 * q + j; };
     const float s = scale ? __ldg(scale + adapter) : 1.f;
     float* dst = h + (int64_t)blockIdx.y * T_rows * RP;
-    if constexpr (WM == 1) {
-        stage_wait<0>();
-        __syncthreads();
-        float* red = reinterpret_cast<float*>(smem);  // [kWarps][BM][RP]
+    stage_wait<0>();
+    __syncthreads();
+    float* red = reinterpret_cast<float*>(smem);  // [WK][BM][RP]
 #pragma unroll
-        for (int b = 0; b < RB; b++)
+    for (int b = 0; b < RB; b++)
 #pragma unroll
-            for (int k = 0; k < 4; k++) red[(warp * BM + g + 8 * (k >> 1)) * RP + column(b, k & 1)] = result(b, k);
-        __syncthreads();
-        for (int e = threadIdx.x; e < rows * RP; e += kThreads) {
-            float v = 0.f;
+        for (int k = 0; k < 4; k++) red[(wk * BM + 16 * wm + g + 8 * (k >> 1)) * RP + column(b, k & 1)] = result(b, k);
+    __syncthreads();
+    for (int e = threadIdx.x; e < rows * RP; e += kThreads) {
+        float v = 0.f;
 #pragma unroll
-            for (int k = 0; k < kWarps; k++) v += red[k * BM * RP + e];
-            dst[(int64_t)tr.row[e / RP] * RP + e % RP] = s * v;
-        }
-    } else {
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-            const int r = 16 * wm + g + 8 * u;
-            if (r < rows) {
-                float* d = dst + (int64_t)tr.row[r] * RP;
-#pragma unroll
-                for (int b = 0; b < RB; b++)
-#pragma unroll
-                    for (int j = 0; j < 2; j++) d[column(b, j)] = s * result(b, 2 * u + j);
-            }
-        }
+        for (int k = 0; k < WK; k++) v += red[k * BM * RP + e];
+        dst[(int64_t)row_of[e / RP] * RP + e % RP] = s * v;
     }
 }
 
@@ -1410,6 +1403,7 @@ __global__ void __launch_bounds__(kThreads) k_weight(Plan plan, const int32_t* _
     constexpr int HV = TK * RP / 4 / kThreads;  // float4 of h a thread stages
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ Scan scan;
+    __shared__ int32_t ids[4][C::TK];  // positions of stages i .. i + 3, -1 past the last
     __shared__ float block_max[kWarps];
     uint8_t* hs = smem + NS * C::X_BYTES;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
@@ -1451,15 +1445,28 @@ __global__ void __launch_bounds__(kThreads) k_weight(Plan plan, const int32_t* _
         take = half_scale(m);
     }
 
+    // A stage's positions are read from memory four stages ahead, so that neither its rows nor its h wait
+    // for them: by the first TK threads, into a register, and into their place one stage later.
+    static_assert(NS == 3, "ids holds a stage more than the ring");
+    const auto id_of = [&](int i) {
+        const int p = (part + i * parts) * TK + (int)threadIdx.x;
+        return i < stages && p < count ? list[p] : -1;
+    };
+    int id_next = -1;
+    if (threadIdx.x < TK) {
+#pragma unroll
+        for (int i = 0; i < 3; i++) ids[i][threadIdx.x] = id_of(i);
+        id_next = id_of(3);
+    }
+    __syncthreads();
     const auto load_x = [&](int i) {
         uint8_t* xs = smem + (i % NS) * C::X_BYTES;
-        const int p0 = (part + i * parts) * TK;
 #pragma unroll
         for (int k = 0; k < TK * FU / kThreads; k++) {
-            const int u = threadIdx.x + k * kThreads, r = u / FU, c = u % FU, p = p0 + r;
+            const int u = threadIdx.x + k * kThreads, r = u / FU, c = u % FU, id = ids[i & 3][r];
             const int to = F32 ? c ^ ((r & 3) << 1) : c ^ (r & 7);
-            stage_unit<T>(xs + r * (FU * 16) + to * 16, x + (p < count ? (int64_t)list[p] * ldx : 0) + f0 + c * E, x,
-                          p < count ? F - f0 - c * E : 0, xvec);
+            stage_unit<T>(xs + r * (FU * 16) + to * 16, x + (int64_t)max(id, 0) * ldx + f0 + c * E, x,
+                          id >= 0 ? F - f0 - c * E : 0, xvec);
         }
         stage_done();
     };
@@ -1467,9 +1474,8 @@ __global__ void __launch_bounds__(kThreads) k_weight(Plan plan, const int32_t* _
     const auto load_h_regs = [&](int i) {
 #pragma unroll
         for (int k = 0; k < HV; k++) {
-            const int e = threadIdx.x + k * kThreads, r = e / (RP / 4), c = e % (RP / 4), p = (part + i * parts) * TK + r;
-            hv[k] = p < count ? load_h(h + (int64_t)list[p] * RP + 4 * c, 1, 0)
-                              : make_float4(0.f, 0.f, 0.f, 0.f);
+            const int e = threadIdx.x + k * kThreads, r = e / (RP / 4), c = e % (RP / 4), id = ids[i & 3][r];
+            hv[k] = id >= 0 ? load_h(h + (int64_t)id * RP + 4 * c, 1, 0) : make_float4(0.f, 0.f, 0.f, 0.f);
         }
     };
     const auto store_h = [&](int i) {
@@ -1513,6 +1519,10 @@ __global__ void __launch_bounds__(kThreads) k_weight(Plan plan, const int32_t* _
         if (i + NS - 1 < stages) load_x(i + NS - 1);
         else stage_done();
         if (i + 1 < stages) load_h_regs(i + 1);
+        if (threadIdx.x < TK) {  // the place of stage i - 1
+            ids[(i + 3) & 3][threadIdx.x] = id_next;
+            id_next = id_of(i + 4);
+        }
         const uint8_t* xs = smem + (i % NS) * C::X_BYTES;
         const uint8_t* hb = hs + (i & 1) * C::H_BYTES;
         if constexpr (F32) {  // lane rows g, g + 8 of block m: ranks 2 RM g + 2 m, + 1; column 8 .. of the warp: NB g + b
@@ -1659,7 +1669,8 @@ Shape shape_of(int64_t T, int n, int rank, int64_t K, int64_t N) {
     s.planned = T > kScanMax || n > kScanAdapters;
     s.tiles = (T + (bm - 1) * groups) / bm;  // as many as there can be
     const auto splits = [&](int64_t width) {
-        const int64_t want = s.tiles > 0 ? ceil_div(2 * kSms, s.tiles) : 1, can = ceil_div(width, 512);
+        const int64_t blocks = s.tiles * (s.wm == 8 ? 2 : 1), want = blocks > 0 ? ceil_div(3 * kSms, blocks) : 1;
+        const int64_t can = ceil_div(width, 512);
         const int64_t k = want < can ? want : can;
         return (int)(k < 1 ? 1 : k > 16 ? 16 : k);
     };
@@ -1751,7 +1762,7 @@ int run_shrink(const Shape& s, const Plan& plan, const int32_t* index, const T* 
     using C = ShrinkCfg<T, RB, WM, TRANS>;
     const int64_t k_split = ceil_div(ceil_div(K, splits), C::KC) * C::KC;
     const bool find = first && !s.planned;
-    return start<k_shrink<T, RB, WM, TRANS>>(dim3((unsigned)s.tiles, (unsigned)splits), kThreads, C::SMEM, !find, st,
+    return start<k_shrink<T, RB, WM, TRANS>>(dim3((unsigned)(s.tiles * C::PARTS), (unsigned)splits), kThreads, C::SMEM, !find, st,
                  plan, (int)(find ? FIND : PLANNED), index, x, ldx, w, scale, s.n, s.rank, K, k_split, (int)s.T,
                  row_units(x, ldx), row_units(w, TRANS ? s.rank : K), h);
 }
