@@ -1382,7 +1382,8 @@ struct Side {
 };
 template <typename T, int RB>
 struct WeightCfg {
-    static constexpr int E = kE<T>, RP = 8 * RB, NB = RB == 16 ? 2 : 4;  // blocks of 8 columns a warp
+    // blocks of 8 columns a warp: as many as the accumulators leave room for
+    static constexpr int E = kE<T>, RP = 8 * RB, NB = RB == 16 ? 2 : 4;
     static constexpr int FC = 4 * 8 * NB, FU = FC / E, TK = 64;
     static constexpr int X_BYTES = TK * FC * (int)sizeof(T);
     // h of a stage: fp32 rows at a pitch of 8 words beyond a multiple of 16; 16 bits: planes hi and lo
@@ -1395,14 +1396,14 @@ struct WeightCfg {
 };
 
 template <typename T, int RB>
-__global__ void __launch_bounds__(kThreads) k_weight(Plan plan, const int32_t* __restrict__ index, Side<T> side_a,
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 && RB <= 4 ? 3 : 1) k_weight(Plan plan, const int32_t* __restrict__ index, Side<T> side_a,
                                                      Side<T> side_b, int first, int n, int rank, int T_rows) {
     using C = WeightCfg<T, RB>;
     constexpr int E = C::E, RP = C::RP, NB = C::NB, FC = C::FC, FU = C::FU, TK = C::TK, NS = C::NS, RM = RB / 2;
     constexpr bool F32 = sizeof(T) == 4;
     constexpr int HV = TK * RP / 4 / kThreads;  // float4 of h a thread stages
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ Scan scan;
+    Scan& scan = *reinterpret_cast<Scan*>(smem + C::SMEM);  // there without a plan only
     __shared__ int32_t ids[4][C::TK];  // positions of stages i .. i + 3, -1 past the last
     __shared__ float block_max[kWarps];
     uint8_t* hs = smem + NS * C::X_BYTES;
@@ -1459,14 +1460,31 @@ __global__ void __launch_bounds__(kThreads) k_weight(Plan plan, const int32_t* _
         id_next = id_of(3);
     }
     __syncthreads();
+    const int64_t column = f0 + threadIdx.x % FU * E;
+    const int column_bytes = column >= F ? 0 : F - column >= E ? 16 : (int)(F - column) * (int)sizeof(T);
+    const T* x_column = column_bytes ? x + column : x;
     const auto load_x = [&](int i) {
         uint8_t* xs = smem + (i % NS) * C::X_BYTES;
+        // a thread's column is the same in all its units: kThreads is a multiple of FU
+        const int c = threadIdx.x % FU, r0 = threadIdx.x / FU;
+        if (xvec) {
+            const uint32_t dst = smem_u32(xs);
 #pragma unroll
-        for (int k = 0; k < TK * FU / kThreads; k++) {
-            const int u = threadIdx.x + k * kThreads, r = u / FU, c = u % FU, id = ids[i & 3][r];
-            const int to = F32 ? c ^ ((r & 3) << 1) : c ^ (r & 7);
-            stage_unit<T>(xs + r * (FU * 16) + to * 16, x + (int64_t)max(id, 0) * ldx + f0 + c * E, x,
-                          id >= 0 ? F - f0 - c * E : 0, xvec);
+            for (int k = 0; k < TK * FU / kThreads; k++) {
+                const int r = r0 + k * (kThreads / FU), id = ids[i & 3][r];
+                const int to = F32 ? c ^ ((r & 3) << 1) : c ^ (r & 7);
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + (r * FU + to) * 16),
+                             "l"(x_column + (int64_t)max(id, 0) * ldx), "r"(id >= 0 ? column_bytes : 0)
+                             : "memory");
+            }
+        } else {
+#pragma unroll 1
+            for (int k = 0; k < TK * FU / kThreads; k++) {
+                const int r = r0 + k * (kThreads / FU), id = ids[i & 3][r];
+                const int to = F32 ? c ^ ((r & 3) << 1) : c ^ (r & 7);
+                stage_unit<T>(xs + (r * FU + to) * 16, x + (int64_t)max(id, 0) * ldx + f0 + c * E, x,
+                              id >= 0 ? F - f0 - c * E : 0, false);
+            }
         }
         stage_done();
     };
@@ -1618,9 +1636,9 @@ __global__ void __launch_bounds__(kThreads) k_weight(Plan plan, const int32_t* _
     if (parts > 1) cluster.sync();
     else __syncthreads();
     T* dst = side.out + (int64_t)a * rank * F;
-    for (int e = threadIdx.x + part * kThreads; e < FC * rank; e += parts * kThreads) {
-        const int r = side.trans ? e % rank : e / FC, c = side.trans ? e / rank : e % FC;
-        if (f0 + c >= F) continue;
+    for (int e = threadIdx.x + part * kThreads; e < FC * RP; e += parts * kThreads) {
+        const int r = side.trans ? e % RP : e / FC, c = side.trans ? e / RP : e % FC;
+        if (r >= rank || f0 + c >= F) continue;
         float v = 0.f;
         for (int k = 0; k < parts; k++) {
             const float* from = parts > 1 ? cluster.map_shared_rank(red, k) : red;
@@ -1825,7 +1843,9 @@ int run_weight(const Shape& s, const Plan& plan, const int32_t* index, const Sid
     const int64_t want = ceil_div(2 * kSms, (blocks_a + blocks_b) * s.n), can = ceil_div(s.T, (int64_t)s.n * C::TK);
     const int64_t most = want < can ? want : can;
     const unsigned parts = most >= 8 ? 8 : most >= 4 ? 4 : most >= 2 ? 2 : 1;
-    return start<k_weight<T, RB>>(dim3((unsigned)(blocks_a + blocks_b), (unsigned)s.n, parts), kThreads, C::SMEM, true, st,
+    constexpr int most_smem = C::SMEM + (int)sizeof(Scan);
+    return start<k_weight<T, RB>, most_smem>(dim3((unsigned)(blocks_a + blocks_b), (unsigned)s.n, parts), kThreads,
+                                  s.planned ? C::SMEM : most_smem, true, st,
                  plan, index, a, b, (int)blocks_a, s.n, s.rank, (int)s.T);
 }
 
