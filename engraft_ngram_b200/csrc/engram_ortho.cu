@@ -524,14 +524,18 @@ constexpr int BM = 128;
 constexpr int kGemmThreads = 320, kEpilogueWarps = 8;
 constexpr int kStageTotal = 192 * 1024;
 
+// A tile is 128 x 256 on one block, or 256 x 256 on a pair (PAIR): a cluster of two blocks whose tensor cores
+// work as one (cta_group::2).  Each block of a pair has half of A's rows and half of B's and reads the other half
+// of B from its partner, so a slice is 32 KB a block where one block needs 48.
 // One K slice of the operands: 32 columns of four planes (A hi, B hi, A lo, B lo) or 64 of two.
-template <int TERMS, int BN>
+template <int TERMS, bool PAIR>
 struct Cfg {
-    static constexpr int KS = TERMS == 3 ? 32 : 64;
-    static constexpr int A_BYTES = BM * KS * 2, B_BYTES = BN * KS * 2;
+    static constexpr int KS = TERMS == 3 ? 32 : 64, BN = 256, B_ROWS = PAIR ? 128 : 256;
+    static constexpr int A_BYTES = BM * KS * 2, B_BYTES = B_ROWS * KS * 2;
     static constexpr int STAGE_BYTES = (TERMS == 3 ? 2 : 1) * (A_BYTES + B_BYTES);
     static constexpr int STAGES = kStageTotal / STAGE_BYTES;
     static constexpr int SMEM = STAGES * STAGE_BYTES + kEpilogueWarps * 4096 + 1024 + 256;
+    static constexpr int TILE_M = PAIR ? 2 * BM : BM;
 };
 
 struct Maps {
@@ -565,27 +569,70 @@ __device__ __forceinline__ uint64_t operand_desc(uint32_t addr) {
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-
-template <bool A_MN, bool B_MN, int BN>
-__device__ __forceinline__ void umma_f16(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t accumulate) {
-    // A and B fp16, D fp32, each operand along K or across it
-    constexpr uint32_t desc = (1u << 4) | ((A_MN ? 1u : 0u) << 15) | ((B_MN ? 1u : 0u) << 16) |
-                              ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
-        "l"(da), "l"(db), "r"(desc), "r"(accumulate)
-        : "memory");
+__device__ __forceinline__ void mbar_arrive_leader(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
-template <bool MN, int KS, int ROWS>
+template <bool A_MN, bool B_MN, bool PAIR>
+__device__ __forceinline__ void umma_f16(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t accumulate) {
+    // A and B fp16, D fp32, each operand along K or across it; M 128, or 256 over the pair; N 256
+    constexpr uint32_t desc = (1u << 4) | ((A_MN ? 1u : 0u) << 15) | ((B_MN ? 1u : 0u) << 16) |
+                              ((uint32_t)(256 >> 3) << 17) | ((uint32_t)((PAIR ? 256 : 128) >> 4) << 24);
+    if constexpr (PAIR)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+            "l"(da), "l"(db), "r"(desc), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+            "l"(da), "l"(db), "r"(desc), "r"(accumulate)
+            : "memory");
+}
+// Arrives at the barrier, of both blocks of a pair, once the MMAs issued so far are done.
+template <bool PAIR>
+__device__ __forceinline__ void commit(uint32_t bar) {
+    if constexpr (PAIR)
+        asm volatile(
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+            "h"((uint16_t)3)
+            : "memory");
+    else
+        umma_commit(bar);
+}
+// The same place in the shared memory of the pair's first block.
+__device__ __forceinline__ uint32_t leaders(uint32_t addr) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// A tile of an operand; PAIR: onto a barrier of the pair's first block.
+template <bool PAIR>
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+    if constexpr (PAIR)
+        asm volatile(
+            "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, "
+            "%4}], [%5];" ::"r"(dst),
+            "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+            : "memory");
+    else
+        tma_load_3d(dst, map, x, y, z, bar);
+}
+template <bool MN, int KS, int ROWS, bool PAIR>
 __device__ __forceinline__ void load_operand(uint32_t dst, const CUtensorMap* map, int row0, int k, int z, uint32_t bar) {
     if constexpr (MN) {
 #pragma unroll
-        for (int b = 0; b < ROWS / 64; b++) tma_load_3d(dst + b * KS * 128, map, row0 + 64 * b, k, z, bar);
+        for (int b = 0; b < ROWS / 64; b++) load_box<PAIR>(dst + b * KS * 128, map, row0 + 64 * b, k, z, bar);
     } else {
-        tma_load_3d(dst, map, k, row0, z, bar);
+        load_box<PAIR>(dst, map, k, row0, z, bar);
     }
 }
 
@@ -614,40 +661,41 @@ __device__ __forceinline__ void put8(const Planes& p, int64_t i, const float* v)
 
 // Tile t of the stack.  Symmetric modes have those with an entry on or above the diagonal: column block b has
 // the first R (b + 1) row blocks, as far as there are any.
-template <bool SYM, int BN, typename J>
+template <bool SYM, int TILE_M, typename J>
 __device__ __forceinline__ void tile_at(const J& job, int t, int& z, int& m0, int& n0) {
     z = t / job.tiles;
     int left = t - z * job.tiles;
     if constexpr (SYM) {
-        constexpr int R = BN / BM;
+        constexpr int R = 256 / TILE_M;
         int b = 0, rows = min(R, job.tiles_m);
         while (left >= rows) left -= rows, b++, rows = min(R * (b + 1), job.tiles_m);
-        m0 = left * BM, n0 = b * BN;
+        m0 = left * TILE_M, n0 = b * 256;
     } else {
-        m0 = left % job.tiles_m * BM, n0 = left / job.tiles_m * BN;
+        m0 = left % job.tiles_m * TILE_M, n0 = left / job.tiles_m * 256;
     }
 }
 
-// BM x BN tiles on persistent blocks, one an SM: warp 0 loads (TMA), one lane of warp 1 issues the MMAs into
+// Tiles on persistent blocks, one an SM: warp 0 loads (TMA), one lane of warp 1 (of a pair's first block) issues the MMAs into
 // two accumulators in turn, and warps 2 to 9 take each through the mode's epilogue (tensor-memory lanes 32
 // (w % 4) .., half of the columns) while the next one is made: the epilogue, up to 8 us a tile beside 11 us
 // of products, costs time only after a block's last tile.  A wait that gives up (never, in a correct run)
-// counts itself in *err and the tile's results become NaN.
-template <int MODE, bool A_MN, bool B_MN, int TERMS, int BN, typename Io>
+// counts itself in *err, and the block's results from then on become NaN.
+template <int MODE, bool A_MN, bool B_MN, int TERMS, bool PAIR, typename Io>
 __global__ void __launch_bounds__(kGemmThreads, 1) k_product(const __grid_constant__ Maps maps, const Job<Io> job) {
-    using G = Cfg<TERMS, BN>;
-    constexpr int KS = G::KS, STAGES = G::STAGES;
+    using G = Cfg<TERMS, PAIR>;
+    constexpr int KS = G::KS, STAGES = G::STAGES, BN = G::BN;
     constexpr bool SYM = MODE == GRAM || MODE == POLY;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* turned = smem + STAGES * G::STAGE_BYTES;  // a 32 x 32 piece of each epilogue warp
     uint64_t* bars = reinterpret_cast<uint64_t*>(turned + kEpilogueWarps * 4096);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 4);
-    volatile uint32_t* gave_up = tmem_slot + 1;
     const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + STAGES), acc_full = smem_u32(bars + 2 * STAGES);
     const uint32_t acc_empty = acc_full + 16;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int slices = (job.K + KS - 1) / KS;
+    const int half = PAIR ? (int)(blockIdx.x & 1) : 0;  // of the pair: the cluster is two blocks along x
+    const int first_tile = PAIR ? blockIdx.x >> 1 : blockIdx.x, tile_step = PAIR ? gridDim.x >> 1 : gridDim.x;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; s++) {
@@ -656,19 +704,27 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_product(const __grid_consta
         }
         for (int a = 0; a < 2; a++) {
             mbar_init(acc_full + 8 * a, 1);
-            mbar_init(acc_empty + 8 * a, kEpilogueWarps);
+            mbar_init(acc_empty + 8 * a, (PAIR ? 2 : 1) * kEpilogueWarps);
         }
-        *gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    if constexpr (PAIR) cluster_sync();  // both blocks are there, with their barriers
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                     "r"((uint32_t)(2 * BN))
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if constexpr (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                         "r"((uint32_t)(2 * BN))
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                         "r"((uint32_t)(2 * BN))
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    __syncthreads();
+    if constexpr (PAIR) cluster_sync();
+    else __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *tmem_slot;
     wait_for_previous();
@@ -678,32 +734,37 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_product(const __grid_consta
         if (lane == 0) {
             int i = 0;
             bool ok = true;
-            for (int t = blockIdx.x; t < job.total && ok; t += gridDim.x) {
+            for (int t = first_tile; t < job.total && ok; t += tile_step) {
                 int z, m0, n0;
-                tile_at<SYM, BN>(job, t, z, m0, n0);
+                tile_at<SYM, G::TILE_M>(job, t, z, m0, n0);
+                m0 += half * BM, n0 += half * G::B_ROWS;
                 for (int k = 0; k < slices; k++, i++) {
                     const int s = i % STAGES, round = i / STAGES;
                     if (round > 0) ok = mbar_wait(empty0 + 8 * s, (uint32_t)((round - 1) & 1), job.err);
                     if (!ok) break;
-                    const uint32_t bar = full0 + 8 * s, st = smem_u32(smem + s * G::STAGE_BYTES);
-                    mbar_expect_tx(bar, G::STAGE_BYTES);
-                    load_operand<A_MN, KS, BM>(st, &maps.a_hi, m0, k * KS, z, bar);
-                    load_operand<B_MN, KS, BN>(st + G::A_BYTES, &maps.b_hi, n0, k * KS, z, bar);
+                    const uint32_t bar = PAIR ? leaders(full0 + 8 * s) : full0 + 8 * s;
+                    const uint32_t st = smem_u32(smem + s * G::STAGE_BYTES);
+                    if (half == 0) mbar_expect_tx(full0 + 8 * s, (PAIR ? 2 : 1) * G::STAGE_BYTES);  // of both blocks
+                    load_operand<A_MN, KS, BM, PAIR>(st, &maps.a_hi, m0, k * KS, z, bar);
+                    load_operand<B_MN, KS, G::B_ROWS, PAIR>(st + G::A_BYTES, &maps.b_hi, n0, k * KS, z, bar);
                     if constexpr (TERMS == 3) {
-                        load_operand<A_MN, KS, BM>(st + G::A_BYTES + G::B_BYTES, &maps.a_lo, m0, k * KS, z, bar);
-                        load_operand<B_MN, KS, BN>(st + 2 * G::A_BYTES + G::B_BYTES, &maps.b_lo, n0, k * KS, z, bar);
+                        load_operand<A_MN, KS, BM, PAIR>(st + G::A_BYTES + G::B_BYTES, &maps.a_lo, m0, k * KS, z, bar);
+                        load_operand<B_MN, KS, G::B_ROWS, PAIR>(st + 2 * G::A_BYTES + G::B_BYTES, &maps.b_lo, n0, k * KS, z,
+                                                                bar);
                     }
                 }
             }
-            // every load issued into this block's shared memory has landed before it ends
-            for (int k = i > STAGES ? i - STAGES : 0; k < i; k++)
-                mbar_wait(full0 + 8 * (k % STAGES), (uint32_t)((k / STAGES) & 1), job.err);
+            // every load issued into this block's shared memory has landed before it ends (a pair's: both
+            // blocks', before either passes the last barrier)
+            if (half == 0)
+                for (int k = i > STAGES ? i - STAGES : 0; k < i; k++)
+                    mbar_wait(full0 + 8 * (k % STAGES), (uint32_t)((k / STAGES) & 1), job.err);
         }
     } else if (warp == 1) {
-        if (lane == 0) {
+        if (lane == 0 && half == 0) {
             int i = 0, made = 0;
             bool ok = true;
-            for (int t = blockIdx.x; t < job.total; t += gridDim.x, made++) {
+            for (int t = first_tile; t < job.total; t += tile_step, made++) {
                 const int acc = made & 1;
                 if (made >= 2) ok = ok && mbar_wait(acc_empty + 8 * acc, (uint32_t)((made / 2 - 1) & 1), job.err);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -721,31 +782,30 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_product(const __grid_consta
                         const uint64_t ah = operand_desc<A_MN, KS>(a + sa * k), bh = operand_desc<B_MN, KS>(b + sb * k);
                         const uint32_t first = (n > 0 || k > 0) ? 1u : 0u;
                         if constexpr (TERMS == 3) {  // the small terms first
-                            umma_f16<A_MN, B_MN, BN>(d, operand_desc<A_MN, KS>(alo + sa * k), bh, first);
-                            umma_f16<A_MN, B_MN, BN>(d, ah, operand_desc<B_MN, KS>(blo + sb * k), 1u);
-                            umma_f16<A_MN, B_MN, BN>(d, ah, bh, 1u);
+                            umma_f16<A_MN, B_MN, PAIR>(d, operand_desc<A_MN, KS>(alo + sa * k), bh, first);
+                            umma_f16<A_MN, B_MN, PAIR>(d, ah, operand_desc<B_MN, KS>(blo + sb * k), 1u);
+                            umma_f16<A_MN, B_MN, PAIR>(d, ah, bh, 1u);
                         } else {
-                            umma_f16<A_MN, B_MN, BN>(d, ah, bh, first);
+                            umma_f16<A_MN, B_MN, PAIR>(d, ah, bh, first);
                         }
                     }
-                    umma_commit(empty0 + 8 * s);
+                    commit<PAIR>(empty0 + 8 * s);
                 }
-                if (!ok) {
-                    *gave_up = 1;
-                    __threadfence_block();
-                }
-                umma_commit(acc_full + 8 * acc);
+                if (!ok) break;  // no accumulator any more: the epilogues' waits give up in their turn
+                commit<PAIR>(acc_full + 8 * acc);
             }
         }
         __syncwarp();
     } else {
         const int w = warp & 3, part = (warp - 2) >> 2;
         int made = 0;
-        for (int t = blockIdx.x; t < job.total; t += gridDim.x, made++) {
+        bool ok = true;
+        for (int t = first_tile; t < job.total; t += tile_step, made++) {
         int z, m0, n0;
-        tile_at<SYM, BN>(job, t, z, m0, n0);
+        tile_at<SYM, G::TILE_M>(job, t, z, m0, n0);
+        m0 += half * BM;
         const int acc = made & 1;
-        const bool ok = mbar_wait(acc_full + 8 * acc, (uint32_t)((made / 2) & 1), job.err) && *gave_up == 0;
+        ok = ok && mbar_wait(acc_full + 8 * acc, (uint32_t)((made / 2) & 1), job.err);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         uint8_t* tile = turned + (warp - 2) * 4096;
         for (int col = part * (BN / 2); col < (part + 1) * (BN / 2); col += 32) {
@@ -763,7 +823,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_product(const __grid_consta
             if (col + 32 == (part + 1) * (BN / 2)) {  // this warp's part of the accumulator has been read
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(acc_empty + 8 * acc);
+                if (lane == 0) {
+                    if constexpr (PAIR) mbar_arrive_leader(leaders(acc_empty + 8 * acc));
+                    else mbar_arrive(acc_empty + 8 * acc);
+                }
             }
             const int r0 = m0 + 32 * w, c0 = n0 + col;
             if (r0 >= job.M || c0 >= job.N) continue;
@@ -860,11 +923,16 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_product(const __grid_consta
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    __syncthreads();
+    if constexpr (PAIR) cluster_sync();  // the partner reads this block's operands, and arrives at its barriers
+    else __syncthreads();
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)(2 * BN))
-                     : "memory");
+        if constexpr (PAIR)
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)(2 * BN))
+                         : "memory");
+        else
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)(2 * BN))
+                         : "memory");
     }
 }
 
@@ -880,7 +948,7 @@ cudaError_t launch(void (*kernel)(P...), const cudaLaunchConfig_t& cfg, A... arg
 
 // Starts a kernel; after = true: it may start while the launch before it still runs (it waits for that
 // one's results itself, griddepcontrol.wait).
-template <auto KERNEL, typename... A>
+template <auto KERNEL, int CLUSTER = 1, typename... A>
 int start(dim3 grid, int threads, int smem, bool after, cudaStream_t st, A... args) {
     if (smem > 48 * 1024) {
         static bool allowed[64] = {false};
@@ -897,11 +965,16 @@ int start(dim3 grid, int threads, int smem, bool after, cudaStream_t st, A... ar
     cfg.blockDim = dim3((unsigned)threads);
     cfg.dynamicSmemBytes = (size_t)smem;
     cfg.stream = st;
-    cudaLaunchAttribute attr = {};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = after ? 1 : 0;
+    cudaLaunchAttribute attr[2] = {};
+    if (after) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (CLUSTER > 1) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attr[cfg.numAttrs++].val.clusterDim = {CLUSTER, 1, 1};
+    }
+    cfg.attrs = attr;
     const cudaError_t e = launch(KERNEL, cfg, args...);
     count_launches(1);
     return e == cudaSuccess && cudaGetLastError() == cudaSuccess ? ENGRAM_OK : ENGRAM_ERR_CUDA;
@@ -998,34 +1071,72 @@ struct Matrix {  // a plane pair and its extent
 
 struct NoIo {};
 
-template <int MODE, bool A_MN, bool B_MN, int TERMS, int BN, typename Io>
-int run_product(const Matrix& a, const Matrix& b, int64_t stack, Job<Io> job, cudaStream_t st) {
-    using G = Cfg<TERMS, BN>;
+// Pairs of blocks that the device runs at once (every k_product takes an SM a block).
+int pairs_at_once(const void* kernel, int smem) {
+    static int cached[64] = {0};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64) return 64;
+    if (cached[dev] == 0) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(148);
+        cfg.blockDim = dim3(kGemmThreads);
+        cfg.dynamicSmemBytes = (size_t)smem;
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim = {2, 1, 1};
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        int n = 0;
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+            cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) {
+            cudaGetLastError();
+            n = 64;
+        }
+        cached[dev] = n;
+    }
+    return cached[dev];
+}
+
+template <int MODE, bool A_MN, bool B_MN, int TERMS, bool PAIR, typename Io>
+int run_tiles(const Matrix& a, const Matrix& b, int64_t stack, Job<Io> job, cudaStream_t st) {
+    using G = Cfg<TERMS, PAIR>;
     Maps maps;
     memset(&maps, 0, sizeof(maps));
     const auto make = [&](CUtensorMap* map, const __half* plane, const Matrix& x, bool mn, int tile_rows) {
         return mn ? plane_map(map, plane, x.rows, x.cols, x.p.ld, x.p.stride, stack, 64, G::KS)
                   : plane_map(map, plane, x.rows, x.cols, x.p.ld, x.p.stride, stack, G::KS, tile_rows);
     };
-    if (!make(&maps.a_hi, a.p.hi, a, A_MN, BM) || !make(&maps.b_hi, b.p.hi, b, B_MN, BN)) return ENGRAM_ERR_CUDA;
-    if (TERMS == 3 && (!make(&maps.a_lo, a.p.lo, a, A_MN, BM) || !make(&maps.b_lo, b.p.lo, b, B_MN, BN)))
+    if (!make(&maps.a_hi, a.p.hi, a, A_MN, BM) || !make(&maps.b_hi, b.p.hi, b, B_MN, G::B_ROWS)) return ENGRAM_ERR_CUDA;
+    if (TERMS == 3 && (!make(&maps.a_lo, a.p.lo, a, A_MN, BM) || !make(&maps.b_lo, b.p.lo, b, B_MN, G::B_ROWS)))
         return ENGRAM_ERR_CUDA;
-    job.tiles_m = (int)ceil_div(job.M, BM), job.tiles_n = (int)ceil_div(job.N, BN);
-    job.tiles = job.tiles_m * job.tiles_n;
+    job.tiles_m = (int)ceil_div(job.M, G::TILE_M), job.tiles_n = (int)ceil_div(job.N, 256);
+    int64_t tiles = (int64_t)job.tiles_m * job.tiles_n;
     if (MODE == GRAM || MODE == POLY) {
-        job.tiles = 0;
-        for (int b = 0; b < job.tiles_n; b++) job.tiles += std::min(BN / BM * (b + 1), job.tiles_m);
+        tiles = 0;
+        for (int b2 = 0; b2 < job.tiles_n; b2++) tiles += std::min(256 / G::TILE_M * (b2 + 1), job.tiles_m);
     }
-    if (job.tiles * stack > INT32_MAX) return ENGRAM_ERR_RANGE;
-    job.total = (int)(job.tiles * stack);
-    return start<k_product<MODE, A_MN, B_MN, TERMS, BN, Io>>(dim3((unsigned)std::min(job.total, sm_count())),
-                                                             kGemmThreads, G::SMEM, true, st, maps, job);
+    if (tiles * stack > INT32_MAX) return ENGRAM_ERR_RANGE;
+    job.tiles = (int)tiles;
+    job.total = (int)(tiles * stack);
+    constexpr auto kernel = k_product<MODE, A_MN, B_MN, TERMS, PAIR, Io>;
+    const int most = PAIR ? pairs_at_once((const void*)kernel, G::SMEM) : sm_count();
+    const int blocks = (PAIR ? 2 : 1) * std::min(job.total, most);
+    return start<kernel, PAIR ? 2 : 1>(dim3((unsigned)blocks), kGemmThreads, G::SMEM, true, st, maps, job);
+}
+
+// Pairs of blocks where that leaves at least half of them a tile: MEASURED.
+template <int MODE, bool A_MN, bool B_MN, int TERMS, typename Io>
+int run_product(const Matrix& a, const Matrix& b, int64_t stack, const Job<Io>& job, cudaStream_t st) {
+    const int64_t tn = ceil_div(job.N, 256), tm = ceil_div(job.M, 256);
+    const int64_t pairs = ((MODE == GRAM || MODE == POLY) ? tn * (tn + 1) / 2 : tm * tn) * stack;
+    if (pairs >= 37) return run_tiles<MODE, A_MN, B_MN, TERMS, true>(a, b, stack, job, st);
+    return run_tiles<MODE, A_MN, B_MN, TERMS, false>(a, b, stack, job, st);
 }
 
 template <int TERMS, typename Io>
 int run_planes(const Shape& s, const Layout& l, const Io& io, const Poly& poly, double eps, uint8_t* ws,
                cudaStream_t st) {
-    constexpr int BN = 256;
     double* part = (double*)(ws + l.part);
     const int64_t ldx = pad64(s.cols), lds = pad64(s.side);
     const auto planes = [&](int64_t at, int64_t plane, int64_t ld, int64_t rows, bool two) {
@@ -1050,30 +1161,30 @@ int run_planes(const Shape& s, const Layout& l, const Io& io, const Poly& poly, 
         job.M = job.N = (int)s.side;
         job.K = (int)s.length;
         job.out = g.p;
-        e = s.tall ? run_product<GRAM, true, true, TERMS, BN>(in, in, s.stack, job, st)
-                   : run_product<GRAM, false, false, TERMS, BN>(in, in, s.stack, job, st);
+        e = s.tall ? run_product<GRAM, true, true, TERMS>(in, in, s.stack, job, st)
+                   : run_product<GRAM, false, false, TERMS>(in, in, s.stack, job, st);
         if (e) break;
         job.K = (int)s.side;
         job.out = b.p;
         job.g = g.p;
         job.c0 = (float)poly.c[i][0], job.c1 = (float)poly.c[i][1], job.c2 = (float)poly.c[i][2];
-        e = run_product<POLY, false, false, TERMS, BN>(g, g, s.stack, job, st);
+        e = run_product<POLY, false, false, TERMS>(g, g, s.stack, job, st);
         if (e) break;
         job.M = (int)s.rows;
         job.N = (int)s.cols;
         job.out = next.p;
         job.g = in.p;
         if (i + 1 < poly.steps) {
-            e = s.tall ? run_product<UPDATE, false, false, TERMS, BN>(in, b, s.stack, job, st)
-                       : run_product<UPDATE, false, true, TERMS, BN>(b, in, s.stack, job, st);
+            e = s.tall ? run_product<UPDATE, false, false, TERMS>(in, b, s.stack, job, st)
+                       : run_product<UPDATE, false, true, TERMS>(b, in, s.stack, job, st);
         } else {
             Job<Io> result = {};
             result.M = job.M, result.N = job.N, result.K = job.K, result.err = job.err;
             result.io = io;
             result.vec = vec;
             result.g = in.p, result.c0 = job.c0;
-            e = s.tall ? run_product<RESULT, false, false, TERMS, BN>(in, b, s.stack, result, st)
-                       : run_product<RESULT, false, true, TERMS, BN>(b, in, s.stack, result, st);
+            e = s.tall ? run_product<RESULT, false, false, TERMS>(in, b, s.stack, result, st)
+                       : run_product<RESULT, false, true, TERMS>(b, in, s.stack, result, st);
         }
     }
     return e;
