@@ -108,7 +108,7 @@ struct Plain {
     __device__ __forceinline__ void put(const Raw&, int64_t i, int left, bool vec, float4 o) const {
         store4(out, i, left, vec, o);
     }
-    __device__ __forceinline__ void finish(int64_t i, int left, bool vec, float4 o) const { store4(out, i, left, vec, o); }
+    __device__ __forceinline__ void before(Raw&, int64_t, int, bool) const {}  // what put() needs
 };
 template <typename T>
 struct MuonIo {
@@ -146,11 +146,7 @@ struct MuonIo {
                make_float4(__fmaf_rn(-step, o.x, decay * r.p.x), __fmaf_rn(-step, o.y, decay * r.p.y),
                            __fmaf_rn(-step, o.z, decay * r.p.z), __fmaf_rn(-step, o.w, decay * r.p.w)));
     }
-    __device__ __forceinline__ void finish(int64_t i, int left, bool vec, float4 o) const {
-        Raw r;
-        r.p = load4(p, i, left, vec);
-        put(r, i, left, vec, o);
-    }
+    __device__ __forceinline__ void before(Raw& r, int64_t i, int left, bool vec) const { r.p = load4(p, i, left, vec); }
 };
 
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
@@ -466,7 +462,7 @@ __device__ __forceinline__ void put(const Planes& p, int64_t i, float y) {
     if (p.lo) p.lo[i] = __float2half_rn(y - __half2float(h));
 }
 
-// planes = 2^12 U / max(|U|, eps); a warp takes a row at a time.
+// planes = 2^12 U / max(|U|, eps); a warp takes 512 columns of a row at a time.
 template <typename Io>
 __global__ void __launch_bounds__(kNormThreads) k_planes(Io io, int64_t rows, int64_t cols, bool vec,
                                                          const double* part, int parts, double eps, Planes out) {
@@ -485,10 +481,12 @@ __global__ void __launch_bounds__(kNormThreads) k_planes(Io io, int64_t rows, in
     const double norm = sqrt(total);
     const double inv = (double)kPlaneScale / (norm < eps ? eps : norm);
     const int64_t base = blockIdx.y * rows * cols;
-    for (int64_t r = blockIdx.x * (int64_t)(kNormThreads / 32) + warp; r < rows;
-         r += (int64_t)gridDim.x * (kNormThreads / 32)) {
-        constexpr int N = 4;  // pieces of four under way a lane
-        for (int64_t c0 = 4 * lane; c0 < cols; c0 += N * 128) {
+    constexpr int N = 4;  // pieces of four under way a lane
+    const int64_t per_row = (cols + N * 128 - 1) / (N * 128), units = rows * per_row;
+    for (int64_t unit = blockIdx.x * (int64_t)(kNormThreads / 32) + warp; unit < units;
+         unit += (int64_t)gridDim.x * (kNormThreads / 32)) {
+        const int64_t r = unit / per_row, c0 = (unit - r * per_row) * (N * 128) + 4 * lane;
+        {
             typename Io::Raw raw[N];
 #pragma unroll
             for (int k = 0; k < N; k++) {
@@ -518,6 +516,10 @@ __global__ void __launch_bounds__(kNormThreads) k_planes(Io io, int64_t rows, in
 
 // ---- longer sides: the products -----------------------------------------------------
 
+struct NoIo {
+    struct Raw {};
+};
+
 enum Mode { GRAM, POLY, UPDATE, RESULT };
 
 constexpr int BM = 128;
@@ -526,11 +528,12 @@ constexpr int kStageTotal = 192 * 1024;
 
 // A tile is 128 x 256 on one block, or 256 x 256 on a pair (PAIR): a cluster of two blocks whose tensor cores
 // work as one (cta_group::2).  Each block of a pair has half of A's rows and half of B's and reads the other half
-// of B from its partner, so a slice is 32 KB a block where one block needs 48.
+// of B from its partner, so a slice is 32 KB a block where one block needs 48.  Small products take 128 x 64 on
+// one block, and sums over a long K with few tiles are split over blocks.
 // One K slice of the operands: 32 columns of four planes (A hi, B hi, A lo, B lo) or 64 of two.
-template <int TERMS, bool PAIR>
+template <int TERMS, bool PAIR, int BN>
 struct Cfg {
-    static constexpr int KS = TERMS == 3 ? 32 : 64, BN = 256, B_ROWS = PAIR ? 128 : 256;
+    static constexpr int KS = TERMS == 3 ? 32 : 64, B_ROWS = PAIR ? BN / 2 : BN;
     static constexpr int A_BYTES = BM * KS * 2, B_BYTES = B_ROWS * KS * 2;
     static constexpr int STAGE_BYTES = (TERMS == 3 ? 2 : 1) * (A_BYTES + B_BYTES);
     static constexpr int STAGES = kStageTotal / STAGE_BYTES;
@@ -546,7 +549,9 @@ template <typename Io>
 struct Job {
     int M, N, K;       // D [M, N] = sum over K
     int tiles_m, tiles_n, tiles;  // tiles along M, along N, of a matrix
-    int total;                    // tiles of the stack
+    int total;                    // tiles of the stack, times splits
+    int splits;                   // blocks that share a tile's sum
+    float* partial;               // [tile, split, 128, BN]: where they put theirs
     Planes out;        // GRAM, POLY, UPDATE
     Planes g;          // POLY: the planes of G; UPDATE, RESULT of one term: those of X
     float c0, c1, c2;  // POLY
@@ -573,11 +578,11 @@ __device__ __forceinline__ void mbar_arrive_leader(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
-template <bool A_MN, bool B_MN, bool PAIR>
+template <bool A_MN, bool B_MN, bool PAIR, int BN>
 __device__ __forceinline__ void umma_f16(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t accumulate) {
-    // A and B fp16, D fp32, each operand along K or across it; M 128, or 256 over the pair; N 256
+    // A and B fp16, D fp32, each operand along K or across it; M 128, or 256 over the pair
     constexpr uint32_t desc = (1u << 4) | ((A_MN ? 1u : 0u) << 15) | ((B_MN ? 1u : 0u) << 16) |
-                              ((uint32_t)(256 >> 3) << 17) | ((uint32_t)((PAIR ? 256 : 128) >> 4) << 24);
+                              ((uint32_t)(BN >> 3) << 17) | ((uint32_t)((PAIR ? 256 : 128) >> 4) << 24);
     if constexpr (PAIR)
         asm volatile(
             "{\n\t.reg .pred p;\n\t"
@@ -636,18 +641,6 @@ __device__ __forceinline__ void load_operand(uint32_t dst, const CUtensorMap* ma
     }
 }
 
-__device__ __forceinline__ void load_planes8(const Planes& p, int64_t i, float* v) {
-    alignas(16) __half h[8];
-    *reinterpret_cast<uint4*>(h) = *reinterpret_cast<const uint4*>(p.hi + i);
-#pragma unroll
-    for (int k = 0; k < 8; k++) v[k] = __half2float(h[k]);
-    if (p.lo) {
-        *reinterpret_cast<uint4*>(h) = *reinterpret_cast<const uint4*>(p.lo + i);
-#pragma unroll
-        for (int k = 0; k < 8; k++) v[k] += __half2float(h[k]);
-    }
-}
-
 __device__ __forceinline__ void put8(const Planes& p, int64_t i, const float* v) {
     alignas(16) __half h[8], l[8];
 #pragma unroll
@@ -659,19 +652,138 @@ __device__ __forceinline__ void put8(const Planes& p, int64_t i, const float* v)
     if (p.lo) *reinterpret_cast<uint4*>(p.lo + i) = *reinterpret_cast<const uint4*>(l);
 }
 
-// Tile t of the stack.  Symmetric modes have those with an entry on or above the diagonal: column block b has
-// the first R (b + 1) row blocks, as far as there are any.
-template <bool SYM, int TILE_M, typename J>
+// Tile t of the stack.  Symmetric modes have those with an entry on or above the diagonal: of column block b
+// the row blocks that begin above its last column.
+template <bool SYM, int TILE_M, int BN, typename J>
 __device__ __forceinline__ void tile_at(const J& job, int t, int& z, int& m0, int& n0) {
     z = t / job.tiles;
     int left = t - z * job.tiles;
     if constexpr (SYM) {
-        constexpr int R = 256 / TILE_M;
-        int b = 0, rows = min(R, job.tiles_m);
-        while (left >= rows) left -= rows, b++, rows = min(R * (b + 1), job.tiles_m);
-        m0 = left * TILE_M, n0 = b * 256;
+        int b = 0, rows = min((BN - 1) / TILE_M + 1, job.tiles_m);
+        while (left >= rows) left -= rows, b++, rows = min((BN * (b + 1) - 1) / TILE_M + 1, job.tiles_m);
+        m0 = left * TILE_M, n0 = b * BN;
     } else {
-        m0 = left % job.tiles_m * TILE_M, n0 = left / job.tiles_m * 256;
+        m0 = left % job.tiles_m * TILE_M, n0 = left / job.tiles_m * BN;
+    }
+}
+
+// What a lane needs from memory for its part of a 32 x 32 piece: fetched together, ahead of the accumulator (one by
+// one, each waits for the one before: 11 us a tile).
+template <int MODE, int TERMS, typename Io>
+struct Before {
+    static constexpr bool SYM = MODE == GRAM || MODE == POLY, PLANES = MODE == POLY || (TERMS == 1 && !SYM);
+    static constexpr bool TWO = PLANES && (TERMS == 3 || !SYM);
+    uint4 hi[PLANES ? 4 : 1], lo[TWO ? 4 : 1];
+    typename Io::Raw raw[MODE == RESULT ? 8 : 1];
+    __device__ __forceinline__ void fetch(const Job<Io>& job, int z, int r0, int c0, int lane) {
+#pragma unroll
+        for (int it = 0; it < 4; it++) {
+            const int row = r0 + 8 * it + (lane >> 2), c = c0 + 8 * (lane & 3);
+            if (row >= job.M || c >= job.N) continue;
+            if constexpr (PLANES) {
+                const int64_t at = (int64_t)z * job.g.stride + (int64_t)row * job.g.ld + c;
+                hi[it] = *reinterpret_cast<const uint4*>(job.g.hi + at);
+                if constexpr (TWO) lo[it] = *reinterpret_cast<const uint4*>(job.g.lo + at);
+            }
+            if constexpr (MODE == RESULT) {
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const int left = job.N - c - 4 * j;
+                    if (left > 0)
+                        job.io.before(raw[2 * it + j], ((int64_t)z * job.M + row) * job.N + c + 4 * j, left < 4 ? left : 4,
+                                      job.vec && left >= 4);
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void planes(int it, float* v) const {
+        if constexpr (PLANES) {
+            const __half* h = reinterpret_cast<const __half*>(&hi[it]);
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[k] = __half2float(h[k]);
+            if constexpr (TWO) {
+                const __half* l = reinterpret_cast<const __half*>(&lo[it]);
+#pragma unroll
+                for (int k = 0; k < 8; k++) v[k] += __half2float(l[k]);
+            }
+        }
+    }
+};
+
+// The mode's work on the 32 x 32 piece of products at (r0, c0), which lies in shared memory in rows of 128 bytes
+// whose units of 16 are swapped by row: four lanes take 64 consecutive bytes of a row.
+template <int MODE, int TERMS, typename Io>
+__device__ __forceinline__ void finish_piece(const Job<Io>& job, uint8_t* tile, const Before<MODE, TERMS, Io>& before, int z,
+                                             int r0, int c0, int lane) {
+    constexpr bool SYM = MODE == GRAM || MODE == POLY;
+#pragma unroll
+    for (int it = 0; it < 4; it++) {
+        const int lr = 8 * it + (lane >> 2), u = 2 * (lane & 3), row = r0 + lr, c = c0 + 4 * u;
+        float* lo4 = reinterpret_cast<float*>(tile + lr * 128 + ((u ^ (lr & 7)) << 4));
+        float* hi4 = reinterpret_cast<float*>(tile + lr * 128 + (((u + 1) ^ (lr & 7)) << 4));
+        float v[8];
+        *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(lo4);
+        *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(hi4);
+        const bool in = row < job.M && c < job.N;
+        float other[8];
+        before.planes(it, other);
+        if constexpr (TERMS == 1 && !SYM) {  // c0 X, at the product's scale
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j] = fmaf(job.c0 * kPlaneScale, other[j], v[j]);
+        }
+        if constexpr (MODE == RESULT) {
+            const int64_t at = ((int64_t)z * job.M + row) * job.N + c;
+            constexpr float one = 1.f / (kPlaneScale * kPlaneScale);
+#pragma unroll
+            for (int j = 0; j < 8; j += 4) {
+                const int left = job.N - c - j;
+                if (in && left > 0)
+                    job.io.put(before.raw[2 * it + j / 4], at + j, left < 4 ? left : 4, job.vec && left >= 4,
+                               make_float4(v[j] * one, v[j + 1] * one, v[j + 2] * one, v[j + 3] * one));
+            }
+        } else {
+            // products carry the square of the planes' scale; the rows' padding (to ld) may be written
+            const int64_t at = (int64_t)z * job.out.stride + (int64_t)row * job.out.ld + c;
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j] *= 1.f / kPlaneScale;
+            if constexpr (MODE == POLY) {
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    v[j] = fmaf(job.c2, v[j], job.c1 * other[j]) +
+                           (TERMS == 3 && c + j == row ? job.c0 * kPlaneScale : 0.f);
+            }
+            if (in && (!SYM || c > row)) {
+                put8(job.out, at, v);
+            } else if (in && c + 7 >= row) {
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    if (c + j >= row && c + j < job.N) put(job.out, at + j, v[j]);
+            }
+            if constexpr (SYM) {
+                *reinterpret_cast<float4*>(lo4) = *reinterpret_cast<const float4*>(v);
+                *reinterpret_cast<float4*>(hi4) = *reinterpret_cast<const float4*>(v + 4);
+            }
+        }
+    }
+    if constexpr (SYM) {  // the mirrored entries: row c0 + ., eight columns of it a lane
+        __syncwarp();
+#pragma unroll
+        for (int it = 0; it < 4; it++) {
+            const int lc = 8 * it + (lane >> 2), lr = 8 * (lane & 3), row = c0 + lc, c = r0 + lr;
+            if (row >= job.N || c >= job.M || c >= row) continue;
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                v[j] = *reinterpret_cast<const float*>(tile + (lr + j) * 128 + (((lc >> 2) ^ j) << 4) + 4 * (lc & 3));
+            const int64_t at = (int64_t)z * job.out.stride + (int64_t)row * job.out.ld + c;
+            if (c + 7 < row && c + 7 < job.M) {
+                put8(job.out, at, v);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    if (c + j < row && c + j < job.M) put(job.out, at + j, v[j]);
+            }
+        }
     }
 }
 
@@ -680,10 +792,11 @@ __device__ __forceinline__ void tile_at(const J& job, int t, int& z, int& m0, in
 // (w % 4) .., half of the columns) while the next one is made: the epilogue, up to 8 us a tile beside 11 us
 // of products, costs time only after a block's last tile.  A wait that gives up (never, in a correct run)
 // counts itself in *err, and the block's results from then on become NaN.
-template <int MODE, bool A_MN, bool B_MN, int TERMS, bool PAIR, typename Io>
+template <int MODE, bool A_MN, bool B_MN, int TERMS, bool PAIR, int BN, typename Io>
 __global__ void __launch_bounds__(kGemmThreads, 1) k_product(const __grid_constant__ Maps maps, const Job<Io> job) {
-    using G = Cfg<TERMS, PAIR>;
-    constexpr int KS = G::KS, STAGES = G::STAGES, BN = G::BN;
+    using G = Cfg<TERMS, PAIR, BN>;
+    constexpr int KS = G::KS, STAGES = G::STAGES;
+    constexpr bool SPLIT = MODE == GRAM && BN == 64;  // may share tiles
     constexpr bool SYM = MODE == GRAM || MODE == POLY;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -736,9 +849,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_product(const __grid_consta
             bool ok = true;
             for (int t = first_tile; t < job.total && ok; t += tile_step) {
                 int z, m0, n0;
-                tile_at<SYM, G::TILE_M>(job, t, z, m0, n0);
+                tile_at<SYM, G::TILE_M, BN>(job, SPLIT ? t / job.splits : t, z, m0, n0);
                 m0 += half * BM, n0 += half * G::B_ROWS;
-                for (int k = 0; k < slices; k++, i++) {
+                const int part = SPLIT ? t % job.splits : 0, parts = SPLIT ? job.splits : 1;
+                for (int k = slices * part / parts; k < slices * (part + 1) / parts; k++, i++) {
                     const int s = i % STAGES, round = i / STAGES;
                     if (round > 0) ok = mbar_wait(empty0 + 8 * s, (uint32_t)((round - 1) & 1), job.err);
                     if (!ok) break;
@@ -769,7 +883,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_product(const __grid_consta
                 if (made >= 2) ok = ok && mbar_wait(acc_empty + 8 * acc, (uint32_t)((made / 2 - 1) & 1), job.err);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t d = tmem + acc * BN;
-                for (int n = 0; n < slices && ok; n++, i++) {
+                const int part = SPLIT ? t % job.splits : 0, parts = SPLIT ? job.splits : 1;
+                const int n0 = slices * part / parts, n1 = slices * (part + 1) / parts;
+                for (int n = n0; n < n1 && ok; n++, i++) {
                     const int s = i % STAGES;
                     ok = mbar_wait(full0 + 8 * s, (uint32_t)((i / STAGES) & 1), job.err);
                     if (!ok) break;
@@ -780,13 +896,13 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_product(const __grid_consta
                     for (int k = 0; k < KS / 16; k++) {  // 16 of K: 32 bytes along it, 16 rows of 128 bytes across it
                         constexpr uint32_t sa = A_MN ? 2048 : 32, sb = B_MN ? 2048 : 32;
                         const uint64_t ah = operand_desc<A_MN, KS>(a + sa * k), bh = operand_desc<B_MN, KS>(b + sb * k);
-                        const uint32_t first = (n > 0 || k > 0) ? 1u : 0u;
+                        const uint32_t first = (n > n0 || k > 0) ? 1u : 0u;
                         if constexpr (TERMS == 3) {  // the small terms first
-                            umma_f16<A_MN, B_MN, PAIR>(d, operand_desc<A_MN, KS>(alo + sa * k), bh, first);
-                            umma_f16<A_MN, B_MN, PAIR>(d, ah, operand_desc<B_MN, KS>(blo + sb * k), 1u);
-                            umma_f16<A_MN, B_MN, PAIR>(d, ah, bh, 1u);
+                            umma_f16<A_MN, B_MN, PAIR, BN>(d, operand_desc<A_MN, KS>(alo + sa * k), bh, first);
+                            umma_f16<A_MN, B_MN, PAIR, BN>(d, ah, operand_desc<B_MN, KS>(blo + sb * k), 1u);
+                            umma_f16<A_MN, B_MN, PAIR, BN>(d, ah, bh, 1u);
                         } else {
-                            umma_f16<A_MN, B_MN, PAIR>(d, ah, bh, first);
+                            umma_f16<A_MN, B_MN, PAIR, BN>(d, ah, bh, first);
                         }
                     }
                     commit<PAIR>(empty0 + 8 * s);
@@ -802,13 +918,16 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_product(const __grid_consta
         bool ok = true;
         for (int t = first_tile; t < job.total; t += tile_step, made++) {
         int z, m0, n0;
-        tile_at<SYM, G::TILE_M>(job, t, z, m0, n0);
+        tile_at<SYM, G::TILE_M, BN>(job, SPLIT ? t / job.splits : t, z, m0, n0);
         m0 += half * BM;
         const int acc = made & 1;
         ok = ok && mbar_wait(acc_full + 8 * acc, (uint32_t)((made / 2) & 1), job.err);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         uint8_t* tile = turned + (warp - 2) * 4096;
         for (int col = part * (BN / 2); col < (part + 1) * (BN / 2); col += 32) {
+            const int r0 = m0 + 32 * w, c0 = n0 + col;
+            Before<MODE, TERMS, Io> before;
+            before.fetch(job, z, r0, c0, lane);
             uint32_t r[32];
             asm volatile(
                 "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
@@ -828,96 +947,32 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_product(const __grid_consta
                     else mbar_arrive(acc_empty + 8 * acc);
                 }
             }
-            const int r0 = m0 + 32 * w, c0 = n0 + col;
             if (r0 >= job.M || c0 >= job.N) continue;
             if constexpr (SYM)
                 if (c0 + 31 < r0) continue;  // below the diagonal: its mirror image is computed
             // Through shared memory, so that four lanes take 64 consecutive bytes of a row: a lane has a row of
             // the accumulator, and 16 bytes of each of 32 rows a store are half a sector each, at a fifth of
-            // the rate.  Units of 16 bytes are swapped by row: no bank twice.
+            // the rate.
             __syncwarp();
 #pragma unroll
-            for (int u = 0; u < 8; u++)
+            for (int u = 0; u < 8; u++) {
+                const uint32_t nan = 0x7fc00000u;
                 *reinterpret_cast<uint4*>(tile + lane * 128 + ((u ^ (lane & 7)) << 4)) =
-                    make_uint4(r[4 * u], r[4 * u + 1], r[4 * u + 2], r[4 * u + 3]);
-            __syncwarp();
-#pragma unroll
-            for (int it = 0; it < 4; it++) {
-                const int lr = 8 * it + (lane >> 2), u = 2 * (lane & 3), row = r0 + lr, c = c0 + 4 * u;
-                float* lo4 = reinterpret_cast<float*>(tile + lr * 128 + ((u ^ (lr & 7)) << 4));
-                float* hi4 = reinterpret_cast<float*>(tile + lr * 128 + (((u + 1) ^ (lr & 7)) << 4));
-                float v[8];
-                *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(lo4);
-                *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(hi4);
-                if (!ok)
-#pragma unroll
-                    for (int j = 0; j < 8; j++) v[j] = __uint_as_float(0x7fc00000u);
-                const bool in = row < job.M && c < job.N;
-                if constexpr (TERMS == 1 && !SYM) {  // c0 X, at the product's scale
-                    if (in) {
-                        float xv[8];
-                        load_planes8(job.g, (int64_t)z * job.g.stride + (int64_t)row * job.g.ld + c, xv);
-#pragma unroll
-                        for (int j = 0; j < 8; j++) v[j] = fmaf(job.c0 * kPlaneScale, xv[j], v[j]);
-                    }
-                }
-                if constexpr (MODE == RESULT) {
-                    const int64_t at = ((int64_t)z * job.M + row) * job.N + c;
-                    constexpr float one = 1.f / (kPlaneScale * kPlaneScale);
-#pragma unroll
-                    for (int j = 0; j < 8; j += 4) {
-                        const int left = job.N - c - j;
-                        if (in && left > 0)
-                            job.io.finish(at + j, left < 4 ? left : 4, job.vec && left >= 4,
-                                          make_float4(v[j] * one, v[j + 1] * one, v[j + 2] * one, v[j + 3] * one));
-                    }
-                } else {
-                    // products carry the square of the planes' scale; the rows' padding (to ld) may be written
-                    const int64_t at = (int64_t)z * job.out.stride + (int64_t)row * job.out.ld + c;
-#pragma unroll
-                    for (int j = 0; j < 8; j++) v[j] *= 1.f / kPlaneScale;
-                    if constexpr (MODE == POLY) {
-                        if (in) {
-                            float gv[8];
-                            load_planes8(job.g, (int64_t)z * job.g.stride + (int64_t)row * job.g.ld + c, gv);
-#pragma unroll
-                            for (int j = 0; j < 8; j++)
-                                v[j] = fmaf(job.c2, v[j], job.c1 * gv[j]) +
-                                       (TERMS == 3 && c + j == row ? job.c0 * kPlaneScale : 0.f);
-                        }
-                    }
-                    if (in && (!SYM || c > row)) {
-                        put8(job.out, at, v);
-                    } else if (in) {
-#pragma unroll
-                        for (int j = 0; j < 8; j++)
-                            if (c + j >= row && c + j < job.N) put(job.out, at + j, v[j]);
-                    }
-                    if constexpr (SYM) {
-                        *reinterpret_cast<float4*>(lo4) = *reinterpret_cast<const float4*>(v);
-                        *reinterpret_cast<float4*>(hi4) = *reinterpret_cast<const float4*>(v + 4);
-                    }
-                }
+                    ok ? make_uint4(r[4 * u], r[4 * u + 1], r[4 * u + 2], r[4 * u + 3]) : make_uint4(nan, nan, nan, nan);
             }
-            if constexpr (SYM) {  // the mirrored entries: row c0 + ., eight columns of it a lane
-                __syncwarp();
+            __syncwarp();
+            if (SPLIT && job.partial) {
+                float* to = job.partial + ((int64_t)t * BM + 32 * w) * BN + col;
 #pragma unroll
                 for (int it = 0; it < 4; it++) {
-                    const int lc = 8 * it + (lane >> 2), lr = 8 * (lane & 3), row = c0 + lc, c = r0 + lr;
-                    float v[8];
+                    const int lr = 8 * it + (lane >> 2), u = 2 * (lane & 3);
 #pragma unroll
-                    for (int j = 0; j < 8; j++)
-                        v[j] = *reinterpret_cast<const float*>(tile + (lr + j) * 128 + (((lc >> 2) ^ j) << 4) + 4 * (lc & 3));
-                    if (row >= job.N || c >= job.M) continue;
-                    const int64_t at = (int64_t)z * job.out.stride + (int64_t)row * job.out.ld + c;
-                    if (c + 7 < row && c + 7 < job.M) {
-                        put8(job.out, at, v);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 8; j++)
-                            if (c + j < row && c + j < job.M) put(job.out, at + j, v[j]);
-                    }
+                    for (int j = 0; j < 2; j++)
+                        *reinterpret_cast<uint4*>(to + lr * BN + 4 * (u + j)) =
+                            *reinterpret_cast<const uint4*>(tile + lr * 128 + (((u + j) ^ (lr & 7)) << 4));
                 }
+            } else {
+                finish_piece<MODE, TERMS, Io>(job, tile, before, z, r0, c0, lane);
             }
         }
         }
@@ -934,6 +989,51 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_product(const __grid_consta
             asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)(2 * BN))
                          : "memory");
     }
+}
+
+// The tiles that blocks shared: their sums, and the mode's work.  A block a 32 x 32 piece: warp w sums splits w, w + 8,
+// .., and the warps are added in their order.
+template <int TERMS, typename Io>
+__global__ void __launch_bounds__(256) k_sum_tiles(const Job<Io> job) {
+    constexpr int BN = 64;
+    __shared__ __align__(128) float4 sums[8][8][32];
+    __shared__ __align__(128) uint8_t tile[4096];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, piece = blockIdx.x & 7, t = blockIdx.x >> 3;
+    int z, m0, n0;
+    tile_at<true, BM, BN>(job, t, z, m0, n0);
+    const int r0 = m0 + 32 * (piece & 3), c0 = n0 + 32 * (piece >> 2);
+    wait_for_previous();
+    let_next_start();
+    if (r0 >= job.M || c0 >= job.N || c0 + 31 < r0) return;
+    const float* from = job.partial + ((int64_t)t * job.splits * BM + 32 * (piece & 3)) * BN + 32 * (piece >> 2);
+    const int u = 2 * (lane & 3);
+    float4 v[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = warp; k < job.splits; k += 8)
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int lr = 8 * (i >> 1) + (lane >> 2);
+            const float4 p = *reinterpret_cast<const float4*>(from + ((int64_t)k * BM + lr) * BN + 4 * (u + (i & 1)));
+            v[i].x += p.x, v[i].y += p.y, v[i].z += p.z, v[i].w += p.w;
+        }
+#pragma unroll
+    for (int i = 0; i < 8; i++) sums[warp][i][lane] = v[i];
+    __syncthreads();
+    if (warp != 0) return;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        float4 w = sums[0][i][lane];
+        for (int k = 1; k < 8; k++) {
+            const float4 p = sums[k][i][lane];
+            w.x += p.x, w.y += p.y, w.z += p.z, w.w += p.w;
+        }
+        const int lr = 8 * (i >> 1) + (lane >> 2);
+        *reinterpret_cast<float4*>(tile + lr * 128 + (((u + (i & 1)) ^ (lr & 7)) << 4)) = w;
+    }
+    __syncwarp();
+    const Before<GRAM, TERMS, Io> before = {};
+    finish_piece<GRAM, TERMS, Io>(job, tile, before, z, r0, c0, lane);
 }
 
 // ---- host ---------------------------------------------------------------------------
@@ -1000,9 +1100,11 @@ int64_t norm_blocks(const Shape& s) {
 
 int64_t pad64(int64_t c) { return (c + 63) & ~int64_t(63); }
 
+constexpr int kSplitTiles = 148;  // 128 x 64 tiles' sums that blocks share
+
 struct Layout {
     int64_t part, pmat;                     // small
-    int64_t err, x[2], g, b, bytes;         // planes: hi, then lo
+    int64_t err, partial, x[2], g, b, bytes;  // planes: hi, then lo
     int64_t x_plane, s_plane;               // bytes of one plane
 };
 
@@ -1021,6 +1123,7 @@ Layout layout_of(const Shape& s, int terms) {
     } else {
         l.part = take(s.stack * norm_blocks(s) * 8);
         l.err = take(4);
+        l.partial = take(kSplitTiles * (int64_t)BM * 64 * 4);
         l.x_plane = align256(s.stack * s.rows * pad64(s.cols) * 2);
         l.s_plane = align256(s.stack * s.side * pad64(s.side) * 2);
         const int planes = terms == 3 ? 2 : 1;
@@ -1069,8 +1172,6 @@ struct Matrix {  // a plane pair and its extent
     int64_t rows, cols;
 };
 
-struct NoIo {};
-
 // Pairs of blocks that the device runs at once (every k_product takes an SM a block).
 int pairs_at_once(const void* kernel, int smem) {
     static int cached[64] = {0};
@@ -1098,9 +1199,19 @@ int pairs_at_once(const void* kernel, int smem) {
     return cached[dev];
 }
 
-template <int MODE, bool A_MN, bool B_MN, int TERMS, bool PAIR, typename Io>
+// Tiles of TILE_M x BN of an M x N product (symmetric: those that reach the diagonal or lie above it).
+int64_t count_tiles(bool sym, int64_t M, int64_t N, int tile_m, int bn) {
+    const int64_t tm = ceil_div(M, tile_m), tn = ceil_div(N, bn);
+    if (!sym) return tm * tn;
+    int64_t n = 0;
+    for (int64_t b = 0; b < tn; b++) n += std::min((bn * (b + 1) - 1) / tile_m + 1, tm);
+    return n;
+}
+
+template <int MODE, bool A_MN, bool B_MN, int TERMS, bool PAIR, int BN, typename Io>
 int run_tiles(const Matrix& a, const Matrix& b, int64_t stack, Job<Io> job, cudaStream_t st) {
-    using G = Cfg<TERMS, PAIR>;
+    using G = Cfg<TERMS, PAIR, BN>;
+    constexpr bool SYM = MODE == GRAM || MODE == POLY;
     Maps maps;
     memset(&maps, 0, sizeof(maps));
     const auto make = [&](CUtensorMap* map, const __half* plane, const Matrix& x, bool mn, int tile_rows) {
@@ -1110,28 +1221,39 @@ int run_tiles(const Matrix& a, const Matrix& b, int64_t stack, Job<Io> job, cuda
     if (!make(&maps.a_hi, a.p.hi, a, A_MN, BM) || !make(&maps.b_hi, b.p.hi, b, B_MN, G::B_ROWS)) return ENGRAM_ERR_CUDA;
     if (TERMS == 3 && (!make(&maps.a_lo, a.p.lo, a, A_MN, BM) || !make(&maps.b_lo, b.p.lo, b, B_MN, G::B_ROWS)))
         return ENGRAM_ERR_CUDA;
-    job.tiles_m = (int)ceil_div(job.M, G::TILE_M), job.tiles_n = (int)ceil_div(job.N, 256);
-    int64_t tiles = (int64_t)job.tiles_m * job.tiles_n;
-    if (MODE == GRAM || MODE == POLY) {
-        tiles = 0;
-        for (int b2 = 0; b2 < job.tiles_n; b2++) tiles += std::min(256 / G::TILE_M * (b2 + 1), job.tiles_m);
-    }
+    job.tiles_m = (int)ceil_div(job.M, G::TILE_M), job.tiles_n = (int)ceil_div(job.N, BN);
+    const int64_t tiles = count_tiles(SYM, job.M, job.N, G::TILE_M, BN);
     if (tiles * stack > INT32_MAX) return ENGRAM_ERR_RANGE;
     job.tiles = (int)tiles;
-    job.total = (int)(tiles * stack);
-    constexpr auto kernel = k_product<MODE, A_MN, B_MN, TERMS, PAIR, Io>;
+    job.splits = 1;
+    if (MODE == GRAM && BN == 64 && job.partial)
+        job.splits = (int)std::max<int64_t>(1, std::min<int64_t>(kSplitTiles / (tiles * stack), ceil_div(job.K, 4 * G::KS)));
+    if (job.splits == 1) job.partial = nullptr;
+    job.total = (int)(tiles * stack * job.splits);
+    constexpr auto kernel = k_product<MODE, A_MN, B_MN, TERMS, PAIR, BN, Io>;
     const int most = PAIR ? pairs_at_once((const void*)kernel, G::SMEM) : sm_count();
     const int blocks = (PAIR ? 2 : 1) * std::min(job.total, most);
-    return start<kernel, PAIR ? 2 : 1>(dim3((unsigned)blocks), kGemmThreads, G::SMEM, true, st, maps, job);
+    int e = start<kernel, PAIR ? 2 : 1>(dim3((unsigned)blocks), kGemmThreads, G::SMEM, true, st, maps, job);
+    if constexpr (MODE == GRAM && BN == 64) {
+        if (!e && job.partial)
+            e = start<k_sum_tiles<TERMS, Io>>(dim3((unsigned)(8 * tiles * stack)), 256, 0, true, st, job);
+    }
+    return e;
 }
 
-// Pairs of blocks where that leaves at least half of them a tile: MEASURED.
+// Which tiles: 256 x 256 on pairs of blocks where there are 50 or more of them, else 128 x 64 while every block gets
+// at most one, else 128 x 256.  Pairs against 128 x 256, all steps: 10240 x 2560 in bf16 1124 against 1183 us, 2560 x
+// 2560 in fp32 1041 against 1056; but 2048 x 2048 in bf16 362 against 350, 1024 x 1024 266 against 250.  128 x 64
+// against 128 x 256: 1024 x 1024 in fp32 310 against 389, 256 x 256 147 against 218; but, at two a block, 1536 x 1536
+// 619 against 514.
 template <int MODE, bool A_MN, bool B_MN, int TERMS, typename Io>
 int run_product(const Matrix& a, const Matrix& b, int64_t stack, const Job<Io>& job, cudaStream_t st) {
-    const int64_t tn = ceil_div(job.N, 256), tm = ceil_div(job.M, 256);
-    const int64_t pairs = ((MODE == GRAM || MODE == POLY) ? tn * (tn + 1) / 2 : tm * tn) * stack;
-    if (pairs >= 37) return run_tiles<MODE, A_MN, B_MN, TERMS, true>(a, b, stack, job, st);
-    return run_tiles<MODE, A_MN, B_MN, TERMS, false>(a, b, stack, job, st);
+    constexpr bool SYM = MODE == GRAM || MODE == POLY;
+    if (count_tiles(SYM, job.M, job.N, 256, 256) * stack >= 50)
+        return run_tiles<MODE, A_MN, B_MN, TERMS, true, 256>(a, b, stack, job, st);
+    if (count_tiles(SYM, job.M, job.N, 128, 64) * stack <= 148)
+        return run_tiles<MODE, A_MN, B_MN, TERMS, false, 64>(a, b, stack, job, st);
+    return run_tiles<MODE, A_MN, B_MN, TERMS, false, 256>(a, b, stack, job, st);
 }
 
 template <int TERMS, typename Io>
@@ -1151,11 +1273,12 @@ int run_planes(const Shape& s, const Layout& l, const Io& io, const Poly& poly, 
     int e = start<k_norm<Io>>(dim3((unsigned)nb, (unsigned)s.stack), kNormThreads, 0, false, st, io, s.rows * s.cols,
                               io.aligned && s.rows * s.cols % 4 == 0, part);
     if (e) return e;
-    const int64_t row_blocks = ceil_div(s.rows, kNormThreads / 32), most = ceil_div(8 * 148, s.stack);
+    const int64_t row_blocks = ceil_div(s.rows * ceil_div(s.cols, 512), kNormThreads / 32), most = ceil_div(8 * 148, s.stack);
     e = start<k_planes<Io>>(dim3((unsigned)(row_blocks < most ? row_blocks : most), (unsigned)s.stack), kNormThreads, 0,
                             true, st, io, s.rows, s.cols, vec, part, nb, eps, x[0].p);
     Job<NoIo> job = {};
     job.err = (int*)(ws + l.err);
+    job.partial = (float*)(ws + l.partial);
     for (int i = 0; i < poly.steps && !e; i++) {
         const Matrix &in = x[i & 1], &next = x[(i & 1) ^ 1];
         job.M = job.N = (int)s.side;

@@ -102,7 +102,8 @@ def test_short_sides_match_the_singular_values(shape, dtype):
 
 LONG = [(1, 65, 65), (1, 128, 128), (1, 130, 257), (2, 257, 130), (1, 256, 512), (1, 512, 384), (3, 100, 90),
         (1, 300, 1000), (1, 1001, 299), (1, 1024, 640), (2, 70, 4097),
-        (1, 2200, 2100), (1, 2100, 2300), (40, 100, 130), (3, 1300, 700)]  # pairs of blocks
+        (1, 2200, 2100), (1, 2100, 2300), (40, 100, 130), (3, 1300, 700),  # pairs of blocks
+        (1, 90, 9000), (1, 6000, 200), (2, 66, 3000)]  # sums over a long side shared by blocks
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=str)
