@@ -182,4 +182,6 @@ def adapter_add(base: torch.Tensor | None, x: torch.Tensor, a: torch.Tensor, b: 
         if out is not None:
             raise ValueError("adapter_add: out= is for calls that need no gradients")
         return _AdapterFn.apply(base, x, a, b, index, scale)
+    if out is not None and out.requires_grad and torch.is_grad_enabled():
+        raise ValueError("adapter_add: out requires grad")
     return forward_into(out, base, x, a, b, index, scale)

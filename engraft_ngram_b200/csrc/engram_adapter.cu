@@ -986,7 +986,8 @@ __global__ void __launch_bounds__(kThreads, RB * (int)sizeof(T) <= 8 ? 3 : RB * 
 // The factors' rows are loaded in an order (a five-dimensional tensor map) that makes a lane's columns of 32
 // (fp32: 16) one 16-byte unit of the row: column 8 k + 2 q + j of the product is feature 8 q + 2 k + j (fp32: 4 q
 // + 2 k + j).  Blocks are persistent, one an SM, and share all (tile, stage) pairs evenly in their order.
-// Every wait is bounded: one that gives up ends its warp's loop (results stay unwritten).
+// Every wait is bounded: one that gives up (never, in a correct run) ends its warp's loop, the waits on that warp
+// give up in their turn, and the results that are then missing are written as NaN.
 template <typename T, int RB>
 struct WideCfg {
     static constexpr int SIZE = sizeof(T), RP = 8 * RB, BM = 128;
@@ -1153,12 +1154,13 @@ __global__ void __launch_bounds__(kWideThreads, 1) k_expand_wide(const __grid_co
         bool ok = true, fresh = true;
         int slot = 0;
         const int tile_first = (int)(begin / per_tile);
-        for (int i = first; i < steps && ok; i += 2) {
+        for (int i = first; i < steps; i += 2) {
             if (fresh) read_rows(row, at.tile);
             const bool real = at.tile < real_tiles;
             const int a = i & 3;
             if (real) {
-                ok = mbar_wait(acc_full + 8 * a, (uint32_t)((i >> 2) & 1), nullptr, kWideSpins);
+                ok = ok && mbar_wait(acc_full + 8 * a, (uint32_t)((i >> 2) & 1), nullptr, kWideSpins);
+                ok = __all_sync(0xffffffffu, ok);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             }
             stage_wait<C::DEPTH - 1>();
@@ -1221,7 +1223,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) k_expand_wide(const __grid_co
                                 }
                             }
                         }
-                        if (ok && row[k] >= 0 && f < F) *reinterpret_cast<uint4*>(out + (int64_t)row[k] * ldo + f) = v;
+                        if (real && !ok) v = make_uint4(~0u, ~0u, ~0u, ~0u);  // NaN in every type
+                        if (row[k] >= 0 && f < F) *reinterpret_cast<uint4*>(out + (int64_t)row[k] * ldo + f) = v;
                     }
             }
             fetch(i + 2 * C::DEPTH, slot);

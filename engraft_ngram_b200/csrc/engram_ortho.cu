@@ -44,7 +44,6 @@ struct Poly {
 };
 
 template <typename T> __device__ __forceinline__ float to_f32(T v);
-template <> __device__ __forceinline__ float to_f32(float v) { return v; }
 template <> __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
 template <> __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
 template <typename T> __device__ __forceinline__ T from_f32(float v);
@@ -557,7 +556,6 @@ struct Job {
     float c0, c1, c2;  // POLY
     Io io;             // RESULT
     bool vec;          // RESULT: rows of whole, aligned fours
-    int* err;
 };
 
 // Shared-memory matrix descriptor.  Along K (rows of KS fp16, 64- or 128-byte swizzle): 8-row groups
@@ -791,7 +789,7 @@ __device__ __forceinline__ void finish_piece(const Job<Io>& job, uint8_t* tile, 
 // two accumulators in turn, and warps 2 to 9 take each through the mode's epilogue (tensor-memory lanes 32
 // (w % 4) .., half of the columns) while the next one is made: the epilogue, up to 8 us a tile beside 11 us
 // of products, costs time only after a block's last tile.  A wait that gives up (never, in a correct run)
-// counts itself in *err, and the block's results from then on become NaN.
+// makes the block's results from then on NaN.
 template <int MODE, bool A_MN, bool B_MN, int TERMS, bool PAIR, int BN, typename Io>
 __global__ void __launch_bounds__(kGemmThreads, 1) k_product(const __grid_constant__ Maps maps, const Job<Io> job) {
     using G = Cfg<TERMS, PAIR, BN>;
@@ -854,7 +852,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_product(const __grid_consta
                 const int part = SPLIT ? t % job.splits : 0, parts = SPLIT ? job.splits : 1;
                 for (int k = slices * part / parts; k < slices * (part + 1) / parts; k++, i++) {
                     const int s = i % STAGES, round = i / STAGES;
-                    if (round > 0) ok = mbar_wait(empty0 + 8 * s, (uint32_t)((round - 1) & 1), job.err);
+                    if (round > 0) ok = mbar_wait(empty0 + 8 * s, (uint32_t)((round - 1) & 1), nullptr);
                     if (!ok) break;
                     const uint32_t bar = PAIR ? leaders(full0 + 8 * s) : full0 + 8 * s;
                     const uint32_t st = smem_u32(smem + s * G::STAGE_BYTES);
@@ -872,7 +870,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_product(const __grid_consta
             // blocks', before either passes the last barrier)
             if (half == 0)
                 for (int k = i > STAGES ? i - STAGES : 0; k < i; k++)
-                    mbar_wait(full0 + 8 * (k % STAGES), (uint32_t)((k / STAGES) & 1), job.err);
+                    mbar_wait(full0 + 8 * (k % STAGES), (uint32_t)((k / STAGES) & 1), nullptr);
         }
     } else if (warp == 1) {
         if (lane == 0 && half == 0) {
@@ -880,14 +878,14 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_product(const __grid_consta
             bool ok = true;
             for (int t = first_tile; t < job.total; t += tile_step, made++) {
                 const int acc = made & 1;
-                if (made >= 2) ok = ok && mbar_wait(acc_empty + 8 * acc, (uint32_t)((made / 2 - 1) & 1), job.err);
+                if (made >= 2) ok = ok && mbar_wait(acc_empty + 8 * acc, (uint32_t)((made / 2 - 1) & 1), nullptr);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t d = tmem + acc * BN;
                 const int part = SPLIT ? t % job.splits : 0, parts = SPLIT ? job.splits : 1;
                 const int n0 = slices * part / parts, n1 = slices * (part + 1) / parts;
                 for (int n = n0; n < n1 && ok; n++, i++) {
                     const int s = i % STAGES;
-                    ok = mbar_wait(full0 + 8 * s, (uint32_t)((i / STAGES) & 1), job.err);
+                    ok = mbar_wait(full0 + 8 * s, (uint32_t)((i / STAGES) & 1), nullptr);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint32_t a = smem_u32(smem + s * G::STAGE_BYTES), b = a + G::A_BYTES;
@@ -921,7 +919,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_product(const __grid_consta
         tile_at<SYM, G::TILE_M, BN>(job, SPLIT ? t / job.splits : t, z, m0, n0);
         m0 += half * BM;
         const int acc = made & 1;
-        ok = ok && mbar_wait(acc_full + 8 * acc, (uint32_t)((made / 2) & 1), job.err);
+        ok = ok && mbar_wait(acc_full + 8 * acc, (uint32_t)((made / 2) & 1), nullptr);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         uint8_t* tile = turned + (warp - 2) * 4096;
         for (int col = part * (BN / 2); col < (part + 1) * (BN / 2); col += 32) {
@@ -1104,7 +1102,7 @@ constexpr int kSplitTiles = 148;  // 128 x 64 tiles' sums that blocks share
 
 struct Layout {
     int64_t part, pmat;                     // small
-    int64_t err, partial, x[2], g, b, bytes;  // planes: hi, then lo
+    int64_t partial, x[2], g, b, bytes;     // planes: hi, then lo
     int64_t x_plane, s_plane;               // bytes of one plane
 };
 
@@ -1122,7 +1120,6 @@ Layout layout_of(const Shape& s, int terms) {
         l.pmat = take(s.stack * rm * rm * 8);
     } else {
         l.part = take(s.stack * norm_blocks(s) * 8);
-        l.err = take(4);
         l.partial = take(kSplitTiles * (int64_t)BM * 64 * 4);
         l.x_plane = align256(s.stack * s.rows * pad64(s.cols) * 2);
         l.s_plane = align256(s.stack * s.side * pad64(s.side) * 2);
@@ -1142,7 +1139,7 @@ int run_small(const Shape& s, const Layout& l, const Io& io, const Poly& poly, d
     double *part = (double*)(ws + l.part), *pmat = (double*)(ws + l.pmat);
     const dim3 grid((unsigned)chunks, (unsigned)s.stack);
     const bool vec = io.aligned && (TALL ? s.side : s.length) % 4 == 0;
-    constexpr int RM = 8 * MB, SP = RM + 4, NT = MB * (MB + 1) / 2;
+    constexpr int RM = 8 * MB, SP = RM + 4;
     int e = start<k_small_gram<MB, TALL, Io>>(grid, kSmallThreads, 0, false, st, io, (int)s.side, s.length, chunk, vec,
                                               part);
     if (!e)
@@ -1277,7 +1274,6 @@ int run_planes(const Shape& s, const Layout& l, const Io& io, const Poly& poly, 
     e = start<k_planes<Io>>(dim3((unsigned)(row_blocks < most ? row_blocks : most), (unsigned)s.stack), kNormThreads, 0,
                             true, st, io, s.rows, s.cols, vec, part, nb, eps, x[0].p);
     Job<NoIo> job = {};
-    job.err = (int*)(ws + l.err);
     job.partial = (float*)(ws + l.partial);
     for (int i = 0; i < poly.steps && !e; i++) {
         const Matrix &in = x[i & 1], &next = x[(i & 1) ^ 1];
@@ -1302,7 +1298,7 @@ int run_planes(const Shape& s, const Layout& l, const Io& io, const Poly& poly, 
                        : run_product<UPDATE, false, true, TERMS>(b, in, s.stack, job, st);
         } else {
             Job<Io> result = {};
-            result.M = job.M, result.N = job.N, result.K = job.K, result.err = job.err;
+            result.M = job.M, result.N = job.N, result.K = job.K;
             result.io = io;
             result.vec = vec;
             result.g = in.p, result.c0 = job.c0;
@@ -1423,6 +1419,7 @@ extern "C" int engram_muon_step(int32_t grad_dtype, const float* p, const void* 
     if (!grad || !aligned_to(grad, grad_dtype) || !workspace || !aligned16(workspace)) return ENGRAM_ERR_ARG;
     for (const float* f : {p, m, (const float*)p_out, (const float*)m_out})
         if (!f || !aligned_to(f, ENGRAM_DTYPE_F32)) return ENGRAM_ERR_ARG;
+    if (p_out == m_out || p == m_out || p_out == m || p == m || grad == p_out || grad == m_out) return ENGRAM_ERR_ARG;
     const Layout l = layout_of(s, 3);
     if (workspace_bytes < l.bytes) return ENGRAM_ERR_WORKSPACE;
     const double ratio = rows > cols ? sqrt((double)rows / (double)cols) : 1.0;

@@ -25,6 +25,8 @@ _DTYPES = {torch.float32: L.DTYPE_F32, torch.bfloat16: L.DTYPE_BF16, torch.float
 
 @functools.lru_cache(maxsize=64)
 def _table(coefficients: tuple, steps: int):
+    if not coefficients:
+        raise ValueError("coefficients: none given")
     rows = coefficients if isinstance(coefficients[0], (tuple, list)) else (coefficients,) * steps
     if len(rows) != steps or any(len(r) != 3 for r in rows):
         raise ValueError(f"coefficients: expected 3 numbers, or 3 for each of the {steps} steps")
@@ -68,7 +70,7 @@ def orthogonalize(update: torch.Tensor, steps: int = 5, coefficients=COEFFICIENT
     Frobenius norm (at least eps) and taken through `steps` steps
     X <- c0 X + (c1 G + c2 G G) X, G = X X^T over the shorter side.
     coefficients: (c0, c1, c2), or one such triple a step.  A zero matrix stays
-    zero.  out (may be update): where to write.  Not differentiable."""
+    zero.  out (update itself, or no part of it): where to write.  Not differentiable."""
     stack, rows, cols = _stack(update, "update")
     table = _coefficients(coefficients, steps)
     if out is None:
@@ -94,7 +96,8 @@ def muon_step(param: torch.Tensor, grad: torch.Tensor, momentum: torch.Tensor, l
         u = grad + beta (momentum - grad) if nesterov else momentum
         param <- (1 - lr weight_decay) param - lr sqrt(max(1, rows / cols)) orthogonalize(u)
     param and momentum: float32, updated in place, or written to out = (param,
-    momentum); grad: float32, bfloat16 or float16.  Returns (param, momentum)."""
+    momentum); grad: float32, bfloat16 or float16.  param, grad and momentum must
+    not overlap one another (an output and its own input may be one).  Returns (param, momentum)."""
     stack, rows, cols = _stack(grad, "grad")
     _same(param, grad, "param", torch.float32)
     _same(momentum, grad, "momentum", torch.float32)

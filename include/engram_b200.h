@@ -724,6 +724,7 @@ ENGRAM_API int engram_adapter_backward(int32_t dtype, const void* grad, int64_t 
  *   m' = m + (1 - beta)(g - m);  u = nesterov ? g + beta (m' - g) : m'
  *   p' = (1 - lr weight_decay) p - lr sqrt(max(1, rows / cols)) O(u)
  * p, m, p_out (may be p), m_out (may be m): fp32; grad of type grad_dtype.
+ * No other two of the five arrays may be the same (ENGRAM_ERR_ARG) or overlap.
  * workspace: 16-byte aligned device scratch of
  * engram_orthogonalize_workspace_bytes(dtype, ...) bytes, for engram_muon_step
  * with dtype = ENGRAM_DTYPE_F32.

@@ -245,6 +245,41 @@ def test_another_stream_and_a_captured_call_replayed_on_new_inputs():
     assert torch.equal(out, want_d) and all(torch.equal(u, v) for u, v in zip(grads, grads_d))
 
 
+def test_two_streams_at_once():
+    """Calls whose kernels overlap keep to their own workspaces: planned and small batches, both directions."""
+    cases = [make(2000, 256, 1024, 16, 3, BF16, "segments", seed=30), make(300, 512, 640, 16, 20, BF16, "random", seed=31)]
+    want = [(eb.adapter_add(**c), *eb.adapter_gradients(g, c["x"], c["a"], c["b"], c["index"], c["scale"]))
+            for c, g in cases]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(8):
+        for k, (c, g) in enumerate(cases):
+            with torch.cuda.stream(streams[k]):
+                got[k].append((eb.adapter_add(**c),
+                               *eb.adapter_gradients(g, c["x"], c["a"], c["b"], c["index"], c["scale"])))
+    torch.cuda.synchronize()
+    for k in range(2):
+        for run in got[k]:
+            assert all(torch.equal(u, v) for u, v in zip(run, want[k]))
+
+
+def test_hundred_thousands_of_positions():
+    test_forward_and_gradients_match_the_formula((200003, 24, 40, 8, 3, F32, "random"))
+    test_forward_and_gradients_match_the_formula((131072, 32, 64, 16, 2, BF16, "segments"))
+
+
+@pytest.mark.parametrize("T", [40, 1500])
+def test_inference_mode_and_an_output_that_needs_gradients(T):
+    c, _ = make(T, 64, 96, 8, 3, F32, "random", seed=32)
+    want = eb.adapter_add(**c)
+    with torch.inference_mode():
+        assert torch.equal(eb.adapter_add(**c), want)
+        held = c["base"].clone()
+        assert torch.equal(eb.adapter_add(**{**c, "base": held}, out=held), want)
+    with pytest.raises(ValueError, match="requires grad"):
+        eb.adapter_add(**c, out=torch.nn.Parameter(c["base"].clone()))
+
+
 @pytest.mark.parametrize("bad, text", [
     (lambda c: dict(x=c["x"].double()), "x:"), (lambda c: dict(a=c["a"][:, :, :-1]), "a "),
     (lambda c: dict(a=c["a"].transpose(1, 2).contiguous().transpose(1, 2)), "contiguous"),

@@ -239,6 +239,33 @@ def test_another_stream_and_a_captured_step_replayed_on_new_gradients():
         assert torch.equal(p, want[k][0]) and torch.equal(o, want[k][1])
 
 
+def test_two_streams_at_once():
+    """Calls whose kernels overlap keep to their own workspaces: pairs of blocks, single blocks and short sides."""
+    xs = [make(1, 2560, 2560, "noise", seed=40).to(BF16), make(1, 300, 1200, "noise", seed=41), make(9, 16, 400, "noise", seed=42)]
+    want = [eb.orthogonalize(x) for x in xs]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in xs], [[] for _ in xs]
+    for _ in range(6):
+        for k, x in enumerate(xs):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(eb.orthogonalize(x))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[k]) for k in range(len(xs)) for y in got[k])
+
+
+def test_inference_mode_and_overlapping_arrays():
+    p, g, m = (make(2, 20, 90, "noise", seed=50 + k) for k in range(3))
+    want = eb.muon_step(p, g, m, 0.1, out=(torch.empty_like(p), torch.empty_like(m)))
+    with torch.inference_mode():
+        q, n = p.clone(), m.clone()
+        eb.muon_step(q, g, n, 0.1)
+        assert torch.equal(q, want[0]) and torch.equal(n, want[1])
+        assert torch.equal(eb.orthogonalize(g), eb.orthogonalize(g, out=g.clone()))
+    for arrays in ((p, g, p), (g, g, m), (p, m, m)):
+        with pytest.raises(ValueError):
+            eb.muon_step(*arrays, 0.1)
+
+
 @pytest.mark.parametrize("bad", [
     lambda x: eb.orthogonalize(x.double()), lambda x: eb.orthogonalize(x.mT), lambda x: eb.orthogonalize(x[0, 0]),
     lambda x: eb.orthogonalize(x, out=x.to(BF16)), lambda x: eb.orthogonalize(x, out=x[:1]),

@@ -63,6 +63,11 @@ def test_muon_refuses_missing_and_misaligned_arrays(lib, name):
     assert muon(lib, **{name: X + 2}) == L.ERR_ARG
 
 
+@pytest.mark.parametrize("alias", [dict(p=M), dict(p_out=M), dict(m_out=X), dict(p_out=M2), dict(g=P2), dict(g=M2)])
+def test_muon_refuses_arrays_that_would_overwrite_one_another(lib, alias):
+    assert muon(lib, **alias) == L.ERR_ARG
+
+
 def test_nothing_to_do_and_the_workspace(lib):
     assert ortho(lib, stack=0, x=None, out=None, ws=None, ws_bytes=0) == 0
     size = lib.engram_orthogonalize_workspace_bytes
@@ -81,6 +86,8 @@ def test_python_calls_refuse():
         MU._coefficients(MU.COEFFICIENTS, 0)
     with pytest.raises(ValueError, match="coefficients"):
         MU._coefficients((1.0, 2.0), 5)
+    with pytest.raises(ValueError, match="coefficients"):
+        MU._coefficients((), 5)
     with pytest.raises(ValueError, match="coefficients"):
         MU._coefficients(((1.0, 0.0, 0.0),) * 4, 5)
     assert list(MU._coefficients([[1, 2, 3], (4, 5, 6)], 2)) == [1, 2, 3, 4, 5, 6]
