@@ -223,8 +223,8 @@ def stream_of(device) -> int:
 def on_device(device, call):
     """call(stream) with the device current (a launch goes to the current device) and its current stream."""
     import torch
-    if device.index == torch.cuda.current_device():
-        return call(torch.cuda.current_stream().cuda_stream)
+    if device.index == torch.cuda.current_device():  # the raw handle: 0.1 us, where a Stream object of it takes 3
+        return call(torch._C._cuda_getCurrentRawStream(device.index))
     with torch.cuda.device(device):
         return call(torch.cuda.current_stream().cuda_stream)
 

@@ -63,7 +63,6 @@ def _workspace_bytes(code, stack, rows, cols) -> int:
     return max(size, 1)
 
 
-@torch.no_grad()
 def orthogonalize(update: torch.Tensor, steps: int = 5, coefficients=COEFFICIENTS, eps: float = 1e-7,
                   out: torch.Tensor | None = None) -> torch.Tensor:
     """Each matrix of update [rows, cols] or [stack, rows, cols], divided by its
@@ -87,7 +86,6 @@ def orthogonalize(update: torch.Tensor, steps: int = 5, coefficients=COEFFICIENT
     return out
 
 
-@torch.no_grad()
 def muon_step(param: torch.Tensor, grad: torch.Tensor, momentum: torch.Tensor, lr: float, beta: float = 0.95,
               nesterov: bool = True, weight_decay: float = 0.0, steps: int = 5, coefficients=COEFFICIENTS,
               eps: float = 1e-7, out: tuple[torch.Tensor, torch.Tensor] | None = None):

@@ -268,6 +268,26 @@ def test_hundred_thousands_of_positions():
     test_forward_and_gradients_match_the_formula((131072, 32, 64, 16, 2, BF16, "segments"))
 
 
+@pytest.mark.parametrize("T", [60, 1100])
+def test_the_largest_stack_of_adapters(T):
+    c, grad = make(T, 24, 40, 4, 3, F32, "random", seed=33)
+    want, mag = formula(c, grad), formula(c, grad, mag=True)
+    used = torch.tensor([0, 9000, 16383], device=DEV)
+    d = dict(c)
+    for k in ("a", "b", "scale"):
+        d[k] = torch.full((16384, *c[k].shape[1:]), float("nan"), device=DEV)
+        d[k][used] = c[k]
+    d["index"] = torch.where(c["index"] < 0, -1, used[c["index"].clamp(min=0)]).to(torch.int32)
+    check(eb.adapter_add(**d), want[0], mag[0], 24 + 4, F32)
+    dx, da, db = eb.adapter_gradients(grad, d["x"], d["a"], d["b"], d["index"], d["scale"])
+    check(dx, want[1], mag[1], 40 + 4, F32)
+    check(da[used], want[2], mag[2], 40 + T, F32)
+    check(db[used], want[3], mag[3], 24 + T, F32)
+    others = torch.ones(16384, dtype=torch.bool, device=DEV)
+    others[used] = False
+    assert (da[others] == 0).all() and (db[others] == 0).all()
+
+
 @pytest.mark.parametrize("T", [40, 1500])
 def test_inference_mode_and_an_output_that_needs_gradients(T):
     c, _ = make(T, 64, 96, 8, 3, F32, "random", seed=32)
