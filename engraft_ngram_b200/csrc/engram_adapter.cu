@@ -1381,7 +1381,7 @@ struct Side {
     const float* h;
     int64_t F;
     T* out;
-    bool trans, vec;
+    bool trans, vec, ovec;  // vec: rows of x start on 16 bytes; ovec: whole 16-byte units of out
 };
 template <typename T, int RB>
 struct WeightCfg {
@@ -1639,6 +1639,36 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 && RB <= 4 ? 3 : 1) k
     if (parts > 1) cluster.sync();
     else __syncthreads();
     T* dst = side.out + (int64_t)a * rank * F;
+    if (side.ovec) {  // 16 bytes a thread: along the columns, or along the ranks of a column
+        for (int u = threadIdx.x + part * kThreads; u < FC * RP / E; u += parts * kThreads) {
+            const int c = side.trans ? u % FC : u % (FC / E) * E, r = side.trans ? u / FC * E : u / (FC / E);
+            if (r >= rank || f0 + c >= F) continue;
+            float v[E];
+#pragma unroll
+            for (int j = 0; j < E; j++) v[j] = 0.f;
+            for (int k = 0; k < parts; k++) {
+                const float* from = (parts > 1 ? cluster.map_shared_rank(red, k) : red) + r * RS + c;
+                if (side.trans) {
+#pragma unroll
+                    for (int j = 0; j < E; j++) v[j] += from[j * RS] + from[(RP + j) * RS];
+                } else {
+#pragma unroll
+                    for (int j = 0; j < E; j += 4) {
+                        const float4 p = *reinterpret_cast<const float4*>(from + j);
+                        const float4 q4 = *reinterpret_cast<const float4*>(from + RP * RS + j);
+                        v[j] += p.x + q4.x, v[j + 1] += p.y + q4.y, v[j + 2] += p.z + q4.z, v[j + 3] += p.w + q4.w;
+                    }
+                }
+            }
+            alignas(16) T o[E];
+#pragma unroll
+            for (int j = 0; j < E; j++) o[j] = narrow<T>(v[j]);
+            T* to = dst + (side.trans ? (f0 + c) * rank + r : (int64_t)r * F + f0 + c);
+            *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(o);
+        }
+        if (parts > 1) cluster.sync();  // its shared memory is read until here
+        return;
+    }
     for (int e = threadIdx.x + part * kThreads; e < FC * RP; e += parts * kThreads) {
         const int r = side.trans ? e % RP : e / FC, c = side.trans ? e / RP : e % FC;
         if (r >= rank || f0 + c >= F) continue;
@@ -1893,8 +1923,10 @@ int backward(const Shape& s, const Layout& l, const Args& g) {
         e = run_expand<T, RB, WM, true>(s, plan, dh, 1, (const T*)g.a, s.K, (const T*)g.base, g.ldbase, (T*)g.dx,
                                         g.lddx, g.st);
     if (!e && (g.da || g.db)) {
-        const Side<T> da = {(const T*)g.x, g.ldx, dh, s.K, (T*)g.da, false, row_units((const T*)g.x, g.ldx)};
-        const Side<T> db = {(const T*)g.grad, g.ldgrad, h, s.N, (T*)g.db, true, row_units((const T*)g.grad, g.ldgrad)};
+        const Side<T> da = {(const T*)g.x, g.ldx, dh, s.K, (T*)g.da, false, row_units((const T*)g.x, g.ldx),
+                            row_units((const T*)g.da, s.K)};
+        const Side<T> db = {(const T*)g.grad, g.ldgrad, h, s.N, (T*)g.db, true, row_units((const T*)g.grad, g.ldgrad),
+                            row_units((const T*)g.db, s.rank)};
         e = run_weight<T, RB>(s, plan, g.index, da, db, g.st);
     }
     return e;
