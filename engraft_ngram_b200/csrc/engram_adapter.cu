@@ -426,17 +426,29 @@ struct ShrinkCfg {
 // Where a block finds its tile: k_plan's, found here and written to `plan`, or written by a launch before.
 enum Tiles { PLANNED, FIND };
 
+// One of the two sums: its operands, width and columns of a split, and where it goes.
+template <typename T>
+struct Shrink {
+    const T* x;
+    int64_t ldx;
+    const T* w;
+    int64_t K, k_split;
+    int splits;
+    bool xvec, wvec;
+    float* h;
+};
+
 template <typename T, int RB, int WM, bool TRANS>
-__global__ void __launch_bounds__(kThreads, RB <= 4 ? 3 : 1) k_shrink(Plan plan, int tiles, const int32_t* __restrict__ index,
-                                                     const T* __restrict__ x, int64_t ldx, const T* __restrict__ w,
-                                                     const float* __restrict__ scale, int n, int rank, int64_t K,
-                                                     int64_t k_split, int T_rows, bool xvec, bool wvec,
-                                                     float* __restrict__ h) {
+__device__ __forceinline__ void shrink_tile(uint8_t* smem, TileRows<16 * WM>& tr, const Plan& plan, int tiles,
+                                            const int32_t* __restrict__ index, const Shrink<T>& side,
+                                            const float* __restrict__ scale, int n, int rank, int T_rows, int split) {
     using C = ShrinkCfg<T, RB, WM, TRANS>;
     constexpr int E = C::E, RP = C::RP, BM = C::BM, WK = C::WK, NCH = C::NCH, KC = C::KC, NS = C::NS;
     constexpr bool F32 = sizeof(T) == 4;
-    extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ TileRows<C::TILE> tr;
+    const T* __restrict__ x = side.x;
+    const T* __restrict__ w = side.w;
+    const int64_t ldx = side.ldx, K = side.K, k_split = side.k_split;
+    const bool xvec = side.xvec, wvec = side.wvec;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
     const int wm = warp % C::WR, wk = warp / C::WR;
     int from = 0;  // this block's first position of the tile
@@ -459,7 +471,7 @@ __global__ void __launch_bounds__(kThreads, RB <= 4 ? 3 : 1) k_shrink(Plan plan,
     const int adapter = tr.adapter, rows = min(BM, tr.rows - from);
     const int32_t* row_of = tr.row + from;
     const T* wi = w + (int64_t)adapter * rank * K;
-    const int64_t k_begin = blockIdx.y * k_split, k_end = k_begin + k_split < K ? k_begin + k_split : K;
+    const int64_t k_begin = split * k_split, k_end = k_begin + k_split < K ? k_begin + k_split : K;
     const int stages = k_begin < k_end ? (int)((k_end - k_begin + KC - 1) / KC) : 0;
 
     constexpr int XU = NCH * 4, WU = TRANS ? RP / E : NCH * 4, WR = TRANS ? KC : RP;
@@ -604,7 +616,7 @@ __global__ void __launch_bounds__(kThreads, RB <= 4 ? 3 : 1) k_shrink(Plan plan,
     const auto result = [&](int b, int k) { return F32 ? sum[F32 ? b : 0][k] : acc[b][k]; };
     const auto column = [&](int b, int j) { return F32 && TRANS ? RB * (2 * q + j) + b : 8 * b + 2 * q + j; };
     const float s = scale ? __ldg(scale + adapter) : 1.f;
-    float* dst = h + (int64_t)blockIdx.y * T_rows * RP;
+    float* dst = side.h + (int64_t)split * T_rows * RP;
     stage_wait<0>();
     __syncthreads();
     float* red = reinterpret_cast<float*>(smem);  // [WK][BM][RP]
@@ -619,6 +631,30 @@ __global__ void __launch_bounds__(kThreads, RB <= 4 ? 3 : 1) k_shrink(Plan plan,
         for (int k = 0; k < WK; k++) v += red[k * BM * RP + e];
         dst[(int64_t)row_of[e / RP] * RP + e % RP] = s * v;
     }
+}
+
+template <typename T, int RB, int WM>
+__global__ void __launch_bounds__(kThreads, RB <= 4 ? 3 : 1) k_shrink(Plan plan, int tiles, const int32_t* __restrict__ index,
+                                                                      Shrink<T> side, const float* __restrict__ scale, int n,
+                                                                      int rank, int T_rows) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ TileRows<16 * WM> tr;
+    shrink_tile<T, RB, WM, false>(smem, tr, plan, tiles, index, side, scale, n, rank, T_rows, (int)blockIdx.y);
+}
+
+// Both sums of the gradients, dh over grad's columns and h over x's, either of which may have no splits: blocks of
+// one fill the SMs that the other's last wave leaves (two launches: 43 us for 2048 positions of 12800 + 2560 fp32).
+template <typename T, int RB, int WM>
+__global__ void __launch_bounds__(kThreads, RB <= 4 ? 3 : 1)
+    k_shrink_both(Plan plan, int tiles, const int32_t* __restrict__ index, Shrink<T> dh, Shrink<T> h,
+                  const float* __restrict__ scale, int n, int rank, int T_rows) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ TileRows<16 * WM> tr;
+    const int y = (int)blockIdx.y;
+    if (y < dh.splits)
+        shrink_tile<T, RB, WM, true>(smem, tr, plan, tiles, index, dh, scale, n, rank, T_rows, y);
+    else
+        shrink_tile<T, RB, WM, false>(smem, tr, plan, tiles, index, h, scale, n, rank, T_rows, y - dh.splits);
 }
 
 // 4 consecutive ranks of a position's h, summed over the splits.
@@ -1808,14 +1844,30 @@ bool row_units(const T* p, int64_t ld) {  // every row starts on 16 bytes
 }
 
 template <typename T, int RB, int WM, bool TRANS>
-int run_shrink(const Shape& s, const Plan& plan, const int32_t* index, const T* x, int64_t ldx, const T* w,
-               const float* scale, int64_t K, int splits, float* h, bool first, cudaStream_t st) {
-    using C = ShrinkCfg<T, RB, WM, TRANS>;
-    const int64_t k_split = ceil_div(ceil_div(K, splits), C::KC) * C::KC;
-    const bool find = first && !s.planned;
-    return start<k_shrink<T, RB, WM, TRANS>>(dim3((unsigned)(s.tiles * C::PARTS), (unsigned)splits), kThreads, C::SMEM, !find, st,
-                 plan, (int)(find ? FIND : PLANNED), index, x, ldx, w, scale, s.n, s.rank, K, k_split, (int)s.T,
-                 row_units(x, ldx), row_units(w, TRANS ? s.rank : K), h);
+Shrink<T> shrink_of(const Shape& s, const T* x, int64_t ldx, const T* w, int64_t K, int splits, float* h) {
+    constexpr int KC = ShrinkCfg<T, RB, WM, TRANS>::KC;
+    return Shrink<T>{x, ldx, w, K, splits ? ceil_div(ceil_div(K, splits), KC) * KC : 0, splits, row_units(x, ldx),
+                     row_units(w, TRANS ? s.rank : K), h};
+}
+
+// The first launch after the plan; without one its blocks find their tiles, and it waits for no launch before it.
+template <typename T, int RB, int WM>
+int run_shrink(const Shape& s, const Plan& plan, const int32_t* index, const Shrink<T>& h, const float* scale,
+               cudaStream_t st) {
+    using C = ShrinkCfg<T, RB, WM, false>;
+    return start<k_shrink<T, RB, WM>>(dim3((unsigned)(s.tiles * C::PARTS), (unsigned)h.splits), kThreads, C::SMEM,
+                                      s.planned, st, plan, (int)(s.planned ? PLANNED : FIND), index, h, scale, s.n, s.rank,
+                                      (int)s.T);
+}
+template <typename T, int RB, int WM>
+int run_shrink_both(const Shape& s, const Plan& plan, const int32_t* index, const Shrink<T>& dh, const Shrink<T>& h,
+                    const float* scale, cudaStream_t st) {
+    using C = ShrinkCfg<T, RB, WM, false>;
+    using B = ShrinkCfg<T, RB, WM, true>;
+    constexpr int smem = C::SMEM > B::SMEM ? C::SMEM : B::SMEM;
+    return start<k_shrink_both<T, RB, WM>>(dim3((unsigned)(s.tiles * C::PARTS), (unsigned)(dh.splits + h.splits)), kThreads,
+                                           smem, s.planned, st, plan, (int)(s.planned ? PLANNED : FIND), index, dh, h,
+                                           scale, s.n, s.rank, (int)s.T);
 }
 
 int run_sum(const Shape& s, float* h, int h_splits, float* dh, int dh_splits, cudaStream_t st) {
@@ -1898,8 +1950,9 @@ int forward(const Shape& s, const Layout& l, const Args& g) {
     float* h = reinterpret_cast<float*>(g.ws + l.h);
     int e = run_plan(s, g.index, plan, g.st);
     if (!e)
-        e = run_shrink<T, RB, WM, false>(s, plan, g.index, (const T*)g.x, g.ldx, (const T*)g.a, g.scale, s.K,
-                                         s.splits_k, h, true, g.st);
+        e = run_shrink<T, RB, WM>(
+            s, plan, g.index, shrink_of<T, RB, WM, false>(s, (const T*)g.x, g.ldx, (const T*)g.a, s.K, s.splits_k, h),
+            g.scale, g.st);
     if (!e)
         e = run_expand<T, RB, WM, false>(s, plan, h, s.splits_k, (const T*)g.b, s.N, (const T*)g.base, g.ldbase,
                                          (T*)g.out, g.ldout, g.st);
@@ -1911,13 +1964,14 @@ int backward(const Shape& s, const Layout& l, const Args& g) {
     const Plan plan = plan_at(g.ws, s, l);
     float *h = reinterpret_cast<float*>(g.ws + l.h), *dh = reinterpret_cast<float*>(g.ws + l.dh);
     const bool inner = g.dx || g.da;
+    if (!inner && !g.db) return ENGRAM_OK;
     int e = run_plan(s, g.index, plan, g.st);
-    if (!e && inner)
-        e = run_shrink<T, RB, WM, true>(s, plan, g.index, (const T*)g.grad, g.ldgrad, (const T*)g.b, g.scale, s.N,
-                                        s.splits_n, dh, true, g.st);
-    if (!e && g.db)
-        e = run_shrink<T, RB, WM, false>(s, plan, g.index, (const T*)g.x, g.ldx, (const T*)g.a, g.scale, s.K,
-                                         s.splits_k, h, !inner, g.st);
+    if (!e)
+        e = run_shrink_both<T, RB, WM>(
+            s, plan, g.index,
+            shrink_of<T, RB, WM, true>(s, (const T*)g.grad, g.ldgrad, (const T*)g.b, s.N, inner ? s.splits_n : 0, dh),
+            shrink_of<T, RB, WM, false>(s, (const T*)g.x, g.ldx, (const T*)g.a, s.K, g.db ? s.splits_k : 0, h), g.scale,
+            g.st);
     if (!e) e = run_sum(s, h, g.db ? s.splits_k : 1, dh, inner ? s.splits_n : 1, g.st);
     if (!e && g.dx)
         e = run_expand<T, RB, WM, true>(s, plan, dh, 1, (const T*)g.a, s.K, (const T*)g.base, g.ldbase, (T*)g.dx,
