@@ -76,14 +76,23 @@ __global__ void __launch_bounds__(kPlanThreads) k_plan(const int32_t* __restrict
     for (int i = tid; i < 2 * (n + 1); i += kPlanThreads) sm[i] = 0;
     if (tid < 2) carry[tid] = 0;
     __syncthreads();
-    for (int t0 = 0; t0 < T; t0 += kPlanThreads) {
-        const int t = t0 + tid;
-        const int a = t < T ? clamp_adapter(__ldg(index + t), n) : -1;
-        const uint32_t same = __match_any_sync(0xffffffffu, a);
-        const uint32_t before = __ballot_sync(0xffffffffu, t < c0) & same;
-        if (a >= 0 && lane == __ffs(same) - 1) {
-            atomicAdd(cnt + a, __popc(same));
-            if (before) atomicAdd(pre + a, __popc(before));
+    // a warp whose positions share an adapter (packed prompts) adds once, another lane by lane
+    constexpr int N = 4;  // loads under way a thread
+    for (int t0 = 0; t0 < T; t0 += N * kPlanThreads) {
+        int a[N];
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            const int t = t0 + j * kPlanThreads + tid;
+            a[j] = t < T ? clamp_adapter(__ldg(index + t), n) : -1;
+        }
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            const bool before = t0 + j * kPlanThreads < c0;  // chunks are whole multiples of kPlanThreads
+            const bool one = __all_sync(0xffffffffu, a[j] == __shfl_sync(0xffffffffu, a[j], 0));
+            if (a[j] >= 0 && (!one || lane == 0)) {
+                atomicAdd(cnt + a[j], one ? 32 : 1);
+                if (before) atomicAdd(pre + a[j], one ? 32 : 1);
+            }
         }
     }
     __syncthreads();
