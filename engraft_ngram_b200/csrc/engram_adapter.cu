@@ -38,8 +38,11 @@ namespace {
 
 constexpr int kThreads = 256, kWarps = 8;
 constexpr int kPlanThreads = 1024;
-constexpr int kScanMax = 1024;       // positions and
-constexpr int kScanAdapters = 2048;  // adapters up to which a block finds its tile by itself
+// Positions and adapters up to which a block finds its tile by itself.  Against k_plan, 12800 columns of fp32 at
+// rank 16: 64 positions of 16 adapters 15 and 19 us, 1024 of 16 45 and 52, 1024 of 1000 202 and 203.  The
+// gradients look through the positions once more, in each block of k_weight: 77 positions of 4 adapters 26.3 and
+// 26.6 us (bf16 18 and 21), but 128 of 16 57 and 47 (bf16 28 and 31), 256 of 64 188 and 134, 1024 of 16 103 and 81.
+constexpr int kScanMax = 1024, kScanMaxGradients = 128, kScanAdapters = 2048;
 constexpr int kMaxAdapters = 16384;  // k_plan counts them in shared memory
 constexpr int kMaxRank = 128;
 
@@ -1045,7 +1048,7 @@ struct WideCfg {
     static constexpr int FETCH = 16 * 4096;  // a stage of all sixteen warps
     static constexpr int FIT = (220 * 1024 - 2 * H_BYTES - NS * STAGE) / FETCH, DEPTH = FIT > 2 ? 2 : FIT;
     static constexpr int SMEM = 2 * H_BYTES + NS * STAGE + DEPTH * FETCH + 1024;
-    static constexpr bool OK = DEPTH >= 1;
+    static constexpr bool OK = RB >= 4 && DEPTH >= 1;  // ranks over 16: run_expand's rule
     static constexpr uint32_t SWIZZLE = SPAN == 128 ? 2 : SPAN == 64 ? 4 : 6;
 };
 
@@ -1755,14 +1758,17 @@ int check_shape(int64_t T, int32_t n, int32_t rank, int64_t K, int64_t N) {
 
 constexpr int kSms = 148;
 
-Shape shape_of(int64_t T, int n, int rank, int64_t K, int64_t N) {
+Shape shape_of(int64_t T, int n, int rank, int64_t K, int64_t N, bool backward) {
     Shape s;
     s.T = T, s.K = K, s.N = N, s.n = n, s.rank = rank;
     s.rb = rank_blocks(rank);
     const int64_t groups = T < (int64_t)n + 1 ? T : (int64_t)n + 1;
-    s.wm = groups > 0 && T / groups >= 32 ? 8 : 1;
+    // Tiles of 128 positions from 96 an adapter on, else of 16.  16 against 128, 12800 columns at rank 16: 64 an adapter
+    // 68 and 76 us (2048 positions, fp32; their gradients 132 and 136), 64 and 75 (4096, bf16); 122 an adapter 44.5
+    // and 45.0; 128 an adapter 117 and 108 (4096, fp32), 65 and 61 (bf16); 256 an adapter 112 and 100, 62 and 60.
+    s.wm = groups > 0 && T / groups >= 96 ? 8 : 1;
     const int bm = 16 * s.wm;
-    s.planned = T > kScanMax || n > kScanAdapters;
+    s.planned = T > (backward ? kScanMaxGradients : kScanMax) || n > kScanAdapters;
     s.tiles = (T + (bm - 1) * groups) / bm;  // as many as there can be
     // Blocks that share a sum: about two an SM.  For 2, 3, 4 and 6 an SM: gradients of 8192 positions (rank 32, bf16)
     // 193, 197, 197 and 198 us, of 2048 (rank 16, fp32) 86, 88, 87 and 92, 16384 positions (rank 64, bf16) 237, 237,
@@ -1917,8 +1923,13 @@ template <typename T, int RB, int WM, bool TRANS>
 int run_expand(const Shape& s, const Plan& plan, const float* h, int splits, const T* w, int64_t F, const T* base,
                int64_t ldb, T* out, int64_t ldo, cudaStream_t st) {
     using C = ExpandCfg<T, RB, WM == 8, TRANS>;
+    // The tcgen05 kernel, where ranks over 16 and enough work pay for its start.  k_expand against it, the whole call
+    // at 12800 columns: rank 16 never (16384 positions 187 and 198 us in bf16, 352 and 371 in fp32); rank 32 in bf16
+    // 88 and 88 at 4096 positions, 154 and 125 at 8192, in fp32 211 and 220 at 8192, 407 and 384 at 16384; rank 64 in
+    // bf16 87 and 94 at 2048, 136 and 126 at 4096, 380 and 238 at 16384, in fp32 148 and 154, 250 and 219, 784 and
+    // 624; rank 128 in bf16 186 and 147 at 2048, 383 and 215 at 8192.
     if constexpr (WM == 8 && !TRANS && WideCfg<T, RB>::OK) {
-        if (s.planned && s.n > 0 && F % WideCfg<T, RB>::GROUP == 0 && s.n * F / WideCfg<T, RB>::GROUP < (1ll << 31) &&
+        if (s.T * F >= (3ll << 30) / (8 * RB) && s.planned && s.n > 0 && F % WideCfg<T, RB>::GROUP == 0 && s.n * F / WideCfg<T, RB>::GROUP < (1ll << 31) &&
             (!base || row_units(base, ldb)) && row_units((const T*)out, ldo) && row_units(w, s.rank))
             return run_expand_wide<T, RB>(s, plan, h, splits, w, F, base, ldb, out, ldo, st);
     }
@@ -2033,7 +2044,7 @@ extern "C" int64_t engram_adapter_workspace_bytes(int64_t T, int32_t n_adapters,
                                                   int32_t backward) {
     const int e = check_shape(T, n_adapters, rank, K, N);
     if (e) return e;
-    return layout_of(shape_of(T, n_adapters, rank, K, N), backward != 0).bytes;
+    return layout_of(shape_of(T, n_adapters, rank, K, N, backward != 0), backward != 0).bytes;
 }
 
 extern "C" int engram_adapter_forward(int32_t dtype, const void* x, int64_t ldx, const void* a, const void* b,
@@ -2049,7 +2060,7 @@ extern "C" int engram_adapter_forward(int32_t dtype, const void* x, int64_t ldx,
     if (ldx < K || ldout < N || (base && ldbase < N) || (base == out && ldbase != ldout)) return ENGRAM_ERR_ARG;
     for (const void* p : {x, a, b, base, (const void*)out})
         if (!aligned_to(p, dtype)) return ENGRAM_ERR_ARG;
-    const Shape s = shape_of(T, n_adapters, rank, K, N);
+    const Shape s = shape_of(T, n_adapters, rank, K, N, false);
     const Layout l = layout_of(s, false);
     if (workspace_bytes < l.bytes) return ENGRAM_ERR_WORKSPACE;
     Args g = {};
@@ -2081,7 +2092,7 @@ extern "C" int engram_adapter_backward(int32_t dtype, const void* grad, int64_t 
         return ENGRAM_ERR_ARG;
     for (const void* p : {grad, x, a, b, dx_base, (const void*)dx, (const void*)da, (const void*)db})
         if (!aligned_to(p, dtype)) return ENGRAM_ERR_ARG;
-    const Shape s = shape_of(T, n_adapters, rank, K, N);
+    const Shape s = shape_of(T, n_adapters, rank, K, N, true);
     const Layout l = layout_of(s, true);
     if (workspace_bytes < l.bytes) return ENGRAM_ERR_WORKSPACE;
     Args g = {};

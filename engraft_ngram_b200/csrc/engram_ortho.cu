@@ -300,15 +300,33 @@ __device__ __forceinline__ void small_product(const double* x, const double* y, 
     __syncthreads();
 }
 
-// The steps on the small matrices: pmat[s] = P / max(|U|, eps).
+// The chunks' sums, in their order, into the first chunk's: an element a thread, where one block a matrix would wait
+// for too many of them.
+__global__ void __launch_bounds__(kSmallThreads) k_small_sum(double* part, int chunks, int size, int64_t total) {
+    wait_for_previous();
+    let_next_start();
+    const int64_t i = blockIdx.x * (int64_t)kSmallThreads + threadIdx.x;
+    if (i >= total) return;
+    double* p = part + i / size * chunks * size + i % size;
+    double v = 0.0;
+#pragma unroll 16
+    for (int c = 0; c < chunks; c++) v += p[(int64_t)c * size];
+    *p = v;
+}
+
+// The steps on the small matrices: pmat[s] = P / max(|U|, eps).  A matrix has `stride` chunks, of which the first
+// `chunks` are summed here.  Twenty products one after the other, on one block: 45 us of the 63 that a 64 x 2560 fp32
+// matrix takes.  Sides over 16 have blocks enough for sixteen warps (eight: 74 us).
 template <int MB>
-__global__ void __launch_bounds__(kSmallThreads) k_small_poly(const double* part, int chunks, int m,
+constexpr int kPolyThreads = MB >= 4 ? 512 : 256;
+template <int MB>
+__global__ void __launch_bounds__(kPolyThreads<MB>) k_small_poly(const double* part, int chunks, int stride, int m,
                                                               Poly poly, double eps, double* __restrict__ pmat) {
     constexpr int RM = 8 * MB, S = RM + 4;
     extern __shared__ double sd[];
     double *A = sd, *B = A + RM * S, *P = B + RM * S, *Q = P + RM * S;
     __shared__ double inv_norm;
-    const double* src = part + (int64_t)blockIdx.x * chunks * RM * RM;
+    const double* src = part + (int64_t)blockIdx.x * stride * RM * RM;
     wait_for_previous();
     let_next_start();
     for (int e = threadIdx.x; e < RM * RM; e += blockDim.x) {
@@ -1131,6 +1149,11 @@ Layout layout_of(const Shape& s, int terms) {
     return l;
 }
 
+// Elements of a matrix's chunks above which k_small_sum adds them.  In k_small_poly and in a launch of its own, fp32:
+// 16 x 2560 (5120 elements) 11.4 and 12.4 us, 40 of 16 x 12800 (3840) 39 and 45, 8 x 12800 (6400) 12.9 and 12.7; 40 of
+// 32 x 12800 (15360) 129 and 108, 64 x 2560 (163840) 99 and 74, 64 x 12800 (819200) 239 and 96.
+constexpr int kSumElements = 8192;
+
 template <int MB, bool TALL, typename Io>
 int run_small(const Shape& s, const Layout& l, const Io& io, const Poly& poly, double eps, uint8_t* ws,
               cudaStream_t st) {
@@ -1142,9 +1165,14 @@ int run_small(const Shape& s, const Layout& l, const Io& io, const Poly& poly, d
     constexpr int RM = 8 * MB, SP = RM + 4;
     int e = start<k_small_gram<MB, TALL, Io>>(grid, kSmallThreads, 0, false, st, io, (int)s.side, s.length, chunk, vec,
                                               part);
+    const bool sum = chunks * RM * RM > kSumElements;
+    const int64_t total = s.stack * RM * RM;
+    if (!e && sum)
+        e = start<k_small_sum>(dim3((unsigned)ceil_div(total, kSmallThreads)), kSmallThreads, 0, true, st, part, (int)chunks,
+                               RM * RM, total);
     if (!e)
-        e = start<k_small_poly<MB>>(dim3((unsigned)s.stack), kSmallThreads, 4 * RM * SP * 8, true, st,
-                                    part, (int)chunks, (int)s.side, poly, eps, pmat);
+        e = start<k_small_poly<MB>>(dim3((unsigned)s.stack), kPolyThreads<MB>, 4 * RM * SP * 8, true, st, part,
+                                    sum ? 1 : (int)chunks, (int)chunks, (int)s.side, poly, eps, pmat);
     if (!e)
         e = start<k_small_apply<MB, TALL, Io>>(grid, kSmallThreads, RM * SP * 8 + S::SIZE * 4, true, st, io, (int)s.side,
                                                s.length, chunk, vec, pmat);

@@ -98,8 +98,7 @@ def test_forward_and_gradients_match_the_formula(case):
         grad, c["x"], c["a"], c["b"], c["index"], c["scale"])))
 
 
-# many positions and rows on 16 bytes: the tensor-memory kernel, at each of its operand layouts (rows of 32, 64,
-# 128 and more bytes of the rank), ranks that end inside one, widths that end inside a stage and inside 128 bytes
+# many positions and rows on 16 bytes, ranks that end inside 16, widths that end inside a stage and inside 128 bytes
 WIDE = [(1500, 96, 264, 16, 3, F32, "random"), (1300, 64, 520, 12, 2, F32, "segments"), (1200, 128, 100, 32, 4, F32, "random"),
         (1100, 64, 1300, 64, 3, F32, "random"), (1400, 72, 264, 128, 2, F32, "random"),
         (1500, 128, 264, 16, 3, BF16, "random"), (1300, 64, 520, 8, 2, BF16, "segments"), (1200, 136, 104, 32, 4, BF16, "random"),
@@ -120,6 +119,24 @@ def test_many_positions(case):
     assert torch.equal(wide[:, 8:8 + case[2]], want) and (wide[:, :8] == 7).all() and (wide[:, 8 + case[2]:] == 7).all()
     zeros = {**c, "base": torch.zeros_like(c["base"])}
     assert torch.equal(eb.adapter_add(None, *list(c.values())[1:]), eb.adapter_add(**zeros))
+
+
+# as much work as the tensor-memory kernel takes, at each of its operand layouts (rows of 64, 128 and more bytes of the
+# rank), ranks that end inside one and widths that end inside a stage
+HUGE = [(96003, 40, 1072, 24, 3, F32, "random"), (50001, 40, 1040, 40, 2, F32, "segments"), (100001, 64, 1056, 32, 5, BF16, "random"),
+        (50007, 64, 1056, 48, 3, F16, "segments"), (26001, 72, 1056, 128, 9, BF16, "random"), (26001, 72, 1056, 104, 2, F16, "segments"),
+        (100001, 64, 1056, 24, 1, F16, "0"), (50001, 40, 1056, 64, 4, BF16, "outside")]
+
+
+@pytest.mark.parametrize("case", HUGE, ids=str)
+def test_much_work(case):
+    test_many_positions(case)
+    c, _ = make(*case)
+    c["x"][::5] *= 100 if case[5] == F16 else 1e4
+    c["x"][1::5] /= 100 if case[5] == F16 else 1e4
+    if case[5] == F16:
+        c["b"] /= 64  # keeps the results inside the type
+    check(eb.adapter_add(**c), formula(c, _)[0], formula(c, _, mag=True)[0], case[1] + case[3], case[5])
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=str)
