@@ -1017,7 +1017,8 @@ __global__ void __launch_bounds__(kThreads, RB * (int)sizeof(T) <= 8 ? 3 : RB * 
 }
 
 // ---- expand on the tcgen05 tensor cores -------------------------------------------
-// The same product, TRANS = false, for many positions, rows of base and out that start on 16 bytes and whole
+// The same product, TRANS = false, for much work at ranks over 16 (run_expand's rule), rows of base and out that start on
+// 16 bytes and whole
 // groups of 32 columns (fp32: 16).  What the kernel above spends its time on is instructions, 400 to 500 a
 // 32 x 32 piece; here the products and the factors' way to them cost the streaming warps nothing:
 //   warps 0-15  out = base + accumulator, 16 positions x 256 bytes a warp and stage, eight warps a stage in
