@@ -1365,8 +1365,9 @@ int check_shape(int64_t stack, int64_t rows, int64_t cols, Shape* s) {
 
 // The iterates have to stay within what the planes hold: from singular values in [0, 1] on, each step's
 // G, polynomial and result below 15.  `top` is the largest singular value that a step can meet, found on a
-// grid over all that the step before can leave.
-int check_poly(int32_t steps, const double* c, double eps, Poly* poly) {
+// grid over all that the step before can leave.  apart: c0 X is added beside the product (one term of longer
+// sides), so the plane holds the polynomial without c0, which may be the larger one.
+int check_poly(int32_t steps, const double* c, double eps, bool apart, Poly* poly) {
     if (steps < 1 || !c || !(eps > 0.0)) return ENGRAM_ERR_ARG;
     if (steps > kMaxSteps) return ENGRAM_ERR_RANGE;
     poly->steps = steps;
@@ -1378,9 +1379,10 @@ int check_poly(int32_t steps, const double* c, double eps, Poly* poly) {
         double f_most = 0.0, x_most = 0.0;
         bool number = true;
         for (int p = 0; p <= kPoints; p++) {
-            const double x = top * p / kPoints, g = x * x, f = fabs(c0 + g * (c1 + g * c2)), y = x * f;
-            number = number && f < 1e30;
-            f_most = f > f_most ? f : f_most;
+            const double x = top * p / kPoints, g = x * x, rest = g * (c1 + g * c2), f = fabs(c0 + rest), y = x * f;
+            const double held = apart && fabs(rest) > f ? fabs(rest) : f;
+            number = number && held < 1e30;
+            f_most = held > f_most ? held : f_most;
             x_most = y > x_most ? y : x_most;
         }
         if (!number || !(top * top < 15.0) || !(f_most < 15.0) || !(x_most < 3.8)) return ENGRAM_ERR_RANGE;
@@ -1413,7 +1415,7 @@ extern "C" int engram_orthogonalize(int32_t dtype, const void* x, int64_t stack,
     int e = check_shape(stack, rows, cols, &s);
     if (e) return e;
     Poly poly;
-    e = check_poly(steps, coefficients, eps, &poly);
+    e = check_poly(steps, coefficients, eps, terms_of(dtype) == 1 && s.side > kSmallSide, &poly);
     if (e) return e;
     if (stack == 0) return ENGRAM_OK;
     if (!x || !out || !aligned_to(x, dtype) || !aligned_to(out, dtype) || !workspace || !aligned16(workspace))
@@ -1441,7 +1443,7 @@ extern "C" int engram_muon_step(int32_t grad_dtype, const float* p, const void* 
     int e = check_shape(stack, rows, cols, &s);
     if (e) return e;
     Poly poly;
-    e = check_poly(steps, coefficients, eps, &poly);
+    e = check_poly(steps, coefficients, eps, false, &poly);
     if (e) return e;
     if (stack == 0) return ENGRAM_OK;
     if (!grad || !aligned_to(grad, grad_dtype) || !workspace || !aligned16(workspace)) return ENGRAM_ERR_ARG;

@@ -714,7 +714,9 @@ ENGRAM_API int engram_adapter_backward(int32_t dtype, const void* grad, int64_t 
  * from the right) and (c0, c1, c2) = coefficients[3 s ..] of step s (HOST
  * doubles [steps, 3], 1 <= steps <= 32).  out (may be x) gets X.  A zero matrix
  * stays zero.  Coefficients under which a singular value of the iterates could
- * leave (-3.8, 3.8), or the polynomial (-15, 15), are ENGRAM_ERR_RANGE.
+ * leave (-3.8, 3.8), or the polynomial (-15, 15), are ENGRAM_ERR_RANGE; for bf16
+ * matrices whose shorter side is over 64 so are those under which the polynomial
+ * without c0 could.
  * Shorter sides up to 64 are summed in fp64; longer ones in products of split
  * fp16 operands with fp32 accumulation (fp32-level results; for bf16 one
  * unsplit product, within 2^-8 of the largest entries).  Shorter side <= 32768,

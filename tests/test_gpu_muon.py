@@ -276,3 +276,29 @@ def test_inference_mode_and_overlapping_arrays():
 def test_refusals(bad):
     with pytest.raises(ValueError):
         bad(make(2, 6, 9, "noise"))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=str)
+@pytest.mark.parametrize("c", [(12.0, -25.0, 13.5), (2.0, -14.0, 13.0)], ids=str)
+def test_polynomials_near_the_limit_on_matrices_along_the_axes(c, dtype):
+    """Entries of the polynomial reach its largest value, with c0 and without, where the singular vectors are axes.
+
+    One entry a row and column, so no sums: each entry's result is s (c0 + c1 g + c2 g g), g = s s, off by the rounding
+    of six operands at most (2^-22 each, in bf16 2^-12 beside an exact c0 s), of fp32's products and of its own type."""
+    x = torch.zeros(3, 100, 130, device=DEV)
+    x[0, 3, 5] = 2.0
+    x[1].fill_diagonal_(0.25)
+    x[2, 7, 0], x[2, 8, 1] = 1.0, -0.3
+    x = x.to(dtype)
+    s = x.double()
+    s = s / s.square().sum((1, 2), keepdim=True).sqrt()
+    g = s * s
+    want = s * (c[0] + c[1] * g + c[2] * g * g)
+    apart = s.abs() * (abs(c[1]) * g + abs(c[2]) * g * g)
+    bound = 12 * 2.0 ** -22 * (c[0] * s.abs() + apart) + torch.finfo(dtype).eps / 2 * want.abs()
+    if dtype == BF16:
+        bound += 6 * 2.0 ** -12 * apart
+    got = eb.orthogonalize(x, steps=1, coefficients=c)
+    assert ((got.double() - want).abs() <= bound).all()
+    with pytest.raises(ValueError):
+        eb.orthogonalize(x.to(BF16), steps=1, coefficients=(14.0, -40.0, 23.0))

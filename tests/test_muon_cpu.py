@@ -95,3 +95,18 @@ def test_python_calls_refuse():
         eb.Muon([torch.nn.Parameter(torch.zeros(5))])
     with pytest.raises(ValueError, match="hyper-parameters"):
         eb.Muon([torch.nn.Parameter(torch.zeros(5, 5))], momentum=1.0)
+
+
+# |c1 g + c2 g g| reaches 17 and 19.3 while the polynomial with c0 stays below 15: more than bf16's plane of longer sides
+# holds, which has no c0
+@pytest.mark.parametrize("triple", [(14.0, -40.0, 23.0), (14.9, -57.0, 42.0)])
+def test_bf16_of_longer_sides_refuses_a_polynomial_that_leaves_the_range_without_c0(lib, triple):
+    c = coefficients(*triple, steps=1)
+    grid = torch.linspace(0, 1, 1001, dtype=torch.float64)
+    rest = triple[1] * grid + triple[2] * grid ** 2
+    assert rest.abs().max() > 65504 / 4096 and (triple[0] + rest).abs().max() < 15
+    assert ortho(lib, dtype=1, rows=100, cols=100, steps=1, c=c) == L.ERR_RANGE
+    assert ortho(lib, dtype=1, rows=300, cols=65, steps=1, c=c) == L.ERR_RANGE
+    for dtype, rows in ((0, 100), (2, 100), (1, 64)):  # c0 on the diagonal, or sums in fp64: taken (and then no room)
+        assert ortho(lib, dtype=dtype, rows=rows, cols=100, steps=1, c=c, ws_bytes=16) == L.ERR_WORKSPACE
+    assert muon(lib, dtype=1, rows=100, cols=100, steps=1, c=c, ws_bytes=16) == L.ERR_WORKSPACE
