@@ -121,7 +121,7 @@ def forward_into(out, base, x, a, b, index, scale) -> torch.Tensor:
 
 def backward_into(grad, x, a, b, index, scale, dx=None, dx_base=None, da=None, db=None) -> None:
     """The gradients wanted (dx, da, db given) of the adapters' product; dx = dx_base (None: zeros) + its own
-    part, and dx_base may be dx."""
+    part, and dx_base may be dx.  Otherwise no output may overlap another one or an input."""
     code, T, K, N, rank, n, ws_bytes = _check(x, a, b, index, scale, 1)
     dev = x.device
     ldx, ldg = _rows(x, "x", T, K, x), _rows(grad, "grad", T, N, x)

@@ -2093,6 +2093,13 @@ extern "C" int engram_adapter_backward(int32_t dtype, const void* grad, int64_t 
         return ENGRAM_ERR_ARG;
     for (const void* p : {grad, x, a, b, dx_base, (const void*)dx, (const void*)da, (const void*)db})
         if (!aligned_to(p, dtype)) return ENGRAM_ERR_ARG;
+    // dx is written before da's sum reads x and db's reads grad, and those are written while other blocks read
+    if (n_adapters > 0) {
+        if (dx && ((da && dx == x) || (db && dx == grad) || dx == da || dx == db)) return ENGRAM_ERR_ARG;
+        for (const void* p : {(const void*)da, (const void*)db})
+            if (p && (p == x || p == grad)) return ENGRAM_ERR_ARG;
+        if (da && da == db) return ENGRAM_ERR_ARG;
+    }
     const Shape s = shape_of(T, n_adapters, rank, K, N, true);
     const Layout l = layout_of(s, true);
     if (workspace_bytes < l.bytes) return ENGRAM_ERR_WORKSPACE;

@@ -697,7 +697,10 @@ ENGRAM_API int engram_adapter_forward(int32_t dtype, const void* x, int64_t ldx,
  * dx [T, K] (row stride lddx), da and db (contiguous, as a and b) are each
  * nullable: not wanted.  Every row of dx is written (dx_base's, or zero, where
  * there is no adapter) and all of da and db (zero for an adapter no position
- * uses).  workspace: ..._workspace_bytes(..., backward = 1).
+ * uses).  The outputs must not overlap one another or an input, but for dx_base:
+ * dx that is x where da is wanted, or grad where db is, da or db that is x or
+ * grad, and two outputs that are one are ENGRAM_ERR_ARG.
+ * workspace: ..._workspace_bytes(..., backward = 1).
  */
 ENGRAM_API int engram_adapter_backward(int32_t dtype, const void* grad, int64_t ldgrad, const void* x, int64_t ldx,
                                        const void* a, const void* b, const int32_t* index, const float* scale,

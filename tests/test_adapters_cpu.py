@@ -89,3 +89,13 @@ def test_row_strides(stride, T, ok):
     else:
         with pytest.raises(ValueError, match="strides"):
             AD._rows(v, "v", T, 8, like)
+
+
+# the workspace is too small: what is accepted ends with ERR_WORKSPACE, before any launch
+@pytest.mark.parametrize("alias, refused", [
+    (dict(dx=X), True), (dict(dx=BASE, lddx=64, ldg=64, N=64), True), (dict(da=X), True), (dict(db=X), True),
+    (dict(da=BASE), True), (dict(db=BASE), True), (dict(dx=OUT, da=OUT), True), (dict(dx=OUT, db=OUT), True),
+    (dict(da=B + 64, db=B + 64), True), (dict(dx=X, da=None), False), (dict(dx=BASE, ldg=64, N=64, db=None), False),
+    (dict(dx_base=OUT, lddb=64), False), (dict(), False)])
+def test_backward_refuses_outputs_that_destroy_what_it_still_reads(lib, alias, refused):
+    assert backward(lib, ws_bytes=64, **alias) == (L.ERR_ARG if refused else L.ERR_WORKSPACE)
