@@ -134,11 +134,19 @@ def backward_into(grad, x, a, b, index, scale, dx=None, dx_base=None, da=None, d
     L.check(st, "engram_adapter_backward")
 
 
+def refuse_scale_gradient(scale) -> None:
+    """No gradient of scale is built: an error where one would be lost."""
+    if scale is not None and scale.requires_grad and torch.is_grad_enabled():
+        raise ValueError("scale requires grad, but adapters have no gradient of it: pass scale.detach(), or train it "
+                         "inside b")
+
+
 def adapter_gradients(grad: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, index: torch.Tensor,
                       scale: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(dx, da, db): the gradients of x, a and b from grad [T, N], the gradient
     of adapter_add's result (base's own gradient is grad itself).  A position
-    without an adapter gets dx = 0, an adapter that no position uses da = db = 0."""
+    without an adapter gets dx = 0, an adapter that no position uses da = db = 0.
+    The results carry no graph, whatever the inputs require."""
     grad, x, a, b = grad.detach(), x.detach(), a.detach(), b.detach()
     dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     da = torch.empty_like(a, memory_format=torch.contiguous_format)
@@ -174,9 +182,11 @@ def adapter_add(base: torch.Tensor | None, x: torch.Tensor, a: torch.Tensor, b: 
     x [T, K] and base: row-strided views are taken as they are; a [n, rank, K]
     and b [n, N, rank]: contiguous, ranks up to 128; index: int32 [T], outside
     [0, n) for a position without an adapter (its row is base's); scale:
-    float32 [n], not differentiable, or None (1).  out: where to write (base
-    itself adds in place); only for calls that need no gradients, and it must
-    not overlap x, a or b, nor base in any other way."""
+    float32 [n], not differentiable (refused where it requires grad), or None
+    (1).  out: where to write (base itself adds in place); only for calls that
+    need no gradients, and it must not overlap x, a or b, nor base in any other
+    way."""
+    refuse_scale_gradient(scale)
     if torch.is_grad_enabled() and (x.requires_grad or a.requires_grad or b.requires_grad
                                     or (base is not None and base.requires_grad)):
         if out is not None:

@@ -41,7 +41,7 @@ import ctypes as C
 import torch
 
 from . import _lib as L
-from .adapters import PleAdapters, backward_into, forward_into
+from .adapters import PleAdapters, backward_into, forward_into, refuse_scale_gradient
 
 _GRAD_FIELDS = ("w_key", "w_value", "norm_key", "norm_query", "norm_conv", "conv1d")
 PROJECTION = "3xtf32"  # or "fp32", "tcgen05"
@@ -292,6 +292,8 @@ def ple_forward(emb: torch.Tensor, hidden: torch.Tensor, w, hist: torch.Tensor, 
     if weights_need_grad(w):
         raise NotImplementedError("engraft_ngram_b200.ple_forward does not build gradients of the block's weights; "
                                   "install_ple routes such calls to the reference's ple_forward")
+    if adapters is not None:
+        refuse_scale_gradient(adapters.scale)
     hc, n = int(hparams.hc_mult), int(hparams.n_embd)
     eps, dil = float(hparams.f_norm_rms_eps), int(hparams.ple_ngram_size)
     T = emb.shape[0]

@@ -1,6 +1,8 @@
 """The adapter entry points without a GPU: what the C ABI and the Python calls refuse, and with which error."""
 from __future__ import annotations
 
+import types
+
 import pytest
 import torch
 
@@ -99,3 +101,26 @@ def test_row_strides(stride, T, ok):
     (dict(dx_base=OUT, lddb=64), False), (dict(), False)])
 def test_backward_refuses_outputs_that_destroy_what_it_still_reads(lib, alias, refused):
     assert backward(lib, ws_bytes=64, **alias) == (L.ERR_ARG if refused else L.ERR_WORKSPACE)
+
+
+def test_a_scale_that_requires_grad_is_refused_where_its_gradient_would_be_lost():
+    x, a, b = torch.zeros(5, 8), torch.zeros(2, 3, 8), torch.zeros(2, 6, 3)
+    index, scale = torch.zeros(5, dtype=torch.int32), torch.ones(2, requires_grad=True)
+    for leaf in (x, x.clone().requires_grad_()):
+        with pytest.raises(ValueError, match="scale requires grad"):
+            eb.adapter_add(None, leaf, a, b, index, scale)
+    with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):  # nothing is lost: on to the other checks
+        eb.adapter_add(None, x, a, b, index, scale)
+    with pytest.raises(ValueError, match="CUDA"):
+        eb.adapter_add(None, x, a, b, index, scale.detach())
+
+
+def test_ple_forward_refuses_a_scale_that_requires_grad():
+    n, hc = 8, 2
+    w = types.SimpleNamespace(w_key=torch.zeros(hc * n, n), w_value=torch.zeros(n, n), norm_key=torch.zeros(hc, n),
+                              norm_query=torch.zeros(hc, n), norm_conv=torch.zeros(hc, n), conv1d=torch.zeros(hc * n, 4))
+    hp = types.SimpleNamespace(hc_mult=hc, n_embd=n, f_norm_rms_eps=1e-6, ple_ngram_size=3)
+    ad = eb.PleAdapters(torch.zeros(2, 3, n), torch.zeros(2, hc * n + n, 3), torch.zeros(4, dtype=torch.int32),
+                        torch.ones(2, requires_grad=True))
+    with pytest.raises(ValueError, match="scale requires grad"):
+        eb.ple_forward(torch.zeros(4, n), torch.zeros(4, hc, n), w, torch.zeros(0, hc, n), hp, adapters=ad)
