@@ -39,6 +39,7 @@ import contextlib
 import ctypes as C
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib as L
 from .adapters import PleAdapters, backward_into, forward_into, refuse_scale_gradient
@@ -235,6 +236,7 @@ class _PleBlockFn(torch.autograd.Function):
         return out, new_hist, gate, s
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout, dtail, _dgate, _ds):
         hidden, hist, kv, gate, s, normed, nk, nq, nc, cw, emb, a, b, index, scale = ctx.saved_tensors
         hc, n, K, eps, dil, detach_value, detach_gate = ctx.meta

@@ -419,3 +419,15 @@ def test_ple_block_refuses_adapters_of_other_widths():
         eb.ple_forward(emb, hidden, w, hist, hp, adapters=eb.PleAdapters(ad.a, ad.b[:, :-1], ad.index))
     with pytest.raises(ValueError, match="index"):
         eb.ple_forward(emb, hidden, w, hist, hp, adapters=eb.PleAdapters(ad.a, ad.b, ad.index[:-1]))
+
+
+def test_second_derivatives_of_the_ple_block_are_an_error_and_not_left_out():
+    emb, hidden, w, hist, hp, ad = ple_case()
+    leaves = [v.clone().requires_grad_() for v in (emb, ad.a, ad.b)]
+    for k in (slice(0, 1), slice(1, 3), slice(0, 3)):  # emb alone is the block without adapters' factors
+        use = [v if i in range(3)[k] else v.detach() for i, v in enumerate(leaves)]
+        adapters = None if k == slice(0, 1) else eb.PleAdapters(use[1], use[2], ad.index, ad.scale)
+        out, _ = eb.ple_forward(use[0], hidden, w, hist, hp, adapters=adapters)
+        grads = torch.autograd.grad(out.square().sum(), leaves[k], create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            sum(g.sum() for g in grads).backward()
