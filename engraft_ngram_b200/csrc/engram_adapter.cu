@@ -1486,8 +1486,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 && RB <= 4 ? 3 : 1) k
     float take = 1.f;  // fp16: h's scale
     if constexpr (std::is_same_v<T, __half>) {
         float m = 0.f;
-        for (int e = threadIdx.x; e < count * (RP / 4); e += kThreads) {
-            const float4 v = load_h(h + (int64_t)list[e / (RP / 4)] * RP + 4 * (e % (RP / 4)), 1, 0);
+        for (int64_t e = threadIdx.x; e < (int64_t)count * (RP / 4); e += kThreads) {  // count reaches 2^30
+            const float4 v = load_h(h + (int64_t)list[e / (RP / 4)] * RP + 4 * (int)(e % (RP / 4)), 1, 0);
             m = fmaxf(fmaxf(fmaxf(m, fabsf(v.x)), fmaxf(fabsf(v.y), fabsf(v.z))), fabsf(v.w));
         }
 #pragma unroll

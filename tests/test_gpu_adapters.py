@@ -431,3 +431,26 @@ def test_second_derivatives_of_the_ple_block_are_an_error_and_not_left_out():
         grads = torch.autograd.grad(out.square().sum(), leaves[k], create_graph=True)
         with pytest.raises(RuntimeError, match="once_differentiable"):
             sum(g.sum() for g in grads).backward()
+
+
+def test_scale_of_the_weight_gradients_over_more_positions_than_32_bits_of_elements():
+    """fp16 at rank 65: 2^26 positions of one adapter are 2^31 fours of h, whose largest magnitude sets their scale.
+
+    h is 2^17, beyond fp16 unless scaled, and of few significant bits, so that every product is exact: db sums the 40
+    positions whose gradient is not zero, and da (whose dh they alone have) 40 terms more."""
+    T, rank = (1 << 26) + 7, 65
+    if torch.cuda.mem_get_info()[0] < 90 << 30:
+        pytest.skip("needs 90 GB of device memory")
+    x = torch.full((T, 1), 512.0, dtype=F16, device=DEV)
+    a = torch.full((1, rank, 1), 256.0, dtype=F16, device=DEV)
+    a[0, ::2] = -128.0
+    b = torch.full((1, 1, rank), 2.0 ** -4, dtype=F16, device=DEV)
+    grad = torch.zeros(T, 1, dtype=F16, device=DEV)
+    grad[T % (T // 39) - 1::T // 39] = 2.0 ** -8  # 40, the last position among them
+    assert int(torch.count_nonzero(grad)) == 40
+    dx, da, db = eb.adapter_gradients(grad, x, a, b, torch.zeros(T, dtype=torch.int32, device=DEV))
+    assert (db[0, 0].float() == 40 * 2.0 ** -8 * 512 * a[0, :, 0].float()).all()
+    assert (da.float() == 40 * 2.0 ** -12 * 512).all()
+    dh = 2.0 ** -12 * float(a.double().sum())
+    assert (dx.float() == (grad != 0) * dh).all()
+    torch.cuda.empty_cache()
