@@ -14,7 +14,9 @@
 //
 // Longer sides: three tcgen05 products a step on planes of fp16.  A value is
 // kept as y = 2^12 x = hi + lo, two fp16 (22 significant bits); a product is
-// hi hi + hi lo + lo hi in fp32 accumulators in tensor memory.  Every iterate has
+// hi hi + hi lo + lo hi in fp32 accumulators in tensor memory.  22 bits of operands and sums that round toward zero
+// leave results of noise 6e-5 off at 2560 x 2560 (plain fp32 4e-6): an update is a direction to step in, and 33 bits in
+// three planes would take twice the products.  Every iterate has
 // entries below 16 (checked for the coefficients on the host), so hi is far from
 // fp16's limits, and lo's steps of 2^-24 are 2^-36 of x.  c0 is added to the
 // diagonal of the polynomial, so X' is one product.  Results rounded to bf16 take
@@ -542,6 +544,11 @@ enum Mode { GRAM, POLY, UPDATE, RESULT };
 constexpr int BM = 128;
 constexpr int kGemmThreads = 320, kEpilogueWarps = 8;
 constexpr int kStageTotal = 192 * 1024;
+// Longest sum that one accumulator takes, in products of three terms and of one (results of 8 bits).  An MMA cuts its
+// 16 products to a grid of 2^-25 of the sum, toward zero, so what a sum of one sign loses grows with its length, by
+// 2^-23 an MMA.  Without an end, 66 x 2^21 in fp32 was 2.0e-4 off and 1536 x 131072 2.9e-4, now 2.6e-5 and 1.4e-5
+// (2.9e-6 and 1.5e-5 in plain fp32).  Ends at 2048: 1.3e-5 and 9e-6, but 1060 us where 2560 x 2560 takes 955.
+constexpr int kChunk3 = 4096, kChunk1 = 16384;
 
 // A tile is 128 x 256 on one block, or 256 x 256 on a pair (PAIR): a cluster of two blocks whose tensor cores
 // work as one (cta_group::2).  Each block of a pair has half of A's rows and half of B's and reads the other half
@@ -556,6 +563,7 @@ struct Cfg {
     static constexpr int STAGES = kStageTotal / STAGE_BYTES;
     static constexpr int SMEM = STAGES * STAGE_BYTES + kEpilogueWarps * 4096 + 1024 + 256;
     static constexpr int TILE_M = PAIR ? 2 * BM : BM;
+    static constexpr int CHUNK = (TERMS == 3 ? kChunk3 : kChunk1) / KS;  // slices that one accumulator takes
 };
 
 struct Maps {
@@ -569,6 +577,7 @@ struct Job {
     int total;                    // tiles of the stack, times splits
     int splits;                   // blocks that share a tile's sum
     float* partial;               // [tile, split, 128, BN]: where they put theirs
+    float4* carry;                // [block, 128 BN / 4]: a tile's sum so far, where it takes more than one accumulator
     Planes out;        // GRAM, POLY, UPDATE
     Planes g;          // POLY: the planes of G; UPDATE, RESULT of one term: those of X
     float c0, c1, c2;  // POLY
@@ -803,12 +812,42 @@ __device__ __forceinline__ void finish_piece(const Job<Io>& job, uint8_t* tile, 
     }
 }
 
+// pieces x 32 columns of a warp's 32 rows of an accumulator, added to what stands in global memory (first: put there).
+// A lane comes back to its own places, in order.
+__device__ __forceinline__ void add_piece(uint32_t tmem, int pieces, bool first, float4* so_far) {
+#pragma unroll 1
+    for (int b = 0; b < pieces; b++) {
+        uint32_t r[32];
+        asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+            "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+              "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+              "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+              "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+            : "r"(tmem + 32 * b));
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+        for (int u = 0; u < 8; u++) {
+            float4 v = make_float4(__uint_as_float(r[4 * u]), __uint_as_float(r[4 * u + 1]), __uint_as_float(r[4 * u + 2]),
+                                   __uint_as_float(r[4 * u + 3]));
+            float4* to = so_far + 256 * b + 32 * u;
+            if (!first) {
+                const float4 p = *to;
+                v = make_float4(p.x + v.x, p.y + v.y, p.z + v.z, p.w + v.w);
+            }
+            *to = v;
+        }
+    }
+}
+
 // Tiles on persistent blocks, one an SM: warp 0 loads (TMA), one lane of warp 1 (of a pair's first block) issues the MMAs into
 // two accumulators in turn, and warps 2 to 9 take each through the mode's epilogue (tensor-memory lanes 32
 // (w % 4) .., half of the columns) while the next one is made: the epilogue, up to 8 us a tile beside 11 us
 // of products, costs time only after a block's last tile.  A wait that gives up (never, in a correct run)
-// makes the block's results from then on NaN.
-template <int MODE, bool A_MN, bool B_MN, int TERMS, bool PAIR, int BN, typename Io>
+// makes the block's results from then on NaN.  LONG: sums that take more than one accumulator; all but a tile's last are
+// added up in global memory, by the lanes that read them, while the next one is made.
+template <int MODE, bool A_MN, bool B_MN, int TERMS, bool PAIR, int BN, bool LONG, typename Io>
 __global__ void __launch_bounds__(kGemmThreads, 1) k_product(const __grid_constant__ Maps maps, const Job<Io> job) {
     using G = Cfg<TERMS, PAIR, BN>;
     constexpr int KS = G::KS, STAGES = G::STAGES;
@@ -894,37 +933,41 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_product(const __grid_consta
         if (lane == 0 && half == 0) {
             int i = 0, made = 0;
             bool ok = true;
-            for (int t = first_tile; t < job.total; t += tile_step, made++) {
-                const int acc = made & 1;
-                if (made >= 2) ok = ok && mbar_wait(acc_empty + 8 * acc, (uint32_t)((made / 2 - 1) & 1), nullptr);
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t d = tmem + acc * BN;
+            for (int t = first_tile; t < job.total && ok; t += tile_step) {
                 const int part = SPLIT ? t % job.splits : 0, parts = SPLIT ? job.splits : 1;
-                const int n0 = slices * part / parts, n1 = slices * (part + 1) / parts;
-                for (int n = n0; n < n1 && ok; n++, i++) {
-                    const int s = i % STAGES;
-                    ok = mbar_wait(full0 + 8 * s, (uint32_t)((i / STAGES) & 1), nullptr);
-                    if (!ok) break;
+                const int begin = slices * part / parts, count = slices * (part + 1) / parts - begin;
+                const int chunks = LONG ? (count + G::CHUNK - 1) / G::CHUNK : 1;
+                for (int c = 0; c < chunks; c++, made++) {
+                    const int acc = made & 1;
+                    if (made >= 2) ok = ok && mbar_wait(acc_empty + 8 * acc, (uint32_t)((made / 2 - 1) & 1), nullptr);
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t a = smem_u32(smem + s * G::STAGE_BYTES), b = a + G::A_BYTES;
-                    const uint32_t alo = b + G::B_BYTES, blo = alo + G::A_BYTES;
+                    const uint32_t d = tmem + acc * BN;
+                    const int n0 = count * c / chunks, n1 = count * (c + 1) / chunks;
+                    for (int n = n0; n < n1 && ok; n++, i++) {
+                        const int s = i % STAGES;
+                        ok = mbar_wait(full0 + 8 * s, (uint32_t)((i / STAGES) & 1), nullptr);
+                        if (!ok) break;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        const uint32_t a = smem_u32(smem + s * G::STAGE_BYTES), b = a + G::A_BYTES;
+                        const uint32_t alo = b + G::B_BYTES, blo = alo + G::A_BYTES;
 #pragma unroll
-                    for (int k = 0; k < KS / 16; k++) {  // 16 of K: 32 bytes along it, 16 rows of 128 bytes across it
-                        constexpr uint32_t sa = A_MN ? 2048 : 32, sb = B_MN ? 2048 : 32;
-                        const uint64_t ah = operand_desc<A_MN, KS>(a + sa * k), bh = operand_desc<B_MN, KS>(b + sb * k);
-                        const uint32_t first = (n > n0 || k > 0) ? 1u : 0u;
-                        if constexpr (TERMS == 3) {  // the small terms first
-                            umma_f16<A_MN, B_MN, PAIR, BN>(d, operand_desc<A_MN, KS>(alo + sa * k), bh, first);
-                            umma_f16<A_MN, B_MN, PAIR, BN>(d, ah, operand_desc<B_MN, KS>(blo + sb * k), 1u);
-                            umma_f16<A_MN, B_MN, PAIR, BN>(d, ah, bh, 1u);
-                        } else {
-                            umma_f16<A_MN, B_MN, PAIR, BN>(d, ah, bh, first);
+                        for (int k = 0; k < KS / 16; k++) {  // 16 of K: 32 bytes along it, 16 rows of 128 bytes across it
+                            constexpr uint32_t sa = A_MN ? 2048 : 32, sb = B_MN ? 2048 : 32;
+                            const uint64_t ah = operand_desc<A_MN, KS>(a + sa * k), bh = operand_desc<B_MN, KS>(b + sb * k);
+                            const uint32_t first = (n > n0 || k > 0) ? 1u : 0u;
+                            if constexpr (TERMS == 3) {  // the small terms first
+                                umma_f16<A_MN, B_MN, PAIR, BN>(d, operand_desc<A_MN, KS>(alo + sa * k), bh, first);
+                                umma_f16<A_MN, B_MN, PAIR, BN>(d, ah, operand_desc<B_MN, KS>(blo + sb * k), 1u);
+                                umma_f16<A_MN, B_MN, PAIR, BN>(d, ah, bh, 1u);
+                            } else {
+                                umma_f16<A_MN, B_MN, PAIR, BN>(d, ah, bh, first);
+                            }
                         }
+                        commit<PAIR>(empty0 + 8 * s);
                     }
-                    commit<PAIR>(empty0 + 8 * s);
+                    if (!ok) break;  // no accumulator any more: the epilogues' waits give up in their turn
+                    commit<PAIR>(acc_full + 8 * acc);
                 }
-                if (!ok) break;  // no accumulator any more: the epilogues' waits give up in their turn
-                commit<PAIR>(acc_full + 8 * acc);
             }
         }
         __syncwarp();
@@ -932,10 +975,26 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_product(const __grid_consta
         const int w = warp & 3, part = (warp - 2) >> 2;
         int made = 0;
         bool ok = true;
+        float4* so_far = job.carry + ((int64_t)blockIdx.x * kEpilogueWarps + warp - 2) * (BN * 4) + lane;
         for (int t = first_tile; t < job.total; t += tile_step, made++) {
         int z, m0, n0;
         tile_at<SYM, G::TILE_M, BN>(job, SPLIT ? t / job.splits : t, z, m0, n0);
         m0 += half * BM;
+        const int share = SPLIT ? t % job.splits : 0, shares = SPLIT ? job.splits : 1;
+        const int count = slices * (share + 1) / shares - slices * share / shares;
+        const int chunks = LONG ? (count + G::CHUNK - 1) / G::CHUNK : 1;
+        for (int c = 0; c + 1 < chunks; c++, made++) {  // all but the last accumulator of a long sum
+            const int acc = made & 1;
+            ok = ok && mbar_wait(acc_full + 8 * acc, (uint32_t)((made / 2) & 1), nullptr);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            add_piece(tmem + ((uint32_t)(32 * w) << 16) + (uint32_t)(acc * BN + part * (BN / 2)), BN / 64, c == 0, so_far);
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+                if constexpr (PAIR) mbar_arrive_leader(leaders(acc_empty + 8 * acc));
+                else mbar_arrive(acc_empty + 8 * acc);
+            }
+        }
         const int acc = made & 1;
         ok = ok && mbar_wait(acc_full + 8 * acc, (uint32_t)((made / 2) & 1), nullptr);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -975,6 +1034,14 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_product(const __grid_consta
                 const uint32_t nan = 0x7fc00000u;
                 *reinterpret_cast<uint4*>(tile + lane * 128 + ((u ^ (lane & 7)) << 4)) =
                     ok ? make_uint4(r[4 * u], r[4 * u + 1], r[4 * u + 2], r[4 * u + 3]) : make_uint4(nan, nan, nan, nan);
+            }
+            if (LONG && chunks > 1) {
+#pragma unroll
+                for (int u = 0; u < 8; u++) {
+                    const float4 p = so_far[(col - part * (BN / 2)) * 8 + 32 * u];
+                    float4* v = reinterpret_cast<float4*>(tile + lane * 128 + ((u ^ (lane & 7)) << 4));
+                    *v = make_float4(v->x + p.x, v->y + p.y, v->z + p.z, v->w + p.w);
+                }
             }
             __syncwarp();
             if (SPLIT && job.partial) {
@@ -1117,10 +1184,11 @@ int64_t norm_blocks(const Shape& s) {
 int64_t pad64(int64_t c) { return (c + 63) & ~int64_t(63); }
 
 constexpr int kSplitTiles = 148;  // 128 x 64 tiles' sums that blocks share
+constexpr int kMostBlocks = 148;  // of k_product: the workspace holds a tile's sum for each
 
 struct Layout {
     int64_t part, pmat;                     // small
-    int64_t partial, x[2], g, b, bytes;     // planes: hi, then lo
+    int64_t partial, carry, x[2], g, b, bytes;  // planes: hi, then lo
     int64_t x_plane, s_plane;               // bytes of one plane
 };
 
@@ -1139,6 +1207,7 @@ Layout layout_of(const Shape& s, int terms) {
     } else {
         l.part = take(s.stack * norm_blocks(s) * 8);
         l.partial = take(kSplitTiles * (int64_t)BM * 64 * 4);
+        l.carry = take(s.length > (terms == 3 ? kChunk3 : kChunk1) ? kMostBlocks * (int64_t)BM * 256 * 4 : 0);
         l.x_plane = align256(s.stack * s.rows * pad64(s.cols) * 2);
         l.s_plane = align256(s.stack * s.side * pad64(s.side) * 2);
         const int planes = terms == 3 ? 2 : 1;
@@ -1255,10 +1324,19 @@ int run_tiles(const Matrix& a, const Matrix& b, int64_t stack, Job<Io> job, cuda
         job.splits = (int)std::max<int64_t>(1, std::min<int64_t>(kSplitTiles / (tiles * stack), ceil_div(job.K, 4 * G::KS)));
     if (job.splits == 1) job.partial = nullptr;
     job.total = (int)(tiles * stack * job.splits);
-    constexpr auto kernel = k_product<MODE, A_MN, B_MN, TERMS, PAIR, BN, Io>;
-    const int most = PAIR ? pairs_at_once((const void*)kernel, G::SMEM) : sm_count();
+    // Where a sum is longer than an accumulator takes.  But for a Gram matrix the sums are as long as the short side,
+    // and those of 4096 and more have tiles for pairs.
+    constexpr bool MAY = PAIR || MODE == GRAM;
+    const bool longer = ceil_div(ceil_div(job.K, G::KS), job.splits) > G::CHUNK;
+    constexpr auto kernel = k_product<MODE, A_MN, B_MN, TERMS, PAIR, BN, false, Io>;
+    constexpr auto kernel_longer = k_product<MODE, A_MN, B_MN, TERMS, PAIR, BN, MAY, Io>;
+    if (longer && !MAY) return ENGRAM_ERR_RANGE;
+    const int most = PAIR ? std::min(pairs_at_once((const void*)kernel, G::SMEM), kMostBlocks / 2)
+                          : std::min(sm_count(), kMostBlocks);
     const int blocks = (PAIR ? 2 : 1) * std::min(job.total, most);
-    int e = start<kernel, PAIR ? 2 : 1>(dim3((unsigned)blocks), kGemmThreads, G::SMEM, true, st, maps, job);
+    const dim3 grid((unsigned)blocks);
+    int e = longer ? start<kernel_longer, PAIR ? 2 : 1>(grid, kGemmThreads, G::SMEM, true, st, maps, job)
+                   : start<kernel, PAIR ? 2 : 1>(grid, kGemmThreads, G::SMEM, true, st, maps, job);
     if constexpr (MODE == GRAM && BN == 64) {
         if (!e && job.partial)
             e = start<k_sum_tiles<TERMS, Io>>(dim3((unsigned)(8 * tiles * stack)), 256, 0, true, st, job);
@@ -1303,6 +1381,7 @@ int run_planes(const Shape& s, const Layout& l, const Io& io, const Poly& poly, 
                             true, st, io, s.rows, s.cols, vec, part, nb, eps, x[0].p);
     Job<NoIo> job = {};
     job.partial = (float*)(ws + l.partial);
+    job.carry = (float4*)(ws + l.carry);
     for (int i = 0; i < poly.steps && !e; i++) {
         const Matrix &in = x[i & 1], &next = x[(i & 1) ^ 1];
         job.M = job.N = (int)s.side;
@@ -1329,7 +1408,7 @@ int run_planes(const Shape& s, const Layout& l, const Io& io, const Poly& poly, 
             result.M = job.M, result.N = job.N, result.K = job.K;
             result.io = io;
             result.vec = vec;
-            result.g = in.p, result.c0 = job.c0;
+            result.g = in.p, result.c0 = job.c0, result.carry = job.carry;
             e = s.tall ? run_product<RESULT, false, false, TERMS>(in, b, s.stack, result, st)
                        : run_product<RESULT, false, true, TERMS>(b, in, s.stack, result, st);
         }

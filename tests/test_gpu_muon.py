@@ -302,3 +302,81 @@ def test_polynomials_near_the_limit_on_matrices_along_the_axes(c, dtype):
     assert ((got.double() - want).abs() <= bound).all()
     with pytest.raises(ValueError):
         eb.orthogonalize(x.to(BF16), steps=1, coefficients=(14.0, -40.0, 23.0))
+
+
+def iterated(x, steps=5, c=C):
+    """The definition step by step in 64 bits."""
+    tall = x.shape[-2] > x.shape[-1]
+    x = x.double().mT if tall else x.double()
+    x = x / x.square().sum((-2, -1), keepdim=True).sqrt()
+    for _ in range(steps):
+        g = x @ x.mT
+        x = c[0] * x + (c[1] * g + c[2] * (g @ g)) @ x
+    return x.mT if tall else x
+
+
+# 128 x 64 tiles whose blocks share sums, 128 x 256 tiles, a stack of them, pairs of blocks; each sum of 10^5 terms or
+# more but the second
+VERY_LONG = [(1, 66, 1 << 21), (150, 70, 20000), (1, 1536, 131072), (1, 140000, 1300), (1, 2600, 100001)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=str)
+@pytest.mark.parametrize("shape", VERY_LONG, ids=str)
+def test_the_gram_matrix_of_a_very_long_side(shape, dtype):
+    """One step of X <- G X on matrices of nearly one direction, where G is a sum of squares and any loss is one-sided.
+
+    Each MMA cuts its 16 products and the sum so far to one grid, 2^-25 of the sum: half of it for each of 16 products
+    of heads (those with a remainder are 2^-11 of them) is 2^-22 of the sum so far, and 2^-23 of the whole sum, which
+    grows from zero.  An accumulator takes 4096 / 16 = 256 of them in fp32: 3.1e-5, 1024 of one term in bf16: 1.2e-4.
+    2^-14 for fp32 and fp16, 2^-13 for bf16 leave room for nothing but the update's own sums, of 2600 or fewer and of
+    both signs.
+    Without an end to a sum, 131072 terms lost 9e-4 in fp32.  The loss is looked for along the result itself,
+    where errors of rounding average out.  Not all of bf16's: its values lie on the grid of the 11-bit operands, and all
+    of a matrix are multiplied by the same 1 / |U|; where that is (1 + e) 2^k with |e| < 2^-12 they all round back to the
+    grid, so all of X is off by e, G by 2 e and G X by 3 e, and rounding G adds 2^-12 at most: 2^-10 in all.  (The next
+    test takes that away.)"""
+    torch.manual_seed(160)
+    x = make(*shape, "noise", seed=60) * 0.05
+    x = (x + torch.randn(shape[0], shape[1], 1, device=DEV) * torch.randn(shape[0], 1, shape[2], device=DEV)).to(dtype)
+    want = iterated(x, 1, (0.0, 1.0, 0.0))
+    got = eb.orthogonalize(x, steps=1, coefficients=(0.0, 1.0, 0.0)).double()
+    along = (got * want).sum((1, 2)) / want.square().sum((1, 2)) - 1
+    assert float(along.abs().max()) <= (2.0 ** -13 + 2.0 ** -10 if dtype == BF16 else 2.0 ** -14), along
+    off = (got - want).norm() / want.norm()
+    assert float(off) <= (2.0 ** -8 if dtype == BF16 else 2.0 ** -13 + torch.finfo(dtype).eps / 2)
+    del x, want, got
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("shape", [(1, 1536, 131072), (1, 131072, 1536), (1, 2600, 131072)], ids=str)
+def test_the_gram_matrix_of_a_very_long_side_in_bf16(shape):
+    """As above, divided by a power of two (eps, above the norm), so that the operands hold bf16's values as they are.
+    G's entries are rounded to 2^-12, each its own way, and average out over some 10^5 of them: 2^-13 for the sums."""
+    torch.manual_seed(162)
+    x = make(*shape, "noise", seed=62) * 0.05
+    x = (x + torch.randn(shape[0], shape[1], 1, device=DEV) * torch.randn(shape[0], 1, shape[2], device=DEV)).to(BF16)
+    eps = 2.0 ** math.ceil(math.log2(float(x.double().norm())))
+    tall = shape[1] > shape[2]
+    want = x.double().mT / eps if tall else x.double() / eps
+    want = (want @ want.mT) @ want
+    got = eb.orthogonalize(x, steps=1, coefficients=(0.0, 1.0, 0.0), eps=eps).double()
+    got = got.mT if tall else got
+    along = float((got * want).sum() / want.square().sum()) - 1
+    assert abs(along) <= 2.0 ** -13
+    del x, want, got
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("shape", [(1, 66, 1 << 21), (1, 1536, 131072), (1, 4200, 4300), (1, 4300, 4200)], ids=str)
+def test_all_steps_of_very_long_sides(shape):
+    """fp32.  A sum of one sign loses 3.1e-5 (above), one of both signs less, and the five steps hand on what they lose:
+    2^-13 of the result in all, and the plain fp32 form's own error."""
+    x = make(*shape, "noise", seed=61)
+    want, own = iterated(x), plain(x).double()
+    own = float((own - want).norm())
+    got = eb.orthogonalize(x).double()
+    assert float((got - want).norm()) <= 2.0 ** -13 * float(want.norm()) + own
+    y = x.to(BF16)
+    want = iterated(y)
+    assert float((eb.orthogonalize(y).double() - want).norm()) <= (2.0 ** -8 + 2.0 ** -9) * float(want.norm())
+    torch.cuda.empty_cache()
