@@ -15,7 +15,8 @@ applies them to the PLE block's key and value projections.  The reference has
 no adapters: its descent trains table rows only.
 
 float32, bfloat16 and float16; sums in fp32, results rounded once and, for the
-same inputs, the same bits.
+same inputs, the same bits.  Infinities and NaN stay in the rows and gradients of
+the positions' own adapters.
 """
 from __future__ import annotations
 

@@ -409,6 +409,22 @@ constexpr int fit_stages(int bytes) {
            : 2 * bytes <= 108 * 1024 ? 2 : 3 * bytes <= 216 * 1024 ? 3 : 2;
 }
 
+// What split operands make of values that are not finite, or that round to infinity in the operand's type, is NaN
+// (inf - inf), never a finite number; zeros that fill a tile do the same.  So a result that is not finite is summed
+// once more, term by term in fp32, which gives the infinity, the NaN or the finite value that the formula has.  Threads
+// find out from the sum of their results, which costs less than a look at each.
+__device__ __forceinline__ bool finite(float v) { return fabsf(v) <= 3.402823466e38f; }
+__device__ __forceinline__ float finite_abs(float v) { return finite(v) ? fabsf(v) : 0.f; }
+struct Total {  // of many results, two at a time
+    uint64_t two = 0;
+    __device__ __forceinline__ void add(float a, float b) {
+        asm("{\n\t.reg .b64 t;\n\tmov.b64 t, {%1, %2};\n\tadd.rn.f32x2 %0, %0, t;\n\t}" : "+l"(two) : "f"(a), "f"(b));
+    }
+    __device__ __forceinline__ bool ok() const {
+        return finite(__uint_as_float((uint32_t)two) + __uint_as_float((uint32_t)(two >> 32)));
+    }
+};
+
 // ---- shrink --------------------------------------------------------------------
 // h[split, t, :] = scale_i * sum over this split's columns k of x[t, k] W_i[:, k].
 // TRANS = false: W_i = A_i [rank, K] (K consecutive); true: W_i = B_i [K, rank] (rank consecutive).
@@ -449,6 +465,17 @@ struct Shrink {
     bool xvec, wvec;
     float* h;
 };
+
+// A position's sum over columns k_begin .. k_end for one rank; beyond the last there is nothing.
+template <bool TRANS, typename T>
+__device__ __forceinline__ float plain_shrink(const T* x, const T* w, int64_t K, int rank, int r, int64_t k_begin,
+                                              int64_t k_end) {
+    float v = 0.f;
+    if (r < rank)
+#pragma unroll 1
+        for (int64_t k = k_begin; k < k_end; k++) v = fmaf(wide(x[k]), wide(TRANS ? w[k * rank + r] : w[r * K + k]), v);
+    return v;
+}
 
 template <typename T, int RB, int WM, bool TRANS>
 __device__ __forceinline__ void shrink_tile(uint8_t* smem, TileRows<16 * WM>& tr, const Plan& plan, int tiles,
@@ -637,11 +664,20 @@ __device__ __forceinline__ void shrink_tile(uint8_t* smem, TileRows<16 * WM>& tr
 #pragma unroll
         for (int k = 0; k < 4; k++) red[(wk * BM + 16 * wm + g + 8 * (k >> 1)) * RP + column(b, k & 1)] = result(b, k);
     __syncthreads();
+    float all = 0.f;  // of this thread's sums: not finite where one is not
     for (int e = threadIdx.x; e < rows * RP; e += kThreads) {
         float v = 0.f;
 #pragma unroll
         for (int k = 0; k < WK; k++) v += red[k * BM * RP + e];
         dst[(int64_t)row_of[e / RP] * RP + e % RP] = s * v;
+        all += v;
+    }
+    if (!finite(all)) {
+#pragma unroll 1
+        for (int e = threadIdx.x; e < rows * RP; e += kThreads) {
+            float* h = dst + (int64_t)row_of[e / RP] * RP + e % RP;
+            if (!finite(*h)) *h = s * plain_shrink<TRANS>(x + (int64_t)row_of[e / RP] * ldx, wi, K, rank, e % RP, k_begin, k_end);
+        }
     }
 }
 
@@ -696,6 +732,20 @@ __global__ void __launch_bounds__(kThreads) k_sum_splits(float4* h, int h_splits
         f.x += u.x, f.y += u.y, f.z += u.z, f.w += u.w;
     }
     p[i] = f;
+}
+
+// The sum over ranks of a position's h and one column of factors, `step` elements apart.
+template <typename T>
+__device__ __forceinline__ float plain_expand(const float* h, int splits, int64_t stride, const T* w, int64_t step, int rank) {
+    float y = 0.f;
+#pragma unroll 1
+    for (int r = 0; r < rank; r++) {
+        float v = h[r];
+#pragma unroll 1
+        for (int k = 1; k < splits; k++) v += h[r + k * stride];
+        y = fmaf(v, wide(w[r * step]), y);
+    }
+    return y;
 }
 
 // 2^(14 - e) for m in [2^e, 2^(e + 1)): brings m into fp16 below 2^15; 1 for zero and for what is not finite.
@@ -762,6 +812,23 @@ __device__ __forceinline__ void copy_rows(const int32_t* row, int rows, const T*
                     if (c + e < f_end) dst[c + e] = base ? src[c + e] : narrow<T>(0.f);
             }
         }
+    }
+}
+
+// The results of a lane's rows and columns (of 32) that are not finite, once more.  bs: the rows' base, or null.
+template <typename T, typename C, bool TRANS>
+__device__ __noinline__ void patch_piece(const int32_t* row, int rows, int first, const uint8_t* bs, const float* h, int splits,
+                                         int T_rows, const T* w, int64_t F, int rank, int left, T* out, int64_t ldo) {
+    constexpr int E = C::E;
+    const int q = threadIdx.x & 3;
+    for (int i = 0; i < 16 * C::MT; i++) {
+        const int e = i % 8, r = first + 8 * (i / 8), f = (4 * (e / E) + q) * E + e % E;
+        if (r >= rows || f >= left) continue;
+        const int64_t t = row[r];
+        if (finite(wide(out[t * ldo + f]))) continue;
+        const float y = plain_expand<T>(h + t * C::RP, splits, (int64_t)T_rows * C::RP, w + (TRANS ? f : (int64_t)f * rank),
+                                        TRANS ? F : 1, rank);
+        out[t * ldo + f] = narrow<T>(bs ? wide(reinterpret_cast<const T*>(bs + r * C::B_PITCH)[f]) + y : y);
     }
 }
 
@@ -873,7 +940,7 @@ __global__ void __launch_bounds__(kThreads, RB * (int)sizeof(T) <= 8 ? 3 : RB * 
         if constexpr (std::is_same_v<T, __half>) {
             float most = 0.f;
 #pragma unroll
-            for (int i = 0; i < RP / 4; i++) most = fmaxf(most, fabsf(v[i]));
+            for (int i = 0; i < RP / 4; i++) most = fmaxf(most, finite_abs(v[i]));
             most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
             most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
             const float s = half_scale(most);
@@ -985,6 +1052,11 @@ __global__ void __launch_bounds__(kThreads, RB * (int)sizeof(T) <= 8 ? 3 : RB * 
                         for (int m = 0; m < MT; m++) mma<T>(acc[m][b], hi[m][s], w0[b], w1[b]);
                 }
             }
+            float all = 0.f;  // not finite where a product is not
+#pragma unroll
+            for (int m = 0; m < MT; m++)
+#pragma unroll
+                for (int b = 0; b < 4; b++) all += (acc[m][b][0] + acc[m][b][1]) + (acc[m][b][2] + acc[m][b][3]);
 #pragma unroll
             for (int m = 0; m < 2 * MT; m++) {
                 if (!live[m]) continue;
@@ -1012,6 +1084,9 @@ __global__ void __launch_bounds__(kThreads, RB * (int)sizeof(T) <= 8 ? 3 : RB * 
                     }
                 }
             }
+            if (!finite(all))
+                patch_piece<T, C, TRANS>(tr.row, rows, 16 * MT * wm + g, base ? bs + fs * (int)sizeof(T) : nullptr, h, splits, T_rows,
+                                         wi + (TRANS ? 1 : rank) * (f0 + fs), F, rank, left, out + f0 + fs, ldo);
         }
     }
 }
@@ -1110,8 +1185,8 @@ struct WideStep {
 
 template <typename T, int RB>
 __global__ void __launch_bounds__(kWideThreads, 1) k_expand_wide(const __grid_constant__ CUtensorMap w_map, Plan plan,
-                                                                 const float* h, int splits, int n, int64_t F,
-                                                                 int T_rows, const T* base, int64_t ldb, T* out,
+                                                                 const float* h, int splits, const T* w_all, int rank,
+                                                                 int64_t F, int T_rows, const T* base, int64_t ldb, T* out,
                                                                  int64_t ldo) {
     using C = WideCfg<T, RB>;
     constexpr int RP = C::RP, FS = C::FS, NS = C::NS, SPAN = C::SPAN, KB = C::KB, SIZE = C::SIZE, BM = C::BM;
@@ -1213,6 +1288,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) k_expand_wide(const __grid_co
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             }
             stage_wait<C::DEPTH - 1>();
+            Total all;  // not finite where a product is not
             float back[2] = {1.f, 1.f};
             if constexpr (std::is_same_v<T, __half>) {
                 if (real)
@@ -1244,6 +1320,11 @@ __global__ void __launch_bounds__(kWideThreads, 1) k_expand_wide(const __grid_co
                                 : "r"(from));
                     }
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                    for (int m = 0; m < 2; m++)
+#pragma unroll
+                        for (int j = 0; j < 4 * C::BLOCKS; j += 2)
+                            all.add(__uint_as_float(r[m][j]), __uint_as_float(r[m][j + 1]));
                     if (c2 == 2) {  // the accumulator, and the rows' scales, have been read
                         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                         __syncwarp();
@@ -1275,6 +1356,19 @@ __global__ void __launch_bounds__(kWideThreads, 1) k_expand_wide(const __grid_co
                         if (real && !ok) v = make_uint4(~0u, ~0u, ~0u, ~0u);  // NaN in every type
                         if (row[k] >= 0 && f < F) *reinterpret_cast<uint4*>(out + (int64_t)row[k] * ldo + f) = v;
                     }
+            }
+            if (real && ok && !all.ok()) {
+                const T* wi = w_all + (int64_t)plan.tile[at.tile].adapter * F * rank;
+#pragma unroll 1
+                for (int u = 0; u < 8 * E; u++) {
+                    const int e = u % E, unit = u / E;  // 4 k + c
+                    const int t = unit < 4 ? row[0] : row[1];
+                    const int64_t f = (int64_t)at.stage * FS + (unit & 3) * C::GROUP + q * E + e;
+                    if (t < 0 || f >= F || finite(wide(out[(int64_t)t * ldo + f]))) continue;
+                    const float y = plain_expand<T>(h + (int64_t)t * RP, splits, (int64_t)T_rows * RP, wi + f * rank, 1, rank);
+                    const T* b = reinterpret_cast<const T*>(fetched + slot * C::FETCH + warp * 4096 + lane * 16 + unit * 512) + e;
+                    out[(int64_t)t * ldo + f] = narrow<T>(base ? wide(*b) + y : y);
+                }
             }
             fetch(i + 2 * C::DEPTH, slot);
             slot = slot + 1 == C::DEPTH ? 0 : slot + 1;
@@ -1348,7 +1442,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) k_expand_wide(const __grid_co
                     float most = 0.f;
                     for (int c = 0; c < RP; c += 4) {
                         const float4 f = load_h(hp + c, splits, (int64_t)T_rows * RP);
-                        most = fmaxf(fmaxf(fmaxf(most, fabsf(f.x)), fmaxf(fabsf(f.y), fabsf(f.z))), fabsf(f.w));
+                        most = fmaxf(fmaxf(most, finite_abs(f.x)), fmaxf(fmaxf(finite_abs(f.y), finite_abs(f.z)), finite_abs(f.w)));
                     }
                     s = half_scale(most);
                     undo[tiles % 6][r] = 1.f / s;
@@ -1447,6 +1541,15 @@ struct WeightCfg {
     static_assert(SMEM <= 220 * 1024, "a block's shared memory");
 };
 
+// The sum over the positions listed of one column of x and one rank of h.
+template <typename T>
+__device__ __forceinline__ float plain_weight(const T* x, int64_t ldx, const float* h, int ldh, const int32_t* list, int count) {
+    float v = 0.f;
+#pragma unroll 1
+    for (int p = 0; p < count; p++) v = fmaf(wide(x[list[p] * ldx]), h[(int64_t)list[p] * ldh], v);
+    return v;
+}
+
 template <typename T, int RB>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 && RB <= 4 ? 3 : 1) k_weight(Plan plan, const int32_t* __restrict__ index, Side<T> side_a,
                                                      Side<T> side_b, int first, int n, int rank, int T_rows) {
@@ -1489,6 +1592,12 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 && RB <= 4 ? 3 : 1) k
         for (int64_t e = threadIdx.x; e < (int64_t)count * (RP / 4); e += kThreads) {  // count reaches 2^30
             const float4 v = load_h(h + (int64_t)list[e / (RP / 4)] * RP + 4 * (int)(e % (RP / 4)), 1, 0);
             m = fmaxf(fmaxf(fmaxf(m, fabsf(v.x)), fmaxf(fabsf(v.y), fabsf(v.z))), fabsf(v.w));
+        }
+        if (!finite(m)) {
+            m = 0.f;
+#pragma unroll 1
+            for (int64_t e = threadIdx.x; e < (int64_t)count * RP; e += kThreads)
+                m = fmaxf(m, finite_abs(h[(int64_t)list[e / RP] * RP + (int)(e % RP)]));
         }
 #pragma unroll
         for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
@@ -1688,6 +1797,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 && RB <= 4 ? 3 : 1) k
     if (parts > 1) cluster.sync();
     else __syncthreads();
     T* dst = side.out + (int64_t)a * rank * F;
+    float total = 0.f;  // of this thread's sums: not finite where one is not
     if (side.ovec) {  // 16 bytes a thread: along the columns, or along the ranks of a column
         for (int u = threadIdx.x + part * kThreads; u < FC * RP / E; u += parts * kThreads) {
             const int c = side.trans ? u % FC : u % (FC / E) * E, r = side.trans ? u / FC * E : u / (FC / E);
@@ -1711,9 +1821,25 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 && RB <= 4 ? 3 : 1) k
             }
             alignas(16) T o[E];
 #pragma unroll
-            for (int j = 0; j < E; j++) o[j] = narrow<T>(v[j]);
+            for (int j = 0; j < E; j++) {
+                total += v[j];
+                o[j] = narrow<T>(v[j]);
+            }
             T* to = dst + (side.trans ? (f0 + c) * rank + r : (int64_t)r * F + f0 + c);
             *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(o);
+        }
+        if (!finite(total)) {
+#pragma unroll 1
+            for (int u = threadIdx.x + part * kThreads; u < FC * RP / E; u += parts * kThreads) {
+                const int c = side.trans ? u % FC : u % (FC / E) * E, r = side.trans ? u / FC * E : u / (FC / E);
+                if (r >= rank || f0 + c >= F) continue;
+                T* to = dst + (side.trans ? (f0 + c) * rank + r : (int64_t)r * F + f0 + c);
+#pragma unroll 1
+                for (int j = 0; j < E; j++)
+                    if (!finite(wide(to[j])))
+                        to[j] = narrow<T>(plain_weight<T>(x + f0 + c + (side.trans ? 0 : j), ldx,
+                                                          h + r + (side.trans ? j : 0), RP, list, count));
+            }
         }
         if (parts > 1) cluster.sync();  // its shared memory is read until here
         return;
@@ -1726,7 +1852,17 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 && RB <= 4 ? 3 : 1) k
             const float* from = parts > 1 ? cluster.map_shared_rank(red, k) : red;
             v += from[r * RS + c] + from[(RP + r) * RS + c];
         }
+        total += v;
         dst[side.trans ? (f0 + c) * rank + r : (int64_t)r * F + f0 + c] = narrow<T>(v);
+    }
+    if (!finite(total)) {
+#pragma unroll 1
+        for (int e = threadIdx.x + part * kThreads; e < FC * RP; e += parts * kThreads) {
+            const int r = side.trans ? e % RP : e / FC, c = side.trans ? e / RP : e % FC;
+            if (r >= rank || f0 + c >= F) continue;
+            T* to = dst + (side.trans ? (f0 + c) * rank + r : (int64_t)r * F + f0 + c);
+            if (!finite(wide(*to))) *to = narrow<T>(plain_weight<T>(x + f0 + c, ldx, h + r, RP, list, count));
+        }
     }
     if (parts > 1) cluster.sync();  // its shared memory is read until here
 }
@@ -1917,7 +2053,7 @@ int run_expand_wide(const Shape& s, const Plan& plan, const float* h, int splits
            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return ENGRAM_ERR_CUDA;
     return start<k_expand_wide<T, RB>>(dim3((unsigned)sm_count()), kWideThreads, C::SMEM, true, st, map, plan, h,
-                 splits, s.n, F, (int)s.T, base, ldb, out, ldo);
+                 splits, w, s.rank, F, (int)s.T, base, ldb, out, ldo);
 }
 
 template <typename T, int RB, int WM, bool TRANS>

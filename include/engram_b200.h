@@ -680,7 +680,10 @@ ENGRAM_API int engram_gemm_3xtf32(const float* a_hi, const float* a_lo, const fl
  * 16-byte aligned rows (pointers, strides, K and N) take wide loads.
  * workspace: device scratch, 16-byte aligned, of
  * engram_adapter_workspace_bytes(..., backward = 0) bytes.
- * Sums run in one fixed order: the same inputs give the same bits.
+ * Sums run in one fixed order: the same inputs give the same bits.  Infinities,
+ * NaN and values up to the type's largest give what the formula gives in fp32, in
+ * their own adapter's rows and gradients only (such results are summed once more,
+ * term by term: calls full of them are slow).
  */
 ENGRAM_API int64_t engram_adapter_workspace_bytes(int64_t T, int32_t n_adapters, int32_t rank, int64_t K, int64_t N,
                                                   int32_t backward);

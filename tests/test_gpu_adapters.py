@@ -454,3 +454,83 @@ def test_scale_of_the_weight_gradients_over_more_positions_than_32_bits_of_eleme
     dh = 2.0 ** -12 * float(a.double().sum())
     assert (dx.float() == (grad != 0) * dh).all()
     torch.cuda.empty_cache()
+
+
+def formula_with_sums_in_fp32(c, grad):
+    """The formula in 64 bits where its sums and products in fp32 are finite, and those where they are not: h, dh and
+    every sum are fp32 by definition, so a product beyond fp32 is an infinity, and one of each sign make a NaN."""
+    def evaluate(up):
+        base, x, a, b, grad_ = (up(v) for v in (c["base"], c["x"], c["a"], c["b"], grad))
+        out, dx, da, db = base.clone(), torch.zeros_like(x), torch.zeros_like(a), torch.zeros_like(b)
+        for i in range(a.shape[0]):
+            t = (c["index"] == i).nonzero().flatten()
+            h, dh = (c["scale"][i] * v for v in (x[t] @ a[i].T, grad_[t] @ b[i]))
+            out[t] += h @ b[i].T
+            dx[t] = dh @ a[i]
+            da[i] = dh.T @ x[t]
+            db[i] = grad_[t].T @ h
+        return out, dx, da, db
+    return [torch.where(torch.isfinite(v), w, v.double()) for v, w in zip(evaluate(torch.Tensor.float),
+                                                                          evaluate(torch.Tensor.double))]
+
+
+def same_as_formula(got, want, mag, k, dtype):
+    """NaN and infinities where the formula has them (or leaves the type), and check()'s bound elsewhere."""
+    half = torch.finfo(dtype).eps / 2
+    rounded = want.to(dtype)
+    assert torch.equal(torch.isnan(got), torch.isnan(rounded))
+    there = torch.isinf(rounded)
+    assert torch.equal(torch.isinf(got), there) and torch.equal(got[there], rounded[there])
+    ok = torch.isfinite(rounded)
+    bound = (2.0 ** -20 + k * 2.0 ** -23) * mag[ok] * (1 + half) + half * want[ok].abs()
+    bound += torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    assert ((got[ok].double() - want[ok]).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=str)
+@pytest.mark.parametrize("shape", [(60, 40, 56, 12), (100, 41, 57, 11), (1100, 41, 57, 11), (1500, 96, 264, 16), (1500, 64, 136, 48),
+                                   (1400, 72, 264, 100), (26001, 72, 1056, 128), (50001, 40, 1056, 40)], ids=str)
+def test_values_that_are_not_finite_or_near_the_types_largest(shape, dtype):
+    """Infinities and NaN in x, grad, base and the factors, and the type's largest values where products of them are
+    finite: as the formula has them, in their own adapters only."""
+    T, K, N, rank = shape
+    n = 8 if T > 200 else 7
+    c, grad = make(T, K, N, rank, n, dtype, "random", seed=70)
+    inf, most, small = float("inf"), torch.finfo(dtype).max, 2.0 ** -14 if dtype == F16 else 2.0 ** -100
+    c["scale"].copy_(2.0 ** torch.arange(n, device=DEV).remainder(3))
+    c["index"][:n] = torch.arange(n, device=DEV)
+    at = [(c["index"] == i).nonzero().flatten() for i in range(n)]
+    c["x"][at[0][0], 3] = inf
+    c["x"][at[0][-1], 5] = -inf
+    c["x"][at[1][0], 0] = float("nan")
+    c["x"][at[2][0], 7] = most  # an infinity in TF32's 11 bits
+    c["a"][2, :, 7] = small
+    grad[at[3][0], 2] = -inf
+    grad[at[3][-1], 4] = most
+    c["b"][3, 4] = small
+    c["a"][4, 0, 6] = most
+    c["x"][at[4], 6] = small
+    c["b"][5, 9, 1] = inf
+    c["b"][5, 8, 0] = -most
+    c["base"][at[6], 1] = -inf
+    c["base"][at[6][0], 2] = float("nan")
+    want, mag = formula_with_sums_in_fp32(c, grad), formula(c, grad, mag=True)
+    out = eb.adapter_add(**c)
+    same_as_formula(out, want[0], mag[0], K + rank, dtype)
+    if rank * K * N < 1 << 20:  # in place, where the base is overwritten
+        held = c["base"].clone()
+        assert torch.equal(eb.adapter_add(held, *list(c.values())[1:], out=held).nan_to_num(), out.nan_to_num())
+    for k, (got, w, m, terms) in enumerate(zip(eb.adapter_gradients(grad, c["x"], c["a"], c["b"], c["index"], c["scale"]),
+                                               want[1:], mag[1:], (N + rank, N + T, K + T))):
+        same_as_formula(got, w, m, terms, dtype)
+    assert torch.isfinite(out[at[2]]).all() and torch.isfinite(out[at[6][0], 3:]).all()
+
+
+def test_one_adapter_of_rank_one_hands_on_infinities_and_large_values():
+    for dtype in (F32, BF16, F16):
+        x = torch.zeros(2, 8, device=DEV, dtype=dtype)
+        x[0, 0], x[1, 0] = -float("inf"), torch.finfo(dtype).max
+        a, b = torch.zeros(1, 1, 8, device=DEV, dtype=dtype), torch.full((1, 4, 1), 0.5, device=DEV, dtype=dtype)
+        a[0, 0] = 0.25
+        out = eb.adapter_add(None, x, a, b, torch.zeros(2, dtype=torch.int32, device=DEV))
+        assert (out[0] == -float("inf")).all() and (out[1].double() == torch.finfo(dtype).max / 8).all()
