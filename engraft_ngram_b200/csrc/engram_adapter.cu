@@ -1550,7 +1550,7 @@ __device__ __forceinline__ float plain_weight(const T* x, int64_t ldx, const flo
     return v;
 }
 
-template <typename T, int RB>
+template <typename T, int RB, bool LONG>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 && RB <= 4 ? 3 : 1) k_weight(Plan plan, const int32_t* __restrict__ index, Side<T> side_a,
                                                      Side<T> side_b, int first, int n, int rank, int T_rows) {
     using C = WeightCfg<T, RB>;
@@ -1675,6 +1675,11 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 && RB <= 4 ? 3 : 1) k
         }
     };
 
+    // fp32 sums are taken out of the accumulators every stage.  For 16-bit results, of 8 or 11 bits, every 16384 positions
+    // do (2^20 of one sign were 4e-4 off without, 2^23 3e-3), into memory: registers are what bounds the blocks an SM.
+    // LONG: there may be so many (run_weight; 200 us of gradients take 203 with the look at each stage).
+    constexpr int DEEP = 256;
+    volatile float deep[LONG ? RM * NB * 4 : 1];
     float acc[RM][NB][4], sum[F32 ? RM : 1][NB][4];
 #pragma unroll
     for (int m = 0; m < RM; m++)
@@ -1773,7 +1778,27 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 && RB <= 4 ? 3 : 1) k
                     for (int b = 0; b < NB; b++) mma<T>(acc[m][b], fh, fb[b][0], fb[b][1]);
                 }
             }
+            if (LONG && (i + 1) % DEEP == 0) {
+#pragma unroll
+                for (int m = 0; m < RM; m++)
+#pragma unroll
+                    for (int b = 0; b < NB; b++)
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            volatile float& d = deep[(m * NB + b) * 4 + k];
+                            d = i < DEEP ? acc[m][b][k] : d + acc[m][b][k];
+                            acc[m][b][k] = 0.f;
+                        }
+            }
         }
+    }
+    if (LONG && stages >= DEEP) {
+#pragma unroll
+        for (int m = 0; m < RM; m++)
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) acc[m][b][k] += deep[(m * NB + b) * 4 + k];
     }
     stage_wait<0>();
     __syncthreads();
@@ -1914,7 +1939,9 @@ Shape shape_of(int64_t T, int n, int rank, int64_t K, int64_t N, bool backward) 
         const int64_t blocks = s.tiles * (s.wm == 8 ? 2 : 1), want = blocks > 0 ? ceil_div(2 * kSms, blocks) : 1;
         const int64_t can = ceil_div(width, 512);
         const int64_t k = want < can ? want : can;
-        return (int)(k < 1 ? 1 : k > 16 ? 16 : k);
+        // and no more than 2^17 columns a split: the accumulators' sums round toward zero, 7e-5 of 2^17 / 16 of one sign
+        const int64_t fewest = ceil_div(width, 1 << 17), some = k < 1 ? 1 : k > 16 ? 16 : k;
+        return (int)(some < fewest ? fewest : some);
     };
     s.splits_k = splits(K);
     s.splits_n = splits(N);
@@ -2078,6 +2105,8 @@ int run_expand(const Shape& s, const Plan& plan, const float* h, int splits, con
                  base && row_units(base, ldb), row_units(w, TRANS ? F : s.rank), row_units((const T*)out, ldo));
 }
 
+constexpr int64_t kManyPositions = 1 << 17;  // 16-bit sums over as many, all of one adapter, are 7e-5 off
+
 // Either side may be missing (out null).
 template <typename T, int RB>
 int run_weight(const Shape& s, const Plan& plan, const int32_t* index, const Side<T>& a, const Side<T>& b,
@@ -2089,9 +2118,12 @@ int run_weight(const Shape& s, const Plan& plan, const int32_t* index, const Sid
     const int64_t most = want < can ? want : can;
     const unsigned parts = most >= 8 ? 8 : most >= 4 ? 4 : most >= 2 ? 2 : 1;
     constexpr int most_smem = C::SMEM + (int)sizeof(Scan);
-    return start<k_weight<T, RB>, most_smem>(dim3((unsigned)(blocks_a + blocks_b), (unsigned)s.n, parts), kThreads,
-                                  s.planned ? C::SMEM : most_smem, true, st,
-                 plan, index, a, b, (int)blocks_a, s.n, s.rank, (int)s.T);
+    const dim3 grid((unsigned)(blocks_a + blocks_b), (unsigned)s.n, parts);
+    if (sizeof(T) == 2 && s.T > kManyPositions)  // planned
+        return start<k_weight<T, RB, sizeof(T) == 2>, most_smem>(grid, kThreads, C::SMEM, true, st, plan, index, a, b,
+                                                                 (int)blocks_a, s.n, s.rank, (int)s.T);
+    return start<k_weight<T, RB, false>, most_smem>(grid, kThreads, s.planned ? C::SMEM : most_smem, true, st, plan, index, a,
+                                                    b, (int)blocks_a, s.n, s.rank, (int)s.T);
 }
 
 struct Args {

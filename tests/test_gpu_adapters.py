@@ -534,3 +534,54 @@ def test_one_adapter_of_rank_one_hands_on_infinities_and_large_values():
         a[0, 0] = 0.25
         out = eb.adapter_add(None, x, a, b, torch.zeros(2, dtype=torch.int32, device=DEV))
         assert (out[0] == -float("inf")).all() and (out[1].double() == torch.finfo(dtype).max / 8).all()
+
+
+def along(got, want):
+    """How far got is along want: what is lost of sums of one sign, beside the rounding of the results."""
+    return float((got.double() * want).sum() / want.square().sum()) - 1
+
+
+# Truncating accumulators lose at most 2^-22 of the sum so far an MMA of 16 terms (16 products cut to a grid of 2^-25), half
+# of that over a sum that grows from zero: 2^-23 a time.  h is split to 2^-17.  Sums of so many values are nearly equal,
+# so the rounding of the results (half a step, 2^-9 or 2^-12) may be the same for all of them and does not average out.
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=str)
+@pytest.mark.parametrize("rank", [16, 40, 100])
+def test_weight_gradients_of_millions_of_positions_of_one_sign(dtype, rank):
+    """16384 positions an accumulator, of which half a block's warps have each half: 512 MMAs, 2^-14, twice that for the
+    two sums."""
+    T, K, N, half = (1 << 22) + 5, 48, 64, torch.finfo(dtype).eps / 2
+    g = torch.Generator(device=DEV).manual_seed(80)
+    one = lambda *s: torch.rand(*s, device=DEV, generator=g) + 0.5  # noqa: E731
+    x, a, b = one(T, K).to(dtype), (one(2, rank, K) / 64).to(dtype), (one(2, N, rank) / 64).to(dtype)
+    grad = (one(T, N) * 2.0 ** -10).to(dtype)
+    index = torch.ones(T, dtype=torch.int32, device=DEV)
+    index[::4096] = 0
+    dx, da, db = eb.adapter_gradients(grad, x, a, b, index)
+    for i in range(2):
+        t = (index == i).nonzero().flatten()
+        xi, gi = x[t].double(), grad[t].double()
+        assert abs(along(da[i], (gi @ b[i].double()).T @ xi)) <= 2.0 ** -13 + half
+        assert abs(along(db[i], gi.T @ (xi @ a[i].double().T))) <= 2.0 ** -13 + half
+        del xi, gi
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=str)
+@pytest.mark.parametrize("T", [20, 200])
+def test_widths_of_millions_of_one_sign(T, dtype):
+    """2^17 columns a split, of which two groups of warps have half each: 4096 MMAs, 2^-11.  2^24 columns in 16 splits
+    would be 32768 MMAs, 2^-8."""
+    K, N = 1 << 24, 24
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GB of device memory")
+    g = torch.Generator(device=DEV).manual_seed(81)
+    x = torch.empty(T, K, dtype=dtype, device=DEV)
+    for t in range(T):
+        x[t] = torch.rand(K, device=DEV, generator=g) + 0.5
+    a = ((torch.rand(1, 2, K, device=DEV, generator=g) + 0.5) * 2.0 ** -12).to(dtype)
+    b = (torch.rand(1, N, 2, device=DEV, generator=g) * 2.0 ** -4 + 2.0 ** -4).to(dtype)
+    out = eb.adapter_add(None, x, a, b, torch.zeros(T, dtype=torch.int32, device=DEV))
+    h = torch.cat([x[t:t + 1].double() @ a[0].double().T for t in range(T)])
+    assert abs(along(out, h @ b[0].double().T)) <= 2.0 ** -11 + torch.finfo(dtype).eps / 2
+    del x
+    torch.cuda.empty_cache()
