@@ -1675,7 +1675,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 && RB <= 4 ? 3 : 1) k
         }
     };
 
-    // fp32 sums are taken out of the accumulators every stage.  For 16-bit results, of 8 or 11 bits, every 16384 positions
+    // fp32 sums are taken out of the accumulators every stage.  For 16-bit results (of 8 or 11 bits) every 16384 positions
     // do (2^20 of one sign were 4e-4 off without, 2^23 3e-3), into memory: registers are what bounds the blocks an SM.
     // LONG: there may be so many (run_weight; 200 us of gradients take 203 with the look at each stage).
     constexpr int DEEP = 256;
