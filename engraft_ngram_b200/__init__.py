@@ -14,7 +14,8 @@ Drop-in use with the reference:
 from __future__ import annotations
 
 from . import _lib
-from ._lib import FMT_F32, FMT_IQ4_NL, FMT_IQ4_XS, MODE_CONCAT_F32, MODE_PAIRSUM_ADD_BF16
+from ._lib import (FMT_F32, FMT_IQ4_NL, FMT_IQ4_XS, MODE_CONCAT_F32, MODE_PAIRSUM_ADD_BF16,
+                   waits_given_up)
 from .adapters import PleAdapters, adapter_add, adapter_gradients
 from .muon import Muon, muon_step, orthogonalize
 from .optim import OverlayAdam, reg_scale
@@ -36,7 +37,7 @@ __all__ = [
     "write_pleo", "read_pleo_device", "FMT_F32", "FMT_IQ4_NL", "FMT_IQ4_XS", "MODE_CONCAT_F32",
     "MODE_PAIRSUM_ADD_BF16", "load_library", "scan_hits", "ple_forward", "install_ple", "uninstall_ple",
     "forget_overlay_map", "adapter_add", "adapter_gradients", "PleAdapters", "orthogonalize",
-    "muon_step", "Muon",
+    "muon_step", "Muon", "waits_given_up",
 ]
 
 

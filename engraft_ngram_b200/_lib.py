@@ -181,6 +181,8 @@ SIGNATURES = {
                                    C.c_void_p, C.c_double, C.c_void_p, C.c_int64, C.c_void_p]),
     "engram_selftest_mod": (C.c_int, [C.c_void_p, C.c_int64, C.c_uint32, C.c_void_p]),
     "engram_launch_count": (C.c_int64, []),
+    "engram_waits_given_up": (C.c_int64, []),
+    "engram_selftest_wait": (C.c_int, [C.c_void_p]),
 }
 
 _lib = None
@@ -227,6 +229,16 @@ def on_device(device, call):
         return call(torch._C._cuda_getCurrentRawStream(device.index))
     with torch.cuda.device(device):
         return call(torch.cuda.current_stream().cuda_stream)
+
+
+def waits_given_up(device=None) -> int:
+    """Barrier waits of kernels on the device that gave up instead of hanging it: 0 in a correct run.  Results that are
+    then missing are NaN; this tells them from NaN of other causes.  Waits for the device."""
+    import torch
+    with torch.cuda.device(device):
+        count = load().engram_waits_given_up()
+    check(min(count, 0), "engram_waits_given_up")
+    return count
 
 
 def ptr(t) -> int | None:

@@ -2209,6 +2209,8 @@ bool aligned_to(const void* p, int32_t dtype) {
 
 }  // namespace
 
+int64_t engram::adapter_waits_given_up() { return read_given_up(g_waits_given_up); }
+
 extern "C" int64_t engram_adapter_workspace_bytes(int64_t T, int32_t n_adapters, int32_t rank, int64_t K, int64_t N,
                                                   int32_t backward) {
     const int e = check_shape(T, n_adapters, rank, K, N);

@@ -264,6 +264,8 @@ int check_shape(int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb, int64
 
 }  // namespace
 
+int64_t engram::gemm_waits_given_up() { return read_given_up(g_waits_given_up); }
+
 extern "C" int engram_gemm_tf32(int32_t n_terms, const float* const* a, const float* const* b, int64_t M, int64_t N,
                                 int64_t K, int64_t lda, int64_t ldb, float* c, int64_t ldc, int32_t* err,
                                 void* stream) {

@@ -1478,6 +1478,32 @@ bool aligned_to(const void* p, int32_t dtype) {
 
 }  // namespace
 
+int64_t engram::ortho_waits_given_up() { return read_given_up(g_waits_given_up); }
+
+namespace {
+__global__ void k_wait_for_nothing() {
+    __shared__ uint64_t bar;
+    mbar_init(smem_u32(&bar), 1);
+    mbar_wait(smem_u32(&bar), 0, nullptr, 1000);
+}
+}  // namespace
+
+extern "C" int64_t engram_waits_given_up(void) {
+    if (cudaDeviceSynchronize() != cudaSuccess) return ENGRAM_ERR_CUDA;
+    int64_t sum = 0;
+    for (const int64_t v : {gemm_waits_given_up(), adapter_waits_given_up(), ortho_waits_given_up()}) {
+        if (v < 0) return v;
+        sum += v;
+    }
+    return sum;
+}
+
+extern "C" int engram_selftest_wait(void* stream) {
+    k_wait_for_nothing<<<1, 1, 0, (cudaStream_t)stream>>>();
+    count_launches(1);
+    return cudaGetLastError() == cudaSuccess ? ENGRAM_OK : ENGRAM_ERR_CUDA;
+}
+
 extern "C" int64_t engram_orthogonalize_workspace_bytes(int32_t dtype, int64_t stack, int64_t rows, int64_t cols) {
     if (dtype < ENGRAM_DTYPE_F32 || dtype > ENGRAM_DTYPE_F16) return ENGRAM_ERR_FORMAT;
     Shape s;

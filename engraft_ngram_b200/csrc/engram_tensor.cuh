@@ -13,6 +13,16 @@ namespace engram {
 
 constexpr long long kSpinLimit = 1ll << 24;  // polls of a barrier before a wait gives up
 
+// Waits that gave up in this source file's kernels, where no counter was given (engram_waits_given_up adds the files').
+static __device__ int g_waits_given_up;
+inline int64_t read_given_up(const int& symbol) {
+    int v = 0;
+    return cudaMemcpyFromSymbol(&v, symbol, sizeof(v)) == cudaSuccess ? v : ENGRAM_ERR_CUDA;
+}
+int64_t gemm_waits_given_up();
+int64_t adapter_waits_given_up();
+int64_t ortho_waits_given_up();
+
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
@@ -32,11 +42,11 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
-// Bounded wait for the phase with the given parity; false (and *err raised) on timeout.
+// Bounded wait for the phase with the given parity; false (and *err, or this file's own count, raised) on timeout.
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int* err, long long limit = kSpinLimit) {
     for (long long it = 0; it < limit; it++)
         if (mbar_try_wait(bar, parity)) return true;
-    if (err) atomicAdd(err, 1);
+    atomicAdd(err ? err : &g_waits_given_up, 1);
     return false;
 }
 

@@ -579,6 +579,17 @@ ENGRAM_API int engram_selftest_mod(const uint64_t* x, int64_t count, uint32_t d,
  * entry points, all devices); lets callers verify that the CUDA path ran. */
 ENGRAM_API int64_t engram_launch_count(void);
 
+/* Barrier waits that gave up on the current device, in all kernels that have
+ * such waits and got no counter of their own (engram_gemm_*'s err): 0 in a
+ * correct run.  A wait gives up after a bounded number of polls instead of
+ * hanging the device; its kernel then ends with NaN in the results that are
+ * missing, and this tells such NaN from others.  Waits for the device; not
+ * inside a stream capture.  Negative: a status. */
+ENGRAM_API int64_t engram_waits_given_up(void);
+/* Launches one thread that polls a barrier nothing arrives at, a thousand
+ * times: raises the count by one. */
+ENGRAM_API int engram_selftest_wait(void* stream);
+
 /* Library version (major*10000 + minor*100 + patch). */
 ENGRAM_API int engram_version(void);
 
