@@ -166,9 +166,6 @@ __global__ void __launch_bounds__(kPlanThreads) k_plan(const int32_t* __restrict
     }
 }
 
-__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-
 // Few positions need no launch for the plan: each block of the first launch looks through all indexes
 // itself, and writes its tile down for the launches after it.  List, in ascending order, of the positions
 // with adapter a (n: without one); every thread of the block calls it.
@@ -1131,9 +1128,6 @@ struct WideCfg {
 constexpr int kWideThreads = 640;
 constexpr long long kWideSpins = 1 << 20;  // polls of a barrier before a wait gives up: over ten milliseconds
 
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
     asm volatile(
@@ -1902,8 +1896,6 @@ struct Shape {
     int splits_k, splits_n;  // blocks per tile that share the sum over K, over N
 };
 
-int64_t align256(int64_t b) { return (b + 255) & ~int64_t(255); }
-int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Places of the workspace; bytes = its size.
 struct Layout {
@@ -1970,47 +1962,6 @@ Plan plan_at(uint8_t* ws, const Shape& s, const Layout& l) {
     return Plan{s.planned ? reinterpret_cast<int32_t*>(ws + l.off) : nullptr,
                 reinterpret_cast<int32_t*>(ws + l.perm),
                 s.planned ? reinterpret_cast<int32_t*>(ws + l.tiles) : nullptr, reinterpret_cast<Tile*>(ws + l.tile)};
-}
-
-template <typename... P, typename... A>
-cudaError_t launch(void (*kernel)(P...), const cudaLaunchConfig_t& cfg, A... args) {
-    return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
-}
-
-// Starts a kernel; after = true: it may start while the launch before it still runs (it waits for that
-// one's results itself, griddepcontrol.wait), which hides the start and its first loads.
-// MOST: the most dynamic shared memory a launch of the kernel takes (0: always `smem`).
-template <auto KERNEL, int MOST = 0, typename... A>
-int start(dim3 grid, int threads, int smem, bool after, cudaStream_t st, A... args) {
-    if (smem > 48 * 1024 || MOST > 48 * 1024) {
-        static bool allowed[64] = {false};
-        int dev = 0;
-        cudaGetDevice(&dev);
-        if (dev < 0 || dev >= 64 || !allowed[dev]) {
-            if (cudaFuncSetAttribute((const void*)KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     MOST ? MOST : smem) != cudaSuccess)
-                return ENGRAM_ERR_CUDA;
-            if (dev >= 0 && dev < 64) allowed[dev] = true;
-        }
-    }
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3((unsigned)threads);
-    cfg.dynamicSmemBytes = (size_t)smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[2] = {};
-    if (after) {
-        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
-    }
-    if (grid.z > 1) {  // a cluster shares its grid's third dimension
-        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
-        attr[cfg.numAttrs++].val.clusterDim = {1, 1, grid.z};
-    }
-    cfg.attrs = attr;
-    const cudaError_t e = launch(KERNEL, cfg, args...);
-    count_launches(1);
-    return e == cudaSuccess && cudaGetLastError() == cudaSuccess ? ENGRAM_OK : ENGRAM_ERR_CUDA;
 }
 
 int run_plan(const Shape& s, const int32_t* index, const Plan& plan, cudaStream_t st) {
@@ -2203,9 +2154,6 @@ int by_type(int32_t dtype, const Shape& s, const Layout& l, const Args& g, bool 
     return ENGRAM_ERR_FORMAT;
 }
 
-bool aligned_to(const void* p, int32_t dtype) {
-    return ((uintptr_t)p & (dtype == ENGRAM_DTYPE_F32 ? 3u : 1u)) == 0;
-}
 
 }  // namespace
 

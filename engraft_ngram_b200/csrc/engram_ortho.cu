@@ -150,9 +150,6 @@ struct MuonIo {
     __device__ __forceinline__ void before(Raw& r, int64_t i, int left, bool vec) const { r.p = load4(p, i, left, vec); }
 };
 
-__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-
 // ---- short sides up to 64 -------------------------------------------------------
 
 __device__ __forceinline__ void dmma(double* d, double a, double b) {
@@ -596,9 +593,6 @@ __device__ __forceinline__ uint64_t operand_desc(uint32_t addr) {
            ((uint64_t)1 << 46) | (swizzle << 61);
 }
 
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
 __device__ __forceinline__ void mbar_arrive_leader(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
@@ -1121,47 +1115,6 @@ __global__ void __launch_bounds__(256) k_sum_tiles(const Job<Io> job) {
 
 // ---- host ---------------------------------------------------------------------------
 
-int64_t align256(int64_t b) { return (b + 255) & ~int64_t(255); }
-int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-
-template <typename... P, typename... A>
-cudaError_t launch(void (*kernel)(P...), const cudaLaunchConfig_t& cfg, A... args) {
-    return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
-}
-
-// Starts a kernel; after = true: it may start while the launch before it still runs (it waits for that
-// one's results itself, griddepcontrol.wait).
-template <auto KERNEL, int CLUSTER = 1, typename... A>
-int start(dim3 grid, int threads, int smem, bool after, cudaStream_t st, A... args) {
-    if (smem > 48 * 1024) {
-        static bool allowed[64] = {false};
-        int dev = 0;
-        cudaGetDevice(&dev);
-        if (dev < 0 || dev >= 64 || !allowed[dev]) {
-            if (cudaFuncSetAttribute((const void*)KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-                return ENGRAM_ERR_CUDA;
-            if (dev >= 0 && dev < 64) allowed[dev] = true;
-        }
-    }
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3((unsigned)threads);
-    cfg.dynamicSmemBytes = (size_t)smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[2] = {};
-    if (after) {
-        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
-    }
-    if (CLUSTER > 1) {
-        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
-        attr[cfg.numAttrs++].val.clusterDim = {CLUSTER, 1, 1};
-    }
-    cfg.attrs = attr;
-    const cudaError_t e = launch(KERNEL, cfg, args...);
-    count_launches(1);
-    return e == cudaSuccess && cudaGetLastError() == cudaSuccess ? ENGRAM_OK : ENGRAM_ERR_CUDA;
-}
 
 struct Shape {
     int64_t stack, rows, cols, side, length;  // side <= length
@@ -1335,8 +1288,8 @@ int run_tiles(const Matrix& a, const Matrix& b, int64_t stack, Job<Io> job, cuda
                           : std::min(sm_count(), kMostBlocks);
     const int blocks = (PAIR ? 2 : 1) * std::min(job.total, most);
     const dim3 grid((unsigned)blocks);
-    int e = longer ? start<kernel_longer, PAIR ? 2 : 1>(grid, kGemmThreads, G::SMEM, true, st, maps, job)
-                   : start<kernel, PAIR ? 2 : 1>(grid, kGemmThreads, G::SMEM, true, st, maps, job);
+    int e = longer ? start<kernel_longer, 0, PAIR ? 2 : 1>(grid, kGemmThreads, G::SMEM, true, st, maps, job)
+                   : start<kernel, 0, PAIR ? 2 : 1>(grid, kGemmThreads, G::SMEM, true, st, maps, job);
     if constexpr (MODE == GRAM && BN == 64) {
         if (!e && job.partial)
             e = start<k_sum_tiles<TERMS, Io>>(dim3((unsigned)(8 * tiles * stack)), 256, 0, true, st, job);
@@ -1472,9 +1425,6 @@ int check_poly(int32_t steps, const double* c, double eps, bool apart, Poly* pol
 
 int terms_of(int32_t dtype) { return dtype == ENGRAM_DTYPE_BF16 ? 1 : 3; }
 
-bool aligned_to(const void* p, int32_t dtype) {
-    return ((uintptr_t)p & (dtype == ENGRAM_DTYPE_F32 ? 3u : 1u)) == 0;
-}
 
 }  // namespace
 

@@ -1,5 +1,6 @@
 // engram_tensor.cuh -- what the tcgen05 kernels share: mbarriers with bounded
-// waits, TMA tile loads (no multicast), MMA commits and tensor-map encoding.
+// waits, TMA tile loads (no multicast), MMA commits and tensor-map encoding; and
+// how they and the kernels around them are launched.
 #pragma once
 
 #include <cuda.h>
@@ -30,6 +31,9 @@ __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
 }
 __device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
     uint32_t ok;
@@ -68,6 +72,59 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
 __device__ __forceinline__ void umma_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
                  : "memory");
+}
+
+// ---- launches that overlap the one before them -----------------------------------
+
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+inline int64_t align256(int64_t b) { return (b + 255) & ~int64_t(255); }
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+inline bool aligned_to(const void* p, int32_t dtype) {
+    return ((uintptr_t)p & (dtype == ENGRAM_DTYPE_F32 ? 3u : 1u)) == 0;
+}
+
+template <typename... P, typename... A>
+inline cudaError_t launch(void (*kernel)(P...), const cudaLaunchConfig_t& cfg, A... args) {
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
+// Starts a kernel; after = true: it may start while the launch before it still runs (it waits for that
+// one's results itself, griddepcontrol.wait), which hides the start and its first loads.
+// MOST: the most dynamic shared memory a launch of the kernel takes (0: always `smem`).  CLUSTER: blocks along x
+// of a cluster; a grid's third dimension of more than one is a cluster too.
+template <auto KERNEL, int MOST = 0, int CLUSTER = 1, typename... A>
+int start(dim3 grid, int threads, int smem, bool after, cudaStream_t st, A... args) {
+    if (smem > 48 * 1024 || MOST > 48 * 1024) {
+        static bool allowed[64] = {false};
+        int dev = 0;
+        cudaGetDevice(&dev);
+        if (dev < 0 || dev >= 64 || !allowed[dev]) {
+            if (cudaFuncSetAttribute((const void*)KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     MOST ? MOST : smem) != cudaSuccess)
+                return ENGRAM_ERR_CUDA;
+            if (dev >= 0 && dev < 64) allowed[dev] = true;
+        }
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2] = {};
+    if (after) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (CLUSTER > 1 || grid.z > 1) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attr[cfg.numAttrs++].val.clusterDim = {CLUSTER, 1, CLUSTER > 1 ? 1 : grid.z};
+    }
+    cfg.attrs = attr;
+    const cudaError_t e = launch(KERNEL, cfg, args...);
+    count_launches(1);
+    return e == cudaSuccess && cudaGetLastError() == cudaSuccess ? ENGRAM_OK : ENGRAM_ERR_CUDA;
 }
 
 inline PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
