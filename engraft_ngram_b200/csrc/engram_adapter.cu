@@ -408,8 +408,8 @@ constexpr int fit_stages(int bytes) {
 
 // What split operands make of values that are not finite, or that round to infinity in the operand's type, is NaN
 // (inf - inf), never a finite number; zeros that fill a tile do the same.  So a result that is not finite is summed
-// once more, term by term in fp32, which gives the infinity, the NaN or the finite value that the formula has.  Threads
-// find out from the sum of their results, which costs less than a look at each.
+// once more, term by term in fp32 up to a NaN, which gives the infinity, the NaN or the finite value that the formula
+// has.  Threads find out from the sum of their results, which costs less than a look at each.
 __device__ __forceinline__ bool finite(float v) { return fabsf(v) <= 3.402823466e38f; }
 __device__ __forceinline__ float finite_abs(float v) { return finite(v) ? fabsf(v) : 0.f; }
 struct Total {  // of many results, two at a time
@@ -470,7 +470,7 @@ __device__ __forceinline__ float plain_shrink(const T* x, const T* w, int64_t K,
     float v = 0.f;
     if (r < rank)
 #pragma unroll 1
-        for (int64_t k = k_begin; k < k_end; k++) v = fmaf(wide(x[k]), wide(TRANS ? w[k * rank + r] : w[r * K + k]), v);
+        for (int64_t k = k_begin; k < k_end && v == v; k++) v = fmaf(wide(x[k]), wide(TRANS ? w[k * rank + r] : w[r * K + k]), v);
     return v;
 }
 
@@ -736,7 +736,7 @@ template <typename T>
 __device__ __forceinline__ float plain_expand(const float* h, int splits, int64_t stride, const T* w, int64_t step, int rank) {
     float y = 0.f;
 #pragma unroll 1
-    for (int r = 0; r < rank; r++) {
+    for (int r = 0; r < rank && y == y; r++) {
         float v = h[r];
 #pragma unroll 1
         for (int k = 1; k < splits; k++) v += h[r + k * stride];
@@ -1126,7 +1126,6 @@ struct WideCfg {
 };
 
 constexpr int kWideThreads = 640;
-constexpr long long kWideSpins = 1 << 20;  // polls of a barrier before a wait gives up: over ten milliseconds
 
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
@@ -1277,7 +1276,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) k_expand_wide(const __grid_co
             const bool real = at.tile < real_tiles;
             const int a = i & 3;
             if (real) {
-                ok = ok && mbar_wait(acc_full + 8 * a, (uint32_t)((i >> 2) & 1), nullptr, kWideSpins);
+                ok = ok && mbar_wait(acc_full + 8 * a, (uint32_t)((i >> 2) & 1), nullptr);
                 ok = __all_sync(0xffffffffu, ok);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             }
@@ -1376,7 +1375,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) k_expand_wide(const __grid_co
                 if (at.next(i) && at.tile < real_tiles) adapter = plan.tile[at.tile].adapter;
                 if (at.tile >= real_tiles) break;
                 const int s = made % NS;
-                if (made >= NS && !mbar_wait(empty + 8 * s, (uint32_t)((made / NS - 1) & 1), nullptr, kWideSpins)) break;
+                if (made >= NS && !mbar_wait(empty + 8 * s, (uint32_t)((made / NS - 1) & 1), nullptr)) break;
                 const uint32_t bar = full + 8 * s, to = smem_u32(smem + s * C::STAGE);
                 mbar_expect_tx(bar, C::W_BYTES);
                 const int y = (int)(((int64_t)adapter * F + (int64_t)at.stage * FS) / C::GROUP);
@@ -1385,7 +1384,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) k_expand_wide(const __grid_co
                 made++;
             }
             for (int k = made > NS ? made - NS : 0; k < made; k++)
-                mbar_wait(full + 8 * (k % NS), (uint32_t)((k / NS) & 1), nullptr, kWideSpins);
+                mbar_wait(full + 8 * (k % NS), (uint32_t)((k / NS) & 1), nullptr);
         }
     } else if (warp == 17) {
         if (lane == 0) {
@@ -1397,10 +1396,10 @@ __global__ void __launch_bounds__(kWideThreads, 1) k_expand_wide(const __grid_co
             for (int i = 0; i < steps && ok; i++) {
                 const bool first = at.next(i);
                 if (at.tile >= real_tiles) break;
-                if (first) ok = mbar_wait(h_full, (uint32_t)(tiles++ & 1), nullptr, kWideSpins);
+                if (first) ok = mbar_wait(h_full, (uint32_t)(tiles++ & 1), nullptr);
                 const int s = made % NS, a = made & 3;
-                ok = ok && mbar_wait((F32 ? low : full) + 8 * s, (uint32_t)((made / NS) & 1), nullptr, kWideSpins);
-                if (made >= 4) ok = ok && mbar_wait(acc_empty + 8 * a, (uint32_t)((made / 4 - 1) & 1), nullptr, kWideSpins);
+                ok = ok && mbar_wait((F32 ? low : full) + 8 * s, (uint32_t)((made / NS) & 1), nullptr);
+                if (made >= 4) ok = ok && mbar_wait(acc_empty + 8 * a, (uint32_t)((made / 4 - 1) & 1), nullptr);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t hh = smem_u32(planes), hl = hh + C::H_BYTES;
@@ -1426,7 +1425,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) k_expand_wide(const __grid_co
             if (!at.next(i)) continue;
             if (at.tile >= real_tiles) break;
             const Tile t = plan.tile[at.tile];
-            if (tiles && !mbar_wait(h_empty, (uint32_t)((tiles - 1) & 1), nullptr, kWideSpins)) break;
+            if (tiles && !mbar_wait(h_empty, (uint32_t)((tiles - 1) & 1), nullptr)) break;
 #pragma unroll 1
             for (int m = 0; m < BM; m += 32) {  // a row a lane
                 const int r = m + lane;
@@ -1479,7 +1478,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) k_expand_wide(const __grid_co
             at.next(i);
             if (at.tile >= real_tiles) break;
             const int s = made % NS;
-            if (!mbar_wait(full + 8 * s, (uint32_t)((made / NS) & 1), nullptr, kWideSpins)) break;
+            if (!mbar_wait(full + 8 * s, (uint32_t)((made / NS) & 1), nullptr)) break;
             uint8_t* w = smem + s * C::STAGE;
 #pragma unroll 4
             for (int u = lane; u < C::W_BYTES / 16; u += 32) {
@@ -1540,7 +1539,7 @@ template <typename T>
 __device__ __forceinline__ float plain_weight(const T* x, int64_t ldx, const float* h, int ldh, const int32_t* list, int count) {
     float v = 0.f;
 #pragma unroll 1
-    for (int p = 0; p < count; p++) v = fmaf(wide(x[list[p] * ldx]), h[(int64_t)list[p] * ldh], v);
+    for (int p = 0; p < count && v == v; p++) v = fmaf(wide(x[list[p] * ldx]), h[(int64_t)list[p] * ldh], v);
     return v;
 }
 
@@ -2044,7 +2043,9 @@ int run_expand(const Shape& s, const Plan& plan, const float* h, int splits, con
     // bf16 87 and 94 at 2048, 136 and 126 at 4096, 380 and 238 at 16384, in fp32 148 and 154, 250 and 219, 784 and
     // 624; rank 128 in bf16 186 and 147 at 2048, 383 and 215 at 8192.
     if constexpr (WM == 8 && !TRANS && WideCfg<T, RB>::OK) {
-        if (s.T * F >= (3ll << 30) / (8 * RB) && s.planned && s.n > 0 && F % WideCfg<T, RB>::GROUP == 0 && s.n * F / WideCfg<T, RB>::GROUP < (1ll << 31) &&
+        // More than 16 splits only widths over 2^21 have: adding them up once more for results that are not finite would
+        // take milliseconds a stage, which the waits' limit leaves no room for.
+        if (s.T * F >= (3ll << 30) / (8 * RB) && splits <= 16 && s.planned && s.n > 0 && F % WideCfg<T, RB>::GROUP == 0 && s.n * F / WideCfg<T, RB>::GROUP < (1ll << 31) &&
             (!base || row_units(base, ldb)) && row_units((const T*)out, ldo) && row_units(w, s.rank))
             return run_expand_wide<T, RB>(s, plan, h, splits, w, F, base, ldb, out, ldo, st);
     }

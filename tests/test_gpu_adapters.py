@@ -623,3 +623,24 @@ def test_gradients_of_many_positions_to_the_accuracy_of_the_plain_form(case):
             bound = 4 * own + half * size
             assert bound <= 2.0 ** -7 * size and float((got[k][i].double() - w).norm()) <= bound, (k, size, own)
     assert (got[0][c["index"] < 0] == 0).all()
+
+
+@pytest.mark.parametrize("case", [(2048, 6400, 12800, 128, 3, BF16), (2048, 4096, 12800, 100, 3, F32)], ids=str)
+def test_a_poisoned_adapter_leaves_the_others_their_bits(case):
+    """Each result of an adapter that is all NaN is summed twice, from sums of several splits, while the other adapters'
+    accumulators wait: no wait may give up, and no other row may change."""
+    c, grad = make(*case, index="random", seed=95)
+    before = eb.waits_given_up()
+    want = eb.adapter_add(**c)
+    grads = eb.adapter_gradients(grad, c["x"], c["a"], c["b"], c["index"], c["scale"])
+    for k in ("a", "b"):
+        c[k][1] = float("nan")
+    got = eb.adapter_add(**c)
+    sick = c["index"] == 1
+    assert torch.isnan(got[sick]).all() and torch.equal(got[~sick], want[~sick])
+    dx, da, db = eb.adapter_gradients(grad, c["x"], c["a"], c["b"], c["index"], c["scale"])
+    well = [0, 2]
+    assert torch.isnan(dx[sick]).all() and torch.equal(dx[~sick], grads[0][~sick])
+    assert torch.equal(da[well], grads[1][well]) and torch.equal(db[well], grads[2][well])
+    assert torch.isnan(da[1]).all() and torch.isnan(db[1]).all()
+    assert eb.waits_given_up() == before
