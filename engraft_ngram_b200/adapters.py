@@ -37,7 +37,9 @@ class PleAdapters:
     """Adapters of the PLE block's projections: a [n, rank, n_embd] and
     b [n, hc*n_embd + n_embd, rank] (key columns, then value columns, as the
     stacked projection [w_key; w_value] has its rows), index int32 [T] of the
-    positions' adapters, scale float32 [n] or None (1)."""
+    positions' adapters, scale float32 [n] or None (1).  The block computes in
+    float32, so a and b are float32; 16-bit adapters are for adapter_add beside
+    a caller's own projection."""
     a: torch.Tensor
     b: torch.Tensor
     index: torch.Tensor

@@ -289,8 +289,8 @@ def ple_forward(emb: torch.Tensor, hidden: torch.Tensor, w, hist: torch.Tensor, 
     """(hidden + gated + silu(conv), new history tail): see the reference's
     docstring.  Differentiable in emb, hidden and hist (detach_value /
     detach_gate as in the reference); diag receives the same five tensors.
-    adapters: low-rank adapters of the positions' requests, added to the key and
-    value projections; differentiable in their factors too."""
+    adapters: low-rank adapters (float32, as the block) of the positions' requests,
+    added to the key and value projections; differentiable in their factors too."""
     if weights_need_grad(w):
         raise NotImplementedError("engraft_ngram_b200.ple_forward does not build gradients of the block's weights; "
                                   "install_ple routes such calls to the reference's ple_forward")
