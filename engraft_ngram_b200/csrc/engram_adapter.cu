@@ -1595,8 +1595,10 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 && RB <= 4 ? 3 : 1) k
         if (!finite(m)) {
             m = 0.f;
 #pragma unroll 1
-            for (int64_t e = threadIdx.x; e < (int64_t)count * RP; e += kThreads)
-                m = fmaxf(m, finite_abs(h[(int64_t)list[e / RP] * RP + (int)(e % RP)]));
+            for (int64_t e = threadIdx.x; e < (int64_t)count * (RP / 4); e += kThreads) {
+                const float4 v = load_h(h + (int64_t)list[e / (RP / 4)] * RP + 4 * (int)(e % (RP / 4)), 1, 0);
+                m = fmaxf(fmaxf(m, finite_abs(v.x)), fmaxf(fmaxf(finite_abs(v.y), finite_abs(v.z)), finite_abs(v.w)));
+            }
         }
 #pragma unroll
         for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));

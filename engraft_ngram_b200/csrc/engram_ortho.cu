@@ -936,7 +936,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_product(const __grid_consta
                     if (made >= 2) ok = ok && mbar_wait(acc_empty + 8 * acc, (uint32_t)((made / 2 - 1) & 1), nullptr);
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint32_t d = tmem + acc * BN;
-                    const int n0 = count * c / chunks, n1 = count * (c + 1) / chunks;
+                    const int n0 = (int)((int64_t)count * c / chunks), n1 = (int)((int64_t)count * (c + 1) / chunks);
                     for (int n = n0; n < n1 && ok; n++, i++) {
                         const int s = i % STAGES;
                         ok = mbar_wait(full0 + 8 * s, (uint32_t)((i / STAGES) & 1), nullptr);
